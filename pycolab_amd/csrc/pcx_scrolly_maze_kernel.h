@@ -593,20 +593,13 @@ __device__ __forceinline__ void ps_dma_row(const uint32_t* base, uint32_t voff, 
       : "v"(voff), "s"(base), "s"(lds_addr)
       : "memory");
 }
-// The next ticket of the work counter: a SCALAR atomic (s_atomic_add; gfx950 has them, coherent across the XCDs:
-// tools/experiments/satomic_probe.hip).  It travels through the scalar cache path, not behind the CU's queue of plane
-// stores, and is waited for on lgkmcnt -- about a microsecond -- so a worker knows its next unit just before it
-// needs it and reserves nothing further ahead (what a worker holds in reserve when the tickets run out is the tail).
-__device__ __forceinline__ uint32_t ps_ticket(uint32_t* ctr_any) {
-  // (uniform by construction; readfirstlane makes it provably so, and the SALU copy inside the statement keeps the scalar
-  // memory instruction from reading an SGPR pair a VALU instruction has just written)
-  const uint64_t v = reinterpret_cast<uint64_t>(ctr_any);
-  const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)v), hi = __builtin_amdgcn_readfirstlane((uint32_t)(v >> 32));
-  uint32_t* const ctr = reinterpret_cast<uint32_t*>(((uint64_t)hi << 32) | lo);
-  uint32_t t = 1u;
-  uint64_t own;
-  asm volatile("s_mov_b64 %1, %2\n\ts_atomic_add %0, %1, 0x0 glc\n\ts_waitcnt lgkmcnt(0)" : "+s"(t), "=&s"(own) : "s"(ctr) : "memory");
-  return t;
+// The next ticket of the work counter: one returning vector atomic by the wave's first lane, drawn just before the worker
+// needs its next unit, so that it reserves nothing further ahead (what a worker holds in reserve when the tickets run out
+// is the tail).  The unit's logic phase, some 20 us, lies between the last plane stores and this wait.
+__device__ __forceinline__ uint32_t ps_ticket(uint32_t* ctr) {
+  uint32_t t = 0;
+  if ((threadIdx.x & 63u) == 0) t = atomicAdd(ctr, 1u);
+  return __builtin_amdgcn_readfirstlane(t);
 }
 __device__ __forceinline__ uint32_t lds_byte_address(const uint32_t* p) {
   return (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const uint32_t*)p;
@@ -1474,7 +1467,7 @@ __global__ __launch_bounds__(COOP ? 8 * WAVE : PS == 3 ? 12 * WAVE : WAVE) void 
   const uint32_t env_stride = (uint32_t)(1 + L) * (uint32_t)pitch;
   const int64_t env0 = env0_render;
   if constexpr (PS == 3) {
-    // the next unit is drawn (scalar atomic, ~1 us) and its state words start travelling now, in front of this unit's
+    // the next unit is drawn (one atomic) and its state words start travelling now, in front of this unit's
     // plane stores: they have landed when the loop below is through (vmcnt is in order, 63 at most)
     if (ps_prof) { const uint32_t t = ps_now(); pt_c += t - pt_mark; pt_mark = t; ++pt_units; }
     if (P.ps_dynamic) {

@@ -61,16 +61,13 @@ __device__ __forceinline__ uint32_t lds_byte_address(const uint32_t* p) {
 // front of the current unit's plane stores (vmcnt counts in order and holds 63: after 64 plane stores they have landed),
 // and at most `lock` workers of a workgroup in the streaming loop at a time.  pcx_scrolly_maze.hip has the measurements.
 
-// The next ticket of a work counter: a SCALAR atomic (s_atomic_add; coherent across the XCDs: tools/experiments/
-// satomic_probe.hip) -- through the scalar cache, not behind the CU's queue of plane stores; waited for on lgkmcnt.
-__device__ __forceinline__ uint32_t scalar_ticket(uint32_t* ctr_any) {
-  const uint64_t v = reinterpret_cast<uint64_t>(ctr_any);
-  const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)v), hi = __builtin_amdgcn_readfirstlane((uint32_t)(v >> 32));
-  uint32_t* const ctr = reinterpret_cast<uint32_t*>(((uint64_t)hi << 32) | lo);
-  uint32_t t = 1u;
-  uint64_t own;
-  asm volatile("s_mov_b64 %1, %2\n\ts_atomic_add %0, %1, 0x0 glc\n\ts_waitcnt lgkmcnt(0)" : "+s"(t), "=&s"(own) : "s"(ctr) : "memory");
-  return t;
+// The next ticket of a work counter: one returning vector atomic by the wave's first lane, the same number for every lane.
+// It queues behind the wave's own plane stores, but a worker draws only after a logic phase of some 20 us, when those have
+// left: the wait is the atomic's own round trip.
+__device__ __forceinline__ uint32_t wave_ticket(uint32_t* ctr) {
+  uint32_t t = 0;
+  if ((threadIdx.x & 63u) == 0) t = atomicAdd(ctr, 1u);
+  return __builtin_amdgcn_readfirstlane(t);
 }
 // A counting semaphore in LDS around the streaming loop: lane 0 alone adds; a wave that finds the count at the limit takes
 // its increment back and tries again a little later.  Giving up after SLOT_SPINS tries (seconds) costs nothing but speed:
@@ -125,7 +122,7 @@ struct WorkQueue {
     while (stolen < shards) {
       const uint32_t y = x + stolen >= shards ? x + stolen - shards : x + stolen;
       const uint32_t nwk_y = ((gridDim.x - y + shards - 1u) / shards) * wpw;
-      const uint32_t cand = y + shards * (nwk_y + scalar_ticket(ctr + 16u * y));
+      const uint32_t cand = y + shards * (nwk_y + wave_ticket(ctr + 16u * y));
       if (cand < n) return cand;
       ++stolen;
     }
