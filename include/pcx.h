@@ -613,6 +613,49 @@ int pcx_post_error_poll(pcx_post* p, void* stream, int32_t* seen);
 int pcx_post_errors(pcx_post* p, uint8_t* errors_host);
 
 /* ------------------------------------------------------------------------ */
+/* Policy operators: what a policy computes between an observation and an action, over the batch layouts of this library.
+ * They have no handle: every call takes plain device pointers and the stream it runs on, allocates nothing, waits for
+ * nothing and may be captured into a graph.  The calling thread's current device must be the pointers' device.  Where a
+ * workspace is asked for, it belongs to that one call until the stream has passed it: two calls that may run at the same
+ * time (two streams, two captured graphs) need two. */
+
+enum pcx_policy_dtype { PCX_F16 = 6, PCX_BF16 = 7 }; /* besides PCX_F32 = 3 */
+enum pcx_activation { PCX_ACT_NONE = 0, PCX_ACT_RELU = 1, PCX_ACT_SILU = 2, PCX_ACT_TANH = 3, PCX_ACT_GELU = 4 };
+
+/* out = act(features . weight^T + bias) + residual, with `features` the 0/1 layer stack that
+ * rendering.ObservationToFeatureArray (rendering.py:545-661) would make of the boards, which is never written:
+ *   stacked == 0: `boards` holds uint8 characters [n][cells] (board b at b * row_stride): layer k of a cell is
+ *     (character == chars[k]); the chars are distinct, characters that are none of them count nowhere;
+ *   stacked != 0: `boards` holds uint8 layers (layer k of board b at b * row_stride + layer_offset[k], or nowhere, all
+ *     zero, where the offset is negative), set where nonzero -- for observations whose layers overlap
+ *     (occlusion_in_layers=False).
+ * weight, bias, residual, out: `dtype` (PCX_F32, PCX_F16, PCX_BF16); weight [hidden][n_layers][cells], bias [hidden] or
+ * NULL, residual and out [n][hidden], contiguous.  Sums are float32. */
+typedef struct pcx_project_desc {
+  int64_t n;              /* boards                                          */
+  int64_t row_stride;     /* bytes from one board to the next                */
+  int64_t layer_offset[PCX_POST_MAX_DEPTH]; /* stacked: bytes from a board's start to its layers */
+  int32_t cells;          /* rows * columns                                  */
+  int32_t n_layers;       /* 1 .. PCX_POST_MAX_DEPTH                         */
+  int32_t hidden;
+  int32_t dtype, activation, stacked;
+  uint8_t chars[PCX_POST_MAX_DEPTH];
+} pcx_project_desc;
+
+/* Bytes of the laid-out weight and of the two workspaces (any pointer may be NULL; 0: none needed).  The weight's bytes
+ * do not depend on n; the workspaces' do. */
+int pcx_project_sizes(const pcx_project_desc* d, uint64_t* packed_bytes, uint64_t* forward_bytes, uint64_t* backward_bytes);
+/* Lays the weight out for pcx_project_forward (16-byte aligned `packed`); again after every change of the weight. */
+int pcx_project_pack(const pcx_project_desc* d, const void* weight, void* packed, void* stream);
+/* slope: NULL, or [n][hidden] that receives act'(...) for pcx_project_backward. */
+int pcx_project_forward(const pcx_project_desc* d, const uint8_t* boards, const void* packed, const void* bias,
+                        const void* residual, void* out, void* slope, void* workspace, uint64_t workspace_bytes, void* stream);
+/* Gradients from grad_out [n][hidden]: grad_weight [hidden][n_layers][cells] and grad_bias [hidden] (either may be
+ * NULL); the residual's gradient is grad_out itself.  slope may be NULL for PCX_ACT_NONE. */
+int pcx_project_backward(const pcx_project_desc* d, const uint8_t* boards, const void* grad_out, const void* slope,
+                         void* grad_weight, void* grad_bias, void* workspace, uint64_t workspace_bytes, void* stream);
+
+/* ------------------------------------------------------------------------ */
 /* Node-level gather of the step results: environments never
  * interact (one Engine per environment, pycolab/engine.py:102-104), so a batch
  * sharded over the GPUs of a node needs no data-path collective; the one

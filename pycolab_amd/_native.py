@@ -129,6 +129,16 @@ class EpilogueDesc(ctypes.Structure):
               ('mapped', ctypes.c_void_p)]
 
 
+F16, BF16 = 6, 7
+ACT_NONE, ACT_RELU, ACT_SILU, ACT_TANH, ACT_GELU = 0, 1, 2, 3, 4
+
+
+class ProjectDesc(ctypes.Structure):
+  _fields_ = [('n', c_i64), ('row_stride', c_i64), ('layer_offset', c_i64 * POST_MAX_DEPTH), ('cells', c_i32), ('n_layers', c_i32),
+              ('hidden', c_i32), ('dtype', c_i32), ('activation', c_i32), ('stacked', c_i32),
+              ('chars', c_u8 * POST_MAX_DEPTH)]
+
+
 # Every symbol include/pcx.h declares: (name, restype, argtypes).
 _VP = ctypes.c_void_p
 SYMBOLS = [
@@ -193,6 +203,10 @@ SYMBOLS = [
     ('pcx_post_bind_output', c_i32, [_VP, _VP, c_u64]),
     ('pcx_post_error_buffer', c_i32, [_VP, ctypes.POINTER(_VP)]),
     ('pcx_post_error_poll', c_i32, [_VP, _VP, ctypes.POINTER(c_i32)]),
+    ('pcx_project_sizes', c_i32, [ctypes.POINTER(ProjectDesc), ctypes.POINTER(c_u64), ctypes.POINTER(c_u64), ctypes.POINTER(c_u64)]),
+    ('pcx_project_pack', c_i32, [ctypes.POINTER(ProjectDesc), _VP, _VP, _VP]),
+    ('pcx_project_forward', c_i32, [ctypes.POINTER(ProjectDesc), _VP, _VP, _VP, _VP, _VP, _VP, _VP, c_u64, _VP]),
+    ('pcx_project_backward', c_i32, [ctypes.POINTER(ProjectDesc), _VP, _VP, _VP, _VP, _VP, _VP, c_u64, _VP]),
     ('pcx_gather_create', c_i32, [ctypes.POINTER(_VP), c_i32, ctypes.POINTER(_VP)]),
     ('pcx_gather_destroy', None, [_VP]),
     ('pcx_gather_scalars', c_i32, [_VP, ctypes.POINTER(_VP)]),

@@ -96,3 +96,26 @@ def synchronize(device_id):
     torch.cuda.synchronize(device_id)
   else:
     N.check(N.lib().pcx_stream_synchronize(None))
+
+
+# ---- the policy operators (rendering.project, actions.sample, actions.log_prob) work on PyTorch tensors ----------------
+
+
+def require_torch(what):
+  torch = torch_module()
+  if torch is None:
+    raise RuntimeError('{} needs PyTorch-ROCm and a GPU'.format(what))
+  return torch
+
+
+def policy_dtype(tensor, name):
+  """The C ABI's number for a floating tensor's type."""
+  torch = torch_module()
+  kinds = {torch.float32: N.F32, torch.float16: N.F16, torch.bfloat16: N.BF16}
+  if tensor.dtype not in kinds:
+    raise TypeError('{} must be float32, float16 or bfloat16, not {}'.format(name, tensor.dtype))
+  return kinds[tensor.dtype]
+
+
+def pointer(tensor):
+  return None if tensor is None else tensor.data_ptr()

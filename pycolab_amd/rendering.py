@@ -626,3 +626,301 @@ class _RepaintedPlanes(object):
     for i, ch in enumerate(self._out_chars):
       view.chars[i] = ord(ch)
     return view, self._device_id
+
+
+# ---------------------------------------------------------------------- the first layer of a policy
+#
+# What a learner does with the stack ObservationToFeatureArray makes is, first of all, to multiply it by a weight.  The
+# operators below do that from the boards themselves (csrc/pcx_project.hip): the float32 stack -- 9.6 KB per scrolly_maze
+# board of 300 bytes -- is never written.  They need PyTorch-ROCm.
+
+_ACTIVATIONS = {None: N.ACT_NONE, 'relu': N.ACT_RELU, 'silu': N.ACT_SILU, 'tanh': N.ACT_TANH, 'gelu': N.ACT_GELU}
+
+
+def _occluded(source):
+  """Are this source's layers exactly `board == character`?"""
+  engine = getattr(source, '_engine', None) or source
+  return bool(getattr(engine, '_occlusion_in_layers', False))
+
+
+class _Boards(object):
+  """Where a projection's boards lie: an Observation of this package, a uint8 tensor [n, rows, cols] of characters, or a
+  uint8 / bool tensor [n, layers, rows, cols] of stacked layers."""
+
+  def __init__(self, boards, layers):
+    torch = dev.require_torch('a projection of observations')
+    self.single = False
+    self.offsets = None  # stacked layers: byte offsets within a board
+    if isinstance(boards, torch.Tensor):
+      self.keep, shape = boards, boards.shape
+      if not boards.is_cuda:
+        raise ValueError('boards must be a device tensor')
+      if boards.dim() == 4:
+        if boards.dtype not in (torch.uint8, torch.bool):
+          raise TypeError('stacked layers must be uint8 or bool, not {}'.format(boards.dtype))
+        if shape[1] != len(layers):
+          raise ValueError('{} stacked layers for the {} characters {}'.format(shape[1], len(layers), repr(layers)))
+        self.offsets = [k * boards.stride(1) for k in range(len(layers))]
+      elif boards.dim() == 3:
+        if boards.dtype != torch.uint8:
+          raise TypeError('boards must be uint8 characters, not {}'.format(boards.dtype))
+      else:
+        raise ValueError('boards must be [n, rows, cols] characters or [n, layers, rows, cols] stacked layers, not '
+                         '{}'.format(list(shape)))
+      self.n, self.rows, self.cols = int(shape[0]), int(shape[-2]), int(shape[-1])
+      if (self.cols > 1 and boards.stride(-1) != 1) or (self.rows > 1 and boards.stride(-2) != self.cols):
+        raise ValueError('the cells of a board must lie one after the other (rows * cols contiguous bytes)')
+      self.device_id, self.ptr, self.row_stride = boards.device.index, boards.data_ptr(), int(boards.stride(0))
+    else:
+      source = _source_of(boards)
+      view, self.device_id = source._planes_view()
+      present = bytes(view.chars)[:view.n_chars]
+      if not any(ord(c) < 256 and ord(c) in present for c in layers):
+        raise RuntimeError('The layers {} have no entry that refers to an actual feature in the input observation, whose '
+                           'features are {}.'.format(repr(layers), repr(present.decode('latin-1'))))
+      self.keep = boards
+      self.n, self.rows, self.cols = int(view.batch), view.rows, view.cols
+      self.ptr, self.row_stride = view.planes, (1 + view.n_chars) * view.pitch
+      self.single = self.n == 1
+      if not _occluded(source):
+        self.offsets = [(1 + present.index(ord(c))) * view.pitch if ord(c) in present else -1 for c in layers]
+
+
+class _Projection(object):
+  """The checked arguments of one projection: what the C ABI's description is made of."""
+
+  def __init__(self, layers, weight, bias, activation):
+    torch = dev.require_torch('a projection of observations')
+    if activation not in _ACTIVATIONS:
+      raise ValueError('activation must be one of {}, not {}'.format(list(_ACTIVATIONS), repr(activation)))
+    depth = len(layers)
+    if not 1 <= depth <= N.POST_MAX_DEPTH:
+      raise NotImplementedError('a projection takes 1 to {} layers, not {}'.format(N.POST_MAX_DEPTH, depth))
+    if any(ord(c) > 255 for c in layers) or len(set(layers)) != depth:
+      raise ValueError('layers must be distinct one-byte characters, not {}'.format(repr(layers)))
+    if not isinstance(weight, torch.Tensor) or not weight.is_cuda:
+      raise ValueError('weight must be a device tensor')
+    self.dtype = dev.policy_dtype(weight, 'weight')
+    if weight.dim() not in (2, 4) or weight.numel() == 0 or (weight.shape[1] != depth if weight.dim() == 4 else weight.shape[1] % depth):
+      raise ValueError('weight must be [hidden, {0}, rows, cols] or [hidden, {0} * rows * cols], not {1}'.format(depth, list(weight.shape)))
+    self.layers, self.hidden, self.device = layers, int(weight.shape[0]), weight.device
+    self.cells = int(weight.numel()) // (self.hidden * depth)
+    self.board = tuple(weight.shape[2:]) if weight.dim() == 4 else None
+    self.check_row(bias, 'bias', weight)
+    if bias is not None and tuple(bias.shape) != (self.hidden,):
+      raise ValueError('bias must be [{}], not {}'.format(self.hidden, list(bias.shape)))
+    self.torch_dtype = weight.dtype
+    d = self.desc = N.ProjectDesc()
+    d.cells, d.n_layers, d.hidden, d.dtype, d.activation = self.cells, depth, self.hidden, self.dtype, _ACTIVATIONS[activation]
+    for i, c in enumerate(layers):
+      d.chars[i] = ord(c)
+
+  def check_row(self, tensor, name, weight):
+    if tensor is not None and (tensor.dtype != weight.dtype or tensor.device != weight.device):
+      raise ValueError('{} must be {} on {}, like the weight'.format(name, weight.dtype, weight.device))
+
+  def check_rows(self, tensor, name, n):
+    if tensor is None:
+      return
+    if tensor.dtype != self.torch_dtype or tensor.device != self.device or tuple(tensor.shape) != (n, self.hidden):
+      raise ValueError('{} must be {} [{}, {}] on {}'.format(name, self.torch_dtype, n, self.hidden, self.device))
+
+  def at(self, boards):
+    """The description for these boards."""
+    if boards.device_id != self.device.index:
+      raise ValueError('the boards are on GPU {}, the weight is on GPU {}'.format(boards.device_id, self.device.index))
+    if boards.rows * boards.cols != self.cells or (self.board and self.board != (boards.rows, boards.cols)):
+      raise ValueError('the weight is for boards of {} cells, these are {} x {}'.format(
+          '{} x {}'.format(*self.board) if self.board else self.cells, boards.rows, boards.cols))
+    d = self.desc
+    d.n, d.row_stride, d.stacked = boards.n, boards.row_stride, int(boards.offsets is not None)
+    if boards.offsets is not None:
+      for i, o in enumerate(boards.offsets):
+        d.layer_offset[i] = o
+    return d
+
+  def sizes(self):
+    out = (N.c_u64(0), N.c_u64(0), N.c_u64(0))
+    N.check(N.lib().pcx_project_sizes(ctypes.byref(self.desc), *[ctypes.byref(x) for x in out]))
+    return [int(x.value) for x in out]
+
+  def pack(self, weight, packed=None):
+    torch = dev.torch_module()
+    if packed is None:
+      packed = torch.empty(self.sizes()[0], dtype=torch.uint8, device=self.device)
+    weight = weight.detach().contiguous()
+    N.check(N.lib().pcx_project_pack(ctypes.byref(self.desc), weight.data_ptr(), packed.data_ptr(), dev.current_stream(self.device.index)))
+    return packed
+
+  def forward(self, boards, packed, bias, residual, want_slope=False):
+    torch = dev.torch_module()
+    d = self.at(boards)
+    self.check_rows(residual, 'residual', boards.n)
+    out = torch.empty((boards.n, self.hidden), dtype=self.torch_dtype, device=self.device)
+    slope = torch.empty_like(out) if want_slope else None
+    scratch = self.sizes()[1]
+    ws = torch.empty(scratch, dtype=torch.uint8, device=self.device) if scratch else None
+    bias = None if bias is None else bias.detach().contiguous()
+    residual = None if residual is None else residual.detach().contiguous()
+    N.check(N.lib().pcx_project_forward(
+        ctypes.byref(d), boards.ptr, packed.data_ptr(), dev.pointer(bias), dev.pointer(residual), out.data_ptr(),
+        dev.pointer(slope), dev.pointer(ws), scratch, dev.current_stream(self.device.index)))
+    return out, slope
+
+  def backward(self, boards, grad, slope, want_weight, want_bias, weight_shape):
+    torch = dev.torch_module()
+    d = self.at(boards)
+    self.check_rows(grad, 'grad', boards.n)
+    self.check_rows(slope, 'slope', boards.n)
+    make = torch.zeros if boards.n == 0 else torch.empty
+    dw = make(weight_shape, dtype=self.torch_dtype, device=self.device) if want_weight else None
+    db = make((self.hidden,), dtype=self.torch_dtype, device=self.device) if want_bias else None
+    if boards.n and (want_weight or want_bias):
+      scratch = self.sizes()[2]
+      ws = torch.empty(scratch, dtype=torch.uint8, device=self.device)
+      grad = grad.contiguous()
+      slope = None if slope is None else slope.contiguous()
+      N.check(N.lib().pcx_project_backward(ctypes.byref(d), boards.ptr, grad.data_ptr(), dev.pointer(slope), dev.pointer(dw),
+                                           dev.pointer(db), ws.data_ptr(), scratch, dev.current_stream(self.device.index)))
+    return dw, db
+
+
+class ObservationProjection(object):
+  """`act(features @ weight.T + bias) + residual` of every board, with `features` the stack that
+  `ObservationToFeatureArray(layers)` would make of it -- for a policy that is only asked.
+
+  `weight`: float32, float16 or bfloat16 device tensor, [hidden, len(layers), rows, cols] or the same flattened to two
+  axes (a Linear layer's weight over the flattened stack); `bias`: [hidden] or None; `activation`: None, 'relu', 'silu',
+  'tanh' or 'gelu' (the exact one).  The weight is copied and laid out once, here and in `load()`: later changes of the
+  tensors do not show until `load()` is called.
+
+  Calling it takes an Observation of this package (engine, cropper or repainter; nothing is copied), a uint8 device
+  tensor [n, rows, cols] of board characters -- say, boards kept from a rollout -- or a uint8 / bool tensor
+  [n, len(layers), rows, cols] of stacked layers, and returns [n, hidden] of the weight's type (a batch-1 Observation:
+  [hidden]).  `residual`: [n, hidden] or None.  Boards whose layers are `board == character` (the default engine) are
+  read as characters; with `occlusion_in_layers=False` the layer planes are read.  Characters of a board that are not
+  among `layers` count nowhere.  Sums are float32.  Nothing waits for the device, so a call can be captured into a graph;
+  gradients are `project()`'s business."""
+
+  def __init__(self, layers, weight, bias=None, activation=None):
+    self._activation = activation
+    self._layers = layers
+    self._plan = _Projection(layers, weight, bias, activation)
+    self._weight = weight.detach().clone()
+    self._bias = None if bias is None else bias.detach().clone()
+    self._packs = {}
+    self._lay_out(0)
+
+  def _lay_out(self, stacked):
+    """The weight in the order the kernel for characters (0) or stacked layers (1) reads it; waits until it lies there,
+    so that calls on any stream may use it."""
+    torch = dev.torch_module()
+    if torch.cuda.is_current_stream_capturing():
+      raise RuntimeError('this ObservationProjection has not laid its weight out for stacked layers yet: call it once before '
+                         'capturing a graph')
+    with torch.cuda.device(self._plan.device):
+      self._plan.desc.stacked = stacked
+      self._packs[stacked] = self._plan.pack(self._weight, self._packs.get(stacked))
+      torch.cuda.current_stream().synchronize()
+
+  def load(self, weight, bias=None):
+    """New values for weight and bias (same shapes and types), in place: graphs that captured a call see them.  Waits for
+    the device, before and after."""
+    torch = dev.torch_module()
+    if torch.cuda.is_current_stream_capturing():
+      raise RuntimeError('load() cannot be captured into a graph')
+    if tuple(weight.shape) != tuple(self._weight.shape) or weight.dtype != self._weight.dtype or (bias is None) != (self._bias is None):
+      raise ValueError('load() takes a weight {} {} and {} bias'.format(self._weight.dtype, list(self._weight.shape),
+                                                                       'no' if self._bias is None else 'a'))
+    _Projection(self._layers, weight, bias, self._activation)  # (checks)
+    torch.cuda.synchronize(self._plan.device)  # nobody reads the old values any more
+    self._weight.copy_(weight.detach())
+    if bias is not None:
+      self._bias.copy_(bias.detach())
+    for stacked in list(self._packs):
+      self._lay_out(stacked)
+    torch.cuda.synchronize(self._plan.device)
+
+  def __call__(self, observation, residual=None):
+    torch = dev.torch_module()
+    boards = _Boards(observation, self._layers)
+    stacked = int(boards.offsets is not None)
+    if stacked not in self._packs:
+      self._lay_out(stacked)
+    with torch.cuda.device(self._plan.device):
+      out, _ = self._plan.forward(boards, self._packs[stacked], self._bias, residual)
+    return out[0] if boards.single else out
+
+
+_project_function = None
+
+
+def _project_autograd():
+  """The autograd function behind `project()` (made on first use: PyTorch is optional here)."""
+  global _project_function
+  if _project_function is None:
+    torch = dev.torch_module()
+
+    class ProjectBoards(torch.autograd.Function):
+
+      @staticmethod
+      def forward(ctx, weight, bias, residual, plan, boards):
+        out, slope = plan.forward(boards, plan.pack(weight), bias, residual, want_slope=plan.desc.activation != N.ACT_NONE)
+        ctx.plan, ctx.boards, ctx.weight_shape = plan, boards, weight.shape
+        # (the boards are an input like any other: a write to them before backward() is noticed where they are a tensor)
+        ctx.save_for_backward(slope, boards.keep if isinstance(boards.keep, torch.Tensor) else None)
+        return out
+
+      @staticmethod
+      @torch.autograd.function.once_differentiable
+      def backward(ctx, grad):
+        slope, _ = ctx.saved_tensors
+        want = ctx.needs_input_grad
+        with torch.cuda.device(ctx.plan.device):
+          dw, db = ctx.plan.backward(ctx.boards, grad, slope, want[0], want[1], ctx.weight_shape)
+        return dw, db, grad if want[2] else None, None, None
+
+    _project_function = ProjectBoards
+  return _project_function
+
+
+def _refuse_recording_in_capture(torch, what, instead, *leaves):
+  if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in leaves) and torch.cuda.is_current_stream_capturing():
+    raise RuntimeError('{0}() does not record gradients while a graph is captured: autograd may hand the captured backward '
+                       'pass to the stream of an earlier one, which ends the process.  Capture {1} instead.'.format(what, instead))
+
+
+def project(boards, layers, weight, bias=None, activation=None, residual=None, return_slope=False):
+  """`act(features @ weight.T + bias) + residual`, differentiable in `weight`, `bias` and `residual`: one training step's
+  first layer.  Arguments, shapes and types as for `ObservationProjection`, which is the form for weights that stay; this
+  one lays the weight out in every call.
+
+  An Observation is a view of the engine's planes, which the next step overwrites: for a backward pass after that, pass a
+  copy of the board (`observation.board.clone()`), a tensor.
+
+  `return_slope=True`: no autograd; returns (out, slope) with slope = act'(...) (None without an activation), what
+  `project_backward` takes -- the pair to capture into a graph."""
+  torch = dev.require_torch('project()')
+  plan = _Projection(layers, weight, bias, activation)
+  view = _Boards(boards, layers)
+  plan.at(view)
+  plan.check_rows(residual, 'residual', view.n)
+  with torch.cuda.device(plan.device):
+    if return_slope:
+      out, slope = plan.forward(view, plan.pack(weight), bias, residual, want_slope=activation is not None)
+      return (out[0] if view.single else out), slope
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (weight, bias, residual)):
+      _refuse_recording_in_capture(torch, 'project', 'project(..., return_slope=True) and project_backward()', weight, bias, residual)
+      out = _project_autograd().apply(weight, bias, residual, plan, view)
+    else:
+      out, _ = plan.forward(view, plan.pack(weight), bias, residual)
+  return out[0] if view.single else out
+
+
+def project_backward(boards, layers, weight, grad, slope=None):
+  """(grad_weight, grad_bias) of `project()` for the gradient `grad` [n, hidden] of its result; `slope` as it returned it.
+  The residual's gradient is `grad`.  Records nothing for autograd and waits for nothing: it may be captured."""
+  torch = dev.require_torch('project_backward()')
+  plan = _Projection(layers, weight, None, None if slope is None else 'relu')  # (which activation it was is in the slopes)
+  with torch.cuda.device(plan.device):
+    return plan.backward(_Boards(boards, layers), grad.detach(), slope, True, True, weight.shape)

@@ -1,0 +1,513 @@
+"""rendering.ObservationProjection / project / project_backward (csrc/pcx_project.hip): the product of a weight with the
+layers of boards, its epilogue and its gradients, against the same formulas in 64 bits.
+
+Tolerances.  A product with a set feature is exact and sums are float32: with S = sum |w| over the set features plus
+|bias|, a sum of m terms is off by at most (m + 2) 2^-23 S (2^-23: a matrix unit may cut off where it adds).  The
+activations are 1.13-Lipschitz (gelu's slope peaks at 1.129) and the device's exp / tanh / erf are good to a few units:
+8 * 2^-24 (|y| + 1) is allowed.  Storing the result rounds by eps / 2 of it.  In the gradients the activation's slope and
+dz are each rounded to the weight's type (eps |dz| together, nothing for float32 beyond its own eps), and the slope moves
+with the sum's error by at most 1.1 of it (silu, tanh and gelu have second derivatives below 1.1)."""
+
+import ctypes
+import math
+
+import numpy as np
+import pytest
+
+from pycolab_amd import _native as N
+from pycolab_amd import rendering
+
+torch = pytest.importorskip('torch')
+
+CHARS = ' #.@Pabcdefghijklmnopqrstuvwxyz01234'
+DTYPES = ['float32', 'float16', 'bfloat16']
+ACTS = [None, 'relu', 'silu', 'tanh', 'gelu']
+
+
+def make(n, layers, rows, cols, hidden, dtype, seed, stacked=False, grid=False):
+  """Boards (one character of them is not stacked), weight, bias and residual on the CPU.  grid: numbers whose sums are
+  exact in float32, so that no sum lies between zero and its rounding (relu's slope is then the same in any precision)."""
+  g = torch.Generator().manual_seed(seed)
+  dt = getattr(torch, dtype)
+  chars = CHARS[:layers]
+  if stacked:
+    boards = (torch.rand(n, layers, rows, cols, generator=g) < 0.3).to(torch.uint8) * torch.randint(1, 256, (n, layers, rows, cols), generator=g).to(torch.uint8)
+  else:
+    table = torch.tensor([ord(c) for c in chars + '~'], dtype=torch.uint8)
+    boards = table[torch.randint(0, layers + 1, (n, rows, cols), generator=g)]
+  if grid:
+    weight = torch.randint(-8, 9, (hidden, layers, rows, cols), generator=g).float() / 16
+    bias = torch.randint(-8, 9, (hidden,), generator=g).float() / 16
+  else:
+    weight = torch.randn(hidden, layers, rows, cols, generator=g) / math.sqrt(rows * cols)
+    bias = torch.randn(hidden, generator=g)
+  residual = torch.randn(n, hidden, generator=g)
+  return chars, boards, weight.to(dt), bias.to(dt), residual.to(dt)
+
+
+def features(chars, boards):
+  if boards.dim() == 4:
+    return (boards != 0).double().flatten(1)
+  return torch.stack([(boards == ord(c)).double() for c in chars], 1).flatten(1)
+
+
+def act64(kind, z):
+  if kind == 'relu':
+    return z.clamp(min=0), (z > 0).double()
+  if kind == 'tanh':
+    return torch.tanh(z), 1 - torch.tanh(z) ** 2
+  if kind == 'silu':
+    s = torch.sigmoid(z)
+    return z * s, s * (1 + z * (1 - s))
+  if kind == 'gelu':
+    c = 0.5 * (1 + torch.erf(z / math.sqrt(2)))
+    return z * c, c + z * torch.exp(-z * z / 2) / math.sqrt(2 * math.pi)
+  return z, torch.ones_like(z)
+
+
+def reference(chars, boards, weight, bias, act, residual):
+  """(y, bound on what may differ from it, slope, bound on the slope)"""
+  x, w = features(chars, boards), weight.double().flatten(1)
+  b = torch.zeros(w.shape[0], dtype=torch.float64) if bias is None else bias.double()
+  z = x @ w.t() + b
+  size = x @ w.abs().t() + b.abs()
+  off = (x.sum(1, keepdim=True) + 2) * 2.0 ** -23 * size
+  y, slope = act64(act, z)
+  tol = 1.13 * off + 8 * 2.0 ** -24 * (y.abs() + 1)
+  if residual is not None:
+    y = y + residual.double()
+    tol = tol + 2.0 ** -24 * y.abs()
+  half = torch.finfo(weight.dtype).eps / 2
+  tiny = torch.finfo(weight.dtype).tiny * half
+  return y, tol + half * (y.abs() + tol) + tiny, slope, (1.1 * off if act not in (None, 'relu') else 0 * off) + 8 * 2.0 ** -24
+
+
+def near(got, want, tol, what):
+  got = got.detach().double().cpu()
+  assert got.shape == want.shape, (what, got.shape, want.shape)
+  bad = ~((got - want).abs() <= tol)
+  assert not bad.any(), '{}: {} of {} off, worst {:.3g} where {:.3g} is allowed'.format(
+      what, int(bad.sum()), bad.numel(), float((got - want).abs().max()), float(tol.flatten()[(got - want).abs().flatten().argmax()]))
+
+
+def check(n, layers, rows, cols, hidden, dtype, act, seed, stacked=False, with_bias=True, with_residual=True, train=False):
+  chars, boards, weight, bias, residual = make(n, layers, rows, cols, hidden, dtype, seed, stacked, grid=act == 'relu')
+  bias, residual = bias if with_bias else None, residual if with_residual else None
+  y, tol, slope, slope_tol = reference(chars, boards, weight, bias, act, residual)
+  dev = [None if t is None else t.cuda() for t in (boards, weight, bias, residual)]
+  got = rendering.ObservationProjection(chars, dev[1], dev[2], activation=act)(dev[0], residual=dev[3])
+  assert got.dtype == weight.dtype
+  near(got, y, tol, 'forward')
+  if not train:
+    return
+  leaves = [t for t in dev[1:] if t is not None]
+  for t in leaves:
+    t.requires_grad_()
+  out = rendering.project(dev[0], chars, dev[1], dev[2], activation=act, residual=dev[3])
+  near(out, y, tol, 'forward of a training step')
+  grad = torch.randn(n, hidden, generator=torch.Generator().manual_seed(seed + 1)).to(weight.dtype)
+  grads = list(torch.autograd.grad(out, leaves, grad.cuda()))
+  check_grads(chars, boards, weight, grad, slope, slope_tol, grads[0], grads[1] if with_bias else None)
+  if with_residual:
+    assert torch.equal(grads[-1].cpu(), grad)
+
+
+def check_grads(chars, boards, weight, grad, slope, slope_tol, dw, db):
+  x, eps = features(chars, boards), torch.finfo(weight.dtype).eps
+  dz = grad.double() * slope
+  off = grad.double().abs() * slope_tol + eps * (dz.abs() + grad.double().abs() * slope_tol) + torch.finfo(weight.dtype).tiny * eps
+  n = x.shape[0]
+  for got, left, what in ((dw, x, 'grad weight'), (db, torch.ones(n, 1, dtype=torch.float64), 'grad bias')):
+    if got is None:
+      continue
+    want = (dz.t() @ left)
+    tol = off.t() @ left + (n + 2) * 2.0 ** -23 * (dz.abs().t() @ left)
+    tol = tol + eps / 2 * (want.abs() + tol) + torch.finfo(weight.dtype).tiny * eps
+    near(got.flatten(1) if what == 'grad weight' else got[:, None], want, tol, what)
+
+
+# ---------------------------------------------------------------- without a GPU
+
+
+def desc(**kw):
+  d = N.ProjectDesc()
+  d.n, d.row_stride, d.cells, d.n_layers, d.hidden, d.dtype = 4, 300, 300, 3, 64, N.BF16
+  for i, c in enumerate('P#@'):
+    d.chars[i] = ord(c)
+  for k, v in kw.items():
+    setattr(d, k, v)
+  return d
+
+
+def sizes(d):
+  out = [N.c_u64(77) for _ in range(3)]
+  rc = N.lib().pcx_project_sizes(ctypes.byref(d), *[ctypes.byref(x) for x in out])
+  return rc, [int(x.value) for x in out]
+
+
+def test_description_layout():
+  # n, row_stride, 32 offsets: 34 x 8; six int32; 32 characters
+  assert ctypes.sizeof(N.ProjectDesc) == 34 * 8 + 6 * 4 + 32
+  assert N.ProjectDesc.chars.offset == 34 * 8 + 24
+
+
+def test_sizes():
+  rc, (packed, forward, backward) = sizes(desc())
+  assert rc == 0
+  assert packed == 10 * 4 * 1 * 2 * 2048  # quads of 32 cells x octets x groups of 4 layers x tiles of 32 units x 2 KB
+  assert forward > 0 and backward > 0
+  assert sizes(desc(dtype=N.F32))[1][0] == 3 * packed
+  assert sizes(desc(n=0))[1] == [packed, 0, 0]
+
+
+@pytest.mark.parametrize('kw,text', [
+    (dict(dtype=N.I32), 'float32, float16 or bfloat16'), (dict(activation=5), 'activation'), (dict(activation=-1), 'activation'),
+    (dict(cells=0), 'range'), (dict(n_layers=0), 'range'), (dict(n_layers=33), 'range'), (dict(hidden=0), 'range'),
+    (dict(hidden=1 << 17), 'range'), (dict(n=-1), 'boards'), (dict(n=(1 << 31) + 1), 'boards'), (dict(row_stride=-1), 'stride'),
+    (dict(cells=1 << 20, hidden=1 << 16), 'too large')])
+def test_refused_descriptions(kw, text):
+  rc, _ = sizes(desc(**kw))
+  assert rc == N.E_INVALID and text in N.lib().pcx_last_error().decode()
+
+
+def test_a_layer_twice_is_refused():
+  d = desc()
+  d.chars[2] = ord('P')
+  rc, _ = sizes(d)
+  assert rc == N.E_INVALID and 'twice' in N.lib().pcx_last_error().decode()
+  d.stacked = 1  # (stacked layers have no characters)
+  assert sizes(d)[0] == 0
+
+
+def test_null_and_misaligned_pointers_are_refused_before_any_launch():
+  lib, d, at = N.lib(), desc(), 1 << 20
+  assert lib.pcx_project_sizes(None, None, None, None) == N.E_INVALID
+  assert lib.pcx_project_pack(ctypes.byref(d), None, at, None) == N.E_INVALID
+  assert lib.pcx_project_pack(ctypes.byref(d), at, at + 8, None) == N.E_INVALID
+  big = 1 << 40
+  assert lib.pcx_project_forward(ctypes.byref(d), None, at, None, None, at, None, at, big, None) == N.E_INVALID
+  assert lib.pcx_project_forward(ctypes.byref(d), at, at, None, None, None, None, at, big, None) == N.E_INVALID
+  assert lib.pcx_project_forward(ctypes.byref(d), at, at, at + 1, None, at, None, at, big, None) == N.E_INVALID
+  assert lib.pcx_project_forward(ctypes.byref(d), at, at, None, None, at, None, at, 16, None) == N.E_INVALID  # too small a workspace
+  assert lib.pcx_project_backward(ctypes.byref(d), at, None, None, at, at, at, big, None) == N.E_INVALID
+  assert lib.pcx_project_backward(ctypes.byref(d), at, at, None, at, at, None, 0, None) == N.E_INVALID
+  assert lib.pcx_project_backward(ctypes.byref(desc(activation=N.ACT_RELU)), at, at, None, at, at, at, big, None) == N.E_INVALID  # slopes
+  assert lib.pcx_project_backward(ctypes.byref(desc(n=0)), at, at, None, at, at, at, big, None) == N.E_INVALID
+
+
+def test_needs_a_gpu():
+  if torch.cuda.is_available():
+    pytest.skip('there is one')
+  with pytest.raises(RuntimeError, match='PyTorch-ROCm'):
+    rendering.ObservationProjection('P', torch.zeros(4, 1, 2, 2))
+  with pytest.raises(RuntimeError, match='PyTorch-ROCm'):
+    rendering.project(torch.zeros(1, 2, 2, dtype=torch.uint8), 'P', torch.zeros(4, 1, 2, 2))
+
+
+# ---------------------------------------------------------------- on the GPU
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('dtype', DTYPES)
+@pytest.mark.parametrize('stacked', [False, True])
+def test_one_board(dtype, stacked):
+  check(1, 8, 10, 30, 256, dtype, 'relu', 1, stacked=stacked, train=True)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('act', ACTS)
+@pytest.mark.parametrize('dtype', DTYPES)
+def test_types_and_activations(dtype, act):
+  check(70, 5, 6, 12, 40, dtype, act, 2, train=True)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('stacked', [False, True])
+@pytest.mark.parametrize('layers', [1, 2, 3, 4, 5, 7, 8, 9, 15, 16, 17, 32])
+def test_layers(layers, stacked):
+  check(130, layers, 5, 7, 33, 'bfloat16', 'tanh', 3, stacked=stacked, train=True)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('rows,cols', [(1, 1), (1, 3), (2, 2), (3, 5), (4, 4), (1, 31), (4, 8), (3, 11), (9, 7), (8, 8), (45, 89)])
+def test_cells(rows, cols):
+  for stacked in (False, True):
+    check(37, 6, rows, cols, 24, 'float16', 'silu', 4, stacked=stacked, train=True)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('hidden', [1, 2, 31, 32, 33, 64, 65, 96, 128, 130, 200, 257, 512])
+def test_hidden(hidden):
+  for n in (3, 600):  # (both launch shapes)
+    check(n, 4, 5, 8, hidden, 'bfloat16', 'gelu', 5, train=True)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('n', [0, 1, 2, 31, 32, 33, 63, 64, 65, 127, 128, 129, 511, 512, 513, 1025, 5000])
+def test_boards(n):
+  check(n, 5, 6, 12, 72, 'float32', 'relu', 6, train=True)
+
+
+@pytest.mark.gpu
+def test_no_bias_no_residual():
+  check(50, 3, 4, 9, 36, 'float16', None, 7, with_bias=False, with_residual=False, train=True)
+  check(50, 3, 4, 9, 36, 'float32', 'silu', 8, with_bias=True, with_residual=False, train=True)
+
+
+@pytest.mark.gpu
+def test_many_boards():
+  check(40000, 8, 10, 30, 96, 'bfloat16', 'relu', 9, train=True)
+
+
+@pytest.mark.gpu
+def test_float32_weights_keep_all_their_bits():
+  g = torch.Generator().manual_seed(10)
+  weight = torch.randn(64, 2, 1, 1, generator=g) * torch.exp2(torch.randint(-100, 100, (64, 2, 1, 1), generator=g).float())
+  boards = torch.tensor([ord('a'), ord('b'), ord('c')], dtype=torch.uint8).reshape(3, 1, 1)
+  y = rendering.project(boards.cuda(), 'ab', weight.cuda()).cpu()
+  assert torch.equal(y[0], weight[:, 0, 0, 0]) and torch.equal(y[1], weight[:, 1, 0, 0]) and not y[2].any()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('dtype', DTYPES)
+def test_largest_smallest_and_no_numbers(dtype):
+  """One feature a board: the weight itself comes back, whatever it is; what is not finite stays where it is set."""
+  dt, info = getattr(torch, dtype), torch.finfo(getattr(torch, dtype))
+  values = torch.tensor([info.max, -info.max, info.tiny, info.smallest_normal * info.eps, 0.0, 1.0], dtype=dt)
+  y = rendering.project(torch.full((1, 1, 1), ord('a'), dtype=torch.uint8).cuda(), 'a', values.reshape(6, 1, 1, 1).cuda()).cpu()[0]
+  assert torch.equal(y[:3], values[:3]) and torch.equal(y[4:], values[4:])
+  assert abs(float(y[3]) - float(values[3])) <= float(values[3])  # the smallest subnormal: itself, or flushed to zero
+  w = torch.tensor([math.inf, -math.inf, math.nan, 2.0], dtype=dt).reshape(4, 1, 1, 1)
+  y = rendering.project(torch.full((1, 1, 1), ord('a'), dtype=torch.uint8).cuda(), 'a', w.cuda()).cpu()[0]
+  assert y[0] == math.inf and y[1] == -math.inf and torch.isnan(y[2]) and y[3] == 2
+
+
+@pytest.mark.gpu
+def test_strided_boards_and_planes():
+  chars, boards, weight, bias, _ = make(40, 6, 5, 9, 48, 'float32', 11)
+  y, tol, _, _ = reference(chars, boards, weight, bias, 'relu', None)
+  proj = rendering.ObservationProjection(chars, weight.cuda(), bias.cuda(), activation='relu')
+  wide = torch.zeros(40, 3, 53, dtype=torch.uint8).cuda()  # boards inside larger rows, starting at odd addresses
+  for shift in (0, 1, 2, 3, 5):
+    wide.zero_()
+    inside = wide[:, 1, shift:shift + 45].unflatten(1, (5, 9))
+    inside.copy_(boards.cuda())
+    near(proj(inside), y, tol, 'shift {}'.format(shift))
+  near(proj(boards.cuda().flip(0)), y.flip(0), tol.flip(0), 'flipped')
+  first = boards[:1].cuda().expand(7, 5, 9)  # one board seven times
+  near(proj(first), y[:1].expand(7, -1), tol[:1].expand(7, -1), 'expanded')
+
+
+@pytest.mark.gpu
+def test_last_board_of_an_allocation():
+  """The bytes behind the last board are not read: a board at the very end of its allocation, at every cell count."""
+  for cells in range(1, 40):
+    pool = torch.full((4096,), ord('#'), dtype=torch.uint8).cuda()
+    board = pool[4096 - cells:].reshape(1, 1, cells)
+    w = torch.randn(8, 1, 1, cells)
+    near(rendering.project(board, '#', w.cuda()), w.double().flatten(1).sum(1)[None], (cells + 4) * 2.0 ** -23 * w.double().abs().flatten(1).sum(1)[None], cells)
+
+
+@pytest.mark.gpu
+def test_refusals():
+  w, b = torch.zeros(16, 3, 4, 5).cuda(), torch.zeros(2, 4, 5, dtype=torch.uint8).cuda()
+  ok = rendering.ObservationProjection('P#@', w)
+  ok(b)
+  for bad in (b.cpu(), b[0], b.reshape(2, 20), b.reshape(1, 2, 4, 5), b.transpose(1, 2)[:, :, :], torch.zeros(2, 4, 6, dtype=torch.uint8).cuda(),
+              torch.zeros(2, 5, 4, dtype=torch.uint8).cuda(), torch.zeros(2, 4, 10, dtype=torch.uint8).cuda()[:, :, ::2]):
+    with pytest.raises(ValueError):
+      ok(bad)
+  with pytest.raises(TypeError):
+    ok(b.float())
+  with pytest.raises(TypeError):
+    ok(b.bool())  # (one layer's bools are no characters)
+  with pytest.raises(TypeError):
+    ok('a board')
+  for residual in (torch.zeros(2, 15).cuda(), torch.zeros(3, 16).cuda(), torch.zeros(2, 16).half().cuda(), torch.zeros(2, 16)):
+    with pytest.raises(ValueError):
+      ok(b, residual=residual)
+  for kw in (dict(layers='P#'), dict(layers='P##'), dict(layers='P#一'), dict(activation='swish'), dict(weight=w.cpu()), dict(weight=w[:0]),
+             dict(weight=w.reshape(16, 3, 20)), dict(bias=torch.zeros(15).cuda()), dict(bias=torch.zeros(16).half().cuda())):
+    args = dict(dict(layers='P#@', weight=w), **kw)
+    with pytest.raises(ValueError):
+      rendering.ObservationProjection(**args)
+    with pytest.raises(ValueError):
+      rendering.project(b, **args)
+  with pytest.raises(TypeError):
+    rendering.project(b, 'P#@', w.double())
+  with pytest.raises(NotImplementedError):
+    rendering.project(b, '', w)
+  with pytest.raises(ValueError):
+    ok.load(w.half())
+  with pytest.raises(ValueError):
+    ok.load(w, torch.zeros(16).cuda())
+
+
+@pytest.mark.gpu
+def test_flat_weight_load_and_same_numbers():
+  chars, boards, weight, bias, residual = make(300, 7, 10, 30, 160, 'bfloat16', 12)
+  b, w, c, r = boards.cuda(), weight.cuda(), bias.cuda(), residual.cuda()
+  proj = rendering.ObservationProjection(chars, w, c, activation='silu')
+  first = proj(b, residual=r)
+  assert torch.equal(first, rendering.ObservationProjection(chars, w.flatten(1), c, activation='silu')(b, residual=r))
+  assert torch.equal(first, rendering.project(b, chars, w, c, activation='silu', residual=r))
+  assert torch.equal(first, rendering.project(b, chars, w, c, activation='silu', residual=r))  # sums in a fixed order
+  proj.load(w * 2, c)
+  assert torch.equal(proj(b, residual=r), rendering.project(b, chars, w * 2, c, activation='silu', residual=r))
+  stacked = torch.stack([(b == ord(ch)) for ch in chars], 1)  # bool layers of the same boards
+  y, tol, _, _ = reference(chars, boards, weight * 2, bias, 'silu', residual)
+  near(proj(stacked, residual=r), y, tol, 'bool layers')
+  proj.load(w, c)
+  y, tol, _, _ = reference(chars, boards, weight, bias, 'silu', residual)
+  near(proj(stacked, residual=r), y, tol, 'bool layers after load()')
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('name,stacked', [('scrolly_maze_L0', False), ('marauders_unoccluded', True), ('warehouse_L0', False)])
+def test_observations_of_an_engine(name, stacked):
+  import os
+  from pycolab_amd.compiler import GameTemplate
+  from pycolab_amd.engine import Engine
+  path = os.path.join(os.path.dirname(__file__), 'golden', 'templates', name + '.npz')
+  for batch in (1, 96):
+    eng = Engine.from_template(GameTemplate.load(path), batch=batch, auto_reset=True)
+    obs, _, _ = eng.its_showtime()
+    layers = 'P' + ''.join(sorted(obs.layers)[:3]).replace('P', '') + '\x7f'  # the last one does not exist in the game
+    g = torch.Generator().manual_seed(13)
+    weight = torch.randn(48, len(layers), eng.rows, eng.cols, generator=g)
+    proj = rendering.ObservationProjection(layers, weight.cuda())
+    for step in range(3):
+      obs = eng.play(torch.full((batch,), step % 2, dtype=torch.int32).cuda() if batch > 1 else step % 2)[0]
+      cells = [torch.as_tensor(np.asarray(obs.layers[c].cpu() if batch > 1 else obs.layers[c])) for c in layers if c in obs.layers]
+      cells = torch.stack([x.reshape(batch, eng.rows, eng.cols) for x in cells] + [torch.zeros(batch, eng.rows, eng.cols)] * (len(layers) - len(cells)), 1)
+      y, tol, _, _ = reference(layers, (cells != 0).to(torch.uint8), weight, None, None, None)
+      got = proj(obs)
+      assert got.shape == ((48,) if batch == 1 else (batch, 48))
+      near(got.reshape(batch, 48), y, tol, '{} step {}'.format(name, step))
+      assert torch.equal(got.reshape(batch, 48), rendering.project(obs, layers, weight.cuda()).reshape(batch, 48))
+    with pytest.raises(RuntimeError, match='actual feature'):
+      rendering.project(obs, '\x7f', weight[:, :1].contiguous().cuda())
+    eng.close()
+
+
+@pytest.mark.gpu
+def test_cropped_and_repainted_observations():
+  import os
+  from pycolab_amd import cropping
+  from pycolab_amd.compiler import GameTemplate
+  from pycolab_amd.engine import Engine
+  path = os.path.join(os.path.dirname(__file__), 'golden', 'templates', 'better_scrolly_maze_L0.npz')
+  eng = Engine.from_template(GameTemplate.load(path), batch=33, auto_reset=True)
+  obs, _, _ = eng.its_showtime()
+  cropper = cropping.ScrollingCropper(rows=10, cols=30, to_track=['P'], scroll_margins=(2, 3))
+  cropper.set_engine(eng)
+  window = cropper.crop(obs)
+  weight = torch.randn(64, 4, 10, 30, generator=torch.Generator().manual_seed(14))
+  want = rendering.ObservationToFeatureArray('P#@a')(window).cpu()
+  y, tol, _, _ = reference('P#@a', (want != 0).to(torch.uint8), weight, None, 'tanh', None)
+  near(rendering.ObservationProjection('P#@a', weight.cuda(), activation='tanh')(window), y, tol, 'window')
+  repainter = rendering.ObservationCharacterRepainter({'a': '@', 'b': '@', 'c': '@'})
+  full = repainter(obs)
+  weight = torch.randn(40, 2, 45, 89, generator=torch.Generator().manual_seed(15))
+  want = rendering.ObservationToFeatureArray('P@')(full).cpu()
+  y, tol, _, _ = reference('P@', (want != 0).to(torch.uint8), weight, None, None, None)
+  near(rendering.project(full, 'P@', weight.cuda()), y, tol, 'repainted')
+  eng.close()
+
+
+@pytest.mark.gpu
+def test_gradient_against_differences():
+  """d/dt f(w + t v) at 0 against (f(w + h v) - f(w - h v)) / 2h in float64 of the formula, and of the kernels' own forward
+  pass: with |v| such that z moves by at most 1 per unit of t, h = 2^-5 leaves h^2 / 6 |f'''| <= 2^-12 |g| sums."""
+  chars, boards, weight, bias, _ = make(64, 4, 3, 5, 24, 'float32', 16)
+  v = torch.randn(weight.shape, generator=torch.Generator().manual_seed(17)) / 15
+  grad = torch.randn(64, 24, generator=torch.Generator().manual_seed(18))
+  w = weight.cuda().requires_grad_()
+  out = rendering.project(boards.cuda(), chars, w, bias.cuda(), activation='silu')
+  dw, = torch.autograd.grad(out, [w], grad.cuda())
+  slope = float((dw.cpu().double() * v.double()).sum())
+  h = 2.0 ** -5
+
+  def own(t):
+    return rendering.project(boards.cuda(), chars, (weight + t * v).cuda(), bias.cuda(), activation='silu').cpu().double()
+
+  x = features(chars, boards)
+  dz = (x @ v.double().flatten(1).t()).abs()
+  bound = h * h / 6 * 1.0 * float((grad.double().abs() * dz ** 3).sum()) + 1e-5 * float(grad.abs().sum())
+  for f in (own, lambda t: act64('silu', x @ (weight.double() + t * v.double()).flatten(1).t() + bias.double())[0]):
+    difference = float((grad.double() * (f(h) - f(-h))).sum()) / (2 * h)
+    assert abs(difference - slope) <= bound, (difference, slope, bound)
+  assert bound < 0.05 * float((grad.double().abs() * dz).sum())  # (the bound says something)
+
+
+@pytest.mark.gpu
+def test_only_what_is_asked_for():
+  chars, boards, weight, bias, residual = make(20, 3, 4, 4, 16, 'float32', 19)
+  b = boards.cuda()
+  for which in ((0,), (1,), (2,), (0, 2)):
+    t = [weight.cuda(), bias.cuda(), residual.cuda()]
+    for i in which:
+      t[i].requires_grad_()
+    out = rendering.project(b, chars, t[0], t[1], activation='tanh', residual=t[2])
+    out.sum().backward()
+    assert [x.grad is not None for x in t] == [i in which for i in range(3)]
+  with torch.no_grad():
+    assert not rendering.project(b, chars, t[0], t[1]).requires_grad
+  shared = weight.cuda().requires_grad_()  # the same weight twice: its gradients add up
+  g1, = torch.autograd.grad(rendering.project(b, chars, shared).sum(), shared)
+  g2, = torch.autograd.grad(rendering.project(b, chars, shared).sum() + rendering.project(b, chars, shared).sum(), shared)
+  assert torch.equal(g2, 2 * g1)
+  half = torch.randn(20, 16).cuda()
+  out = rendering.project(b, chars, shared)
+  assert torch.equal(torch.autograd.grad(out, shared, half[:, :1].expand(20, 16), retain_graph=True)[0],
+                     torch.autograd.grad(out, shared, half[:, :1].expand(20, 16).contiguous())[0])  # a broadcast gradient
+  out = rendering.project(b, chars, shared)
+  b.zero_()
+  with pytest.raises(RuntimeError, match='modified by an inplace operation'):
+    out.sum().backward()
+
+
+@pytest.mark.gpu
+def test_other_streams_and_graphs():
+  chars, boards, weight, bias, residual = make(700, 8, 10, 30, 96, 'bfloat16', 20)
+  b, w, c, r = boards.cuda(), weight.cuda(), bias.cuda(), residual.cuda()
+  proj = rendering.ObservationProjection(chars, w, c, activation='relu')
+  want = proj(b, residual=r)
+  grad = torch.randn(700, 96).to(torch.bfloat16).cuda()
+  y, slope = rendering.project(b, chars, w, c, activation='relu', residual=r, return_slope=True)
+  dw, db = rendering.project_backward(b, chars, w, grad, slope)
+  side = torch.cuda.Stream()
+  side.wait_stream(torch.cuda.current_stream())
+  with torch.cuda.stream(side):
+    other = proj(b, residual=r)
+  torch.cuda.current_stream().wait_stream(side)
+  assert torch.equal(other, want)
+  ones = torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()
+  torch.cuda.synchronize()
+  with torch.cuda.graph(ones[0]):
+    first = proj(b, residual=r)
+  with torch.cuda.graph(ones[1]):
+    second, sl = rendering.project(b, chars, w, c, activation='relu', residual=r, return_slope=True)
+    gw, gb = rendering.project_backward(b, chars, w, grad, sl)
+  for i in range(4):
+    b.copy_(boards.cuda().roll(i, 0))
+    expect = proj(b, residual=r)
+    ones[0].replay()
+    ones[1].replay()
+    torch.cuda.synchronize()
+    assert torch.equal(first, expect) and torch.equal(second, expect)
+    _, s2 = rendering.project(b, chars, w, c, activation='relu', residual=r, return_slope=True)
+    e2 = rendering.project_backward(b, chars, w, grad, s2)
+    assert torch.equal(gw, e2[0]) and torch.equal(gb, e2[1])
+  b.copy_(boards)
+  proj.load(w * 2, c)
+  ones[0].replay()
+  assert torch.equal(first, proj(b, residual=r))
+  leaf = w.clone().requires_grad_()
+  torch.cuda.synchronize()
+  graph = torch.cuda.CUDAGraph()
+  with pytest.raises(RuntimeError, match='project_backward'):
+    with torch.cuda.graph(graph):
+      rendering.project(b, chars, leaf, c)
+  torch.cuda.synchronize()
+  assert torch.equal(rendering.project_backward(boards.cuda(), chars, w, grad, slope)[0], dw) and db.shape == (96,)
