@@ -655,6 +655,50 @@ int pcx_project_forward(const pcx_project_desc* d, const uint8_t* boards, const 
 int pcx_project_backward(const pcx_project_desc* d, const uint8_t* boards, const void* grad_out, const void* slope,
                          void* grad_weight, void* grad_bias, void* workspace, uint64_t workspace_bytes, void* stream);
 
+/* Logits over the actions, one row per environment: `dtype` (PCX_F32, PCX_F16, PCX_BF16) at row * row_stride elements,
+ * the actions of a row contiguous.  Wherever `legal` is taken: NULL, or uint8 at row * legal_stride bytes, zero where the
+ * action may not be taken.  An action is allowed where it is legal and its logit is neither -infinity nor a NaN. */
+typedef struct pcx_logits_desc {
+  int64_t n;            /* rows                                              */
+  int64_t row_stride;   /* elements                                          */
+  int64_t legal_stride; /* bytes                                             */
+  int32_t actions;      /* 1 .. 2^24                                         */
+  int32_t dtype;
+} pcx_logits_desc;
+
+/* How actions are drawn; a *_row pointer, where not NULL, is a device array [n] that replaces the number of its name row
+ * by row.  temperature: logits are divided by it; 0 (or less, or a NaN, in temperature_row): the best action.  top_k: how
+ * many of the best actions stay, 0 (or less): all.  top_p: of those, an action stays while the better ones weigh less than
+ * this part of the total; 1 or more: all.  min_p: of those, an action stays if it is at least this part as probable as the
+ * best one.  Better is the higher logit, then the lower index; the best action always stays. */
+typedef struct pcx_sampling {
+  float temperature, top_p, min_p;
+  int32_t top_k;
+  const float* temperature_row;
+  const int32_t* top_k_row;
+  const float* top_p_row;
+  const float* min_p_row;
+} pcx_sampling;
+
+/* actions_out[row] = the first action, by index, at which the running sum of the kept actions' weights exceeds
+ * uniforms[row] (in [0, 1)) of their total; PCX_ACTION_NONE where no action is allowed.  64-bit weights; the result
+ * depends on the row alone.  The workspace (pcx_sample_size: 0 up to 16,384 actions) serves one call at a time. */
+int pcx_sample_size(const pcx_logits_desc* d, uint64_t* bytes);
+int pcx_sample_actions(const pcx_logits_desc* d, const pcx_sampling* rules, const void* logits, const uint8_t* legal,
+                       const float* uniforms, int32_t* actions_out, void* workspace, uint64_t workspace_bytes, void* stream);
+
+/* log_prob[row] of actions[row] under softmax(logits / temperature) over the allowed actions, and the entropy of that
+ * distribution; stats [n][2] for the backward pass.  An action of PCX_ACTION_NONE, or a row that allows nothing, has
+ * log_prob 0 (and the row's entropy); an action that is not allowed -infinity; one that does not exist a NaN. */
+int pcx_log_prob_size(const pcx_logits_desc* d, uint64_t* bytes);
+int pcx_log_prob(const pcx_logits_desc* d, float temperature, const void* logits, const uint8_t* legal, const int32_t* actions,
+                 float* log_prob, float* entropy, float* stats, void* workspace, uint64_t workspace_bytes, void* stream);
+/* grad_logits [n][actions] (contiguous, the logits' type; 0 where not allowed) from the gradients of log_prob and entropy
+ * [n] (NULL: zero), with `entropy` and `stats` as pcx_log_prob left them. */
+int pcx_log_prob_backward(const pcx_logits_desc* d, float temperature, const void* logits, const uint8_t* legal, const int32_t* actions,
+                          const float* entropy, const float* stats, const float* grad_log_prob, const float* grad_entropy,
+                          void* grad_logits, void* stream);
+
 /* ------------------------------------------------------------------------ */
 /* Node-level gather of the step results: environments never
  * interact (one Engine per environment, pycolab/engine.py:102-104), so a batch

@@ -139,6 +139,16 @@ class ProjectDesc(ctypes.Structure):
               ('chars', c_u8 * POST_MAX_DEPTH)]
 
 
+class LogitsDesc(ctypes.Structure):
+  _fields_ = [('n', c_i64), ('row_stride', c_i64), ('legal_stride', c_i64), ('actions', c_i32), ('dtype', c_i32)]
+
+
+class Sampling(ctypes.Structure):
+  _fields_ = [('temperature', ctypes.c_float), ('top_p', ctypes.c_float), ('min_p', ctypes.c_float), ('top_k', c_i32),
+              ('temperature_row', ctypes.c_void_p), ('top_k_row', ctypes.c_void_p), ('top_p_row', ctypes.c_void_p),
+              ('min_p_row', ctypes.c_void_p)]
+
+
 # Every symbol include/pcx.h declares: (name, restype, argtypes).
 _VP = ctypes.c_void_p
 SYMBOLS = [
@@ -207,6 +217,11 @@ SYMBOLS = [
     ('pcx_project_pack', c_i32, [ctypes.POINTER(ProjectDesc), _VP, _VP, _VP]),
     ('pcx_project_forward', c_i32, [ctypes.POINTER(ProjectDesc), _VP, _VP, _VP, _VP, _VP, _VP, _VP, c_u64, _VP]),
     ('pcx_project_backward', c_i32, [ctypes.POINTER(ProjectDesc), _VP, _VP, _VP, _VP, _VP, _VP, c_u64, _VP]),
+    ('pcx_sample_size', c_i32, [ctypes.POINTER(LogitsDesc), ctypes.POINTER(c_u64)]),
+    ('pcx_sample_actions', c_i32, [ctypes.POINTER(LogitsDesc), ctypes.POINTER(Sampling), _VP, _VP, _VP, _VP, _VP, c_u64, _VP]),
+    ('pcx_log_prob_size', c_i32, [ctypes.POINTER(LogitsDesc), ctypes.POINTER(c_u64)]),
+    ('pcx_log_prob', c_i32, [ctypes.POINTER(LogitsDesc), ctypes.c_float, _VP, _VP, _VP, _VP, _VP, _VP, _VP, c_u64, _VP]),
+    ('pcx_log_prob_backward', c_i32, [ctypes.POINTER(LogitsDesc), ctypes.c_float, _VP, _VP, _VP, _VP, _VP, _VP, _VP, _VP, _VP]),
     ('pcx_gather_create', c_i32, [ctypes.POINTER(_VP), c_i32, ctypes.POINTER(_VP)]),
     ('pcx_gather_destroy', None, [_VP]),
     ('pcx_gather_scalars', c_i32, [_VP, ctypes.POINTER(_VP)]),

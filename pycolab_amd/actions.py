@@ -1,4 +1,4 @@
-"""Synthetic action tapes shared by host, oracle and device.
+"""Actions: synthetic tapes shared by host, oracle and device, and actions drawn from a policy's logits.
 
 `pcx_action_hash` (include/pcx.h) is the counter-based generator behind
 `Engine.step_hashed`: action of environment `env` (its GLOBAL index in a
@@ -6,9 +6,19 @@ sharded batch) at step `t` = hash(seed, env, t) % n_actions.  This is its
 vectorised host twin, so that a sharded run can stage on every rank exactly the
 tape an unsharded engine would draw on the device (the global
 environment index drives the actions, never the rank).
+
+`sample` draws one action per environment from a policy's logits (what
+`Engine.play()` / `Engine.step_sampled()` then takes), `log_prob` is the
+log-probability of actions taken and the policy's entropy, differentiable in
+the logits.  Both run as kernels of csrc/pcx_policy.hip on PyTorch tensors.
 """
 
+import ctypes
+
 import numpy as np
+
+from pycolab_amd import _native as N
+from pycolab_amd import device as dev
 
 _M1, _M2, _M3 = np.uint64(0x9E3779B97F4A7C15), np.uint64(0xBF58476D1CE4E5B9), np.uint64(0x94D049BB133111EB)
 
@@ -31,3 +41,194 @@ def hashed_tape(seed, env_lo, n_envs, t0, steps, n_actions):
   env = np.arange(env_lo, env_lo + n_envs, dtype=np.uint64)[None, :]
   t = np.arange(t0, t0 + steps, dtype=np.uint64)[:, None]
   return (action_hash(seed, env, t) % np.uint32(n_actions)).astype(np.int32)
+
+
+# ---------------------------------------------------------------------- a policy's actions
+
+
+def _rows(logits, legal):
+  """(description, legal tensor to keep) of logits [n, actions] whose actions are contiguous."""
+  torch = dev.require_torch('a policy over actions')
+  if not isinstance(logits, torch.Tensor) or not logits.is_cuda or logits.dim() != 2:
+    raise ValueError('logits must be a device tensor [n, actions]')
+  d = N.LogitsDesc()
+  d.dtype = dev.policy_dtype(logits, 'logits')
+  d.n, d.actions = int(logits.shape[0]), int(logits.shape[1])
+  if d.actions < 1:
+    raise ValueError('logits of no action')
+  if d.actions > 1 and logits.stride(1) != 1:
+    raise ValueError('the actions of a row must be contiguous (strides {})'.format(logits.stride()))
+  d.row_stride = int(logits.stride(0))
+  if legal is not None:
+    if not isinstance(legal, torch.Tensor) or legal.device != logits.device or legal.dtype not in (torch.bool, torch.uint8):
+      raise ValueError('legal must be a bool or uint8 tensor on {}'.format(logits.device))
+    if tuple(legal.shape) == (d.actions,):
+      legal = legal.expand(d.n, d.actions)
+    if tuple(legal.shape) != tuple(logits.shape):
+      raise ValueError('legal must be [{}, {}] or [{}]'.format(d.n, d.actions, d.actions))
+    if d.actions > 1 and legal.stride(1) != 1:
+      raise ValueError('the actions of a row of `legal` must be contiguous')
+    d.legal_stride = int(legal.stride(0))
+  return d, legal
+
+
+def _per_row(value, name, n, dtype, device):
+  """A rule's device array [n], or None for a number."""
+  torch = dev.torch_module()
+  if not isinstance(value, torch.Tensor):
+    return None
+  if value.dtype != dtype or value.device != device or tuple(value.shape) != (n,):
+    raise ValueError('{} must be a number or a {} tensor [{}] on {}'.format(name, dtype, n, device))
+  return value.contiguous()
+
+
+def sample(logits, uniforms, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, legal=None, out=None):
+  """One action per row of `logits` (float32, float16 or bfloat16 device tensor [n, actions]): int32 [n], what
+  `Engine.play()` takes.
+
+  `uniforms`: float32 [n], one number of [0, 1) per row; the result is a function of the row and its number alone, so a
+  sharded batch draws what the whole one would.  `legal`: bool / uint8 [n, actions] or [actions]; an action is allowed where
+  it is legal and its logit is neither -infinity nor a NaN.  Of the allowed actions, ordered by (logit descending, index
+  ascending), the first `top_k` stay (0: all), of those each whose predecessors weigh less than `top_p` of the total, of
+  those each at least `min_p` times as probable as the best; the best one always.  Weights are exp(logit / temperature);
+  `temperature` 0 takes the best action.  Each of the four is a number or a device array [n] (float32; `top_k` int32), row by
+  row.  A row that allows nothing gives `_native.ACTION_NONE` (-1), the engine's `None`.
+
+  `out`: an int32 tensor [n] to write into.  Nothing waits for the device; calls can be captured into a graph."""
+  torch = dev.require_torch('sample()')
+  d, legal = _rows(logits, legal)
+  if not isinstance(uniforms, torch.Tensor) or uniforms.dtype != torch.float32 or uniforms.device != logits.device or tuple(uniforms.shape) != (d.n,):
+    raise ValueError('uniforms must be float32 [{}] on {}'.format(d.n, logits.device))
+  r = N.Sampling()
+  rows = [_per_row(v, name, d.n, dtype, logits.device) for v, name, dtype in (
+      (temperature, 'temperature', torch.float32), (top_k, 'top_k', torch.int32), (top_p, 'top_p', torch.float32), (min_p, 'min_p', torch.float32))]
+  r.temperature_row, r.top_k_row, r.top_p_row, r.min_p_row = [dev.pointer(t) for t in rows]
+  if rows[0] is None:
+    r.temperature = float(temperature)
+  if rows[1] is None:
+    if int(top_k) != top_k:
+      raise ValueError('top_k must be a whole number')
+    r.top_k = max(-1, min(int(top_k), 1 << 30))
+  if rows[2] is None:
+    r.top_p = float(top_p)
+  if rows[3] is None:
+    r.min_p = float(min_p)
+  if out is None:
+    out = torch.empty((d.n,), dtype=torch.int32, device=logits.device)
+  elif out.dtype != torch.int32 or out.device != logits.device or tuple(out.shape) != (d.n,) or not out.is_contiguous():
+    raise ValueError('out must be a contiguous int32 tensor [{}] on {}'.format(d.n, logits.device))
+  uniforms = uniforms.contiguous()
+  with torch.cuda.device(logits.device):
+    scratch = N.c_u64(0)
+    N.check(N.lib().pcx_sample_size(ctypes.byref(d), ctypes.byref(scratch)))
+    ws = torch.empty(scratch.value, dtype=torch.uint8, device=logits.device) if scratch.value else None
+    N.check(N.lib().pcx_sample_actions(ctypes.byref(d), ctypes.byref(r), logits.data_ptr(), dev.pointer(legal), uniforms.data_ptr(),
+                                       out.data_ptr(), dev.pointer(ws), scratch.value, dev.current_stream(logits.device.index)))
+  return out
+
+
+def _taken(actions, n, device):
+  torch = dev.torch_module()
+  if not isinstance(actions, torch.Tensor) or actions.dtype != torch.int32 or actions.device != device or tuple(actions.shape) != (n,):
+    raise ValueError('actions must be int32 [{}] on {}'.format(n, device))
+  return actions.contiguous()
+
+
+def _log_prob_forward(d, legal, logits, actions, temperature):
+  torch = dev.torch_module()
+  log_prob, entropy = (torch.empty((d.n,), dtype=torch.float32, device=logits.device) for _ in range(2))
+  stats = torch.empty((d.n, 2), dtype=torch.float32, device=logits.device)
+  with torch.cuda.device(logits.device):
+    scratch = N.c_u64(0)
+    N.check(N.lib().pcx_log_prob_size(ctypes.byref(d), ctypes.byref(scratch)))
+    ws = torch.empty(scratch.value, dtype=torch.uint8, device=logits.device) if scratch.value else None
+    N.check(N.lib().pcx_log_prob(ctypes.byref(d), temperature, logits.data_ptr(), dev.pointer(legal), actions.data_ptr(), log_prob.data_ptr(),
+                                 entropy.data_ptr(), stats.data_ptr(), dev.pointer(ws), scratch.value, dev.current_stream(logits.device.index)))
+  return log_prob, entropy, stats
+
+
+def _log_prob_backward(d, legal, logits, actions, temperature, entropy, stats, grad_log_prob, grad_entropy):
+  torch = dev.torch_module()
+  grad = torch.empty((d.n, d.actions), dtype=logits.dtype, device=logits.device)
+  for g, name in ((grad_log_prob, 'grad_log_prob'), (grad_entropy, 'grad_entropy')):
+    if g is not None and (g.dtype != torch.float32 or tuple(g.shape) != (d.n,) or g.device != logits.device):
+      raise ValueError('{} must be float32 [{}] on {}'.format(name, d.n, logits.device))
+  grad_log_prob, grad_entropy = (None if g is None else g.contiguous() for g in (grad_log_prob, grad_entropy))
+  with torch.cuda.device(logits.device):
+    N.check(N.lib().pcx_log_prob_backward(ctypes.byref(d), temperature, logits.data_ptr(), dev.pointer(legal), actions.data_ptr(), entropy.data_ptr(),
+                                          stats.data_ptr(), dev.pointer(grad_log_prob), dev.pointer(grad_entropy), grad.data_ptr(),
+                                          dev.current_stream(logits.device.index)))
+  return grad
+
+
+_log_prob_function = None
+
+
+def _log_prob_autograd():
+  """The autograd function behind `log_prob()` (made on first use: PyTorch is optional here)."""
+  global _log_prob_function
+  if _log_prob_function is None:
+    torch = dev.torch_module()
+
+    class LogProb(torch.autograd.Function):
+
+      @staticmethod
+      def forward(ctx, logits, actions, legal, temperature, d):
+        ctx.set_materialize_grads(False)
+        log_prob, entropy, stats = _log_prob_forward(d, legal, logits, actions, temperature)
+        ctx.d, ctx.temperature = d, temperature
+        ctx.save_for_backward(logits, actions, legal, entropy, stats)
+        return log_prob, entropy
+
+      @staticmethod
+      @torch.autograd.function.once_differentiable
+      def backward(ctx, grad_log_prob, grad_entropy):
+        logits, actions, legal, entropy, stats = ctx.saved_tensors
+        if grad_log_prob is None and grad_entropy is None:
+          return None, None, None, None, None
+        return (_log_prob_backward(ctx.d, legal, logits, actions, ctx.temperature, entropy, stats, grad_log_prob, grad_entropy),
+                None, None, None, None)
+
+    _log_prob_function = LogProb
+  return _log_prob_function
+
+
+def _positive(temperature):
+  temperature = float(temperature)
+  if not 0.0 < temperature < float('inf'):
+    raise ValueError('temperature must be a positive number, not {}'.format(temperature))
+  return temperature
+
+
+def log_prob(logits, actions, legal=None, temperature=1.0, return_stats=False):
+  """(log-probability of `actions`, entropy) of every row's policy softmax(logits / temperature) over the allowed actions:
+  two float32 tensors [n], differentiable in `logits` (float32, float16 or bfloat16 [n, actions]).
+
+  `actions`: int32 [n], as `sample()` returned them.  -1 (`_native.ACTION_NONE`: nothing was allowed) has log-probability 0
+  and adds nothing to the gradient; so does a row that allows nothing, whose entropy is 0 too.  An action that is not
+  allowed has -infinity, one that does not exist a NaN.  The gradient is 0 where an action is not allowed.  `legal`: as for
+  `sample()`.
+
+  `return_stats=True`: no autograd; returns (log_prob, entropy, stats), what `log_prob_backward` takes -- the pair to
+  capture into a graph."""
+  torch = dev.require_torch('log_prob()')
+  d, legal = _rows(logits, legal)
+  actions, temperature = _taken(actions, d.n, logits.device), _positive(temperature)
+  if return_stats:
+    return _log_prob_forward(d, legal, logits.detach(), actions, temperature)
+  if torch.is_grad_enabled() and logits.requires_grad:
+    dev.refuse_recording_in_capture('log_prob', 'log_prob(..., return_stats=True) and log_prob_backward()')
+    return _log_prob_autograd().apply(logits, actions, legal, temperature, d)
+  return _log_prob_forward(d, legal, logits, actions, temperature)[:2]
+
+
+def log_prob_backward(logits, actions, entropy, stats, grad_log_prob=None, grad_entropy=None, legal=None, temperature=1.0):
+  """The gradient with respect to `logits` of `log_prob()`'s two results, from theirs (float32 [n], None: zero) and from the
+  `entropy` and `stats` it returned.  Records nothing for autograd and waits for nothing: it may be captured."""
+  torch = dev.require_torch('log_prob_backward()')
+  d, legal = _rows(logits, legal)
+  actions, temperature = _taken(actions, d.n, logits.device), _positive(temperature)
+  for t, shape, name in ((entropy, (d.n,), 'entropy'), (stats, (d.n, 2), 'stats')):
+    if t.dtype != torch.float32 or tuple(t.shape) != shape or t.device != logits.device or not t.is_contiguous():
+      raise ValueError('{} must be what log_prob(..., return_stats=True) returned'.format(name))
+  return _log_prob_backward(d, legal, logits, actions, temperature, entropy, stats, grad_log_prob, grad_entropy)

@@ -1,0 +1,1100 @@
+// pcx_policy.hip -- what a policy's logits become: sampled actions, and the log-probability of actions taken and the
+// policy's entropy with the gradient of both with respect to the logits.
+//
+// Definitions, for one row of logits x over the actions, `allowed` where the action is legal, x is no NaN and x > -inf:
+//   w_j = exp((x_j - max x) / T) for the allowed actions (an action that equals the maximum weighs 1, infinite or not).
+//   sample: order the allowed actions by (x descending, index ascending).  Keep the first top_k of them; of those, each
+//   whose predecessors weigh less than top_p of the kept ones' total; of those, each with w_j >= min_p; the first always.
+//   What is kept is a prefix of that order, so it is described by the last kept value and how many of the actions with
+//   that very value are kept (the lowest indices).  The action is the first j in index order whose running sum of kept
+//   weights exceeds u times their total; T <= 0 takes the first of the order.  No allowed action: PCX_ACTION_NONE.
+//   log_prob: with d_j = (x_j - max x) / T and s = sum exp d_j:  log p_a = d_a - log s,
+//   H = log s - (sum d_j exp d_j) / s;  d(log p_a) = (1[j = a] - p_j) / T,  dH = -p_j (log p_j + H) / T.
+//
+// Sampling decides by where one number falls between two sums, so its weights and sums are 64-bit: a float32 sum would
+// pick another action once in some million rows.  MI355X multiplies and adds 64-bit floats at the rate of 32-bit ones,
+// which puts exp at about 25 instructions.  Sums that atomics build are 64-bit fixed point: their order does not matter.
+#include "pcx_internal.h"
+
+#include <cmath>
+
+using pcx::set_error;
+
+namespace {
+
+constexpr int NONE = PCX_ACTION_NONE;
+
+template <int DT> struct Logit;
+template <> struct Logit<PCX_F32> {
+  typedef float T;
+  static __device__ __forceinline__ float get(float v) { return v; }
+  static __device__ __forceinline__ float put(float v) { return v; }
+};
+template <> struct Logit<PCX_F16> {
+  typedef _Float16 T;
+  static __device__ __forceinline__ float get(_Float16 v) { return (float)v; }
+  static __device__ __forceinline__ _Float16 put(float v) { return (_Float16)v; }
+};
+template <> struct Logit<PCX_BF16> {
+  typedef __bf16 T;
+  static __device__ __forceinline__ float get(__bf16 v) { return (float)v; }
+  static __device__ __forceinline__ __bf16 put(float v) { return (__bf16)v; }
+};
+
+struct Rows {
+  int64_t n, row_stride, legal_stride;
+  int32_t actions;
+  const void* logits;
+  const uint8_t* legal;  // or null
+};
+
+template <typename T> struct Quad { T v[4]; };
+
+// A float as an unsigned number of the same order; 0 stands for "not allowed".  (+0 and -0 are one value.)
+__device__ __forceinline__ uint32_t order_of(float x) {
+  const uint32_t u = __float_as_uint(x + 0.0f);
+  return u ^ ((u >> 31) ? 0xFFFFFFFFu : 0x80000000u);
+}
+__device__ __forceinline__ float value_of(uint32_t key) { return __uint_as_float(key ^ ((key >> 31) ? 0x80000000u : 0xFFFFFFFFu)); }
+__device__ __forceinline__ bool allowed(float x, bool legal) { return legal && x > -INFINITY; }  // (a NaN compares false)
+
+// ---------------------------------------------------------------- reductions over a group of THREADS (one wave, or a workgroup)
+
+template <typename V> __device__ __forceinline__ V across(V v, int mask) { return __shfl_xor(v, mask); }
+
+template <int THREADS>
+struct Group {
+  static constexpr int WAVES = THREADS / 64;
+  struct Scratch { double d[WAVES + 1]; uint64_t u[WAVES + 1]; };
+  Scratch* s;
+  int t;  // thread within the group
+  template <typename V, typename F>
+  __device__ __forceinline__ V reduce(V v, V* slots, F f) const {
+#pragma unroll
+    for (int k = 32; k >= 1; k >>= 1) v = f(v, across(v, k));
+    if constexpr (WAVES > 1) {
+      __syncthreads();
+      if ((t & 63) == 0) slots[t >> 6] = v;
+      __syncthreads();
+      v = slots[0];
+#pragma unroll 1
+      for (int i = 1; i < WAVES; ++i) v = f(v, slots[i]);
+    }
+    return v;
+  }
+  __device__ __forceinline__ double sum(double v) const { return reduce(v, s->d, [](double a, double b) { return a + b; }); }
+  __device__ __forceinline__ uint32_t count(uint32_t v) const {
+    return (uint32_t)reduce((uint64_t)v, s->u, [](uint64_t a, uint64_t b) { return a + b; });
+  }
+  __device__ __forceinline__ uint64_t max(uint64_t v) const { return reduce(v, s->u, [](uint64_t a, uint64_t b) { return a > b ? a : b; }); }
+  __device__ __forceinline__ uint64_t min(uint64_t v) const { return reduce(v, s->u, [](uint64_t a, uint64_t b) { return a < b ? a : b; }); }
+  // the sum of the threads before this one, and of all
+  template <typename V>
+  __device__ __forceinline__ V scan(V v, V* slots, V* total) const {
+    V in = v;
+#pragma unroll
+    for (int k = 1; k < 64; k <<= 1) {
+      const V o = __shfl_up(in, k);
+      if ((t & 63) >= k) in += o;
+    }
+    V before = __shfl_up(in, 1);
+    if ((t & 63) == 0) before = V(0);
+    V all = __shfl(in, 63);
+    if constexpr (WAVES > 1) {
+      __syncthreads();
+      if ((t & 63) == 63) slots[t >> 6] = in;
+      __syncthreads();
+      all = V(0);
+#pragma unroll 1
+      for (int i = 0; i < WAVES; ++i) {
+        if (i == (t >> 6)) before = all + before;
+        all += slots[i];
+      }
+    }
+    *total = all;
+    return before;
+  }
+};
+
+// ---------------------------------------------------------------- sampling
+
+struct Rules {
+  float temperature, top_p, min_p;
+  int32_t top_k;
+  const float* temperature_row;
+  const int32_t* top_k_row;
+  const float* top_p_row;
+  const float* min_p_row;
+};
+struct RowRules { float temperature, top_p, min_p; int32_t top_k; };
+__device__ __forceinline__ RowRules rules_of(const Rules& r, int64_t row) {
+  RowRules o;
+  o.temperature = r.temperature_row ? r.temperature_row[row] : r.temperature;
+  o.top_k = r.top_k_row ? r.top_k_row[row] : r.top_k;
+  o.top_p = r.top_p_row ? r.top_p_row[row] : r.top_p;
+  const float m = r.min_p_row ? r.min_p_row[row] : r.min_p;
+  o.min_p = m < 1.0f ? m : (m >= 1.0f ? 1.0f : 0.0f);  // (a NaN asks for nothing)
+  return o;
+}
+
+struct SampleArgs {
+  Rows rows;
+  Rules rules;
+  const float* uniforms;
+  int32_t* out;
+};
+
+__device__ __forceinline__ double weight_of(float x, float best, double rate) {
+  return x == best ? 1.0 : exp(((double)x - (double)best) * rate);
+}
+
+// A thread holds a whole row: few actions, many rows.
+template <int DT, int CAP>
+__global__ __launch_bounds__(256) void pcx_sample_rows(SampleArgs a) {
+  typedef typename Logit<DT>::T T;
+  const int64_t row = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (row >= a.rows.n) return;
+  const T* const x_row = reinterpret_cast<const T*>(a.rows.logits) + row * a.rows.row_stride;
+  const uint8_t* const l_row = a.rows.legal ? a.rows.legal + row * a.rows.legal_stride : nullptr;
+  const RowRules r = rules_of(a.rules, row);
+  const int A = a.rows.actions;
+  float x[CAP];
+  float best = -INFINITY;
+  int first = NONE;
+#pragma unroll
+  for (int j = 0; j < CAP; ++j) {
+    x[j] = -INFINITY;
+    if (j < A) {
+      const float v = Logit<DT>::get(x_row[j]);
+      if (allowed(v, l_row ? l_row[j] != 0 : true)) x[j] = v;
+    }
+    if (x[j] > best) { best = x[j]; first = j; }
+  }
+  if (first == NONE || !(r.temperature > 0.0f)) { a.out[row] = first; return; }
+  const double rate = 1.0 / (double)r.temperature;
+  double w[CAP];
+#pragma unroll
+  for (int j = 0; j < CAP; ++j) w[j] = x[j] > -INFINITY ? weight_of(x[j], best, rate) : 0.0;
+  if (r.top_k > 0 && r.top_k < A) {
+#pragma unroll
+    for (int j = 0; j < CAP; ++j) {
+      int rank = 0;
+#pragma unroll
+      for (int i = 0; i < CAP; ++i) rank += i < j ? x[i] >= x[j] : x[i] > x[j];
+      if (rank >= r.top_k) w[j] = -w[j];  // (dropped: its sign, while the others are still being ranked)
+    }
+#pragma unroll
+    for (int j = 0; j < CAP; ++j)
+      if (!(w[j] > 0.0)) w[j] = 0.0;
+  }
+  if (r.top_p < 1.0f) {
+    double total = 0.0;
+#pragma unroll
+    for (int j = 0; j < CAP; ++j) total += w[j];
+    const double target = (double)r.top_p * total;
+    uint32_t keep = 0;
+#pragma unroll
+    for (int j = 0; j < CAP; ++j) {
+      double ahead = 0.0;
+#pragma unroll
+      for (int i = 0; i < CAP; ++i) ahead += (i < j ? x[i] >= x[j] : x[i] > x[j]) ? w[i] : 0.0;
+      if (j == first || ahead < target) keep |= 1u << j;
+    }
+#pragma unroll
+    for (int j = 0; j < CAP; ++j)
+      if (!((keep >> j) & 1u)) w[j] = 0.0;
+  }
+  double total = 0.0;
+#pragma unroll
+  for (int j = 0; j < CAP; ++j) {
+    if (w[j] < (double)r.min_p) w[j] = 0.0;
+    total += w[j];
+  }
+  const double target = (double)a.uniforms[row] * total;
+  double run = 0.0;
+  int pick = NONE, last = NONE;
+#pragma unroll
+  for (int j = 0; j < CAP; ++j) {
+    run += w[j];
+    if (w[j] > 0.0) last = j;
+    if (pick == NONE && w[j] > 0.0 && run > target) pick = j;
+  }
+  a.out[row] = pick == NONE ? last : pick;
+}
+
+// EP neighbouring actions of one row per thread: their order keys (0: not allowed, or not there).
+template <int DT, int EP>
+__device__ __forceinline__ void load_keys(const Rows& rows, int64_t row, int j0, int end, uint32_t* key) {
+  typedef typename Logit<DT>::T T;
+  const T* const x_row = reinterpret_cast<const T*>(rows.logits) + row * rows.row_stride;
+  const uint8_t* const l_row = rows.legal ? rows.legal + row * rows.legal_stride : nullptr;
+  if constexpr (EP % 4 == 0) {
+#pragma unroll
+    for (int i = 0; i < EP; i += 4) {
+      Quad<T> q = {};
+      uint32_t ok = 0x01010101u;
+      const int j = j0 + i;
+      if (j + 4 <= end) {
+        __builtin_memcpy(&q, x_row + j, sizeof q);
+        if (l_row) __builtin_memcpy(&ok, l_row + j, 4);
+      } else {
+        for (int c = 0; c < 4; ++c)
+          if (j + c < end) {
+            q.v[c] = x_row[j + c];
+            if (l_row && !l_row[j + c]) ok &= ~(0xFFu << (8 * c));
+          }
+      }
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        const float x = Logit<DT>::get(q.v[c]);
+        key[i + c] = j + c < end && allowed(x, ((ok >> (8 * c)) & 255u) != 0) ? order_of(x) : 0u;
+      }
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < EP; ++i) {
+      key[i] = 0;
+      if (j0 + i < end) {
+        const float x = Logit<DT>::get(x_row[j0 + i]);
+        if (allowed(x, l_row ? l_row[j0 + i] != 0 : true)) key[i] = order_of(x);
+      }
+    }
+  }
+}
+
+// Of the elements whose key is `value`, those from the `keep`-th on (in index order) are let go.
+template <int THREADS, int EP>
+__device__ __forceinline__ void drop_ties(const Group<THREADS>& g, uint32_t value, uint32_t keep, uint32_t* key, double* w) {
+  uint64_t mine = 0, total;
+#pragma unroll
+  for (int i = 0; i < EP; ++i) mine += key[i] == value;
+  uint64_t at = g.scan(mine, g.s->u, &total);
+#pragma unroll
+  for (int i = 0; i < EP; ++i)
+    if (key[i] == value && at++ >= keep) { key[i] = 0; w[i] = 0.0; }
+}
+
+// The action at u of the kept weights' total, all threads of the group together.
+template <int THREADS, int EP>
+__device__ __forceinline__ int draw_action(const Group<THREADS>& g, const double* w, int j0, double target_of_total, double offset, bool absolute) {
+  double mine = 0.0, total;
+#pragma unroll
+  for (int i = 0; i < EP; ++i) mine += w[i];
+  const double before = offset + g.scan(mine, g.s->d, &total);
+  const double target = absolute ? target_of_total : target_of_total * total;
+  uint64_t pick = ~0ull;
+  uint64_t last = 0;
+  double run = before;
+#pragma unroll
+  for (int i = 0; i < EP; ++i) {
+    run += w[i];
+    if (w[i] > 0.0) {
+      last = (uint64_t)(j0 + i) + 1;
+      if (run > target && pick == ~0ull) pick = (uint64_t)(j0 + i);
+    }
+  }
+  pick = g.min(pick);
+  if (pick != ~0ull) return (int)pick;
+  last = g.max(last);  // (u is one or more, or no number: the last one kept)
+  return (int)last - 1;
+}
+
+// The largest key t with at least k keys >= t; the keys hold more than k that are not 0.
+template <int THREADS, int EP>
+__device__ __forceinline__ uint32_t find_rank(const Group<THREADS>& g, const uint32_t* key, uint32_t k, uint32_t hi) {
+  uint32_t lo = 1;
+  while (lo < hi) {
+    const uint32_t mid = hi - (hi - lo) / 2;
+    uint32_t c = 0;
+#pragma unroll
+    for (int i = 0; i < EP; ++i) c += key[i] >= mid;
+    if (g.count(c) >= k) lo = mid; else hi = mid - 1;
+  }
+  return lo;
+}
+// The largest key t whose elements >= t weigh at least `target`.
+template <int THREADS, int EP>
+__device__ __forceinline__ uint32_t find_mass(const Group<THREADS>& g, const uint32_t* key, const double* w, double target, uint32_t hi) {
+  uint32_t lo = 1;
+  while (lo < hi) {
+    const uint32_t mid = hi - (hi - lo) / 2;
+    double m = 0.0;
+#pragma unroll
+    for (int i = 0; i < EP; ++i) m += key[i] >= mid ? w[i] : 0.0;
+    if (g.sum(m) >= target) lo = mid; else hi = mid - 1;
+  }
+  return lo;
+}
+
+// A wave or a workgroup holds a row in registers, EP neighbouring actions a thread.
+template <int DT, int THREADS, int EP>
+__global__ __launch_bounds__(THREADS < 256 ? 256 : THREADS) void pcx_sample_group(SampleArgs a) {
+  constexpr int ROWS = THREADS < 256 ? 256 / THREADS : 1;
+  __shared__ typename Group<THREADS>::Scratch scratch[ROWS];
+  Group<THREADS> g{&scratch[threadIdx.x / THREADS], (int)(threadIdx.x % THREADS)};
+  const int64_t row = (int64_t)blockIdx.x * ROWS + threadIdx.x / THREADS;
+  if (row >= a.rows.n) return;  // (a whole group)
+  const RowRules r = rules_of(a.rules, row);
+  const int A = a.rows.actions, j0 = g.t * EP;
+  uint32_t key[EP];
+  load_keys<DT, EP>(a.rows, row, j0, A, key);
+  uint64_t top = 0;
+#pragma unroll
+  for (int i = 0; i < EP; ++i) {
+    const uint64_t v = ((uint64_t)key[i] << 32) | (uint32_t)~(uint32_t)(j0 + i);
+    if (key[i] && v > top) top = v;
+  }
+  top = g.max(top);
+  const uint32_t best_key = (uint32_t)(top >> 32);
+  if (best_key == 0 || !(r.temperature > 0.0f)) {
+    if (g.t == 0) a.out[row] = best_key ? (int)~(uint32_t)top : NONE;
+    return;
+  }
+  const float best = value_of(best_key);
+  const double rate = 1.0 / (double)r.temperature;
+  double w[EP];
+#pragma unroll
+  for (int i = 0; i < EP; ++i) w[i] = key[i] ? weight_of(value_of(key[i]), best, rate) : 0.0;
+  if (r.top_k > 0 && r.top_k < A) {
+    uint32_t c = 0;
+#pragma unroll
+    for (int i = 0; i < EP; ++i) c += key[i] != 0;
+    if (g.count(c) > (uint32_t)r.top_k) {
+      const uint32_t edge = find_rank<THREADS, EP>(g, key, (uint32_t)r.top_k, best_key);
+      uint32_t above = 0;
+#pragma unroll
+      for (int i = 0; i < EP; ++i) {
+        above += key[i] > edge;
+        if (key[i] < edge) { key[i] = 0; w[i] = 0.0; }
+      }
+      above = g.count(above);
+      drop_ties<THREADS, EP>(g, edge, (uint32_t)r.top_k - above, key, w);
+    }
+  }
+  if (r.top_p < 1.0f) {
+    double total = 0.0;
+#pragma unroll
+    for (int i = 0; i < EP; ++i) total += w[i];
+    const double target = (double)r.top_p * g.sum(total);
+    const uint32_t edge = find_mass<THREADS, EP>(g, key, w, target, best_key);
+    double above = 0.0;
+#pragma unroll
+    for (int i = 0; i < EP; ++i) {
+      above += key[i] > edge ? w[i] : 0.0;
+      if (key[i] < edge) { key[i] = 0; w[i] = 0.0; }
+    }
+    above = g.sum(above);
+    const double need = ceil((target - above) / weight_of(value_of(edge), best, rate));
+    drop_ties<THREADS, EP>(g, edge, need >= 1.0 ? (need < 4e9 ? (uint32_t)need : 0xFFFFFFFFu) : 1u, key, w);
+  }
+#pragma unroll
+  for (int i = 0; i < EP; ++i)
+    if (w[i] < (double)r.min_p) w[i] = 0.0;
+  const int pick = draw_action<THREADS, EP>(g, w, j0, (double)a.uniforms[row], 0.0, false);
+  if (g.t == 0) a.out[row] = pick;
+}
+
+// ---- rows that no workgroup holds: divided among workgroups, one launch per question ------------------------------------
+
+constexpr int SLICE = 8192;    // actions per workgroup
+constexpr int WEP = 32;        // ... per thread of 256
+constexpr int BINS = 2048;     // of a digit of the order key: 11, 11 and 10 bits
+struct RowState {
+  uint64_t best;               // (order key, ~index) of the best action
+  double total, target, above; // weights: of what top_k leaves, top_p of it, ahead of the current digit's bin
+  uint64_t count_above;        // actions ahead of the current digit's bin
+  uint32_t prefix;             // the digits found so far
+  uint32_t edge, ties;         // kept: keys above `edge`, and `ties` (lowest indices) that equal it
+  uint32_t active;             // bit 0: the row samples; 1: top_k cuts; 2: top_p cuts
+};
+struct Slot { double weight; uint64_t ties; };
+struct WideArgs {
+  SampleArgs a;
+  int64_t row0;                // first row of this batch of launches
+  int32_t slices, scale;       // fixed-point weights: w * 2^scale
+  RowState* state;             // [rows]
+  uint64_t* mass;              // [2][rows][BINS]: the first digit's, the later digits'
+  uint32_t* count;
+  Slot* slots;                 // [rows][slices]
+  int32_t batch;
+};
+__device__ __forceinline__ int digit_shift(int level) { return level == 0 ? 21 : level == 1 ? 10 : 0; }
+__device__ __forceinline__ uint32_t digit_of(uint32_t key, int level) { return (key >> digit_shift(level)) & (level == 2 ? 1023u : 2047u); }
+__device__ __forceinline__ bool same_prefix(uint32_t key, uint32_t prefix, int level) {
+  return level == 0 || (level == 1 ? key >> 21 == prefix >> 21 : key >> 10 == prefix >> 10);
+}
+
+__global__ __launch_bounds__(256) void pcx_sample_clear(WideArgs w) {
+  const int row = blockIdx.x;
+  for (int i = threadIdx.x; i < 2 * BINS; i += 256) {
+    const int64_t at = ((int64_t)(i / BINS) * w.batch + row) * BINS + i % BINS;
+    w.mass[at] = 0;
+    w.count[at] = 0;
+  }
+  if (threadIdx.x == 0) w.state[row] = RowState{};
+}
+template <int DT>
+__global__ __launch_bounds__(256) void pcx_sample_best(WideArgs w) {
+  __shared__ Group<256>::Scratch scratch;
+  Group<256> g{&scratch, (int)threadIdx.x};
+  const int row = blockIdx.y, lo = blockIdx.x * SLICE;
+  const int end = w.a.rows.actions - lo < SLICE ? w.a.rows.actions : lo + SLICE;
+  uint64_t top = 0;
+  for (int j0 = lo + threadIdx.x * 4; j0 < end; j0 += 1024) {
+    uint32_t key[4];
+    load_keys<DT, 4>(w.a.rows, w.row0 + row, j0, end, key);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint64_t v = ((uint64_t)key[i] << 32) | (uint32_t)~(uint32_t)(j0 + i);
+      if (key[i] && v > top) top = v;
+    }
+  }
+  top = g.max(top);
+  if (threadIdx.x == 0 && top) atomicMax(reinterpret_cast<unsigned long long*>(&w.state[row].best), (unsigned long long)top);
+}
+// Counts and weights per value of one digit, of the keys that agree with the digits found so far.
+template <int DT>
+__global__ __launch_bounds__(256) void pcx_sample_digit(WideArgs w, int level, uint32_t needs) {
+  __shared__ unsigned long long mass[BINS];
+  __shared__ uint32_t count[BINS];
+  const int row = blockIdx.y, lo = blockIdx.x * SLICE;
+  const RowState st = w.state[row];
+  if (level > 0 && !(st.active & needs)) return;
+  const RowRules r = rules_of(w.a.rules, w.row0 + row);
+  const uint32_t best_key = (uint32_t)(st.best >> 32);
+  if (!best_key || !(r.temperature > 0.0f)) return;
+  const float best = value_of(best_key);
+  const double rate = 1.0 / (double)r.temperature;
+  for (int i = threadIdx.x; i < BINS; i += 256) { mass[i] = 0; count[i] = 0; }
+  __syncthreads();
+  const int end = w.a.rows.actions - lo < SLICE ? w.a.rows.actions : lo + SLICE;
+  for (int j0 = lo + threadIdx.x * 4; j0 < end; j0 += 1024) {
+    uint32_t key[4];
+    load_keys<DT, 4>(w.a.rows, w.row0 + row, j0, end, key);
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (key[i] && same_prefix(key[i], st.prefix, level)) {
+        const uint32_t d = digit_of(key[i], level);
+        atomicAdd(&count[d], 1u);
+        atomicAdd(&mass[d], (unsigned long long)(ldexp(weight_of(value_of(key[i]), best, rate), w.scale) + 0.5));
+      }
+  }
+  __syncthreads();
+  const int64_t at = ((int64_t)(level != 0) * w.batch + row) * BINS;
+  for (int i = threadIdx.x; i < BINS; i += 256)
+    if (count[i]) {
+      atomicAdd(&w.count[at + i], count[i]);
+      if (mass[i]) atomicAdd(reinterpret_cast<unsigned long long*>(&w.mass[at + i]), mass[i]);
+    }
+}
+// Which bin of the digit the edge lies in.  by_mass: top_p's edge, else top_k's.
+__global__ __launch_bounds__(256) void pcx_sample_edge(WideArgs w, int level, int by_mass) {
+  __shared__ Group<256>::Scratch scratch;
+  __shared__ RowState next;
+  Group<256> g{&scratch, (int)threadIdx.x};
+  const int row = blockIdx.x;
+  RowState st = w.state[row];
+  const RowRules r = rules_of(w.a.rules, w.row0 + row);
+  const uint32_t best_key = (uint32_t)(st.best >> 32);
+  if (!best_key || !(r.temperature > 0.0f)) return;
+  if (level > 0 && !(st.active & (by_mass ? 4u : 2u))) return;
+  const int64_t at = ((int64_t)(level != 0) * w.batch + row) * BINS;
+  // thread 0 has the highest bins: eight a thread
+  uint64_t counts[8], masses[8], c_mine = 0, m_mine = 0, c_all, m_all;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int bin = BINS - 1 - ((int)threadIdx.x * 8 + i);
+    counts[i] = w.count[at + bin];
+    masses[i] = w.mass[at + bin];
+    c_mine += counts[i];
+    m_mine += masses[i];
+    if (level != 0) { w.count[at + bin] = 0; w.mass[at + bin] = 0; }  // for the next digit
+  }
+  uint64_t c = g.scan(c_mine, g.s->u, &c_all);
+  uint64_t m = g.scan(m_mine, g.s->u, &m_all);
+  if (level == 0) {
+    st.above = 0.0;
+    st.count_above = 0;
+    if (by_mass) {
+      if (!(st.active & 2u)) st.total = ldexp((double)m_all, -w.scale);
+      st.target = (double)r.top_p * st.total;
+      if (r.top_p < 1.0f) st.active |= 4u;
+    } else if (r.top_k > 0 && c_all > (uint64_t)r.top_k) {
+      st.active |= 2u;
+    }
+  }
+  const bool cuts = (st.active & (by_mass ? 4u : 2u)) != 0;
+  if (threadIdx.x == 0) next = st;
+  __syncthreads();
+  if (cuts) {
+    // the first bin, from the top, at which the edge is reached
+    uint64_t found = ~0ull;
+    uint64_t c_run = c, m_run = m, c_at = 0, m_at = 0;  // ahead of the bin taken
+    int bin_at = -1;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      if (!counts[i] || found != ~0ull) continue;
+      c_at = c_run;
+      m_at = m_run;
+      bin_at = BINS - 1 - ((int)threadIdx.x * 8 + i);
+      c_run += counts[i];
+      m_run += masses[i];
+      const bool reached = by_mass ? st.above + ldexp((double)m_run, -w.scale) >= st.target : st.count_above + c_run >= (uint64_t)r.top_k;
+      if (reached) found = threadIdx.x;
+    }
+    uint64_t who = g.min(found);
+    // (sums of fixed-point weights can miss the target by their rounding: then the lowest bin that holds anything)
+    const uint64_t lowest = g.max(bin_at >= 0 ? (uint64_t)threadIdx.x : 0);
+    if (who == ~0ull) who = lowest;
+    const bool mine = who == threadIdx.x && bin_at >= 0;
+    if (mine) {
+      next.count_above = st.count_above + c_at;
+      next.above = st.above + ldexp((double)m_at, -w.scale);
+      next.prefix = (level == 0 ? 0u : st.prefix) | ((uint32_t)bin_at << digit_shift(level));
+      if (level == 2) {
+        const double tie = weight_of(value_of(next.prefix), value_of(best_key), 1.0 / (double)r.temperature);
+        next.edge = next.prefix;
+        if (by_mass) {
+          const double need = ceil((st.target - next.above) / tie);
+          const uint32_t limit = (st.active & 2u) && next.edge == st.edge ? st.ties : 0xFFFFFFFFu;  // (what top_k left of them)
+          next.ties = need >= 1.0 ? (need < 4e9 ? (uint32_t)need : 0xFFFFFFFFu) : 1u;
+          if (next.ties > limit) next.ties = limit;
+        } else {
+          next.ties = (uint32_t)((uint64_t)r.top_k - next.count_above);
+          next.total = next.above + (double)next.ties * tie;
+        }
+      }
+    }
+  }
+  __syncthreads();
+  if (threadIdx.x == 0) w.state[row] = next;
+}
+// What of a slice is kept: weight above the edge, and how many equal it.
+template <int DT>
+__global__ __launch_bounds__(256) void pcx_sample_weigh(WideArgs w) {
+  __shared__ Group<256>::Scratch scratch;
+  Group<256> g{&scratch, (int)threadIdx.x};
+  const int row = blockIdx.y, lo = blockIdx.x * SLICE;
+  const RowState st = w.state[row];
+  const RowRules r = rules_of(w.a.rules, w.row0 + row);
+  const uint32_t best_key = (uint32_t)(st.best >> 32);
+  if (!best_key || !(r.temperature > 0.0f)) return;
+  const float best = value_of(best_key);
+  const double rate = 1.0 / (double)r.temperature;
+  const int end = w.a.rows.actions - lo < SLICE ? w.a.rows.actions : lo + SLICE;
+  double mine = 0.0;
+  uint64_t ties = 0;
+  for (int j0 = lo + threadIdx.x * 4; j0 < end; j0 += 1024) {
+    uint32_t key[4];
+    load_keys<DT, 4>(w.a.rows, w.row0 + row, j0, end, key);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (key[i] > st.edge) {
+        const double v = weight_of(value_of(key[i]), best, rate);
+        if (v >= (double)r.min_p) mine += v;
+      }
+      ties += st.edge && key[i] == st.edge;
+    }
+  }
+  mine = g.sum(mine);
+  ties = g.count((uint32_t)ties);
+  if (threadIdx.x == 0) w.slots[(int64_t)row * w.slices + blockIdx.x] = Slot{mine, ties};
+}
+template <int DT>
+__global__ __launch_bounds__(256) void pcx_sample_pick(WideArgs w) {
+  __shared__ Group<256>::Scratch scratch;
+  __shared__ int chosen;
+  __shared__ double offset, goal;
+  __shared__ uint32_t ties_left;
+  Group<256> g{&scratch, (int)threadIdx.x};
+  const int row = blockIdx.x;
+  const int64_t at = w.row0 + row;
+  const RowState st = w.state[row];
+  const RowRules r = rules_of(w.a.rules, at);
+  const uint32_t best_key = (uint32_t)(st.best >> 32);
+  if (!best_key || !(r.temperature > 0.0f)) {
+    if (threadIdx.x == 0) w.a.out[at] = best_key ? (int)~(uint32_t)st.best : NONE;
+    return;
+  }
+  const float best = value_of(best_key);
+  const double rate = 1.0 / (double)r.temperature;
+  double tie = st.edge ? weight_of(value_of(st.edge), best, rate) : 0.0;
+  if (tie < (double)r.min_p) tie = 0.0;
+  if (threadIdx.x == 0) {
+    const Slot* const slots = w.slots + (int64_t)row * w.slices;
+    double total = 0.0;
+    uint64_t left = st.ties;
+    for (int s = 0; s < w.slices; ++s) {
+      const uint64_t kept = slots[s].ties < left ? slots[s].ties : left;
+      left -= kept;
+      total += slots[s].weight + (double)kept * tie;
+    }
+    const double target = (double)w.a.uniforms[at] * total;
+    double run = 0.0;
+    left = st.ties;
+    chosen = -1;
+    for (int s = 0; s < w.slices; ++s) {
+      const uint64_t kept = slots[s].ties < left ? slots[s].ties : left;
+      const double weight = slots[s].weight + (double)kept * tie;
+      if (weight > 0.0) { chosen = s; offset = run; ties_left = (uint32_t)left; }  // (the last that holds anything, if u asks for more)
+      run += weight;
+      left -= kept;
+      if (weight > 0.0 && run > target) break;
+    }
+    goal = target;
+  }
+  __syncthreads();
+  const int lo = chosen * SLICE, j0 = lo + (int)threadIdx.x * WEP;
+  const int end = w.a.rows.actions - lo < SLICE ? w.a.rows.actions : lo + SLICE;
+  uint32_t key[WEP];
+  double v[WEP];
+  load_keys<DT, WEP>(w.a.rows, at, j0, end, key);
+#pragma unroll
+  for (int i = 0; i < WEP; ++i) {
+    v[i] = key[i] && key[i] >= st.edge ? weight_of(value_of(key[i]), best, rate) : 0.0;
+    if (v[i] < (double)r.min_p) v[i] = 0.0;
+  }
+  if (st.edge) drop_ties<256, WEP>(g, st.edge, ties_left, key, v);
+  const int pick = draw_action<256, WEP>(g, v, j0, goal, offset, true);
+  if (threadIdx.x == 0) w.a.out[at] = pick;
+}
+
+// ---------------------------------------------------------------- log-probability, entropy and their gradient
+
+struct LogProbArgs {
+  Rows rows;
+  float rate;                 // 1 / temperature
+  const int32_t* taken;
+  float* log_prob;            // [n]
+  float* entropy;             // [n]
+  float2* stats;              // [n]: the largest logit, sum exp((x - largest) / T); 0 where nothing is allowed
+  const float* grad_log_prob; // backward, or null
+  const float* grad_entropy;  // backward, or null
+  void* grad;                 // [n][actions]
+  float4* partial;            // [n][slices], when a row is divided
+  int32_t slices;
+};
+
+// exp(d) for d <= 0, d = x log2(e) carried in two parts: good to about 2^-23 however large x is.
+__device__ __forceinline__ float exp_of(float d) {
+  const float hi = d * 1.44269502f;
+  const float lo = fmaf(d, 1.44269502f, -hi) + d * 1.925963033e-8f;
+  const float e = __builtin_amdgcn_exp2f(hi);
+  return d > -200.0f ? fmaf(e, lo * 0.693147181f, e) : 0.0f;
+}
+
+// Running (largest x, sum of exp, sum of d exp) of a part of a row, relative to the largest so far.
+struct Soft {
+  float m, s, t;
+  __device__ __forceinline__ void join(float m2, float s2, float t2, float rate) {
+    if (!(m2 > -INFINITY)) return;
+    if (!(m > -INFINITY)) { m = m2; s = s2; t = t2; return; }
+    const float big = fmaxf(m, m2);
+    const float d1 = m == big ? 0.0f : (m - big) * rate, d2 = m2 == big ? 0.0f : (m2 - big) * rate;
+    const float e1 = exp_of(d1), e2 = exp_of(d2);
+    t = (e1 > 0.0f ? e1 * fmaf(d1, s, t) : 0.0f) + (e2 > 0.0f ? e2 * fmaf(d2, s2, t2) : 0.0f);
+    s = e1 * s + e2 * s2;
+    m = big;
+  }
+};
+template <int DT>
+__device__ __forceinline__ void finish_row(const LogProbArgs& a, int64_t row, const Soft& v) {
+  typedef typename Logit<DT>::T T;
+  const bool some = v.m > -INFINITY;
+  const float ls = some ? logf(v.s) : 0.0f;
+  a.entropy[row] = some ? ls - v.t / v.s : 0.0f;
+  a.stats[row] = some ? make_float2(v.m, v.s) : make_float2(0.0f, 0.0f);
+  const int taken = a.taken[row];
+  float lp = 0.0f;
+  if (taken != NONE && (taken < 0 || taken >= a.rows.actions)) lp = NAN;  // (no such action: not passed over in silence)
+  else if (taken != NONE && some) {
+    const float x = Logit<DT>::get(reinterpret_cast<const T*>(a.rows.logits)[row * a.rows.row_stride + taken]);
+    const bool ok = allowed(x, a.rows.legal ? a.rows.legal[row * a.rows.legal_stride + taken] != 0 : true);
+    lp = ok ? (x == v.m ? 0.0f : (x - v.m) * a.rate) - ls : -INFINITY;
+  }
+  a.log_prob[row] = lp;
+}
+
+template <int DT, int THREADS>
+__global__ __launch_bounds__(256) void pcx_log_prob_forward(LogProbArgs a) {
+  constexpr int ROWS = 256 / THREADS;
+  __shared__ float shared[4][3];
+  const int t = threadIdx.x % THREADS;
+  const int64_t unit = (int64_t)blockIdx.x * ROWS + threadIdx.x / THREADS;
+  if (unit >= a.rows.n * a.slices) return;
+  const int64_t row = unit / a.slices;
+  const int slice = (int)(unit - row * a.slices);
+  const int lo = a.slices > 1 ? slice * SLICE : 0;
+  const int end = a.slices > 1 && a.rows.actions - lo > SLICE ? lo + SLICE : a.rows.actions;
+  Soft v{-INFINITY, 0.0f, 0.0f};
+  for (int j0 = lo + t * 4; j0 < end; j0 += THREADS * 4) {
+    uint32_t key[4];
+    load_keys<DT, 4>(a.rows, row, j0, end, key);
+    const uint32_t k1 = key[0] > key[1] ? key[0] : key[1], k2 = key[2] > key[3] ? key[2] : key[3];
+    const uint32_t top = k1 > k2 ? k1 : k2;
+    if (!top) continue;
+    const float big = value_of(top);
+    float s = 0.0f, tt = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (key[i]) {
+        const float x = value_of(key[i]);
+        const float d = x == big ? 0.0f : (x - big) * a.rate, e = exp_of(d);
+        s += e;
+        if (e > 0.0f) tt = fmaf(d, e, tt);
+      }
+    v.join(big, s, tt, a.rate);
+  }
+#pragma unroll
+  for (int k = 32; k >= 1; k >>= 1) {
+    const float m2 = __shfl_xor(v.m, k), s2 = __shfl_xor(v.s, k), t2 = __shfl_xor(v.t, k);
+    v.join(m2, s2, t2, a.rate);
+  }
+  if constexpr (THREADS > 64) {
+    if ((t & 63) == 0) { shared[t >> 6][0] = v.m; shared[t >> 6][1] = v.s; shared[t >> 6][2] = v.t; }
+    __syncthreads();
+    v = Soft{shared[0][0], shared[0][1], shared[0][2]};
+    for (int i = 1; i < THREADS / 64; ++i) v.join(shared[i][0], shared[i][1], shared[i][2], a.rate);
+  }
+  if (t != 0) return;
+  if (a.slices > 1) a.partial[unit] = make_float4(v.m, v.s, v.t, 0.0f);
+  else finish_row<DT>(a, row, v);
+}
+template <int DT>
+__global__ __launch_bounds__(64) void pcx_log_prob_join(LogProbArgs a) {
+  const int64_t row = blockIdx.x;
+  Soft v{-INFINITY, 0.0f, 0.0f};
+  for (int i = threadIdx.x; i < a.slices; i += 64) {
+    const float4 p = a.partial[row * a.slices + i];
+    v.join(p.x, p.y, p.z, a.rate);
+  }
+#pragma unroll
+  for (int k = 32; k >= 1; k >>= 1) {
+    const float m2 = __shfl_xor(v.m, k), s2 = __shfl_xor(v.s, k), t2 = __shfl_xor(v.t, k);
+    v.join(m2, s2, t2, a.rate);
+  }
+  if (threadIdx.x) return;
+  finish_row<DT>(a, row, v);
+}
+
+// One row's numbers for the gradient of its elements.
+struct RowGrad { float m, inv, ls, h, gl, ge; int taken; bool some; };
+__device__ __forceinline__ RowGrad row_grad(const LogProbArgs& a, int64_t row) {
+  RowGrad g;
+  const float2 st = a.stats[row];
+  g.some = st.y > 0.0f;
+  g.m = st.x;
+  g.inv = 1.0f / st.y;
+  g.ls = logf(st.y);
+  g.h = a.entropy[row];
+  g.taken = a.taken[row];
+  g.gl = a.grad_log_prob && g.taken != NONE ? a.grad_log_prob[row] : 0.0f;
+  if (g.taken != NONE && (g.taken < 0 || g.taken >= a.rows.actions)) g.gl = NAN;
+  g.ge = a.grad_entropy ? a.grad_entropy[row] : 0.0f;
+  return g;
+}
+__device__ __forceinline__ float element_grad(const RowGrad& g, uint32_t key, int j, float rate) {
+  if (!key) return 0.0f;
+  const float x = value_of(key);
+  const float d = x == g.m ? 0.0f : (x - g.m) * rate;
+  const float p = exp_of(d) * g.inv;
+  const float term = p > 0.0f ? p * (d - g.ls + g.h) : 0.0f;
+  return ((j == g.taken ? g.gl : 0.0f) - g.gl * p - g.ge * term) * rate;
+}
+template <int DT, int THREADS>
+__global__ __launch_bounds__(256) void pcx_log_prob_backward_kernel(LogProbArgs a) {
+  typedef typename Logit<DT>::T T;
+  constexpr int ROWS = 256 / THREADS;
+  const int t = threadIdx.x % THREADS;
+  const int64_t unit = (int64_t)blockIdx.x * ROWS + threadIdx.x / THREADS;
+  if (unit >= a.rows.n * a.slices) return;
+  const int64_t row = unit / a.slices;
+  const int slice = (int)(unit - row * a.slices);
+  const int lo = a.slices > 1 ? slice * SLICE : 0;
+  const int end = a.slices > 1 && a.rows.actions - lo > SLICE ? lo + SLICE : a.rows.actions;
+  const RowGrad g = row_grad(a, row);
+  T* const out = reinterpret_cast<T*>(a.grad) + row * a.rows.actions;
+  for (int j0 = lo + t * 4; j0 < end; j0 += THREADS * 4) {
+    uint32_t key[4];
+    load_keys<DT, 4>(a.rows, row, j0, end, key);
+    Quad<T> q;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) q.v[i] = Logit<DT>::put(element_grad(g, key[i], j0 + i, a.rate));
+    if (j0 + 4 <= end) __builtin_memcpy(out + j0, &q, sizeof q);
+    else
+      for (int i = 0; i < 4; ++i)
+        if (j0 + i < end) out[j0 + i] = q.v[i];
+  }
+}
+// Few actions: a thread holds a row.
+template <int DT, int CAP>
+__global__ __launch_bounds__(256) void pcx_log_prob_rows(LogProbArgs a) {
+  const int64_t row = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (row >= a.rows.n) return;
+  uint32_t key[CAP];
+  load_keys<DT, CAP>(a.rows, row, 0, a.rows.actions, key);
+  uint32_t top = 0;
+#pragma unroll
+  for (int i = 0; i < CAP; ++i) top = key[i] > top ? key[i] : top;
+  Soft v{-INFINITY, 0.0f, 0.0f};
+  if (top) {
+    v.m = value_of(top);
+#pragma unroll
+    for (int i = 0; i < CAP; ++i)
+      if (key[i]) {
+        const float x = value_of(key[i]);
+        const float d = x == v.m ? 0.0f : (x - v.m) * a.rate, e = exp_of(d);
+        v.s += e;
+        if (e > 0.0f) v.t = fmaf(d, e, v.t);
+      }
+  }
+  finish_row<DT>(a, row, v);
+}
+template <int DT, int CAP>
+__global__ __launch_bounds__(256) void pcx_log_prob_rows_backward(LogProbArgs a) {
+  typedef typename Logit<DT>::T T;
+  const int64_t row = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (row >= a.rows.n) return;
+  uint32_t key[CAP];
+  load_keys<DT, CAP>(a.rows, row, 0, a.rows.actions, key);
+  const RowGrad g = row_grad(a, row);
+  T* const out = reinterpret_cast<T*>(a.grad) + row * a.rows.actions;
+#pragma unroll
+  for (int i = 0; i < CAP; ++i)
+    if (i < a.rows.actions) out[i] = Logit<DT>::put(element_grad(g, key[i], i, a.rate));
+}
+
+// ---------------------------------------------------------------- plans and entry points
+
+constexpr int ROW_IN_GROUP = 16384;  // actions a workgroup holds in registers
+constexpr int WIDE_BATCH = 1024;     // rows per batch of launches beyond that
+constexpr int64_t CHUNK = 1 << 22;   // rows per launch otherwise (a grid has fewer than 2^32 threads)
+
+int check_rows(const pcx_logits_desc* d, Rows* r, const char* who) {
+  if (!d) return set_error(PCX_E_INVALID, "%s: null description", who);
+  if (d->dtype != PCX_F32 && d->dtype != PCX_F16 && d->dtype != PCX_BF16)
+    return set_error(PCX_E_INVALID, "%s: logits are float32, float16 or bfloat16", who);
+  if (d->n < 0 || d->n > (int64_t)1 << 31) return set_error(PCX_E_INVALID, "%s: %lld rows", who, (long long)d->n);
+  if (d->actions < 1 || d->actions > 1 << 24) return set_error(PCX_E_INVALID, "%s: %d actions", who, d->actions);
+  if (d->row_stride < 0 || d->legal_stride < 0) return set_error(PCX_E_INVALID, "%s: negative stride", who);
+  r->n = d->n; r->row_stride = d->row_stride; r->legal_stride = d->legal_stride; r->actions = d->actions;
+  return 0;
+}
+bool misaligned(const void* p, uintptr_t to) { return (reinterpret_cast<uintptr_t>(p) & (to - 1)) != 0; }
+int elem_size(int dtype) { return dtype == PCX_F32 ? 4 : 2; }
+
+// The rows of one launch, from row0 on.
+Rows rows_from(const Rows& all, int64_t row0, int es) {
+  Rows r = all;
+  r.n = all.n - row0 < CHUNK ? all.n - row0 : CHUNK;
+  r.logits = reinterpret_cast<const uint8_t*>(all.logits) + row0 * all.row_stride * es;
+  if (all.legal) r.legal = all.legal + row0 * all.legal_stride;
+  return r;
+}
+
+int wide_slices(int actions) { return (actions + SLICE - 1) / SLICE; }
+uint64_t wide_bytes(int64_t n, int actions) {
+  if (actions <= ROW_IN_GROUP) return 0;
+  const uint64_t rows = (uint64_t)(n < WIDE_BATCH ? n : WIDE_BATCH);
+  return rows * (sizeof(RowState) + 2ull * BINS * 12 + (uint64_t)wide_slices(actions) * sizeof(Slot)) + 1024;
+}
+// A row of logits is divided among workgroups where there are too few rows to fill the chip.
+int log_prob_slices(int64_t n, int actions) { return actions > 2 * SLICE && n < 2048 ? wide_slices(actions) : 1; }
+
+template <int DT>
+int sample_wide(const SampleArgs& a, void* workspace, hipStream_t st) {
+  const int slices = wide_slices(a.rows.actions);
+  int log2a = 0;
+  while ((1 << log2a) < a.rows.actions) ++log2a;
+  for (int64_t row0 = 0; row0 < a.rows.n; row0 += WIDE_BATCH) {
+    WideArgs w{a};
+    w.row0 = row0;
+    w.batch = (int32_t)(a.rows.n - row0 < WIDE_BATCH ? a.rows.n - row0 : WIDE_BATCH);
+    w.slices = slices;
+    w.scale = 62 - log2a;
+    uint8_t* p = reinterpret_cast<uint8_t*>(workspace);
+    w.mass = reinterpret_cast<uint64_t*>(p); p += (size_t)w.batch * 2 * BINS * 8;
+    w.state = reinterpret_cast<RowState*>(p); p += (size_t)w.batch * sizeof(RowState);
+    w.slots = reinterpret_cast<Slot*>(p); p += (size_t)w.batch * slices * sizeof(Slot);
+    w.count = reinterpret_cast<uint32_t*>(p);
+    const dim3 rows((unsigned)w.batch), grid((unsigned)slices, (unsigned)w.batch), block(256);
+    hipLaunchKernelGGL(pcx_sample_clear, rows, block, 0, st, w);
+    hipLaunchKernelGGL((pcx_sample_best<DT>), grid, block, 0, st, w);
+    const bool k = a.rules.top_k_row || (a.rules.top_k > 0 && a.rules.top_k < a.rows.actions);
+    const bool p_ = a.rules.top_p_row || a.rules.top_p < 1.0f;
+    if (k || p_) {
+      hipLaunchKernelGGL((pcx_sample_digit<DT>), grid, block, 0, st, w, 0, 0u);
+      for (int by_mass = k ? 0 : 1; by_mass <= (p_ ? 1 : 0); ++by_mass)
+        for (int level = 0; level < 3; ++level) {
+          if (level) hipLaunchKernelGGL((pcx_sample_digit<DT>), grid, block, 0, st, w, level, by_mass ? 4u : 2u);
+          hipLaunchKernelGGL(pcx_sample_edge, rows, block, 0, st, w, level, by_mass);
+        }
+    }
+    hipLaunchKernelGGL((pcx_sample_weigh<DT>), grid, block, 0, st, w);
+    hipLaunchKernelGGL((pcx_sample_pick<DT>), rows, block, 0, st, w);
+  }
+  return 0;
+}
+template <int DT>
+int sample_type(const SampleArgs& all, void* workspace, hipStream_t st) {
+  const int A = all.rows.actions;
+  if (A > ROW_IN_GROUP) return sample_wide<DT>(all, workspace, st);
+  for (int64_t row0 = 0; row0 < all.rows.n; row0 += CHUNK) {
+    SampleArgs a = all;
+    a.rows = rows_from(all.rows, row0, elem_size(DT));
+    a.uniforms += row0;
+    a.out += row0;
+    if (a.rules.temperature_row) a.rules.temperature_row += row0;
+    if (a.rules.top_k_row) a.rules.top_k_row += row0;
+    if (a.rules.top_p_row) a.rules.top_p_row += row0;
+    if (a.rules.min_p_row) a.rules.min_p_row += row0;
+    const dim3 block(256), per_thread((unsigned)((a.rows.n + 255) / 256)), per_wave((unsigned)((a.rows.n + 3) / 4)), per_group((unsigned)a.rows.n);
+    if (A <= 8) hipLaunchKernelGGL((pcx_sample_rows<DT, 8>), per_thread, block, 0, st, a);
+    else if (A <= 16) hipLaunchKernelGGL((pcx_sample_rows<DT, 16>), per_thread, block, 0, st, a);
+    else if (A <= 128) hipLaunchKernelGGL((pcx_sample_group<DT, 64, 2>), per_wave, block, 0, st, a);
+    else if (A <= 512) hipLaunchKernelGGL((pcx_sample_group<DT, 64, 8>), per_wave, block, 0, st, a);
+    else if (A <= 4096) hipLaunchKernelGGL((pcx_sample_group<DT, 256, 16>), per_group, block, 0, st, a);
+    else hipLaunchKernelGGL((pcx_sample_group<DT, 512, 32>), per_group, dim3(512), 0, st, a);
+  }
+  return 0;
+}
+template <int DT>
+int log_prob_type(const LogProbArgs& all, bool backward, hipStream_t st) {
+  const int A = all.rows.actions;
+  for (int64_t row0 = 0; row0 < all.rows.n; row0 += CHUNK) {
+    LogProbArgs a = all;
+    a.rows = rows_from(all.rows, row0, elem_size(DT));
+    a.taken += row0;
+    a.entropy += row0;
+    a.stats += row0;
+    if (a.log_prob) a.log_prob += row0;
+    if (a.grad_log_prob) a.grad_log_prob += row0;
+    if (a.grad_entropy) a.grad_entropy += row0;
+    if (a.grad) a.grad = reinterpret_cast<uint8_t*>(a.grad) + row0 * A * elem_size(DT);
+    const int64_t units = a.rows.n * a.slices;  // (slices > 1: few rows, one chunk)
+    const dim3 block(256), per_thread((unsigned)((a.rows.n + 255) / 256)), per_wave((unsigned)((units + 3) / 4)), per_group((unsigned)units);
+    if (!backward) {
+      if (A <= 8) hipLaunchKernelGGL((pcx_log_prob_rows<DT, 8>), per_thread, block, 0, st, a);
+      else if (A <= 32) hipLaunchKernelGGL((pcx_log_prob_rows<DT, 32>), per_thread, block, 0, st, a);
+      else if (A <= 2048) hipLaunchKernelGGL((pcx_log_prob_forward<DT, 64>), per_wave, block, 0, st, a);
+      else hipLaunchKernelGGL((pcx_log_prob_forward<DT, 256>), per_group, block, 0, st, a);
+      if (a.slices > 1) hipLaunchKernelGGL((pcx_log_prob_join<DT>), dim3((unsigned)a.rows.n), dim3(64), 0, st, a);
+    } else {
+      if (A <= 8) hipLaunchKernelGGL((pcx_log_prob_rows_backward<DT, 8>), per_thread, block, 0, st, a);
+      else if (A <= 32) hipLaunchKernelGGL((pcx_log_prob_rows_backward<DT, 32>), per_thread, block, 0, st, a);
+      else if (A <= 2048) hipLaunchKernelGGL((pcx_log_prob_backward_kernel<DT, 64>), per_wave, block, 0, st, a);
+      else hipLaunchKernelGGL((pcx_log_prob_backward_kernel<DT, 256>), per_group, block, 0, st, a);
+    }
+  }
+  return 0;
+}
+
+}  // namespace
+
+extern "C" {
+
+int pcx_sample_size(const pcx_logits_desc* d, uint64_t* bytes) {
+  Rows r;
+  if (int rc = check_rows(d, &r, "pcx_sample_size")) return rc;
+  if (!bytes) return set_error(PCX_E_INVALID, "pcx_sample_size: null");
+  *bytes = wide_bytes(r.n, r.actions);
+  return 0;
+}
+
+int pcx_sample_actions(const pcx_logits_desc* d, const pcx_sampling* rules, const void* logits, const uint8_t* legal,
+                       const float* uniforms, int32_t* actions_out, void* workspace, uint64_t workspace_bytes, void* stream) {
+  SampleArgs a{};
+  if (int rc = check_rows(d, &a.rows, "pcx_sample_actions")) return rc;
+  if (!rules) return set_error(PCX_E_INVALID, "pcx_sample_actions: no rules");
+  if (!rules->temperature_row && !(rules->temperature >= 0.0f)) return set_error(PCX_E_INVALID, "pcx_sample_actions: the temperature must be 0 or more");
+  if (!rules->top_k_row && rules->top_k < 0) return set_error(PCX_E_INVALID, "pcx_sample_actions: top_k must be 0 (all) or more");
+  if (!rules->top_p_row && !(rules->top_p >= 0.0f)) return set_error(PCX_E_INVALID, "pcx_sample_actions: top_p must be 0 or more");
+  if (!rules->min_p_row && !(rules->min_p >= 0.0f && rules->min_p <= 1.0f)) return set_error(PCX_E_INVALID, "pcx_sample_actions: min_p must lie in [0, 1]");
+  if (!a.rows.n) return 0;
+  if (!logits || !uniforms || !actions_out || misaligned(logits, elem_size(d->dtype)) || misaligned(uniforms, 4) || misaligned(actions_out, 4) ||
+      misaligned(rules->temperature_row, 4) || misaligned(rules->top_k_row, 4) || misaligned(rules->top_p_row, 4) || misaligned(rules->min_p_row, 4))
+    return set_error(PCX_E_INVALID, "pcx_sample_actions: null or misaligned pointer");
+  const uint64_t need = wide_bytes(a.rows.n, a.rows.actions);
+  if (need && (!workspace || workspace_bytes < need || misaligned(workspace, 16)))
+    return set_error(PCX_E_INVALID, "pcx_sample_actions: the workspace needs %llu bytes, 16-byte aligned", (unsigned long long)need);
+  a.rows.logits = logits;
+  a.rows.legal = legal;
+  a.rules = Rules{rules->temperature, rules->top_p, rules->min_p, rules->top_k, rules->temperature_row, rules->top_k_row, rules->top_p_row, rules->min_p_row};
+  a.uniforms = uniforms;
+  a.out = actions_out;
+  hipStream_t st = (hipStream_t)stream;
+  int rc;
+  if (d->dtype == PCX_F32) rc = sample_type<PCX_F32>(a, workspace, st);
+  else if (d->dtype == PCX_F16) rc = sample_type<PCX_F16>(a, workspace, st);
+  else rc = sample_type<PCX_BF16>(a, workspace, st);
+  if (rc) return rc;
+  PCX_HIP(hipGetLastError());
+  return 0;
+}
+
+int pcx_log_prob_size(const pcx_logits_desc* d, uint64_t* bytes) {
+  Rows r;
+  if (int rc = check_rows(d, &r, "pcx_log_prob_size")) return rc;
+  if (!bytes) return set_error(PCX_E_INVALID, "pcx_log_prob_size: null");
+  const int slices = log_prob_slices(r.n, r.actions);
+  *bytes = slices > 1 ? (uint64_t)r.n * slices * sizeof(float4) : 0;
+  return 0;
+}
+
+static int log_prob_call(const pcx_logits_desc* d, float temperature, LogProbArgs* a, bool backward, void* stream, const char* who) {
+  if (!(temperature > 0.0f) || !(1.0f / temperature > 0.0f) || !(1.0f / temperature < INFINITY))
+    return set_error(PCX_E_INVALID, "%s: the temperature must be a positive number", who);
+  if (misaligned(a->rows.logits, elem_size(d->dtype)) || misaligned(a->taken, 4) || misaligned(a->log_prob, 4) || misaligned(a->entropy, 4) ||
+      misaligned(a->stats, 8) || misaligned(a->grad_log_prob, 4) || misaligned(a->grad_entropy, 4) || misaligned(a->grad, elem_size(d->dtype)))
+    return set_error(PCX_E_INVALID, "%s: misaligned pointer", who);
+  a->rate = 1.0f / temperature;
+  hipStream_t st = (hipStream_t)stream;
+  int rc;
+  if (d->dtype == PCX_F32) rc = log_prob_type<PCX_F32>(*a, backward, st);
+  else if (d->dtype == PCX_F16) rc = log_prob_type<PCX_F16>(*a, backward, st);
+  else rc = log_prob_type<PCX_BF16>(*a, backward, st);
+  if (rc) return rc;
+  PCX_HIP(hipGetLastError());
+  return 0;
+}
+
+int pcx_log_prob(const pcx_logits_desc* d, float temperature, const void* logits, const uint8_t* legal, const int32_t* actions,
+                 float* log_prob, float* entropy, float* stats, void* workspace, uint64_t workspace_bytes, void* stream) {
+  LogProbArgs a{};
+  if (int rc = check_rows(d, &a.rows, "pcx_log_prob")) return rc;
+  if (!a.rows.n) return 0;
+  if (!logits || !actions || !log_prob || !entropy || !stats) return set_error(PCX_E_INVALID, "pcx_log_prob: null pointer");
+  a.slices = log_prob_slices(a.rows.n, a.rows.actions);
+  const uint64_t need = a.slices > 1 ? (uint64_t)a.rows.n * a.slices * sizeof(float4) : 0;
+  if (need && (!workspace || workspace_bytes < need || misaligned(workspace, 16)))
+    return set_error(PCX_E_INVALID, "pcx_log_prob: the workspace needs %llu bytes, 16-byte aligned", (unsigned long long)need);
+  a.rows.logits = logits;
+  a.rows.legal = legal;
+  a.taken = actions;
+  a.log_prob = log_prob;
+  a.entropy = entropy;
+  a.stats = reinterpret_cast<float2*>(stats);
+  a.partial = reinterpret_cast<float4*>(workspace);
+  return log_prob_call(d, temperature, &a, false, stream, "pcx_log_prob");
+}
+
+int pcx_log_prob_backward(const pcx_logits_desc* d, float temperature, const void* logits, const uint8_t* legal, const int32_t* actions,
+                          const float* entropy, const float* stats, const float* grad_log_prob, const float* grad_entropy,
+                          void* grad_logits, void* stream) {
+  LogProbArgs a{};
+  if (int rc = check_rows(d, &a.rows, "pcx_log_prob_backward")) return rc;
+  if (!a.rows.n) return 0;
+  if (!logits || !actions || !entropy || !stats || !grad_logits) return set_error(PCX_E_INVALID, "pcx_log_prob_backward: null pointer");
+  a.slices = log_prob_slices(a.rows.n, a.rows.actions);
+  a.rows.logits = logits;
+  a.rows.legal = legal;
+  a.taken = actions;
+  a.entropy = const_cast<float*>(entropy);
+  a.stats = reinterpret_cast<float2*>(const_cast<float*>(stats));
+  a.grad_log_prob = grad_log_prob;
+  a.grad_entropy = grad_entropy;
+  a.grad = grad_logits;
+  return log_prob_call(d, temperature, &a, true, stream, "pcx_log_prob_backward");
+}
+
+}  // extern "C"

@@ -859,7 +859,7 @@ int pcx_project_forward(const pcx_project_desc* d, const uint8_t* boards, const 
                 p.splits, p.mblocks, p.nblocks, 0, 0};
   a.wide = s.hidden % 4 == 0 && !misaligned(out, 4 * es) && !misaligned(residual, 4 * es) && !misaligned(slope, 4 * es);
   const int64_t groups = (int64_t)p.mblocks * p.nblocks * p.splits;
-  if (groups > (int64_t)1 << 30) return set_error(PCX_E_INVALID, "pcx_project_forward: too many boards for one call");
+  if (groups >= (int64_t)1 << 23) return set_error(PCX_E_INVALID, "pcx_project_forward: too many boards for one call");
   a.chunk = (int32_t)((groups + 7) / 8);
   const unsigned grid = (unsigned)a.chunk * 8u;
   hipStream_t st = (hipStream_t)stream;
@@ -884,6 +884,7 @@ int pcx_project_backward(const pcx_project_desc* d, const uint8_t* boards, const
     return set_error(PCX_E_INVALID, "pcx_project_backward: null or misaligned pointer");
   if (s.activation != PCX_ACT_NONE && !slope) return set_error(PCX_E_INVALID, "pcx_project_backward: the activation's slopes are missing");
   const BackwardPlan p = plan_backward(s);
+  if ((int64_t)p.hblocks * p.cell_blocks * p.layer_blocks * p.splits >= (int64_t)1 << 23) return set_error(PCX_E_INVALID, "pcx_project_backward: the weight is too large");
   if (!workspace || workspace_bytes < p.frag_bytes + p.bias_bytes + p.part_bytes || misaligned(workspace, 16))
     return set_error(PCX_E_INVALID, "pcx_project_backward: the workspace needs %llu bytes, 16-byte aligned",
                      (unsigned long long)(p.frag_bytes + p.bias_bytes + p.part_bytes));

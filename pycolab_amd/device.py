@@ -119,3 +119,10 @@ def policy_dtype(tensor, name):
 
 def pointer(tensor):
   return None if tensor is None else tensor.data_ptr()
+
+
+def refuse_recording_in_capture(what, instead):
+  """A backward pass captured while an eager graph of the same leaves lives would run on that graph's stream and end the
+  process: differentiable calls are refused under capture, the explicit pair of calls is what a graph holds."""
+  if torch_module().cuda.is_current_stream_capturing():
+    raise RuntimeError('{}() does not record gradients while a graph is captured: capture {} instead'.format(what, instead))

@@ -421,6 +421,18 @@ class Engine(object):
         dev.current_stream(self._device_id)))
     self._steps_launched += int(steps)
 
+  def step_sampled(self, logits, uniforms, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, legal=None):
+    """One step with the actions `actions.sample()` draws from a policy's logits [batch, n_actions] and one number per
+    environment; returns them (int32 device tensor [batch]; -1, the engine's `None`, where an environment may do
+    nothing).  No host synchronisation."""
+    from pycolab_amd import actions as policy
+    self._b  # (raises after close())
+    drawn = policy.sample(logits, uniforms, temperature, top_k, top_p, min_p, legal)
+    if drawn.shape[0] != self._batch or drawn.device.index != self._device_id:
+      raise ValueError('logits must be [{}, actions] on GPU {}'.format(self._batch, self._device_id))
+    self.step(drawn)
+    return drawn
+
   def _stage_actions(self, actions):
     torch = dev.torch_module()
     if torch is not None and isinstance(actions, torch.Tensor):

@@ -884,12 +884,6 @@ def _project_autograd():
   return _project_function
 
 
-def _refuse_recording_in_capture(torch, what, instead, *leaves):
-  if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in leaves) and torch.cuda.is_current_stream_capturing():
-    raise RuntimeError('{0}() does not record gradients while a graph is captured: autograd may hand the captured backward '
-                       'pass to the stream of an earlier one, which ends the process.  Capture {1} instead.'.format(what, instead))
-
-
 def project(boards, layers, weight, bias=None, activation=None, residual=None, return_slope=False):
   """`act(features @ weight.T + bias) + residual`, differentiable in `weight`, `bias` and `residual`: one training step's
   first layer.  Arguments, shapes and types as for `ObservationProjection`, which is the form for weights that stay; this
@@ -910,7 +904,7 @@ def project(boards, layers, weight, bias=None, activation=None, residual=None, r
       out, slope = plan.forward(view, plan.pack(weight), bias, residual, want_slope=activation is not None)
       return (out[0] if view.single else out), slope
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (weight, bias, residual)):
-      _refuse_recording_in_capture(torch, 'project', 'project(..., return_slope=True) and project_backward()', weight, bias, residual)
+      dev.refuse_recording_in_capture('project', 'project(..., return_slope=True) and project_backward()')
       out = _project_autograd().apply(weight, bias, residual, plan, view)
     else:
       out, _ = plan.forward(view, plan.pack(weight), bias, residual)
