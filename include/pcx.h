@@ -647,7 +647,8 @@ typedef struct pcx_project_desc {
 int pcx_project_sizes(const pcx_project_desc* d, uint64_t* packed_bytes, uint64_t* forward_bytes, uint64_t* backward_bytes);
 /* Lays the weight out for pcx_project_forward (16-byte aligned `packed`); again after every change of the weight. */
 int pcx_project_pack(const pcx_project_desc* d, const void* weight, void* packed, void* stream);
-/* slope: NULL, or [n][hidden] that receives act'(...) for pcx_project_backward. */
+/* slope: NULL, or [n][hidden] that receives act'(...) for pcx_project_backward: of the weight's type for PCX_ACT_RELU,
+ * float32 for the others. */
 int pcx_project_forward(const pcx_project_desc* d, const uint8_t* boards, const void* packed, const void* bias,
                         const void* residual, void* out, void* slope, void* workspace, uint64_t workspace_bytes, void* stream);
 /* Gradients from grad_out [n][hidden]: grad_weight [hidden][n_layers][cells] and grad_bias [hidden] (either may be

@@ -719,11 +719,14 @@ class _Projection(object):
     if tensor is not None and (tensor.dtype != weight.dtype or tensor.device != weight.device):
       raise ValueError('{} must be {} on {}, like the weight'.format(name, weight.dtype, weight.device))
 
-  def check_rows(self, tensor, name, n):
+  def slope_dtype(self):
+    return self.torch_dtype if self.desc.activation == N.ACT_RELU else dev.torch_module().float32
+
+  def check_rows(self, tensor, name, n, dtype=None):
     if tensor is None:
       return
-    if tensor.dtype != self.torch_dtype or tensor.device != self.device or tuple(tensor.shape) != (n, self.hidden):
-      raise ValueError('{} must be {} [{}, {}] on {}'.format(name, self.torch_dtype, n, self.hidden, self.device))
+    if tensor.dtype != (dtype or self.torch_dtype) or tensor.device != self.device or tuple(tensor.shape) != (n, self.hidden):
+      raise ValueError('{} must be {} [{}, {}] on {}'.format(name, dtype or self.torch_dtype, n, self.hidden, self.device))
 
   def at(self, boards):
     """The description for these boards."""
@@ -757,7 +760,7 @@ class _Projection(object):
     d = self.at(boards)
     self.check_rows(residual, 'residual', boards.n)
     out = torch.empty((boards.n, self.hidden), dtype=self.torch_dtype, device=self.device)
-    slope = torch.empty_like(out) if want_slope else None
+    slope = torch.empty(out.shape, dtype=self.slope_dtype(), device=self.device) if want_slope else None
     scratch = self.sizes()[1]
     ws = torch.empty(scratch, dtype=torch.uint8, device=self.device) if scratch else None
     bias = None if bias is None else bias.detach().contiguous()
@@ -771,7 +774,7 @@ class _Projection(object):
     torch = dev.torch_module()
     d = self.at(boards)
     self.check_rows(grad, 'grad', boards.n)
-    self.check_rows(slope, 'slope', boards.n)
+    self.check_rows(slope, 'slope', boards.n, self.slope_dtype())
     make = torch.zeros if boards.n == 0 else torch.empty
     dw = make(weight_shape, dtype=self.torch_dtype, device=self.device) if want_weight else None
     db = make((self.hidden,), dtype=self.torch_dtype, device=self.device) if want_bias else None
@@ -915,6 +918,7 @@ def project_backward(boards, layers, weight, grad, slope=None):
   """(grad_weight, grad_bias) of `project()` for the gradient `grad` [n, hidden] of its result; `slope` as it returned it.
   The residual's gradient is `grad`.  Records nothing for autograd and waits for nothing: it may be captured."""
   torch = dev.require_torch('project_backward()')
-  plan = _Projection(layers, weight, None, None if slope is None else 'relu')  # (which activation it was is in the slopes)
+  # (which activation it was is in the slopes: relu's have the weight's type, the others' are float32)
+  plan = _Projection(layers, weight, None, None if slope is None else 'relu' if slope.dtype == weight.dtype else 'silu')
   with torch.cuda.device(plan.device):
     return plan.backward(_Boards(boards, layers), grad.detach(), slope, True, True, weight.shape)
