@@ -17,6 +17,8 @@
 // passes and no accuracy.  All sums are float32.
 #include "pcx_project.h"
 
+#include <type_traits>
+
 namespace pcx {
 namespace project {
 
@@ -61,16 +63,17 @@ constexpr int FRAG = 2048;       // bytes of one right operand: 32 features x 32
 // What a sum of the matrix unit is multiplied by: a feature is 2, and all weights but float16 ones are laid out halved.
 template <int DT> constexpr float SCALE = DT == PCX_F16 ? 0.5f : 1.0f;
 
-__device__ __forceinline__ void activate(int act, float z, float* y, float* slope) {
-  if (act == PCX_ACT_RELU) {
-    *y = z > 0.0f ? z : (z != z ? z : 0.0f); *slope = z > 0.0f ? 1.0f : 0.0f;
-  } else if (act == PCX_ACT_SILU) {
+template <int ACT>
+__device__ __forceinline__ void activate(float z, float* y, float* slope) {
+  if constexpr (ACT == PCX_ACT_RELU) {
+    *y = z < 0.0f ? 0.0f : z; *slope = z > 0.0f ? 1.0f : 0.0f;  // (a NaN stays one)
+  } else if constexpr (ACT == PCX_ACT_SILU) {
     const float s = 1.0f / (1.0f + expf(-z));
     *y = z * s; *slope = s * (1.0f + z * (1.0f - s));
-  } else if (act == PCX_ACT_TANH) {
+  } else if constexpr (ACT == PCX_ACT_TANH) {
     const float t = tanhf(z);
     *y = t; *slope = 1.0f - t * t;
-  } else if (act == PCX_ACT_GELU) {
+  } else if constexpr (ACT == PCX_ACT_GELU) {
     const float cdf = 0.5f * (1.0f + erff(z * 0.70710678118654752f));
     *y = z * cdf; *slope = cdf + z * expf(-0.5f * z * z) * 0.3989422804014327f;
   } else {
@@ -147,50 +150,59 @@ __device__ __forceinline__ f32x16 sparse_step(u32x4 a, u32x8 b, f32x16 c, int in
     return __builtin_amdgcn_smfmac_f32_32x32x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x16, b), c, index, 0, 0);
 }
 
-// Bias, activation and residual on up to four neighbouring sums of one board (count < 4 at the last columns; `wide`: the
-// rows keep four elements aligned).
-template <int DT>
-__device__ __forceinline__ void finish(const ForwardArgs& a, int64_t row, int col, const float* sum, int count, bool wide) {
+// Four neighbouring elements of a row.
+template <typename T> struct __align__(4 * sizeof(T)) Four { T v[4]; };
+template <typename T>
+__device__ __forceinline__ Four<T> load_four(const T* from, int count, bool wide) {
+  Four<T> f = {};
+  if (wide) return *reinterpret_cast<const Four<T>*>(from);
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if (i < count) f.v[i] = from[i];
+  return f;
+}
+template <typename T>
+__device__ __forceinline__ void store_four(T* to, Four<T> f, int count, bool wide) {
+  if (wide) { *reinterpret_cast<Four<T>*>(to) = f; return; }
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if (i < count) to[i] = f.v[i];
+}
+// Bias, activation and residual on up to four neighbouring sums of one board, `at` elements into out (count < 4 at the last
+// columns; a.wide: the rows keep four elements aligned).
+template <int DT, int ACT>
+__device__ __forceinline__ void finish(const ForwardArgs& a, int64_t at, const float* sum, Four<typename Num<DT>::T> bias,
+                                       Four<typename Num<DT>::T> res, int count) {
   typedef typename Num<DT>::T T;
-  struct __align__(4 * sizeof(T)) Four { T v[4]; };
-  const int64_t at = row * a.s.hidden + col;
-  Four bias = {}, res = {}, out;
+  Four<T> out;
   float slope[4];
-  const T* const pb = reinterpret_cast<const T*>(a.bias);
-  const T* const pr = reinterpret_cast<const T*>(a.residual);
-  T* const po = reinterpret_cast<T*>(a.out);
-  if (pb)
-    for (int i = 0; i < count; ++i) bias.v[i] = pb[col + i];
-  if (pr) {
-    if (wide) res = *reinterpret_cast<const Four*>(pr + at);
-    else
-      for (int i = 0; i < count; ++i) res.v[i] = pr[at + i];
-  }
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     float y;
-    activate(a.s.activation, sum[i] + (pb ? Num<DT>::get(bias.v[i]) : 0.0f), &y, &slope[i]);
-    if (pr) y += Num<DT>::get(res.v[i]);
-    out.v[i] = Num<DT>::put(y);
+    activate<ACT>(sum[i] + Num<DT>::get(bias.v[i]), &y, &slope[i]);
+    out.v[i] = Num<DT>::put(a.residual ? y + Num<DT>::get(res.v[i]) : y);
   }
-  if (wide) *reinterpret_cast<Four*>(po + at) = out;
-  else
-    for (int i = 0; i < count; ++i) po[at + i] = out.v[i];
+  store_four(reinterpret_cast<T*>(a.out) + at, out, count, a.wide);
   if (!a.slope) return;
   // relu's slopes are 0 and 1 in any type; the others keep float32, so that the gradients lose nothing but their own rounding
-  if (a.s.activation == PCX_ACT_RELU) {
-    T* const ps = reinterpret_cast<T*>(a.slope);
-    Four k;
+  if constexpr (ACT == PCX_ACT_RELU) {
+    Four<T> k;
 #pragma unroll
     for (int i = 0; i < 4; ++i) k.v[i] = Num<DT>::put(slope[i]);
-    if (wide) *reinterpret_cast<Four*>(ps + at) = k;
-    else
-      for (int i = 0; i < count; ++i) ps[at + i] = k.v[i];
+    store_four(reinterpret_cast<T*>(a.slope) + at, k, count, a.wide);
   } else {
-    float* const ps = reinterpret_cast<float*>(a.slope);
-    if (wide) *reinterpret_cast<float4*>(ps + at) = make_float4(slope[0], slope[1], slope[2], slope[3]);
-    else
-      for (int i = 0; i < count; ++i) ps[at + i] = slope[i];
+    store_four(reinterpret_cast<float*>(a.slope) + at, Four<float>{{slope[0], slope[1], slope[2], slope[3]}}, count, a.wide);
+  }
+}
+// f with the activation as a constant
+template <typename F>
+__device__ __forceinline__ void by_activation(int act, F f) {
+  switch (act) {
+    case PCX_ACT_RELU: f(std::integral_constant<int, PCX_ACT_RELU>()); break;
+    case PCX_ACT_SILU: f(std::integral_constant<int, PCX_ACT_SILU>()); break;
+    case PCX_ACT_TANH: f(std::integral_constant<int, PCX_ACT_TANH>()); break;
+    case PCX_ACT_GELU: f(std::integral_constant<int, PCX_ACT_GELU>()); break;
+    default: f(std::integral_constant<int, PCX_ACT_NONE>()); break;
   }
 }
 
@@ -209,8 +221,8 @@ __global__ __launch_bounds__(256, 2) void pcx_project_forward_kernel(ForwardArgs
   constexpr int PIECES = STAGE / 1024;        // 1 KB copies per stage
   constexpr int MROWS = (4 / WN) * MT * 32;
   const Shape& s = a.s;
+  __shared__ uint32_t lut[256];
   extern __shared__ __align__(16) uint8_t lds[];
-  uint32_t* const lut = reinterpret_cast<uint32_t*>(lds + 2 * STAGE);
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   // consecutive tiles of a board block go to one XCD (workgroup i runs on XCD i % 8), whose L2 then serves the boards once
   const uint32_t id = (blockIdx.x & 7u) * (uint32_t)a.chunk + (blockIdx.x >> 3);
@@ -219,21 +231,15 @@ __global__ __launch_bounds__(256, 2) void pcx_project_forward_kernel(ForwardArgs
   const uint32_t rest = id / (uint32_t)a.nblocks;
   const int split = (int)(rest % (uint32_t)a.splits), mb = (int)(rest / (uint32_t)a.splits);
   const int blocks = STACKED ? 1 : (s.groups + 3) / 4;
-  if constexpr (!STACKED) {
-    // Per block and character: bits 0..3 and again 4..7 the positions of the two slots of a group -- they ascend: (p, 3) with
-    // the feature in the low slot for p < 3, (0, 3) with it in the high one for 3 -- and bit 14 - g (30 - g) a feature of
-    // group g in its low (high) slot.
-    for (int b = 0; b < blocks; ++b) {
-      uint32_t v = 0x44u;  // (0, 1), none
-      for (int l = b * 16; l < s.layers && l < b * 16 + 16; ++l)
-        if (s.chars[l] == tid) {
-          const int p = l & 3, g = (l >> 2) & 3;
-          v = p < 3 ? (0x4000u >> g) | (uint32_t)((p | 12) * 0x11) : (0x40000000u >> g) | 0xCCu;
-        }
-      lut[b * 256 + tid] = v;
-    }
+  // A block's table by character: bits 0..3 and again 4..7 the positions of the two slots of a group -- they ascend: (p, 3)
+  // with the feature in the low slot for p < 3, (0, 3) with it in the high one for 3 -- and bit 14 - g (30 - g) a feature of
+  // group g in its low (high) slot.
+  auto write_table = [&](int b) {  // (the caller has the workgroup's barriers around it)
+    lut[tid] = 0x44u;  // (0, 1), none
     __syncthreads();
-  }
+    const int l = b * 16 + tid, p = l & 3, g = (l >> 2) & 3;
+    if (tid < 16 && l < s.layers) lut[s.chars[l]] = p < 3 ? (0x4000u >> g) | (uint32_t)((p | 12) * 0x11) : (0x40000000u >> g) | 0xCCu;
+  };
   // the run of (block, quad) units of this split
   const int units = blocks * s.quads;
   const int u0 = (int)((int64_t)units * split / a.splits), u1 = (int)((int64_t)units * (split + 1) / a.splits);
@@ -265,13 +271,19 @@ __global__ __launch_bounds__(256, 2) void pcx_project_forward_kernel(ForwardArgs
       for (int i = 0; i < 16; ++i) acc[m][t][i] = 0.0f;
   u32x4 left[MT];
   int index[MT];
-  // one matrix step: step k of the stage at `base`
+  // One matrix step: step k of the stage at `base`.  The right operands are read one ahead, the first of a stage in
+  // front of it.
+  u32x8 ahead;
+  auto read_right = [&](const uint8_t* base, int i) {
+    const uint8_t* const at = base + ((i / NT) * FR + i % NT) * FRAG;
+    const u32x4 b0 = *reinterpret_cast<const u32x4*>(at), b1 = *reinterpret_cast<const u32x4*>(at + 1024);
+    ahead = u32x8{b0[0], b0[1], b0[2], b0[3], b1[0], b1[1], b1[2], b1[3]};
+  };
   auto multiply = [&](const uint8_t* base, int k) {
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
-      const uint8_t* const at = base + (k * FR + t) * FRAG;
-      const u32x4 b0 = *reinterpret_cast<const u32x4*>(at), b1 = *reinterpret_cast<const u32x4*>(at + 1024);
-      const u32x8 right = {b0[0], b0[1], b0[2], b0[3], b1[0], b1[1], b1[2], b1[3]};
+      const u32x8 right = ahead;
+      if (k * NT + t + 1 < STEPS * NT) read_right(base, k * NT + t + 1);
 #pragma unroll
       for (int m = 0; m < MT; ++m) acc[m][t] = sparse_step<DT == PCX_F16>(left[m], right, acc[m][t], index[m]);
     }
@@ -326,6 +338,7 @@ __global__ __launch_bounds__(256, 2) void pcx_project_forward_kernel(ForwardArgs
             else if (q + 1 < u1) fetch(q + 1, 0);
           }
           const uint8_t* const base = stage_base(st);
+          read_right(base, 0);
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
 #pragma unroll
@@ -349,9 +362,15 @@ __global__ __launch_bounds__(256, 2) void pcx_project_forward_kernel(ForwardArgs
       for (int m = 0; m < MT; ++m) nxt[m] = load16(row[m], c);
     };
     fetch(u0);
+    write_table(u0 < s.quads ? 0 : 1);
+    __syncthreads();
 #pragma unroll 1
     for (int u = u0; u < u1; ++u) {
-      const uint8_t* const table = reinterpret_cast<const uint8_t*>(lut) + (u < s.quads ? 0 : 1024);
+      if (u == s.quads && u > u0) {  // (the second block of a stack of more than 16 layers)
+        __syncthreads();
+        write_table(1);
+        __syncthreads();
+      }
 #pragma unroll
       for (int m = 0; m < MT; ++m) cur[m] = nxt[m];
       uint32_t word[MT][4];  // the cells' feature bits
@@ -361,11 +380,12 @@ __global__ __launch_bounds__(256, 2) void pcx_project_forward_kernel(ForwardArgs
           stage_barrier();
           if (st + 1 < stages) stage_in(st + 1);
           if (j == 0 && u + 1 < u1) fetch(u + 1);
+          read_right(stage_base(st), 0);
         }
 #pragma unroll
         for (int m = 0; m < MT; ++m) {
 #pragma unroll
-          for (int c = 0; c < 4; ++c) word[m][c] = *reinterpret_cast<const uint32_t*>(table + ((cur[m][j] >> (8 * c)) & 255u) * 4);
+          for (int c = 0; c < 4; ++c) word[m][c] = lut[(cur[m][j] >> (8 * c)) & 255u];
           const uint32_t lo = (word[m][0] & 0x0Fu) | (word[m][1] & 0xF0u), hi = (word[m][2] & 0x0Fu) | (word[m][3] & 0xF0u);
           index[m] = (int)(lo | hi << 8);
         }
@@ -374,6 +394,7 @@ __global__ __launch_bounds__(256, 2) void pcx_project_forward_kernel(ForwardArgs
           if (part && part % PS == 0) {
             stage_barrier();
             if (st + 1 < stages) stage_in(st + 1);
+            read_right(stage_base(st), 0);
           }
           const uint8_t* const base = stage_base(st);
 #pragma unroll
@@ -390,33 +411,58 @@ __global__ __launch_bounds__(256, 2) void pcx_project_forward_kernel(ForwardArgs
     }
   }
   // Out through LDS, 32 boards at a time and each wave by itself: a lane then has four neighbouring hidden units of one
-  // board, and a wave writes whole rows of its tile.
-  constexpr int PITCH = NT * 32 + 4, LANES = NT * 8;  // lanes per row
+  // board, and a wave writes whole rows of its tile.  The residual's rows are on their way one tile ahead and wait in LDS
+  // too (loaded where they are used, every row cost its own trip to memory: 583 us against 340 for 262,144 boards).
+  typedef typename Num<DT>::T T;
+  constexpr int PITCH = NT * 32 + 4, LANES = NT * 8, ROUNDS = 32 * LANES / 64;  // lanes per row, rows per lane
   __syncthreads();
   float* const mine = reinterpret_cast<float*>(lds) + wave * 32 * PITCH;
+  Four<T>* const kept = reinterpret_cast<Four<T>*>(lds + 4 * 32 * PITCH * 4) + wave * ROUNDS * 64 + lane;
   const int col0 = (tile0 + wn * NT) * 32 + (lane % LANES) * 4;
-  const int count = a.s.hidden - col0 < 4 ? a.s.hidden - col0 : 4;
+  const int count = s.hidden - col0 < 4 ? s.hidden - col0 : 4;
+  const bool whole = a.splits == 1;
+  const T* const residual = whole ? reinterpret_cast<const T*>(a.residual) : nullptr;
+  Four<T> bias = {}, res[ROUNDS] = {};
+  if (whole && a.bias && count > 0) bias = load_four(reinterpret_cast<const T*>(a.bias) + col0, count, false);
+  const T* from = residual + (row0 + lane / LANES) * s.hidden + col0;
+  auto fetch_residual = [&](int m) {
+    if (!residual || count <= 0) return;
+#pragma unroll
+    for (int i = 0; i < ROUNDS; ++i) {
+      const int64_t board = row0 + m * 32 + i * (64 / LANES) + lane / LANES;
+      if (board < s.n) res[i] = load_four(from, count, a.wide);
+      from += (64 / LANES) * s.hidden;
+    }
+  };
+  fetch_residual(0);
 #pragma unroll
   for (int m = 0; m < MT; ++m) {
 #pragma unroll
     for (int t = 0; t < NT; ++t)
 #pragma unroll
       for (int i = 0; i < 16; ++i) mine[(8 * (i >> 2) + 4 * half + (i & 3)) * PITCH + t * 32 + (lane & 31)] = SCALE<DT> * acc[m][t][i];
+#pragma unroll
+    for (int i = 0; i < ROUNDS; ++i) kept[i * 64] = res[i];
+    if (m + 1 < MT) fetch_residual(m + 1);
     __builtin_amdgcn_wave_barrier();
+    const int64_t first = row0 + m * 32 + lane / LANES;
+    const int rows = count <= 0 ? 0 : s.n - first < 32 ? (int)(s.n - first) : 32;  // (from this lane's first row on)
+    if (whole) {
+      by_activation(s.activation, [&](auto act) {
+        int64_t at = first * s.hidden + col0;
 #pragma unroll 1
-    for (int r0 = 0; r0 < 32; r0 += 64 / LANES) {
-      const int r = r0 + lane / LANES;
-      const int64_t board = row0 + m * 32 + r;
-      const float4 v = *reinterpret_cast<const float4*>(mine + r * PITCH + (lane % LANES) * 4);
-      const float sum[4] = {v.x, v.y, v.z, v.w};
-      if (board >= s.n || count <= 0) continue;
-      if (a.splits > 1) {
-        float* const to = a.partial + ((int64_t)split * s.n + board) * s.hidden + col0;
-        if (a.wide) *reinterpret_cast<float4*>(to) = v;
-        else
-          for (int i = 0; i < count; ++i) to[i] = sum[i];
-      } else {
-        finish<DT>(a, board, col0, sum, count, a.wide);
+        for (int i = 0; i < ROUNDS; ++i, at += (64 / LANES) * s.hidden) {
+          const float4 v = *reinterpret_cast<const float4*>(mine + (i * (64 / LANES) + lane / LANES) * PITCH + (lane % LANES) * 4);
+          const float sum[4] = {v.x, v.y, v.z, v.w};
+          if (i * (64 / LANES) < rows) finish<DT, decltype(act)::value>(a, at, sum, bias, kept[i * 64], count);
+        }
+      });
+    } else {
+      float* to = a.partial + ((int64_t)split * s.n + first) * s.hidden + col0;
+#pragma unroll 1
+      for (int i = 0; i < ROUNDS; ++i, to += (64 / LANES) * s.hidden) {
+        const float4 v = *reinterpret_cast<const float4*>(mine + (i * (64 / LANES) + lane / LANES) * PITCH + (lane % LANES) * 4);
+        if (i * (64 / LANES) < rows) store_four(to, Four<float>{{v.x, v.y, v.z, v.w}}, count, a.wide);
       }
     }
     __builtin_amdgcn_wave_barrier();
@@ -426,37 +472,40 @@ __global__ __launch_bounds__(256, 2) void pcx_project_forward_kernel(ForwardArgs
 // The cells' partial sums joined in a fixed order, and the epilogue.
 template <int DT>
 __global__ __launch_bounds__(256) void pcx_project_join(ForwardArgs a) {
+  typedef typename Num<DT>::T T;
   const int quads = (a.s.hidden + 3) / 4;
   const int64_t total = a.s.n * quads, plane = a.s.n * a.s.hidden;
   for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
     const int64_t row = i / quads;
     const int col = (int)(i - row * quads) * 4, count = a.s.hidden - col < 4 ? a.s.hidden - col : 4;
     const float* from = a.partial + row * a.s.hidden + col;
+    Four<T> bias = {}, res = {};
+    if (a.bias) bias = load_four(reinterpret_cast<const T*>(a.bias) + col, count, false);
+    if (a.residual) res = load_four(reinterpret_cast<const T*>(a.residual) + row * a.s.hidden + col, count, a.wide);
     float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 8
     for (int k = 0; k < a.splits; ++k, from += plane) {
-      if (a.wide) {
-        const float4 v = *reinterpret_cast<const float4*>(from);
-        sum[0] += v.x; sum[1] += v.y; sum[2] += v.z; sum[3] += v.w;
-      } else {
-        for (int c = 0; c < count; ++c) sum[c] += from[c];
-      }
+      const Four<float> v = load_four(from, count, a.wide);
+#pragma unroll
+      for (int c = 0; c < 4; ++c) sum[c] += v.v[c];
     }
-    finish<DT>(a, row, col, sum, count, a.wide);
+    by_activation(a.s.activation, [&](auto act) { finish<DT, decltype(act)::value>(a, row * a.s.hidden + col, sum, bias, res, count); });
   }
 }
 
 // ---------------------------------------------------------------- plan
 
-struct ForwardPlan { int mt, wn, mblocks, nblocks, splits; uint64_t bytes; };
+struct ForwardPlan { int mt, nt, wn, mblocks, nblocks, splits; uint64_t bytes; };
 
 ForwardPlan plan_forward(const Shape& s) {
   ForwardPlan p;
   // 4 x 2 tiles a wave make the most of a weight in LDS and of an expanded board; fewer boards than that fills the chip
   // with get smaller tiles before the cells are divided
-  p.wn = s.tiles >= 3 ? 2 : 1;
   p.mt = 4;
-  if (s.n <= 512) { p.mt = 1; p.wn = 4; }
-  const int rows = (4 / p.wn) * p.mt * 32, cols = (p.mt == 1 ? 1 : 2) * p.wn;
+  p.nt = 2;
+  p.wn = s.tiles >= 3 ? 2 : 1;
+  if (s.n <= 512) { p.mt = 1; p.nt = 1; p.wn = 4; }
+  const int rows = (4 / p.wn) * p.mt * 32, cols = p.nt * p.wn;
   p.mblocks = (int)((s.n + rows - 1) / rows);
   p.nblocks = (s.tiles + cols - 1) / cols;
   const int64_t groups = (int64_t)p.mblocks * p.nblocks;
@@ -471,10 +520,10 @@ template <int DT, int G, int MT, int NT, int WN>
 int forward_go(const ForwardArgs& a, unsigned grid, hipStream_t st) {
   constexpr int PARTS = DT == PCX_F32 ? 3 : 1;
   constexpr int STEPS = G == 0 ? 4 : PARTS == 1 ? (G == 3 ? 3 : 4) : (G == 1 ? 3 : G);
-  constexpr int ROWS_OUT = 4 * 32 * (NT * 32 + 4) * 4, STAGES = 2 * STEPS * NT * WN * FRAG + 2048;
+  constexpr int ROWS_OUT = 4 * 32 * (NT * 32 + 4) * 4 + 4 * 32 * NT * 32 * (DT == PCX_F32 ? 4 : 2), STAGES = 2 * STEPS * NT * WN * FRAG;
   constexpr int LDS = ROWS_OUT > STAGES ? ROWS_OUT : STAGES;
   auto* const kernel = &pcx_project_forward_kernel<DT, G, MT, NT, WN>;
-  if (LDS > 65536) PCX_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, LDS));
+  if (LDS + 1024 > 65536) PCX_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, LDS));
   hipLaunchKernelGGL(kernel, dim3(grid), dim3(256), LDS, st, a);
   return 0;
 }

@@ -148,10 +148,9 @@ __global__ __launch_bounds__(256, 2) void pcx_project_weight_grad(BackwardArgs a
   const int lb = (int)(t % (uint32_t)a.layer_blocks), cb = (int)(t / (uint32_t)a.layer_blocks);
   const int l0 = lb * 8, c0 = quad_start(cb, s.cells);
   if constexpr (!STACKED) {
-    uint32_t v = 0;
-    for (int l = 0; l < 8; ++l)
-      if (l0 + l < s.layers && s.chars[l0 + l] == tid) v = 128u << l;
-    lut[tid] = (uint16_t)v;
+    lut[tid] = 0;
+    __syncthreads();
+    if (tid < 8 && l0 + tid < s.layers) lut[s.chars[l0 + tid]] = (uint16_t)(128u << tid);
   }
   const int b0 = (int)((int64_t)a.blocks * split / a.splits), b1 = (int)((int64_t)a.blocks * (split + 1) / a.splits);
   const uint8_t* const src = a.frags + (int64_t)hb * NH * PARTS * 1024 + lane * 16;
