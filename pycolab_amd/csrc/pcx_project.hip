@@ -137,6 +137,10 @@ struct ForwardArgs {
   int32_t wide;          // hidden is a multiple of four and every array aligned for it
 };
 
+// How many octets of a quad a stage holds: as many as leave two workgroups of four waves a CU, or one of eight.
+constexpr int octets_per_stage(int parts, int groups, int waves) {
+  return parts > 1 ? 1 : groups == 1 ? 4 : groups == 2 ? (waves == 8 ? 4 : 2) : groups == 4 && waves == 8 ? 2 : 1;
+}
 // bit 6 of every byte that is not zero
 __device__ __forceinline__ uint32_t set_bytes(uint32_t b) {
   return (((((b & 0x7F7F7F7Fu) + 0x7F7F7F7Fu) | b) >> 1) & 0x40404040u);
@@ -206,22 +210,23 @@ __device__ __forceinline__ void by_activation(int act, F f) {
   }
 }
 
-// A wave holds MT x NT tiles of 32 x 32 sums; 4 / WN waves lie along the boards and WN along the hidden units.  G: groups of
+// A wave holds MT x NT tiles of 32 x 32 sums; WM waves lie along the boards and WN along the hidden units.  G: groups of
 // a block of characters (1..4), 0: stacked layers.  The weights of a stage are copied into LDS one stage ahead, the boards'
 // bytes into registers one quad ahead; a workgroup's waves share the weights, each wave expands its own boards.
-template <int DT, int G, int MT, int NT, int WN>
-__global__ __launch_bounds__(256, 2) void pcx_project_forward_kernel(ForwardArgs a) {
+template <int DT, int G, int MT, int NT, int WM, int WN>
+__global__ __launch_bounds__(64 * WM * WN, 2) void pcx_project_forward_kernel(ForwardArgs a) {
   constexpr bool STACKED = G == 0;
   constexpr int PARTS = DT == PCX_F32 ? 3 : 1;
   constexpr int FR = NT * WN;                                                              // right operands per step
-  constexpr int OCT = STACKED ? 4 : PARTS == 1 ? (G == 1 ? 4 : G == 2 ? 2 : 1) : 1;        // octets per stage
+  constexpr int WAVES = WM * WN;
+  constexpr int OCT = STACKED ? 4 : octets_per_stage(PARTS, G, WAVES);                     // octets per stage
   constexpr int PS = !STACKED && PARTS == 3 && G == 1 ? 3 : 1;                             // parts per stage
   constexpr int STEPS = STACKED ? 4 : OCT * PS * G;                                        // matrix steps per stage
   constexpr int STAGE = STEPS * FR * FRAG;
   constexpr int PIECES = STAGE / 1024;        // 1 KB copies per stage
-  constexpr int MROWS = (4 / WN) * MT * 32;
+  constexpr int MROWS = WM * MT * 32;
   const Shape& s = a.s;
-  __shared__ uint32_t lut[256];
+  __shared__ uint32_t lut[STACKED ? 1 : 256];
   extern __shared__ __align__(16) uint8_t lds[];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   // consecutive tiles of a board block go to one XCD (workgroup i runs on XCD i % 8), whose L2 then serves the boards once
@@ -233,9 +238,10 @@ __global__ __launch_bounds__(256, 2) void pcx_project_forward_kernel(ForwardArgs
   const int blocks = STACKED ? 1 : (s.groups + 3) / 4;
   // A block's table by character: bits 0..3 and again 4..7 the positions of the two slots of a group -- they ascend: (p, 3)
   // with the feature in the low slot for p < 3, (0, 3) with it in the high one for 3 -- and bit 14 - g (30 - g) a feature of
-  // group g in its low (high) slot.
+  // group g in its low (high) slot.  (Two words a character save 6 of 21 instructions a cell quad and lose 6 % to the
+  // wider LDS reads.)
   auto write_table = [&](int b) {  // (the caller has the workgroup's barriers around it)
-    lut[tid] = 0x44u;  // (0, 1), none
+    if (tid < 256) lut[tid] = 0x44u;  // (0, 1), none
     __syncthreads();
     const int l = b * 16 + tid, p = l & 3, g = (l >> 2) & 3;
     if (tid < 16 && l < s.layers) lut[s.chars[l]] = p < 3 ? (0x4000u >> g) | (uint32_t)((p | 12) * 0x11) : (0x40000000u >> g) | 0xCCu;
@@ -257,8 +263,8 @@ __global__ __launch_bounds__(256, 2) void pcx_project_forward_kernel(ForwardArgs
   auto stage_in = [&](int st) {
     uint8_t* const dst = lds + (st & 1) * STAGE;
 #pragma unroll
-    for (int i = 0; i < (PIECES + 3) / 4; ++i) {
-      const int k = wave + 4 * i, step = k / (2 * FR), off = k % (2 * FR);  // 2 FR pieces of 1 KB to a step
+    for (int i = 0; i < (PIECES + WAVES - 1) / WAVES; ++i) {
+      const int k = wave + WAVES * i, step = k / (2 * FR), off = k % (2 * FR);  // 2 FR pieces of 1 KB to a step
       if (k < PIECES && off < 2 * live) copy_in(src + ((int64_t)(st * STEPS + step) * s.tiles) * FRAG + off * 1024, dst + k * 1024);
     }
   };
@@ -417,7 +423,7 @@ __global__ __launch_bounds__(256, 2) void pcx_project_forward_kernel(ForwardArgs
   constexpr int PITCH = NT * 32 + 4, LANES = NT * 8, ROUNDS = 32 * LANES / 64;  // lanes per row, rows per lane
   __syncthreads();
   float* const mine = reinterpret_cast<float*>(lds) + wave * 32 * PITCH;
-  Four<T>* const kept = reinterpret_cast<Four<T>*>(lds + 4 * 32 * PITCH * 4) + wave * ROUNDS * 64 + lane;
+  Four<T>* const kept = reinterpret_cast<Four<T>*>(lds + WAVES * 32 * PITCH * 4) + wave * ROUNDS * 64 + lane;
   const int col0 = (tile0 + wn * NT) * 32 + (lane % LANES) * 4;
   const int count = s.hidden - col0 < 4 ? s.hidden - col0 : 4;
   const bool whole = a.splits == 1;
@@ -495,43 +501,44 @@ __global__ __launch_bounds__(256) void pcx_project_join(ForwardArgs a) {
 
 // ---------------------------------------------------------------- plan
 
-struct ForwardPlan { int mt, nt, wn, mblocks, nblocks, splits; uint64_t bytes; };
+struct ForwardPlan { int mt, wm, wn, mblocks, nblocks, splits; uint64_t bytes; };
 
 ForwardPlan plan_forward(const Shape& s) {
   ForwardPlan p;
-  // 4 x 2 tiles a wave make the most of a weight in LDS and of an expanded board; fewer boards than that fills the chip
-  // with get smaller tiles before the cells are divided
+  // 4 x 2 tiles a wave make the most of a weight in LDS and of an expanded board.  Eight waves share a weight where the
+  // boards fill the chip with them (the weight then leaves L2 half as often); few boards take one tile a wave.
   p.mt = 4;
-  p.nt = 2;
   p.wn = s.tiles >= 3 ? 2 : 1;
-  if (s.n <= 512) { p.mt = 1; p.nt = 1; p.wn = 4; }
-  const int rows = (4 / p.wn) * p.mt * 32, cols = p.nt * p.wn;
+  p.wm = p.wn == 2 && s.n * ((s.tiles + 3) / 4) >= 512 * 192 ? 4 : 4 / p.wn;
+  if (s.n <= 512) { p.mt = 1; p.wm = 1; p.wn = 4; }
+  const int rows = p.wm * p.mt * 32, cols = (p.mt == 1 ? 1 : 2) * p.wn;
   p.mblocks = (int)((s.n + rows - 1) / rows);
   p.nblocks = (s.tiles + cols - 1) / cols;
   const int64_t groups = (int64_t)p.mblocks * p.nblocks;
-  int64_t splits = groups >= SLOTS / 2 ? 1 : SLOTS / groups;
+  int64_t splits = groups >= SLOTS / 2 || p.wm * p.wn == 8 ? 1 : SLOTS / groups;
   if (splits > s.quads) splits = s.quads;
   p.splits = (int)splits;
   p.bytes = splits > 1 ? (uint64_t)splits * s.n * s.hidden * 4 : 0;
   return p;
 }
 
-template <int DT, int G, int MT, int NT, int WN>
+template <int DT, int G, int MT, int NT, int WM, int WN>
 int forward_go(const ForwardArgs& a, unsigned grid, hipStream_t st) {
-  constexpr int PARTS = DT == PCX_F32 ? 3 : 1;
-  constexpr int STEPS = G == 0 ? 4 : PARTS == 1 ? (G == 3 ? 3 : 4) : (G == 1 ? 3 : G);
-  constexpr int ROWS_OUT = 4 * 32 * (NT * 32 + 4) * 4 + 4 * 32 * NT * 32 * (DT == PCX_F32 ? 4 : 2), STAGES = 2 * STEPS * NT * WN * FRAG;
+  constexpr int PARTS = DT == PCX_F32 ? 3 : 1, WAVES = WM * WN;
+  constexpr int STEPS = G == 0 ? 4 : octets_per_stage(PARTS, G, WAVES) * (PARTS == 3 && G == 1 ? 3 : 1) * G;
+  constexpr int ROWS_OUT = WAVES * 32 * (NT * 32 + 4) * 4 + WAVES * 32 * NT * 32 * (DT == PCX_F32 ? 4 : 2), STAGES = 2 * STEPS * NT * WN * FRAG;
   constexpr int LDS = ROWS_OUT > STAGES ? ROWS_OUT : STAGES;
-  auto* const kernel = &pcx_project_forward_kernel<DT, G, MT, NT, WN>;
+  auto* const kernel = &pcx_project_forward_kernel<DT, G, MT, NT, WM, WN>;
   if (LDS + 1024 > 65536) PCX_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, LDS));
-  hipLaunchKernelGGL(kernel, dim3(grid), dim3(256), LDS, st, a);
+  hipLaunchKernelGGL(kernel, dim3(grid), dim3(64 * WAVES), LDS, st, a);
   return 0;
 }
 template <int DT, int G>
 int forward_shape(const ForwardArgs& a, const ForwardPlan& p, unsigned grid, hipStream_t st) {
-  if (p.mt == 1) return forward_go<DT, G, 1, 1, 4>(a, grid, st);
-  if (p.wn == 2) return forward_go<DT, G, 4, 2, 2>(a, grid, st);
-  return forward_go<DT, G, 4, 2, 1>(a, grid, st);
+  if (p.mt == 1) return forward_go<DT, G, 1, 1, 1, 4>(a, grid, st);
+  if (p.wm * p.wn == 8) return forward_go<DT, G, 4, 2, 4, 2>(a, grid, st);
+  if (p.wn == 2) return forward_go<DT, G, 4, 2, 2, 2>(a, grid, st);
+  return forward_go<DT, G, 4, 2, 4, 1>(a, grid, st);
 }
 template <int DT>
 int forward_type(const ForwardArgs& a, const ForwardPlan& p, unsigned grid, hipStream_t st) {
