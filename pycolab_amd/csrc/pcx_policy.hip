@@ -48,73 +48,185 @@ struct Rows {
   const uint8_t* legal;  // or null
 };
 
-template <typename T> struct Quad { T v[4]; };
+template <typename T, int N> struct Pack { T v[N]; };
 
-// A float as an unsigned number of the same order; 0 stands for "not allowed".  (+0 and -0 are one value.)
+// A logit as an unsigned number of the same order, with the bits its type has (a 16-bit search takes half the steps of a
+// 32-bit one); 0 stands for "not allowed".  (+0 and -0 are one value.)
+template <int DT> constexpr int KEY_SHIFT = DT == PCX_BF16 ? 16 : DT == PCX_F16 ? 13 : 0;
+template <int DT>
 __device__ __forceinline__ uint32_t order_of(float x) {
   const uint32_t u = __float_as_uint(x + 0.0f);
-  return u ^ ((u >> 31) ? 0xFFFFFFFFu : 0x80000000u);
+  return (u ^ ((u >> 31) ? 0xFFFFFFFFu : 0x80000000u)) >> KEY_SHIFT<DT>;
 }
-__device__ __forceinline__ float value_of(uint32_t key) { return __uint_as_float(key ^ ((key >> 31) ? 0x80000000u : 0xFFFFFFFFu)); }
+template <int DT>
+__device__ __forceinline__ float value_of(uint32_t key) {
+  const uint32_t k = key << KEY_SHIFT<DT>;
+  return __uint_as_float(k >> 31 ? k ^ 0x80000000u : ~(k | ((1u << KEY_SHIFT<DT>) - 1u)));
+}
 __device__ __forceinline__ bool allowed(float x, bool legal) { return legal && x > -INFINITY; }  // (a NaN compares false)
+
+// N neighbouring logits of a row from j on, -infinity where they are not allowed or not there (j may lie behind the end).
+template <int DT, int N>
+__device__ __forceinline__ void load_logits(const typename Logit<DT>::T* x_row, const uint8_t* l_row, int j, int end, float* x) {
+  typedef typename Logit<DT>::T T;
+  constexpr int W = N % (16 / (int)sizeof(T)) == 0 ? 16 / (int)sizeof(T) : N % 4 == 0 ? 4 : 1;  // elements per load
+#pragma unroll
+  for (int i = 0; i < N; i += W) {
+    Pack<T, W> q = {};
+    Pack<uint8_t, W> ok;
+#pragma unroll
+    for (int c = 0; c < W; ++c) ok.v[c] = 1;
+    if (j + i + W <= end) {
+      __builtin_memcpy(&q, x_row + j + i, sizeof q);
+      if (l_row) __builtin_memcpy(&ok, l_row + j + i, sizeof ok);
+    } else {
+#pragma unroll
+      for (int c = 0; c < W; ++c) {
+        ok.v[c] = 0;
+        if (j + i + c < end) {
+          q.v[c] = x_row[j + i + c];
+          ok.v[c] = l_row ? l_row[j + i + c] : 1;
+        }
+      }
+    }
+#pragma unroll
+    for (int c = 0; c < W; ++c) {
+      const float v = Logit<DT>::get(q.v[c]);
+      x[i + c] = allowed(v, ok.v[c] != 0) ? v : -INFINITY;
+    }
+  }
+}
+template <int DT, int N>
+__device__ __forceinline__ void load_keys(const Rows& rows, int64_t row, int j, int end, uint32_t* key) {
+  float x[N];
+  load_logits<DT, N>(reinterpret_cast<const typename Logit<DT>::T*>(rows.logits) + row * rows.row_stride,
+                     rows.legal ? rows.legal + row * rows.legal_stride : nullptr, j, end, x);
+#pragma unroll
+  for (int i = 0; i < N; ++i) key[i] = x[i] > -INFINITY ? order_of<DT>(x[i]) : 0u;
+}
+
+// exp(d) for d <= 0 in 64 bits, to about a unit in the last place: d = n ln 2 + r with ln 2 in two parts, the upper one short
+// enough that n times it is exact (the reduction of Cody and Waite), the Taylor series
+// of exp(r), |r| <= ln(2) / 2, to r^13 / 13! (the next term is 4e-18), and n in the exponent.
+__device__ __forceinline__ double exp64(double d) {
+  d = fmax(d, -800.0);
+  const double n = rint(d * 1.4426950408889634);
+  const double r = fma(n, -1.9082149292705877e-10, fma(n, -0.6931471803691238, d));
+  double p = 1.0 / 6227020800.0;
+  p = fma(p, r, 1.0 / 479001600.0);
+  p = fma(p, r, 1.0 / 39916800.0);
+  p = fma(p, r, 1.0 / 3628800.0);
+  p = fma(p, r, 1.0 / 362880.0);
+  p = fma(p, r, 1.0 / 40320.0);
+  p = fma(p, r, 1.0 / 5040.0);
+  p = fma(p, r, 1.0 / 720.0);
+  p = fma(p, r, 1.0 / 120.0);
+  p = fma(p, r, 1.0 / 24.0);
+  p = fma(p, r, 1.0 / 6.0);
+  p = fma(p, r, 0.5);
+  p = fma(p, r, 1.0);
+  p = fma(p, r, 1.0);
+  return ldexp(p, (int)n);
+}
 
 // ---------------------------------------------------------------- reductions over a group of THREADS (one wave, or a workgroup)
 
-template <typename V> __device__ __forceinline__ V across(V v, int mask) { return __shfl_xor(v, mask); }
+// v from the lane that a data-parallel primitive names, 0 where it names none.
+template <int CTRL, int ROWS, typename V>
+__device__ __forceinline__ V moved(V v) {
+  if constexpr (sizeof(V) == 8) {
+    uint64_t u = __builtin_bit_cast(uint64_t, v);
+    const uint32_t lo = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)u, CTRL, ROWS, 0xF, true);
+    const uint32_t hi = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)(u >> 32), CTRL, ROWS, 0xF, true);
+    return __builtin_bit_cast(V, (uint64_t)hi << 32 | lo);
+  } else {
+    return __builtin_bit_cast(V, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, ROWS, 0xF, true));
+  }
+}
+template <typename V>
+__device__ __forceinline__ V from_lane(V v, int lane) {
+  if constexpr (sizeof(V) == 8) {
+    const uint64_t u = __builtin_bit_cast(uint64_t, v);
+    const uint32_t lo = __builtin_amdgcn_readlane((int)(uint32_t)u, lane), hi = __builtin_amdgcn_readlane((int)(uint32_t)(u >> 32), lane);
+    return __builtin_bit_cast(V, (uint64_t)hi << 32 | lo);
+  } else {
+    return __builtin_bit_cast(V, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), lane));
+  }
+}
+// Prefix within a wave: each lane with those below it (f's neutral element is 0): steps of 1, 2, 4, 8 within rows of 16
+// lanes, then row to row.
+template <typename V, typename F>
+__device__ __forceinline__ V wave_prefix(V v, F f) {
+  v = f(v, moved<0x111, 0xF>(v));
+  v = f(v, moved<0x112, 0xF>(v));
+  v = f(v, moved<0x114, 0xF>(v));
+  v = f(v, moved<0x118, 0xF>(v));
+  v = f(v, moved<0x142, 0xA>(v));  // the last lane of rows 0 and 2 to rows 1 and 3
+  v = f(v, moved<0x143, 0xC>(v));  // lane 31 to the upper half
+  return v;
+}
 
 template <int THREADS>
 struct Group {
   static constexpr int WAVES = THREADS / 64;
-  struct Scratch { double d[WAVES + 1]; uint64_t u[WAVES + 1]; };
+  struct Scratch { uint64_t slot[2][WAVES]; };
   Scratch* s;
-  int t;  // thread within the group
+  int t;      // thread within the group
+  int phase;  // which half of the slots the next exchange uses: its readers are through before that half is written again
+  // one number per wave (the same in all its lanes), joined in the waves' order
   template <typename V, typename F>
-  __device__ __forceinline__ V reduce(V v, V* slots, F f) const {
+  __device__ __forceinline__ V join(V v, F f) {
+    if constexpr (WAVES == 1) return v;
+    V* const slot = reinterpret_cast<V*>(s->slot[phase]);
+    phase ^= 1;
+    if ((t & 63) == 0) slot[t >> 6] = v;
+    __syncthreads();
+    v = slot[0];
 #pragma unroll
-    for (int k = 32; k >= 1; k >>= 1) v = f(v, across(v, k));
-    if constexpr (WAVES > 1) {
-      __syncthreads();
-      if ((t & 63) == 0) slots[t >> 6] = v;
-      __syncthreads();
-      v = slots[0];
-#pragma unroll 1
-      for (int i = 1; i < WAVES; ++i) v = f(v, slots[i]);
-    }
+    for (int i = 1; i < WAVES; ++i) v = f(v, slot[i]);
     return v;
   }
-  __device__ __forceinline__ double sum(double v) const { return reduce(v, s->d, [](double a, double b) { return a + b; }); }
-  __device__ __forceinline__ uint32_t count(uint32_t v) const {
-    return (uint32_t)reduce((uint64_t)v, s->u, [](uint64_t a, uint64_t b) { return a + b; });
+  __device__ __forceinline__ double sum(double v) {
+    auto add = [](double a, double b) { return a + b; };
+    return join(from_lane(wave_prefix(v, add), 63), add);
   }
-  __device__ __forceinline__ uint64_t max(uint64_t v) const { return reduce(v, s->u, [](uint64_t a, uint64_t b) { return a > b ? a : b; }); }
-  __device__ __forceinline__ uint64_t min(uint64_t v) const { return reduce(v, s->u, [](uint64_t a, uint64_t b) { return a < b ? a : b; }); }
+  __device__ __forceinline__ float sum(float v) {
+    auto add = [](float a, float b) { return a + b; };
+    return join(from_lane(wave_prefix(v, add), 63), add);
+  }
+  __device__ __forceinline__ uint32_t max(uint32_t v) {
+    auto most = [](uint32_t a, uint32_t b) { return a > b ? a : b; };
+    return join(from_lane(wave_prefix(v, most), 63), most);
+  }
+  __device__ __forceinline__ uint32_t min(uint32_t v) { return ~max(~v); }
+  // `mine` counted per wave already (of ballots)
+  __device__ __forceinline__ uint32_t count(uint32_t mine) {
+    return join(mine, [](uint32_t a, uint32_t b) { return a + b; });
+  }
   // the sum of the threads before this one, and of all
   template <typename V>
-  __device__ __forceinline__ V scan(V v, V* slots, V* total) const {
-    V in = v;
-#pragma unroll
-    for (int k = 1; k < 64; k <<= 1) {
-      const V o = __shfl_up(in, k);
-      if ((t & 63) >= k) in += o;
-    }
-    V before = __shfl_up(in, 1);
-    if ((t & 63) == 0) before = V(0);
-    V all = __shfl(in, 63);
+  __device__ __forceinline__ V scan(V v, V* total) {
+    auto add = [](V a, V b) { return a + b; };
+    const V in = wave_prefix(v, add);
+    V before = moved<0x138, 0xF>(in);  // one lane up across the whole wave
+    V all = from_lane(in, 63);
     if constexpr (WAVES > 1) {
-      __syncthreads();
-      if ((t & 63) == 63) slots[t >> 6] = in;
+      V* const slot = reinterpret_cast<V*>(s->slot[phase]);
+      phase ^= 1;
+      if ((t & 63) == 63) slot[t >> 6] = in;
       __syncthreads();
       all = V(0);
-#pragma unroll 1
+#pragma unroll
       for (int i = 0; i < WAVES; ++i) {
         if (i == (t >> 6)) before = all + before;
-        all += slots[i];
+        all += slot[i];
       }
     }
     *total = all;
     return before;
   }
 };
+__device__ __forceinline__ uint32_t ballots(bool b) { return (uint32_t)__popcll(__ballot(b)); }
 
 // ---------------------------------------------------------------- sampling
 
@@ -145,7 +257,7 @@ struct SampleArgs {
 };
 
 __device__ __forceinline__ double weight_of(float x, float best, double rate) {
-  return x == best ? 1.0 : exp(((double)x - (double)best) * rate);
+  return exp64(x == best ? 0.0 : ((double)x - (double)best) * rate);
 }
 
 // A thread holds a whole row: few actions, many rows.
@@ -159,17 +271,12 @@ __global__ __launch_bounds__(256) void pcx_sample_rows(SampleArgs a) {
   const RowRules r = rules_of(a.rules, row);
   const int A = a.rows.actions;
   float x[CAP];
+  load_logits<DT, CAP>(x_row, l_row, 0, A, x);
   float best = -INFINITY;
   int first = NONE;
 #pragma unroll
-  for (int j = 0; j < CAP; ++j) {
-    x[j] = -INFINITY;
-    if (j < A) {
-      const float v = Logit<DT>::get(x_row[j]);
-      if (allowed(v, l_row ? l_row[j] != 0 : true)) x[j] = v;
-    }
+  for (int j = 0; j < CAP; ++j)
     if (x[j] > best) { best = x[j]; first = j; }
-  }
   if (first == NONE || !(r.temperature > 0.0f)) { a.out[row] = first; return; }
   const double rate = 1.0 / (double)r.temperature;
   double w[CAP];
@@ -222,183 +329,207 @@ __global__ __launch_bounds__(256) void pcx_sample_rows(SampleArgs a) {
   a.out[row] = pick == NONE ? last : pick;
 }
 
-// EP neighbouring actions of one row per thread: their order keys (0: not allowed, or not there).
-template <int DT, int EP>
-__device__ __forceinline__ void load_keys(const Rows& rows, int64_t row, int j0, int end, uint32_t* key) {
-  typedef typename Logit<DT>::T T;
-  const T* const x_row = reinterpret_cast<const T*>(rows.logits) + row * rows.row_stride;
-  const uint8_t* const l_row = rows.legal ? rows.legal + row * rows.legal_stride : nullptr;
-  if constexpr (EP % 4 == 0) {
-#pragma unroll
-    for (int i = 0; i < EP; i += 4) {
-      Quad<T> q = {};
-      uint32_t ok = 0x01010101u;
-      const int j = j0 + i;
-      if (j + 4 <= end) {
-        __builtin_memcpy(&q, x_row + j, sizeof q);
-        if (l_row) __builtin_memcpy(&ok, l_row + j, 4);
-      } else {
-        for (int c = 0; c < 4; ++c)
-          if (j + c < end) {
-            q.v[c] = x_row[j + c];
-            if (l_row && !l_row[j + c]) ok &= ~(0xFFu << (8 * c));
-          }
-      }
-#pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        const float x = Logit<DT>::get(q.v[c]);
-        key[i + c] = j + c < end && allowed(x, ((ok >> (8 * c)) & 255u) != 0) ? order_of(x) : 0u;
-      }
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < EP; ++i) {
-      key[i] = 0;
-      if (j0 + i < end) {
-        const float x = Logit<DT>::get(x_row[j0 + i]);
-        if (allowed(x, l_row ? l_row[j0 + i] != 0 : true)) key[i] = order_of(x);
-      }
-    }
-  }
-}
-
 // Of the elements whose key is `value`, those from the `keep`-th on (in index order) are let go.
 template <int THREADS, int EP>
-__device__ __forceinline__ void drop_ties(const Group<THREADS>& g, uint32_t value, uint32_t keep, uint32_t* key, double* w) {
-  uint64_t mine = 0, total;
+__device__ __forceinline__ void drop_ties(Group<THREADS>& g, uint32_t value, uint32_t keep, uint32_t* key, double* w) {
+  uint32_t mine = 0, total;
 #pragma unroll
   for (int i = 0; i < EP; ++i) mine += key[i] == value;
-  uint64_t at = g.scan(mine, g.s->u, &total);
+  uint32_t at = g.scan(mine, &total);
+  if (total <= keep) return;
 #pragma unroll
   for (int i = 0; i < EP; ++i)
     if (key[i] == value && at++ >= keep) { key[i] = 0; w[i] = 0.0; }
 }
 
-// The action at u of the kept weights' total, all threads of the group together.
+// Where among the group's elements (EP neighbouring ones a thread) the running sum of weights passes the target: `part` of
+// their total, or absolutely with what lies before them.
 template <int THREADS, int EP>
-__device__ __forceinline__ int draw_action(const Group<THREADS>& g, const double* w, int j0, double target_of_total, double offset, bool absolute) {
+__device__ __forceinline__ int draw_action(Group<THREADS>& g, const double* w, double part, double offset, bool absolute) {
   double mine = 0.0, total;
 #pragma unroll
   for (int i = 0; i < EP; ++i) mine += w[i];
-  const double before = offset + g.scan(mine, g.s->d, &total);
-  const double target = absolute ? target_of_total : target_of_total * total;
-  uint64_t pick = ~0ull;
-  uint64_t last = 0;
-  double run = before;
+  const double before = g.scan(mine, &total);
+  const double target = absolute ? part : part * total;
+  uint32_t pick = 0xFFFFFFFFu, last = 0;
+  double run = offset + before;
 #pragma unroll
   for (int i = 0; i < EP; ++i) {
     run += w[i];
     if (w[i] > 0.0) {
-      last = (uint64_t)(j0 + i) + 1;
-      if (run > target && pick == ~0ull) pick = (uint64_t)(j0 + i);
+      last = (uint32_t)(g.t * EP + i) + 1;
+      if (run > target && pick == 0xFFFFFFFFu) pick = (uint32_t)(g.t * EP + i);
     }
   }
   pick = g.min(pick);
-  if (pick != ~0ull) return (int)pick;
-  last = g.max(last);  // (u is one or more, or no number: the last one kept)
-  return (int)last - 1;
+  if (pick != 0xFFFFFFFFu) return (int)pick;
+  return (int)g.max(last) - 1;  // (u is one or more, or no number: the last one kept)
 }
 
-// The largest key t with at least k keys >= t; the keys hold more than k that are not 0.
+// The largest key t with at least k keys >= t; more than k keys are not 0.
 template <int THREADS, int EP>
-__device__ __forceinline__ uint32_t find_rank(const Group<THREADS>& g, const uint32_t* key, uint32_t k, uint32_t hi) {
+__device__ __forceinline__ uint32_t find_rank(Group<THREADS>& g, const uint32_t* key, uint32_t k, uint32_t hi) {
   uint32_t lo = 1;
   while (lo < hi) {
     const uint32_t mid = hi - (hi - lo) / 2;
     uint32_t c = 0;
 #pragma unroll
-    for (int i = 0; i < EP; ++i) c += key[i] >= mid;
+    for (int i = 0; i < EP; ++i) c += ballots(key[i] >= mid);
     if (g.count(c) >= k) lo = mid; else hi = mid - 1;
   }
   return lo;
 }
-// The largest key t whose elements >= t weigh at least `target`.
+// The largest key t whose elements >= t weigh at least `target`, and what those above it weigh.
 template <int THREADS, int EP>
-__device__ __forceinline__ uint32_t find_mass(const Group<THREADS>& g, const uint32_t* key, const double* w, double target, uint32_t hi) {
-  uint32_t lo = 1;
+__device__ __forceinline__ uint32_t find_mass(Group<THREADS>& g, const uint32_t* key, const double* w, double target, uint32_t lo, uint32_t hi, double* above) {
+  double over = 0.0;
   while (lo < hi) {
     const uint32_t mid = hi - (hi - lo) / 2;
     double m = 0.0;
 #pragma unroll
     for (int i = 0; i < EP; ++i) m += key[i] >= mid ? w[i] : 0.0;
-    if (g.sum(m) >= target) lo = mid; else hi = mid - 1;
+    m = g.sum(m);
+    if (m >= target) lo = mid;
+    else { hi = mid - 1; over = m; }
   }
+  *above = over;
   return lo;
 }
 
-// A wave or a workgroup holds a row in registers, EP neighbouring actions a thread.
+// The rules on a group's elements, EP neighbouring ones a thread in index order, of which best_key is the largest key (not
+// 0); `of` says how many actions the row has.  Which element is drawn.
+template <int DT, int THREADS, int EP>
+__device__ __forceinline__ int choose(Group<THREADS>& g, uint32_t* key, uint32_t best_key, const RowRules& r, int of, double u) {
+  if (r.top_k > 0 && r.top_k < of) {
+    uint32_t c = 0;
+#pragma unroll
+    for (int i = 0; i < EP; ++i) c += ballots(key[i] != 0);
+    if (g.count(c) > (uint32_t)r.top_k) {
+      const uint32_t edge = find_rank<THREADS, EP>(g, key, (uint32_t)r.top_k, best_key);
+      uint32_t above = 0, equal = 0;
+#pragma unroll
+      for (int i = 0; i < EP; ++i) {
+        above += ballots(key[i] > edge);
+        equal += key[i] == edge;
+        if (key[i] < edge) key[i] = 0;
+      }
+      const uint32_t keep = (uint32_t)r.top_k - g.count(above);
+      uint32_t total;
+      uint32_t at = g.scan(equal, &total);
+      if (total > keep) {
+#pragma unroll
+        for (int i = 0; i < EP; ++i)
+          if (key[i] == edge && at++ >= keep) key[i] = 0;
+      }
+    }
+  }
+  const float best = value_of<DT>(best_key);
+  const double rate = 1.0 / (double)r.temperature;
+  double w[EP];
+#pragma unroll
+  for (int i = 0; i < EP; ++i) {
+    w[i] = 0.0;
+    if (__ballot(key[i] != 0)) w[i] = key[i] ? weight_of(value_of<DT>(key[i]), best, rate) : 0.0;  // (whole waves of nothing left are common)
+  }
+  if (r.top_p < 1.0f) {
+    double total = 0.0;
+#pragma unroll
+    for (int i = 0; i < EP; ++i) total += w[i];
+    total = g.sum(total);
+    const double target = (double)r.top_p * total;
+    // What lies below the edge weighs at most (1 - top_p) of the total: an action of that much / (2 * all) cannot be the edge.
+    uint32_t lo = 1;
+    const float floor_x = best + (float)(log((total - target) / (2.0 * of)) * (double)r.temperature);
+    if (floor_x > -3e38f && floor_x < best) lo = order_of<DT>(floor_x);
+    double above;
+    const uint32_t edge = find_mass<THREADS, EP>(g, key, w, target, lo, best_key, &above);
+#pragma unroll
+    for (int i = 0; i < EP; ++i)
+      if (key[i] < edge) { key[i] = 0; w[i] = 0.0; }
+    const double need = ceil((target - above) / weight_of(value_of<DT>(edge), best, rate));
+    drop_ties<THREADS, EP>(g, edge, need >= 1.0 ? (need < 4e9 ? (uint32_t)need : 0xFFFFFFFFu) : 1u, key, w);
+  }
+#pragma unroll
+  for (int i = 0; i < EP; ++i)
+    if (w[i] < (double)r.min_p) w[i] = 0.0;
+  return draw_action<THREADS, EP>(g, w, u, 0.0, false);
+}
+
+// A wave or a workgroup holds a row in registers, EP neighbouring actions a thread.  Where top_k keeps few of a workgroup's
+// row, it first cuts at the k-th largest of the threads' largest keys -- at least k elements reach that, and seldom many
+// more -- and one wave chooses among those alone: no 64-bit exponentials and no workgroup-wide searches for the rest.
 template <int DT, int THREADS, int EP>
 __global__ __launch_bounds__(THREADS < 256 ? 256 : THREADS) void pcx_sample_group(SampleArgs a) {
   constexpr int ROWS = THREADS < 256 ? 256 / THREADS : 1;
+  constexpr int FEW = 512;  // elements a wave chooses among
   __shared__ typename Group<THREADS>::Scratch scratch[ROWS];
-  Group<THREADS> g{&scratch[threadIdx.x / THREADS], (int)(threadIdx.x % THREADS)};
+  Group<THREADS> g{&scratch[threadIdx.x / THREADS], (int)(threadIdx.x % THREADS), 0};
   const int64_t row = (int64_t)blockIdx.x * ROWS + threadIdx.x / THREADS;
   if (row >= a.rows.n) return;  // (a whole group)
   const RowRules r = rules_of(a.rules, row);
   const int A = a.rows.actions, j0 = g.t * EP;
   uint32_t key[EP];
   load_keys<DT, EP>(a.rows, row, j0, A, key);
-  uint64_t top = 0;
+  uint32_t most = 0;
 #pragma unroll
-  for (int i = 0; i < EP; ++i) {
-    const uint64_t v = ((uint64_t)key[i] << 32) | (uint32_t)~(uint32_t)(j0 + i);
-    if (key[i] && v > top) top = v;
-  }
-  top = g.max(top);
-  const uint32_t best_key = (uint32_t)(top >> 32);
+  for (int i = 0; i < EP; ++i) most = key[i] > most ? key[i] : most;
+  const uint32_t best_key = g.max(most);
   if (best_key == 0 || !(r.temperature > 0.0f)) {
-    if (g.t == 0) a.out[row] = best_key ? (int)~(uint32_t)top : NONE;
+    uint32_t first = 0xFFFFFFFFu;
+#pragma unroll
+    for (int i = EP - 1; i >= 0; --i)
+      if (key[i] == best_key) first = (uint32_t)(j0 + i);
+    first = g.min(first);
+    if (g.t == 0) a.out[row] = best_key ? (int)first : NONE;
     return;
   }
-  const float best = value_of(best_key);
-  const double rate = 1.0 / (double)r.temperature;
-  double w[EP];
+  const double u = (double)a.uniforms[row];
+  if constexpr (THREADS >= 256) {
+    __shared__ uint32_t few_key[FEW];
+    __shared__ uint16_t few_at[FEW];
+    if (r.top_k > 0 && r.top_k <= THREADS / 2 && r.top_k < A) {
+      uint32_t mine[1] = {most};
+      const uint32_t cut = find_rank<THREADS, 1>(g, mine, (uint32_t)r.top_k, best_key);
+      uint32_t c = 0, total;
 #pragma unroll
-  for (int i = 0; i < EP; ++i) w[i] = key[i] ? weight_of(value_of(key[i]), best, rate) : 0.0;
-  if (r.top_k > 0 && r.top_k < A) {
-    uint32_t c = 0;
+      for (int i = 0; i < EP; ++i) c += key[i] >= cut;
+      uint32_t at = g.scan(c, &total);
+      if (total <= FEW) {
 #pragma unroll
-    for (int i = 0; i < EP; ++i) c += key[i] != 0;
-    if (g.count(c) > (uint32_t)r.top_k) {
-      const uint32_t edge = find_rank<THREADS, EP>(g, key, (uint32_t)r.top_k, best_key);
-      uint32_t above = 0;
+        for (int i = 0; i < EP; ++i)
+          if (key[i] >= cut) {
+            few_key[at] = key[i];
+            few_at[at++] = (uint16_t)(j0 + i);
+          }
+        __syncthreads();
+        if (g.t >= 64) return;
+        Group<64> one{nullptr, g.t, 0};
+        int pick;
+        if (total <= 128) {
+          uint32_t k[2];
 #pragma unroll
-      for (int i = 0; i < EP; ++i) {
-        above += key[i] > edge;
-        if (key[i] < edge) { key[i] = 0; w[i] = 0.0; }
+          for (int i = 0; i < 2; ++i) k[i] = (uint32_t)(g.t * 2 + i) < total ? few_key[g.t * 2 + i] : 0;
+          pick = choose<DT, 64, 2>(one, k, best_key, r, A, u);
+        } else {
+          uint32_t k[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) k[i] = (uint32_t)(g.t * 8 + i) < total ? few_key[g.t * 8 + i] : 0;
+          pick = choose<DT, 64, 8>(one, k, best_key, r, A, u);
+        }
+        if (g.t == 0) a.out[row] = few_at[pick];
+        return;
       }
-      above = g.count(above);
-      drop_ties<THREADS, EP>(g, edge, (uint32_t)r.top_k - above, key, w);
     }
   }
-  if (r.top_p < 1.0f) {
-    double total = 0.0;
-#pragma unroll
-    for (int i = 0; i < EP; ++i) total += w[i];
-    const double target = (double)r.top_p * g.sum(total);
-    const uint32_t edge = find_mass<THREADS, EP>(g, key, w, target, best_key);
-    double above = 0.0;
-#pragma unroll
-    for (int i = 0; i < EP; ++i) {
-      above += key[i] > edge ? w[i] : 0.0;
-      if (key[i] < edge) { key[i] = 0; w[i] = 0.0; }
-    }
-    above = g.sum(above);
-    const double need = ceil((target - above) / weight_of(value_of(edge), best, rate));
-    drop_ties<THREADS, EP>(g, edge, need >= 1.0 ? (need < 4e9 ? (uint32_t)need : 0xFFFFFFFFu) : 1u, key, w);
-  }
-#pragma unroll
-  for (int i = 0; i < EP; ++i)
-    if (w[i] < (double)r.min_p) w[i] = 0.0;
-  const int pick = draw_action<THREADS, EP>(g, w, j0, (double)a.uniforms[row], 0.0, false);
+  const int pick = choose<DT, THREADS, EP>(g, key, best_key, r, A, u);
   if (g.t == 0) a.out[row] = pick;
 }
 
 // ---- rows that no workgroup holds: divided among workgroups, one launch per question ------------------------------------
 
 constexpr int SLICE = 8192;    // actions per workgroup
-constexpr int WEP = 32;        // ... per thread of 256
-constexpr int BINS = 2048;     // of a digit of the order key: 11, 11 and 10 bits
+constexpr int WEP = 32;        // ... per thread of 256, all of them in flight before the first is looked at
+constexpr int BINS = 2048;     // of a digit of the order key: at most 11 bits
 struct RowState {
   uint64_t best;               // (order key, ~index) of the best action
   double total, target, above; // weights: of what top_k leaves, top_p of it, ahead of the current digit's bin
@@ -418,10 +549,21 @@ struct WideArgs {
   Slot* slots;                 // [rows][slices]
   int32_t batch;
 };
-__device__ __forceinline__ int digit_shift(int level) { return level == 0 ? 21 : level == 1 ? 10 : 0; }
-__device__ __forceinline__ uint32_t digit_of(uint32_t key, int level) { return (key >> digit_shift(level)) & (level == 2 ? 1023u : 2047u); }
+// The digits of a key, from the top: 11, 11 and 10 bits of 32; 11 and 5 of bfloat16's 16, 11 and 8 of float16's 19.
+template <int DT> constexpr int LEVELS = DT == PCX_F32 ? 3 : 2;
+template <int DT>
+__host__ __device__ __forceinline__ int digit_shift(int level) {
+  constexpr int BITS = 32 - KEY_SHIFT<DT>;
+  return level == 0 ? BITS - 11 : level == 1 && BITS > 22 ? BITS - 22 : 0;
+}
+template <int DT>
+__device__ __forceinline__ uint32_t digit_of(uint32_t key, int level) {
+  const uint32_t bits = level == 0 ? 11u : (uint32_t)(digit_shift<DT>(level - 1) - digit_shift<DT>(level));
+  return (key >> digit_shift<DT>(level)) & ((1u << bits) - 1u);
+}
+template <int DT>
 __device__ __forceinline__ bool same_prefix(uint32_t key, uint32_t prefix, int level) {
-  return level == 0 || (level == 1 ? key >> 21 == prefix >> 21 : key >> 10 == prefix >> 10);
+  return level == 0 || key >> digit_shift<DT>(level - 1) == prefix >> digit_shift<DT>(level - 1);
 }
 
 __global__ __launch_bounds__(256) void pcx_sample_clear(WideArgs w) {
@@ -433,24 +575,35 @@ __global__ __launch_bounds__(256) void pcx_sample_clear(WideArgs w) {
   }
   if (threadIdx.x == 0) w.state[row] = RowState{};
 }
+// The keys of this thread in a slice: SLICE / 256, in packs that lie 256 packs apart.
+template <int DT>
+__device__ __forceinline__ void load_slice(const WideArgs& w, int row, int lo, uint32_t* key) {
+  constexpr int W = 16 / (int)sizeof(typename Logit<DT>::T);
+  const int end = w.a.rows.actions - lo < SLICE ? w.a.rows.actions : lo + SLICE;
+#pragma unroll
+  for (int i = 0; i < WEP / W; ++i) load_keys<DT, W>(w.a.rows, w.row0 + row, lo + (i * 256 + (int)threadIdx.x) * W, end, key + i * W);
+}
+template <int DT>
+__device__ __forceinline__ int slice_index(int lo, int i) {
+  constexpr int W = 16 / (int)sizeof(typename Logit<DT>::T);
+  return lo + ((i / W) * 256 + (int)threadIdx.x) * W + i % W;
+}
 template <int DT>
 __global__ __launch_bounds__(256) void pcx_sample_best(WideArgs w) {
   __shared__ Group<256>::Scratch scratch;
-  Group<256> g{&scratch, (int)threadIdx.x};
+  Group<256> g{&scratch, (int)threadIdx.x, 0};
   const int row = blockIdx.y, lo = blockIdx.x * SLICE;
-  const int end = w.a.rows.actions - lo < SLICE ? w.a.rows.actions : lo + SLICE;
-  uint64_t top = 0;
-  for (int j0 = lo + threadIdx.x * 4; j0 < end; j0 += 1024) {
-    uint32_t key[4];
-    load_keys<DT, 4>(w.a.rows, w.row0 + row, j0, end, key);
+  uint32_t key[WEP];
+  load_slice<DT>(w, row, lo, key);
+  uint32_t top = 0, at = 0xFFFFFFFFu;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const uint64_t v = ((uint64_t)key[i] << 32) | (uint32_t)~(uint32_t)(j0 + i);
-      if (key[i] && v > top) top = v;
-    }
-  }
+  for (int i = 0; i < WEP; ++i) top = key[i] > top ? key[i] : top;
   top = g.max(top);
-  if (threadIdx.x == 0 && top) atomicMax(reinterpret_cast<unsigned long long*>(&w.state[row].best), (unsigned long long)top);
+#pragma unroll
+  for (int i = 0; i < WEP; ++i)
+    if (key[i] == top && (uint32_t)slice_index<DT>(lo, i) < at) at = (uint32_t)slice_index<DT>(lo, i);
+  at = g.min(at);
+  if (threadIdx.x == 0 && top) atomicMax(reinterpret_cast<unsigned long long*>(&w.state[row].best), (unsigned long long)top << 32 | (uint32_t)~at);
 }
 // Counts and weights per value of one digit, of the keys that agree with the digits found so far.
 template <int DT>
@@ -463,22 +616,19 @@ __global__ __launch_bounds__(256) void pcx_sample_digit(WideArgs w, int level, u
   const RowRules r = rules_of(w.a.rules, w.row0 + row);
   const uint32_t best_key = (uint32_t)(st.best >> 32);
   if (!best_key || !(r.temperature > 0.0f)) return;
-  const float best = value_of(best_key);
+  uint32_t key[WEP];
+  load_slice<DT>(w, row, lo, key);
+  const float best = value_of<DT>(best_key);
   const double rate = 1.0 / (double)r.temperature;
   for (int i = threadIdx.x; i < BINS; i += 256) { mass[i] = 0; count[i] = 0; }
   __syncthreads();
-  const int end = w.a.rows.actions - lo < SLICE ? w.a.rows.actions : lo + SLICE;
-  for (int j0 = lo + threadIdx.x * 4; j0 < end; j0 += 1024) {
-    uint32_t key[4];
-    load_keys<DT, 4>(w.a.rows, w.row0 + row, j0, end, key);
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (key[i] && same_prefix(key[i], st.prefix, level)) {
-        const uint32_t d = digit_of(key[i], level);
-        atomicAdd(&count[d], 1u);
-        atomicAdd(&mass[d], (unsigned long long)(ldexp(weight_of(value_of(key[i]), best, rate), w.scale) + 0.5));
-      }
-  }
+  for (int i = 0; i < WEP; ++i)
+    if (key[i] && same_prefix<DT>(key[i], st.prefix, level)) {
+      const uint32_t d = digit_of<DT>(key[i], level);
+      atomicAdd(&count[d], 1u);
+      atomicAdd(&mass[d], (unsigned long long)(ldexp(weight_of(value_of<DT>(key[i]), best, rate), w.scale) + 0.5));
+    }
   __syncthreads();
   const int64_t at = ((int64_t)(level != 0) * w.batch + row) * BINS;
   for (int i = threadIdx.x; i < BINS; i += 256)
@@ -488,10 +638,11 @@ __global__ __launch_bounds__(256) void pcx_sample_digit(WideArgs w, int level, u
     }
 }
 // Which bin of the digit the edge lies in.  by_mass: top_p's edge, else top_k's.
+template <int DT>
 __global__ __launch_bounds__(256) void pcx_sample_edge(WideArgs w, int level, int by_mass) {
   __shared__ Group<256>::Scratch scratch;
   __shared__ RowState next;
-  Group<256> g{&scratch, (int)threadIdx.x};
+  Group<256> g{&scratch, (int)threadIdx.x, 0};
   const int row = blockIdx.x;
   RowState st = w.state[row];
   const RowRules r = rules_of(w.a.rules, w.row0 + row);
@@ -510,8 +661,7 @@ __global__ __launch_bounds__(256) void pcx_sample_edge(WideArgs w, int level, in
     m_mine += masses[i];
     if (level != 0) { w.count[at + bin] = 0; w.mass[at + bin] = 0; }  // for the next digit
   }
-  uint64_t c = g.scan(c_mine, g.s->u, &c_all);
-  uint64_t m = g.scan(m_mine, g.s->u, &m_all);
+  uint64_t c = g.scan(c_mine, &c_all), m = g.scan(m_mine, &m_all);
   if (level == 0) {
     st.above = 0.0;
     st.count_above = 0;
@@ -528,12 +678,12 @@ __global__ __launch_bounds__(256) void pcx_sample_edge(WideArgs w, int level, in
   __syncthreads();
   if (cuts) {
     // the first bin, from the top, at which the edge is reached
-    uint64_t found = ~0ull;
+    uint32_t found = 0xFFFFFFFFu;
     uint64_t c_run = c, m_run = m, c_at = 0, m_at = 0;  // ahead of the bin taken
     int bin_at = -1;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      if (!counts[i] || found != ~0ull) continue;
+      if (!counts[i] || found != 0xFFFFFFFFu) continue;
       c_at = c_run;
       m_at = m_run;
       bin_at = BINS - 1 - ((int)threadIdx.x * 8 + i);
@@ -542,17 +692,17 @@ __global__ __launch_bounds__(256) void pcx_sample_edge(WideArgs w, int level, in
       const bool reached = by_mass ? st.above + ldexp((double)m_run, -w.scale) >= st.target : st.count_above + c_run >= (uint64_t)r.top_k;
       if (reached) found = threadIdx.x;
     }
-    uint64_t who = g.min(found);
+    uint32_t who = g.min(found);
     // (sums of fixed-point weights can miss the target by their rounding: then the lowest bin that holds anything)
-    const uint64_t lowest = g.max(bin_at >= 0 ? (uint64_t)threadIdx.x : 0);
-    if (who == ~0ull) who = lowest;
+    const uint32_t lowest = g.max(bin_at >= 0 ? threadIdx.x : 0u);
+    if (who == 0xFFFFFFFFu) who = lowest;
     const bool mine = who == threadIdx.x && bin_at >= 0;
     if (mine) {
       next.count_above = st.count_above + c_at;
       next.above = st.above + ldexp((double)m_at, -w.scale);
-      next.prefix = (level == 0 ? 0u : st.prefix) | ((uint32_t)bin_at << digit_shift(level));
-      if (level == 2) {
-        const double tie = weight_of(value_of(next.prefix), value_of(best_key), 1.0 / (double)r.temperature);
+      next.prefix = (level == 0 ? 0u : st.prefix) | ((uint32_t)bin_at << digit_shift<DT>(level));
+      if (level == LEVELS<DT> - 1) {
+        const double tie = weight_of(value_of<DT>(next.prefix), value_of<DT>(best_key), 1.0 / (double)r.temperature);
         next.edge = next.prefix;
         if (by_mass) {
           const double need = ceil((st.target - next.above) / tie);
@@ -573,40 +723,37 @@ __global__ __launch_bounds__(256) void pcx_sample_edge(WideArgs w, int level, in
 template <int DT>
 __global__ __launch_bounds__(256) void pcx_sample_weigh(WideArgs w) {
   __shared__ Group<256>::Scratch scratch;
-  Group<256> g{&scratch, (int)threadIdx.x};
+  Group<256> g{&scratch, (int)threadIdx.x, 0};
   const int row = blockIdx.y, lo = blockIdx.x * SLICE;
   const RowState st = w.state[row];
   const RowRules r = rules_of(w.a.rules, w.row0 + row);
   const uint32_t best_key = (uint32_t)(st.best >> 32);
   if (!best_key || !(r.temperature > 0.0f)) return;
-  const float best = value_of(best_key);
+  uint32_t key[WEP];
+  load_slice<DT>(w, row, lo, key);
+  const float best = value_of<DT>(best_key);
   const double rate = 1.0 / (double)r.temperature;
-  const int end = w.a.rows.actions - lo < SLICE ? w.a.rows.actions : lo + SLICE;
   double mine = 0.0;
-  uint64_t ties = 0;
-  for (int j0 = lo + threadIdx.x * 4; j0 < end; j0 += 1024) {
-    uint32_t key[4];
-    load_keys<DT, 4>(w.a.rows, w.row0 + row, j0, end, key);
+  uint32_t ties = 0;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      if (key[i] > st.edge) {
-        const double v = weight_of(value_of(key[i]), best, rate);
-        if (v >= (double)r.min_p) mine += v;
-      }
-      ties += st.edge && key[i] == st.edge;
+  for (int i = 0; i < WEP; ++i) {
+    if (key[i] > st.edge) {
+      const double v = weight_of(value_of<DT>(key[i]), best, rate);
+      if (v >= (double)r.min_p) mine += v;
     }
+    ties += ballots(st.edge && key[i] == st.edge);
   }
   mine = g.sum(mine);
-  ties = g.count((uint32_t)ties);
+  ties = g.count(ties);
   if (threadIdx.x == 0) w.slots[(int64_t)row * w.slices + blockIdx.x] = Slot{mine, ties};
 }
+// The slice that the number falls into, then the action within it.
 template <int DT>
 __global__ __launch_bounds__(256) void pcx_sample_pick(WideArgs w) {
   __shared__ Group<256>::Scratch scratch;
-  __shared__ int chosen;
-  __shared__ double offset, goal;
+  __shared__ double offset;
   __shared__ uint32_t ties_left;
-  Group<256> g{&scratch, (int)threadIdx.x};
+  Group<256> g{&scratch, (int)threadIdx.x, 0};
   const int row = blockIdx.x;
   const int64_t at = w.row0 + row;
   const RowState st = w.state[row];
@@ -616,47 +763,64 @@ __global__ __launch_bounds__(256) void pcx_sample_pick(WideArgs w) {
     if (threadIdx.x == 0) w.a.out[at] = best_key ? (int)~(uint32_t)st.best : NONE;
     return;
   }
-  const float best = value_of(best_key);
+  const float best = value_of<DT>(best_key);
   const double rate = 1.0 / (double)r.temperature;
-  double tie = st.edge ? weight_of(value_of(st.edge), best, rate) : 0.0;
+  double tie = st.edge ? weight_of(value_of<DT>(st.edge), best, rate) : 0.0;
   if (tie < (double)r.min_p) tie = 0.0;
-  if (threadIdx.x == 0) {
-    const Slot* const slots = w.slots + (int64_t)row * w.slices;
-    double total = 0.0;
-    uint64_t left = st.ties;
-    for (int s = 0; s < w.slices; ++s) {
-      const uint64_t kept = slots[s].ties < left ? slots[s].ties : left;
-      left -= kept;
-      total += slots[s].weight + (double)kept * tie;
-    }
-    const double target = (double)w.a.uniforms[at] * total;
-    double run = 0.0;
-    left = st.ties;
-    chosen = -1;
-    for (int s = 0; s < w.slices; ++s) {
-      const uint64_t kept = slots[s].ties < left ? slots[s].ties : left;
-      const double weight = slots[s].weight + (double)kept * tie;
-      if (weight > 0.0) { chosen = s; offset = run; ties_left = (uint32_t)left; }  // (the last that holds anything, if u asks for more)
-      run += weight;
-      left -= kept;
-      if (weight > 0.0 && run > target) break;
-    }
-    goal = target;
+  // neighbouring slices a thread: (2^24 actions are 2048 slices, eight a thread)
+  const Slot* const slots = w.slots + (int64_t)row * w.slices;
+  const int per = (w.slices + 255) / 256, s0 = (int)threadIdx.x * per;
+  uint64_t ties = 0, ties_all;
+  for (int i = s0; i < s0 + per && i < w.slices; ++i) ties += slots[i].ties;
+  const uint64_t ties_before = g.scan(ties, &ties_all);
+  uint64_t left = ties_before < st.ties ? st.ties - ties_before : 0;
+  const uint64_t left0 = left;
+  double mine = 0.0, total;
+  for (int i = s0; i < s0 + per && i < w.slices; ++i) {
+    const uint64_t kept = slots[i].ties < left ? slots[i].ties : left;
+    left -= kept;
+    mine += slots[i].weight + (double)kept * tie;
   }
+  const double before = g.scan(mine, &total);
+  const double goal = (double)w.a.uniforms[at] * total;
+  uint32_t chosen = 0xFFFFFFFFu, last = 0;
+  double run = before, run_at = 0.0, run_last = 0.0;
+  uint64_t left_at = 0, left_last = 0;
+  left = left0;
+  for (int i = s0; i < s0 + per && i < w.slices; ++i) {
+    const uint64_t kept = slots[i].ties < left ? slots[i].ties : left;
+    const double weight = slots[i].weight + (double)kept * tie;
+    if (weight > 0.0) {
+      last = (uint32_t)i + 1;
+      run_last = run;
+      left_last = left;
+      if (run + weight > goal && chosen == 0xFFFFFFFFu) { chosen = (uint32_t)i; run_at = run; left_at = left; }
+    }
+    run += weight;
+    left -= kept;
+  }
+  uint32_t slice = g.min(chosen);
+  if (slice == 0xFFFFFFFFu) {  // (u asks for more than there is: the last slice that holds anything)
+    slice = g.max(last) - 1;
+    chosen = last - 1;
+    run_at = run_last;
+    left_at = left_last;
+  }
+  if (chosen == slice) { offset = run_at; ties_left = (uint32_t)(left_at < 0xFFFFFFFFull ? left_at : 0xFFFFFFFFull); }
   __syncthreads();
-  const int lo = chosen * SLICE, j0 = lo + (int)threadIdx.x * WEP;
+  const int lo = (int)slice * SLICE, j0 = lo + (int)threadIdx.x * WEP;
   const int end = w.a.rows.actions - lo < SLICE ? w.a.rows.actions : lo + SLICE;
   uint32_t key[WEP];
   double v[WEP];
   load_keys<DT, WEP>(w.a.rows, at, j0, end, key);
 #pragma unroll
   for (int i = 0; i < WEP; ++i) {
-    v[i] = key[i] && key[i] >= st.edge ? weight_of(value_of(key[i]), best, rate) : 0.0;
+    v[i] = key[i] && key[i] >= st.edge ? weight_of(value_of<DT>(key[i]), best, rate) : 0.0;
     if (v[i] < (double)r.min_p) v[i] = 0.0;
   }
   if (st.edge) drop_ties<256, WEP>(g, st.edge, ties_left, key, v);
-  const int pick = draw_action<256, WEP>(g, v, j0, goal, offset, true);
-  if (threadIdx.x == 0) w.a.out[at] = pick;
+  const int pick = draw_action<256, WEP>(g, v, goal, offset, true);
+  if (threadIdx.x == 0) w.a.out[at] = lo + pick;
 }
 
 // ---------------------------------------------------------------- log-probability, entropy and their gradient
@@ -715,9 +879,21 @@ __device__ __forceinline__ void finish_row(const LogProbArgs& a, int64_t row, co
   a.log_prob[row] = lp;
 }
 
+// sum of exp and of d exp of N logits relative to `big` (> -infinity); -infinity adds nothing
+template <int N>
+__device__ __forceinline__ void soft_sums(const float* x, float big, float rate, float* s, float* t) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const float d = x[i] == big ? 0.0f : fmaxf((x[i] - big) * rate, -1e4f), e = exp_of(d);  // (d e is 0 long before -1e4)
+    *s += e;
+    *t = fmaf(d, e, *t);
+  }
+}
+// A wave (few actions) or a workgroup takes a row, 16 neighbouring logits a thread and turn.
 template <int DT, int THREADS>
 __global__ __launch_bounds__(256) void pcx_log_prob_forward(LogProbArgs a) {
-  constexpr int ROWS = 256 / THREADS;
+  typedef typename Logit<DT>::T T;
+  constexpr int ROWS = 256 / THREADS, EP = THREADS == 64 ? 8 : 16;
   __shared__ float shared[4][3];
   const int t = threadIdx.x % THREADS;
   const int64_t unit = (int64_t)blockIdx.x * ROWS + threadIdx.x / THREADS;
@@ -726,23 +902,18 @@ __global__ __launch_bounds__(256) void pcx_log_prob_forward(LogProbArgs a) {
   const int slice = (int)(unit - row * a.slices);
   const int lo = a.slices > 1 ? slice * SLICE : 0;
   const int end = a.slices > 1 && a.rows.actions - lo > SLICE ? lo + SLICE : a.rows.actions;
+  const T* const x_row = reinterpret_cast<const T*>(a.rows.logits) + row * a.rows.row_stride;
+  const uint8_t* const l_row = a.rows.legal ? a.rows.legal + row * a.rows.legal_stride : nullptr;
   Soft v{-INFINITY, 0.0f, 0.0f};
-  for (int j0 = lo + t * 4; j0 < end; j0 += THREADS * 4) {
-    uint32_t key[4];
-    load_keys<DT, 4>(a.rows, row, j0, end, key);
-    const uint32_t k1 = key[0] > key[1] ? key[0] : key[1], k2 = key[2] > key[3] ? key[2] : key[3];
-    const uint32_t top = k1 > k2 ? k1 : k2;
-    if (!top) continue;
-    const float big = value_of(top);
-    float s = 0.0f, tt = 0.0f;
+  for (int j = lo + t * EP; j < end; j += THREADS * EP) {
+    float x[EP];
+    load_logits<DT, EP>(x_row, l_row, j, end, x);
+    float big = x[0];
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (key[i]) {
-        const float x = value_of(key[i]);
-        const float d = x == big ? 0.0f : (x - big) * a.rate, e = exp_of(d);
-        s += e;
-        if (e > 0.0f) tt = fmaf(d, e, tt);
-      }
+    for (int i = 1; i < EP; ++i) big = fmaxf(big, x[i]);
+    if (!(big > -INFINITY)) continue;
+    float s = 0.0f, tt = 0.0f;
+    soft_sums<EP>(x, big, a.rate, &s, &tt);
     v.join(big, s, tt, a.rate);
   }
 #pragma unroll
@@ -793,18 +964,16 @@ __device__ __forceinline__ RowGrad row_grad(const LogProbArgs& a, int64_t row) {
   g.ge = a.grad_entropy ? a.grad_entropy[row] : 0.0f;
   return g;
 }
-__device__ __forceinline__ float element_grad(const RowGrad& g, uint32_t key, int j, float rate) {
-  if (!key) return 0.0f;
-  const float x = value_of(key);
-  const float d = x == g.m ? 0.0f : (x - g.m) * rate;
+__device__ __forceinline__ float element_grad(const RowGrad& g, float x, int j, float rate) {
+  const float d = x == g.m ? 0.0f : fmaxf((x - g.m) * rate, -1e4f);
   const float p = exp_of(d) * g.inv;
-  const float term = p > 0.0f ? p * (d - g.ls + g.h) : 0.0f;
-  return ((j == g.taken ? g.gl : 0.0f) - g.gl * p - g.ge * term) * rate;
+  const float v = ((j == g.taken ? g.gl : 0.0f) - p * (g.gl + g.ge * (d - g.ls + g.h))) * rate;
+  return x > -INFINITY ? v : 0.0f;
 }
 template <int DT, int THREADS>
 __global__ __launch_bounds__(256) void pcx_log_prob_backward_kernel(LogProbArgs a) {
   typedef typename Logit<DT>::T T;
-  constexpr int ROWS = 256 / THREADS;
+  constexpr int ROWS = 256 / THREADS, W = 16 / (int)sizeof(T);
   const int t = threadIdx.x % THREADS;
   const int64_t unit = (int64_t)blockIdx.x * ROWS + threadIdx.x / THREADS;
   if (unit >= a.rows.n * a.slices) return;
@@ -812,42 +981,37 @@ __global__ __launch_bounds__(256) void pcx_log_prob_backward_kernel(LogProbArgs 
   const int slice = (int)(unit - row * a.slices);
   const int lo = a.slices > 1 ? slice * SLICE : 0;
   const int end = a.slices > 1 && a.rows.actions - lo > SLICE ? lo + SLICE : a.rows.actions;
+  const T* const x_row = reinterpret_cast<const T*>(a.rows.logits) + row * a.rows.row_stride;
+  const uint8_t* const l_row = a.rows.legal ? a.rows.legal + row * a.rows.legal_stride : nullptr;
   const RowGrad g = row_grad(a, row);
   T* const out = reinterpret_cast<T*>(a.grad) + row * a.rows.actions;
-  for (int j0 = lo + t * 4; j0 < end; j0 += THREADS * 4) {
-    uint32_t key[4];
-    load_keys<DT, 4>(a.rows, row, j0, end, key);
-    Quad<T> q;
+#pragma unroll 2
+  for (int j = lo + t * W; j < end; j += THREADS * W) {
+    float x[W];
+    load_logits<DT, W>(x_row, l_row, j, end, x);
+    Pack<T, W> q;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) q.v[i] = Logit<DT>::put(element_grad(g, key[i], j0 + i, a.rate));
-    if (j0 + 4 <= end) __builtin_memcpy(out + j0, &q, sizeof q);
+    for (int i = 0; i < W; ++i) q.v[i] = Logit<DT>::put(element_grad(g, x[i], j + i, a.rate));
+    if (j + W <= end) __builtin_memcpy(out + j, &q, sizeof q);
     else
-      for (int i = 0; i < 4; ++i)
-        if (j0 + i < end) out[j0 + i] = q.v[i];
+#pragma unroll
+      for (int i = 0; i < W; ++i)
+        if (j + i < end) out[j + i] = q.v[i];
   }
 }
 // Few actions: a thread holds a row.
 template <int DT, int CAP>
 __global__ __launch_bounds__(256) void pcx_log_prob_rows(LogProbArgs a) {
+  typedef typename Logit<DT>::T T;
   const int64_t row = (int64_t)blockIdx.x * 256 + threadIdx.x;
   if (row >= a.rows.n) return;
-  uint32_t key[CAP];
-  load_keys<DT, CAP>(a.rows, row, 0, a.rows.actions, key);
-  uint32_t top = 0;
+  float x[CAP];
+  load_logits<DT, CAP>(reinterpret_cast<const T*>(a.rows.logits) + row * a.rows.row_stride, a.rows.legal ? a.rows.legal + row * a.rows.legal_stride : nullptr,
+                       0, a.rows.actions, x);
+  Soft v{x[0], 0.0f, 0.0f};
 #pragma unroll
-  for (int i = 0; i < CAP; ++i) top = key[i] > top ? key[i] : top;
-  Soft v{-INFINITY, 0.0f, 0.0f};
-  if (top) {
-    v.m = value_of(top);
-#pragma unroll
-    for (int i = 0; i < CAP; ++i)
-      if (key[i]) {
-        const float x = value_of(key[i]);
-        const float d = x == v.m ? 0.0f : (x - v.m) * a.rate, e = exp_of(d);
-        v.s += e;
-        if (e > 0.0f) v.t = fmaf(d, e, v.t);
-      }
-  }
+  for (int i = 1; i < CAP; ++i) v.m = fmaxf(v.m, x[i]);
+  if (v.m > -INFINITY) soft_sums<CAP>(x, v.m, a.rate, &v.s, &v.t);
   finish_row<DT>(a, row, v);
 }
 template <int DT, int CAP>
@@ -855,13 +1019,14 @@ __global__ __launch_bounds__(256) void pcx_log_prob_rows_backward(LogProbArgs a)
   typedef typename Logit<DT>::T T;
   const int64_t row = (int64_t)blockIdx.x * 256 + threadIdx.x;
   if (row >= a.rows.n) return;
-  uint32_t key[CAP];
-  load_keys<DT, CAP>(a.rows, row, 0, a.rows.actions, key);
+  float x[CAP];
+  load_logits<DT, CAP>(reinterpret_cast<const T*>(a.rows.logits) + row * a.rows.row_stride, a.rows.legal ? a.rows.legal + row * a.rows.legal_stride : nullptr,
+                       0, a.rows.actions, x);
   const RowGrad g = row_grad(a, row);
   T* const out = reinterpret_cast<T*>(a.grad) + row * a.rows.actions;
 #pragma unroll
   for (int i = 0; i < CAP; ++i)
-    if (i < a.rows.actions) out[i] = Logit<DT>::put(element_grad(g, key[i], i, a.rate));
+    if (i < a.rows.actions) out[i] = Logit<DT>::put(element_grad(g, x[i], i, a.rate));
 }
 
 // ---------------------------------------------------------------- plans and entry points
@@ -925,9 +1090,9 @@ int sample_wide(const SampleArgs& a, void* workspace, hipStream_t st) {
     if (k || p_) {
       hipLaunchKernelGGL((pcx_sample_digit<DT>), grid, block, 0, st, w, 0, 0u);
       for (int by_mass = k ? 0 : 1; by_mass <= (p_ ? 1 : 0); ++by_mass)
-        for (int level = 0; level < 3; ++level) {
+        for (int level = 0; level < LEVELS<DT>; ++level) {
           if (level) hipLaunchKernelGGL((pcx_sample_digit<DT>), grid, block, 0, st, w, level, by_mass ? 4u : 2u);
-          hipLaunchKernelGGL(pcx_sample_edge, rows, block, 0, st, w, level, by_mass);
+          hipLaunchKernelGGL((pcx_sample_edge<DT>), rows, block, 0, st, w, level, by_mass);
         }
     }
     hipLaunchKernelGGL((pcx_sample_weigh<DT>), grid, block, 0, st, w);
