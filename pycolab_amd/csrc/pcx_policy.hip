@@ -108,21 +108,23 @@ __device__ __forceinline__ void load_keys(const Rows& rows, int64_t row, int j, 
 // exp(d) for d <= 0 in 64 bits, to about a unit in the last place: d = n ln 2 + r with ln 2 in two parts, the upper one short
 // enough that n times it is exact (the reduction of Cody and Waite), the Taylor series
 // of exp(r), |r| <= ln(2) / 2, to r^13 / 13! (the next term is 4e-18), and n in the exponent.
+// (The coefficients are held in scalar registers: left to itself the compiler copies each into vector registers for every
+// element, two instructions a term, and took 454 registers for 16 elements.)
+__device__ __forceinline__ double scalar(double c) { asm("" : "+s"(c)); return c; }
 __device__ __forceinline__ double exp64(double d) {
   d = fmax(d, -800.0);
-  const double n = rint(d * 1.4426950408889634);
-  const double r = fma(n, -1.9082149292705877e-10, fma(n, -0.6931471803691238, d));
-  double p = 1.0 / 6227020800.0;
-  p = fma(p, r, 1.0 / 479001600.0);
-  p = fma(p, r, 1.0 / 39916800.0);
-  p = fma(p, r, 1.0 / 3628800.0);
-  p = fma(p, r, 1.0 / 362880.0);
-  p = fma(p, r, 1.0 / 40320.0);
-  p = fma(p, r, 1.0 / 5040.0);
-  p = fma(p, r, 1.0 / 720.0);
-  p = fma(p, r, 1.0 / 120.0);
-  p = fma(p, r, 1.0 / 24.0);
-  p = fma(p, r, 1.0 / 6.0);
+  const double n = rint(d * scalar(1.4426950408889634));
+  const double r = fma(n, scalar(-1.9082149292705877e-10), fma(n, scalar(-0.6931471803691238), d));
+  double p = fma(r, scalar(1.0 / 6227020800.0), scalar(1.0 / 479001600.0));
+  p = fma(p, r, scalar(1.0 / 39916800.0));
+  p = fma(p, r, scalar(1.0 / 3628800.0));
+  p = fma(p, r, scalar(1.0 / 362880.0));
+  p = fma(p, r, scalar(1.0 / 40320.0));
+  p = fma(p, r, scalar(1.0 / 5040.0));
+  p = fma(p, r, scalar(1.0 / 720.0));
+  p = fma(p, r, scalar(1.0 / 120.0));
+  p = fma(p, r, scalar(1.0 / 24.0));
+  p = fma(p, r, scalar(1.0 / 6.0));
   p = fma(p, r, 0.5);
   p = fma(p, r, 1.0);
   p = fma(p, r, 1.0);
@@ -428,8 +430,8 @@ __device__ __forceinline__ int choose(Group<THREADS>& g, uint32_t* key, uint32_t
   double w[EP];
 #pragma unroll
   for (int i = 0; i < EP; ++i) {
-    w[i] = 0.0;
-    if (__ballot(key[i] != 0)) w[i] = key[i] ? weight_of(value_of<DT>(key[i]), best, rate) : 0.0;  // (whole waves of nothing left are common)
+    const double v = weight_of(value_of<DT>(key[i] ? key[i] : best_key), best, rate);
+    w[i] = key[i] ? v : 0.0;
   }
   if (r.top_p < 1.0f) {
     double total = 0.0;
@@ -459,7 +461,7 @@ __device__ __forceinline__ int choose(Group<THREADS>& g, uint32_t* key, uint32_t
 // row, it first cuts at the k-th largest of the threads' largest keys -- at least k elements reach that, and seldom many
 // more -- and one wave chooses among those alone: no 64-bit exponentials and no workgroup-wide searches for the rest.
 template <int DT, int THREADS, int EP>
-__global__ __launch_bounds__(THREADS < 256 ? 256 : THREADS) void pcx_sample_group(SampleArgs a) {
+__global__ __launch_bounds__(THREADS < 256 ? 256 : THREADS, EP <= 8 ? 5 : EP == 16 ? 4 : 2) void pcx_sample_group(SampleArgs a) {
   constexpr int ROWS = THREADS < 256 ? 256 / THREADS : 1;
   constexpr int FEW = 512;  // elements a wave chooses among
   __shared__ typename Group<THREADS>::Scratch scratch[ROWS];
@@ -1117,7 +1119,9 @@ int sample_type(const SampleArgs& all, void* workspace, hipStream_t st) {
     if (A <= 8) hipLaunchKernelGGL((pcx_sample_rows<DT, 8>), per_thread, block, 0, st, a);
     else if (A <= 16) hipLaunchKernelGGL((pcx_sample_rows<DT, 16>), per_thread, block, 0, st, a);
     else if (A <= 128) hipLaunchKernelGGL((pcx_sample_group<DT, 64, 2>), per_wave, block, 0, st, a);
+    else if (A <= 256) hipLaunchKernelGGL((pcx_sample_group<DT, 64, 4>), per_wave, block, 0, st, a);
     else if (A <= 512) hipLaunchKernelGGL((pcx_sample_group<DT, 64, 8>), per_wave, block, 0, st, a);
+    else if (A <= 1024) hipLaunchKernelGGL((pcx_sample_group<DT, 64, 16>), per_wave, block, 0, st, a);
     else if (A <= 4096) hipLaunchKernelGGL((pcx_sample_group<DT, 256, 16>), per_group, block, 0, st, a);
     else hipLaunchKernelGGL((pcx_sample_group<DT, 512, 32>), per_group, dim3(512), 0, st, a);
   }
