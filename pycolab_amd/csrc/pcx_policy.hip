@@ -108,27 +108,55 @@ __device__ __forceinline__ void load_keys(const Rows& rows, int64_t row, int j, 
 // exp(d) for d <= 0 in 64 bits, to about a unit in the last place: d = n ln 2 + r with ln 2 in two parts, the upper one short
 // enough that n times it is exact (the reduction of Cody and Waite), the Taylor series
 // of exp(r), |r| <= ln(2) / 2, to r^13 / 13! (the next term is 4e-18), and n in the exponent.
-// (The coefficients are held in scalar registers: left to itself the compiler copies each into vector registers for every
-// element, two instructions a term, and took 454 registers for 16 elements.)
+// Four at a time: a chain of twenty dependent instructions leaves the unit idle, four side by side do not (33 million
+// logits: 20 -> 11 us); and the coefficients are held in scalar registers, which the four share -- left to itself the
+// compiler copies each into vector registers for every element.
 __device__ __forceinline__ double scalar(double c) { asm("" : "+s"(c)); return c; }
-__device__ __forceinline__ double exp64(double d) {
-  d = fmax(d, -800.0);
-  const double n = rint(d * scalar(1.4426950408889634));
-  const double r = fma(n, scalar(-1.9082149292705877e-10), fma(n, scalar(-0.6931471803691238), d));
-  double p = fma(r, scalar(1.0 / 6227020800.0), scalar(1.0 / 479001600.0));
-  p = fma(p, r, scalar(1.0 / 39916800.0));
-  p = fma(p, r, scalar(1.0 / 3628800.0));
-  p = fma(p, r, scalar(1.0 / 362880.0));
-  p = fma(p, r, scalar(1.0 / 40320.0));
-  p = fma(p, r, scalar(1.0 / 5040.0));
-  p = fma(p, r, scalar(1.0 / 720.0));
-  p = fma(p, r, scalar(1.0 / 120.0));
-  p = fma(p, r, scalar(1.0 / 24.0));
-  p = fma(p, r, scalar(1.0 / 6.0));
-  p = fma(p, r, 0.5);
-  p = fma(p, r, 1.0);
-  p = fma(p, r, 1.0);
-  return ldexp(p, (int)n);
+template <int N>
+__device__ __forceinline__ void exp64(double* d) {
+  double n[N], p[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) d[i] = fmax(d[i], -800.0);
+  const double log2e = scalar(1.4426950408889634), ln2_hi = scalar(-0.6931471803691238), ln2_lo = scalar(-1.9082149292705877e-10);
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    n[i] = rint(d[i] * log2e);
+    d[i] = fma(n[i], ln2_hi, d[i]);
+    d[i] = fma(n[i], ln2_lo, d[i]);
+    p[i] = 1.0 / 6227020800.0;
+  }
+  constexpr double C[13] = {1.0 / 479001600.0, 1.0 / 39916800.0, 1.0 / 3628800.0, 1.0 / 362880.0, 1.0 / 40320.0, 1.0 / 5040.0, 1.0 / 720.0,
+                            1.0 / 120.0, 1.0 / 24.0, 1.0 / 6.0, 0.5, 1.0, 1.0};
+#pragma unroll
+  for (int k = 0; k < 13; ++k) {
+    const double c = scalar(C[k]);
+#pragma unroll
+    for (int i = 0; i < N; ++i) p[i] = fma(p[i], d[i], c);
+  }
+#pragma unroll
+  for (int i = 0; i < N; ++i) d[i] = ldexp(p[i], (int)n[i]);
+}
+// exp((x - best) * rate); 0 for -infinity, 1 where x is the best, infinite or not.
+template <int N>
+__device__ __forceinline__ void weights(const float* x, float best, double rate, double* w) {
+  constexpr int AT_ONCE = N % 4 == 0 ? 4 : N % 2 == 0 ? 2 : 1;
+#pragma unroll
+  for (int i = 0; i < N; i += AT_ONCE) {
+    double d[AT_ONCE];
+#pragma unroll
+    for (int c = 0; c < AT_ONCE; ++c) {
+      const double v = ((double)x[i + c] - (double)best) * rate;
+      d[c] = x[i + c] == best ? 0.0 : v;
+    }
+    exp64<AT_ONCE>(d);
+#pragma unroll
+    for (int c = 0; c < AT_ONCE; ++c) w[i + c] = d[c];
+  }
+}
+__device__ __forceinline__ double weight_of(float x, float best, double rate) {
+  double w;
+  weights<1>(&x, best, rate, &w);
+  return w;
 }
 
 // ---------------------------------------------------------------- reductions over a group of THREADS (one wave, or a workgroup)
@@ -258,8 +286,13 @@ struct SampleArgs {
   int32_t* out;
 };
 
-__device__ __forceinline__ double weight_of(float x, float best, double rate) {
-  return exp64(x == best ? 0.0 : ((double)x - (double)best) * rate);
+// The weights of N keys (0: none).
+template <int DT, int N>
+__device__ __forceinline__ void key_weights(const uint32_t* key, float best, double rate, double* w) {
+  float x[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) x[i] = key[i] ? value_of<DT>(key[i]) : -INFINITY;
+  weights<N>(x, best, rate, w);
 }
 
 // A thread holds a whole row: few actions, many rows.
@@ -282,8 +315,7 @@ __global__ __launch_bounds__(256) void pcx_sample_rows(SampleArgs a) {
   if (first == NONE || !(r.temperature > 0.0f)) { a.out[row] = first; return; }
   const double rate = 1.0 / (double)r.temperature;
   double w[CAP];
-#pragma unroll
-  for (int j = 0; j < CAP; ++j) w[j] = x[j] > -INFINITY ? weight_of(x[j], best, rate) : 0.0;
+  weights<CAP>(x, best, rate, w);
   if (r.top_k > 0 && r.top_k < A) {
 #pragma unroll
     for (int j = 0; j < CAP; ++j) {
@@ -428,11 +460,7 @@ __device__ __forceinline__ int choose(Group<THREADS>& g, uint32_t* key, uint32_t
   const float best = value_of<DT>(best_key);
   const double rate = 1.0 / (double)r.temperature;
   double w[EP];
-#pragma unroll
-  for (int i = 0; i < EP; ++i) {
-    const double v = weight_of(value_of<DT>(key[i] ? key[i] : best_key), best, rate);
-    w[i] = key[i] ? v : 0.0;
-  }
+  key_weights<DT, EP>(key, best, rate, w);
   if (r.top_p < 1.0f) {
     double total = 0.0;
 #pragma unroll
@@ -624,13 +652,25 @@ __global__ __launch_bounds__(256) void pcx_sample_digit(WideArgs w, int level, u
   const double rate = 1.0 / (double)r.temperature;
   for (int i = threadIdx.x; i < BINS; i += 256) { mass[i] = 0; count[i] = 0; }
   __syncthreads();
+#pragma unroll 1
+  for (int i = 0; i < WEP; i += 4) {
+    bool mine[4];
 #pragma unroll
-  for (int i = 0; i < WEP; ++i)
-    if (key[i] && same_prefix<DT>(key[i], st.prefix, level)) {
-      const uint32_t d = digit_of<DT>(key[i], level);
-      atomicAdd(&count[d], 1u);
-      atomicAdd(&mass[d], (unsigned long long)(ldexp(weight_of(value_of<DT>(key[i]), best, rate), w.scale) + 0.5));
+    for (int c = 0; c < 4; ++c) mine[c] = key[c] && same_prefix<DT>(key[c], st.prefix, level);
+    if (__ballot(mine[0] || mine[1] || mine[2] || mine[3])) {  // (later digits concern few)
+      double v[4];
+      key_weights<DT, 4>(key, best, rate, v);
+#pragma unroll
+      for (int c = 0; c < 4; ++c)
+        if (mine[c]) {
+          const uint32_t d = digit_of<DT>(key[c], level);
+          atomicAdd(&count[d], 1u);
+          atomicAdd(&mass[d], (unsigned long long)(ldexp(v[c], w.scale) + 0.5));
+        }
     }
+#pragma unroll
+    for (int c = 0; c < WEP - 4; ++c) key[c] = key[c + 4];
+  }
   __syncthreads();
   const int64_t at = ((int64_t)(level != 0) * w.batch + row) * BINS;
   for (int i = threadIdx.x; i < BINS; i += 256)
@@ -738,12 +778,16 @@ __global__ __launch_bounds__(256) void pcx_sample_weigh(WideArgs w) {
   double mine = 0.0;
   uint32_t ties = 0;
 #pragma unroll
-  for (int i = 0; i < WEP; ++i) {
-    if (key[i] > st.edge) {
-      const double v = weight_of(value_of<DT>(key[i]), best, rate);
-      if (v >= (double)r.min_p) mine += v;
+  for (int i = 0; i < WEP; i += 4) {
+    double v[4];
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      ties += ballots(st.edge && key[i + c] == st.edge);
+      if (key[i + c] <= st.edge) key[i + c] = 0;
     }
-    ties += ballots(st.edge && key[i] == st.edge);
+    key_weights<DT, 4>(key + i, best, rate, v);
+#pragma unroll
+    for (int c = 0; c < 4; ++c) mine += v[c] >= (double)r.min_p ? v[c] : 0.0;
   }
   mine = g.sum(mine);
   ties = g.count(ties);
@@ -816,10 +860,12 @@ __global__ __launch_bounds__(256) void pcx_sample_pick(WideArgs w) {
   double v[WEP];
   load_keys<DT, WEP>(w.a.rows, at, j0, end, key);
 #pragma unroll
-  for (int i = 0; i < WEP; ++i) {
-    v[i] = key[i] && key[i] >= st.edge ? weight_of(value_of<DT>(key[i]), best, rate) : 0.0;
+  for (int i = 0; i < WEP; ++i)
+    if (key[i] < st.edge) key[i] = 0;
+  key_weights<DT, WEP>(key, best, rate, v);
+#pragma unroll
+  for (int i = 0; i < WEP; ++i)
     if (v[i] < (double)r.min_p) v[i] = 0.0;
-  }
   if (st.edge) drop_ties<256, WEP>(g, st.edge, ties_left, key, v);
   const int pick = draw_action<256, WEP>(g, v, goal, offset, true);
   if (threadIdx.x == 0) w.a.out[at] = lo + pick;
