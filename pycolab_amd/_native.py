@@ -6,6 +6,7 @@ is no CPU fallback behind it.
 
 import ctypes
 import os
+import struct
 
 c_u8, c_i32, c_i64, c_u32, c_u64 = (ctypes.c_uint8, ctypes.c_int32,
                                     ctypes.c_int64, ctypes.c_uint32,
@@ -149,6 +150,11 @@ class Sampling(ctypes.Structure):
               ('min_p_row', ctypes.c_void_p)]
 
 
+# ... and their bytes, in the same order
+PROJECT_HEAD, PROJECT_OFFSETS, PROJECT_TAIL = struct.Struct('=qq'), struct.Struct('=%dq' % POST_MAX_DEPTH), struct.Struct('=6i%ds' % POST_MAX_DEPTH)
+LOGITS_DESC, SAMPLING = struct.Struct('=qqqii'), struct.Struct('=fffiQQQQ')
+
+
 # Every symbol include/pcx.h declares: (name, restype, argtypes).
 _VP = ctypes.c_void_p
 SYMBOLS = [
@@ -213,15 +219,16 @@ SYMBOLS = [
     ('pcx_post_bind_output', c_i32, [_VP, _VP, c_u64]),
     ('pcx_post_error_buffer', c_i32, [_VP, ctypes.POINTER(_VP)]),
     ('pcx_post_error_poll', c_i32, [_VP, _VP, ctypes.POINTER(c_i32)]),
-    ('pcx_project_sizes', c_i32, [ctypes.POINTER(ProjectDesc), ctypes.POINTER(c_u64), ctypes.POINTER(c_u64), ctypes.POINTER(c_u64)]),
-    ('pcx_project_pack', c_i32, [ctypes.POINTER(ProjectDesc), _VP, _VP, _VP]),
-    ('pcx_project_forward', c_i32, [ctypes.POINTER(ProjectDesc), _VP, _VP, _VP, _VP, _VP, _VP, _VP, c_u64, _VP]),
-    ('pcx_project_backward', c_i32, [ctypes.POINTER(ProjectDesc), _VP, _VP, _VP, _VP, _VP, _VP, c_u64, _VP]),
-    ('pcx_sample_size', c_i32, [ctypes.POINTER(LogitsDesc), ctypes.POINTER(c_u64)]),
-    ('pcx_sample_actions', c_i32, [ctypes.POINTER(LogitsDesc), ctypes.POINTER(Sampling), _VP, _VP, _VP, _VP, _VP, c_u64, _VP]),
-    ('pcx_log_prob_size', c_i32, [ctypes.POINTER(LogitsDesc), ctypes.POINTER(c_u64)]),
-    ('pcx_log_prob', c_i32, [ctypes.POINTER(LogitsDesc), ctypes.c_float, _VP, _VP, _VP, _VP, _VP, _VP, _VP, c_u64, _VP]),
-    ('pcx_log_prob_backward', c_i32, [ctypes.POINTER(LogitsDesc), ctypes.c_float, _VP, _VP, _VP, _VP, _VP, _VP, _VP, _VP, _VP]),
+    # (the policy operators' descriptions are passed as the structure's bytes: no ctypes object is built per call)
+    ('pcx_project_sizes', c_i32, [_VP, _VP, _VP, _VP]),
+    ('pcx_project_pack', c_i32, [_VP, _VP, _VP, _VP]),
+    ('pcx_project_forward', c_i32, [_VP, _VP, _VP, _VP, _VP, _VP, _VP, _VP, c_u64, _VP]),
+    ('pcx_project_backward', c_i32, [_VP, _VP, _VP, _VP, _VP, _VP, _VP, c_u64, _VP]),
+    ('pcx_sample_size', c_i32, [_VP, _VP]),
+    ('pcx_sample_actions', c_i32, [_VP, _VP, _VP, _VP, _VP, _VP, _VP, c_u64, _VP]),
+    ('pcx_log_prob_size', c_i32, [_VP, _VP]),
+    ('pcx_log_prob', c_i32, [_VP, ctypes.c_float, _VP, _VP, _VP, _VP, _VP, _VP, _VP, c_u64, _VP]),
+    ('pcx_log_prob_backward', c_i32, [_VP, ctypes.c_float, _VP, _VP, _VP, _VP, _VP, _VP, _VP, _VP, _VP]),
     ('pcx_gather_create', c_i32, [ctypes.POINTER(_VP), c_i32, ctypes.POINTER(_VP)]),
     ('pcx_gather_destroy', None, [_VP]),
     ('pcx_gather_scalars', c_i32, [_VP, ctypes.POINTER(_VP)]),

@@ -13,8 +13,6 @@ log-probability of actions taken and the policy's entropy, differentiable in
 the logits.  Both run as kernels of csrc/pcx_policy.hip on PyTorch tensors.
 """
 
-import ctypes
-
 import numpy as np
 
 from pycolab_amd import _native as N
@@ -46,35 +44,33 @@ def hashed_tape(seed, env_lo, n_envs, t0, steps, n_actions):
 # ---------------------------------------------------------------------- a policy's actions
 
 
-def _rows(logits, legal):
-  """(description, legal tensor to keep) of logits [n, actions] whose actions are contiguous."""
-  torch = dev.require_torch('a policy over actions')
+def _rows(torch, logits, legal):
+  """(description, legal tensor to keep, rows, actions, device index) of logits [n, actions] whose actions are contiguous."""
   if not isinstance(logits, torch.Tensor) or not logits.is_cuda or logits.dim() != 2:
     raise ValueError('logits must be a device tensor [n, actions]')
-  d = N.LogitsDesc()
-  d.dtype = dev.policy_dtype(logits, 'logits')
-  d.n, d.actions = int(logits.shape[0]), int(logits.shape[1])
-  if d.actions < 1:
+  dtype = dev.policy_dtype(logits, 'logits')
+  n, actions = logits.shape
+  row_stride, stride = logits.stride()
+  if actions < 1:
     raise ValueError('logits of no action')
-  if d.actions > 1 and logits.stride(1) != 1:
+  if actions > 1 and stride != 1:
     raise ValueError('the actions of a row must be contiguous (strides {})'.format(logits.stride()))
-  d.row_stride = int(logits.stride(0))
+  legal_stride = 0
   if legal is not None:
     if not isinstance(legal, torch.Tensor) or legal.device != logits.device or legal.dtype not in (torch.bool, torch.uint8):
       raise ValueError('legal must be a bool or uint8 tensor on {}'.format(logits.device))
-    if tuple(legal.shape) == (d.actions,):
-      legal = legal.expand(d.n, d.actions)
-    if tuple(legal.shape) != tuple(logits.shape):
-      raise ValueError('legal must be [{}, {}] or [{}]'.format(d.n, d.actions, d.actions))
-    if d.actions > 1 and legal.stride(1) != 1:
+    if legal.dim() == 1 and legal.shape[0] == actions:
+      legal = legal.expand(n, actions)
+    if legal.shape != logits.shape:
+      raise ValueError('legal must be [{}, {}] or [{}]'.format(n, actions, actions))
+    legal_stride, stride = legal.stride()
+    if actions > 1 and stride != 1:
       raise ValueError('the actions of a row of `legal` must be contiguous')
-    d.legal_stride = int(legal.stride(0))
-  return d, legal
+  return N.LOGITS_DESC.pack(n, row_stride, legal_stride, actions, dtype), legal, n, actions, logits.device.index
 
 
-def _per_row(value, name, n, dtype, device):
+def _per_row(torch, value, name, n, dtype, device):
   """A rule's device array [n], or None for a number."""
-  torch = dev.torch_module()
   if not isinstance(value, torch.Tensor):
     return None
   if value.dtype != dtype or value.device != device or tuple(value.shape) != (n,):
@@ -96,68 +92,60 @@ def sample(logits, uniforms, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, leg
 
   `out`: an int32 tensor [n] to write into.  Nothing waits for the device; calls can be captured into a graph."""
   torch = dev.require_torch('sample()')
-  d, legal = _rows(logits, legal)
-  if not isinstance(uniforms, torch.Tensor) or uniforms.dtype != torch.float32 or uniforms.device != logits.device or tuple(uniforms.shape) != (d.n,):
-    raise ValueError('uniforms must be float32 [{}] on {}'.format(d.n, logits.device))
-  r = N.Sampling()
-  rows = [_per_row(v, name, d.n, dtype, logits.device) for v, name, dtype in (
-      (temperature, 'temperature', torch.float32), (top_k, 'top_k', torch.int32), (top_p, 'top_p', torch.float32), (min_p, 'min_p', torch.float32))]
-  r.temperature_row, r.top_k_row, r.top_p_row, r.min_p_row = [dev.pointer(t) for t in rows]
-  if rows[0] is None:
-    r.temperature = float(temperature)
-  if rows[1] is None:
+  desc, legal, n, _, index = _rows(torch, logits, legal)
+  device = logits.device
+  if (not isinstance(uniforms, torch.Tensor) or uniforms.dtype != torch.float32 or uniforms.device != device or uniforms.dim() != 1 or
+      uniforms.shape[0] != n):
+    raise ValueError('uniforms must be float32 [{}] on {}'.format(n, device))
+  t_row = _per_row(torch, temperature, 'temperature', n, torch.float32, device)
+  k_row = _per_row(torch, top_k, 'top_k', n, torch.int32, device)
+  p_row = _per_row(torch, top_p, 'top_p', n, torch.float32, device)
+  m_row = _per_row(torch, min_p, 'min_p', n, torch.float32, device)
+  if k_row is None:
     if int(top_k) != top_k:
       raise ValueError('top_k must be a whole number')
-    r.top_k = max(-1, min(int(top_k), 1 << 30))
-  if rows[2] is None:
-    r.top_p = float(top_p)
-  if rows[3] is None:
-    r.min_p = float(min_p)
+    top_k = max(-1, min(int(top_k), 1 << 30))
+  rules = N.SAMPLING.pack(0.0 if t_row is not None else float(temperature), 0.0 if p_row is not None else float(top_p),
+                          0.0 if m_row is not None else float(min_p), 0 if k_row is not None else top_k,
+                          dev.pointer(t_row) or 0, dev.pointer(k_row) or 0, dev.pointer(p_row) or 0, dev.pointer(m_row) or 0)
   if out is None:
-    out = torch.empty((d.n,), dtype=torch.int32, device=logits.device)
-  elif out.dtype != torch.int32 or out.device != logits.device or tuple(out.shape) != (d.n,) or not out.is_contiguous():
-    raise ValueError('out must be a contiguous int32 tensor [{}] on {}'.format(d.n, logits.device))
+    out = torch.empty((n,), dtype=torch.int32, device=device)
+  elif out.dtype != torch.int32 or out.device != device or tuple(out.shape) != (n,) or not out.is_contiguous():
+    raise ValueError('out must be a contiguous int32 tensor [{}] on {}'.format(n, device))
   uniforms = uniforms.contiguous()
-  with torch.cuda.device(logits.device):
-    scratch = N.c_u64(0)
-    N.check(N.lib().pcx_sample_size(ctypes.byref(d), ctypes.byref(scratch)))
-    ws = torch.empty(scratch.value, dtype=torch.uint8, device=logits.device) if scratch.value else None
-    N.check(N.lib().pcx_sample_actions(ctypes.byref(d), ctypes.byref(r), logits.data_ptr(), dev.pointer(legal), uniforms.data_ptr(),
-                                       out.data_ptr(), dev.pointer(ws), scratch.value, dev.current_stream(logits.device.index)))
+  scratch, size = dev.workspace('pcx_sample_size', desc, device)
+  dev.launch(index, N.lib().pcx_sample_actions, desc, rules, logits.data_ptr(), dev.pointer(legal), uniforms.data_ptr(), out.data_ptr(),
+             dev.pointer(scratch), size)
   return out
 
 
-def _taken(actions, n, device):
-  torch = dev.torch_module()
+def _taken(torch, actions, n, device):
   if not isinstance(actions, torch.Tensor) or actions.dtype != torch.int32 or actions.device != device or tuple(actions.shape) != (n,):
     raise ValueError('actions must be int32 [{}] on {}'.format(n, device))
   return actions.contiguous()
 
 
-def _log_prob_forward(d, legal, logits, actions, temperature):
-  torch = dev.torch_module()
-  log_prob, entropy = (torch.empty((d.n,), dtype=torch.float32, device=logits.device) for _ in range(2))
-  stats = torch.empty((d.n, 2), dtype=torch.float32, device=logits.device)
-  with torch.cuda.device(logits.device):
-    scratch = N.c_u64(0)
-    N.check(N.lib().pcx_log_prob_size(ctypes.byref(d), ctypes.byref(scratch)))
-    ws = torch.empty(scratch.value, dtype=torch.uint8, device=logits.device) if scratch.value else None
-    N.check(N.lib().pcx_log_prob(ctypes.byref(d), temperature, logits.data_ptr(), dev.pointer(legal), actions.data_ptr(), log_prob.data_ptr(),
-                                 entropy.data_ptr(), stats.data_ptr(), dev.pointer(ws), scratch.value, dev.current_stream(logits.device.index)))
+def _log_prob_forward(torch, desc, legal, logits, actions, temperature):
+  n, device = logits.shape[0], logits.device
+  both = torch.empty((2, n), dtype=torch.float32, device=device)
+  log_prob, entropy = both.unbind(0)
+  stats = torch.empty((n, 2), dtype=torch.float32, device=device)
+  scratch, size = dev.workspace('pcx_log_prob_size', desc, device)
+  start = both.data_ptr()
+  dev.launch(device.index, N.lib().pcx_log_prob, desc, temperature, logits.data_ptr(), dev.pointer(legal), actions.data_ptr(), start,
+             start + 4 * n, stats.data_ptr(), dev.pointer(scratch), size)
   return log_prob, entropy, stats
 
 
-def _log_prob_backward(d, legal, logits, actions, temperature, entropy, stats, grad_log_prob, grad_entropy):
-  torch = dev.torch_module()
-  grad = torch.empty((d.n, d.actions), dtype=logits.dtype, device=logits.device)
+def _log_prob_backward(torch, desc, legal, logits, actions, temperature, entropy, stats, grad_log_prob, grad_entropy):
+  n, device = logits.shape[0], logits.device
+  grad = torch.empty(logits.shape, dtype=logits.dtype, device=device)
   for g, name in ((grad_log_prob, 'grad_log_prob'), (grad_entropy, 'grad_entropy')):
-    if g is not None and (g.dtype != torch.float32 or tuple(g.shape) != (d.n,) or g.device != logits.device):
-      raise ValueError('{} must be float32 [{}] on {}'.format(name, d.n, logits.device))
+    if g is not None and (g.dtype != torch.float32 or g.dim() != 1 or g.shape[0] != n or g.device != device):
+      raise ValueError('{} must be float32 [{}] on {}'.format(name, n, device))
   grad_log_prob, grad_entropy = (None if g is None else g.contiguous() for g in (grad_log_prob, grad_entropy))
-  with torch.cuda.device(logits.device):
-    N.check(N.lib().pcx_log_prob_backward(ctypes.byref(d), temperature, logits.data_ptr(), dev.pointer(legal), actions.data_ptr(), entropy.data_ptr(),
-                                          stats.data_ptr(), dev.pointer(grad_log_prob), dev.pointer(grad_entropy), grad.data_ptr(),
-                                          dev.current_stream(logits.device.index)))
+  dev.launch(device.index, N.lib().pcx_log_prob_backward, desc, temperature, logits.data_ptr(), dev.pointer(legal), actions.data_ptr(),
+             entropy.data_ptr(), stats.data_ptr(), dev.pointer(grad_log_prob), dev.pointer(grad_entropy), grad.data_ptr())
   return grad
 
 
@@ -173,20 +161,20 @@ def _log_prob_autograd():
     class LogProb(torch.autograd.Function):
 
       @staticmethod
-      def forward(ctx, logits, actions, legal, temperature, d):
+      def forward(ctx, logits, actions, legal, temperature, desc):
         ctx.set_materialize_grads(False)
-        log_prob, entropy, stats = _log_prob_forward(d, legal, logits, actions, temperature)
-        ctx.d, ctx.temperature = d, temperature
+        log_prob, entropy, stats = _log_prob_forward(torch, desc, legal, logits, actions, temperature)
+        ctx.desc, ctx.temperature = desc, temperature
         ctx.save_for_backward(logits, actions, legal, entropy, stats)
         return log_prob, entropy
 
       @staticmethod
-      @torch.autograd.function.once_differentiable
       def backward(ctx, grad_log_prob, grad_entropy):
+        dev.refuse_twice('log_prob')
         logits, actions, legal, entropy, stats = ctx.saved_tensors
         if grad_log_prob is None and grad_entropy is None:
           return None, None, None, None, None
-        return (_log_prob_backward(ctx.d, legal, logits, actions, ctx.temperature, entropy, stats, grad_log_prob, grad_entropy),
+        return (_log_prob_backward(torch, ctx.desc, legal, logits, actions, ctx.temperature, entropy, stats, grad_log_prob, grad_entropy),
                 None, None, None, None)
 
     _log_prob_function = LogProb
@@ -212,23 +200,23 @@ def log_prob(logits, actions, legal=None, temperature=1.0, return_stats=False):
   `return_stats=True`: no autograd; returns (log_prob, entropy, stats), what `log_prob_backward` takes -- the pair to
   capture into a graph."""
   torch = dev.require_torch('log_prob()')
-  d, legal = _rows(logits, legal)
-  actions, temperature = _taken(actions, d.n, logits.device), _positive(temperature)
+  desc, legal, n, _, _ = _rows(torch, logits, legal)
+  actions, temperature = _taken(torch, actions, n, logits.device), _positive(temperature)
   if return_stats:
-    return _log_prob_forward(d, legal, logits.detach(), actions, temperature)
-  if torch.is_grad_enabled() and logits.requires_grad:
+    return _log_prob_forward(torch, desc, legal, logits.detach(), actions, temperature)
+  if logits.requires_grad and torch.is_grad_enabled():
     dev.refuse_recording_in_capture('log_prob', 'log_prob(..., return_stats=True) and log_prob_backward()')
-    return _log_prob_autograd().apply(logits, actions, legal, temperature, d)
-  return _log_prob_forward(d, legal, logits, actions, temperature)[:2]
+    return _log_prob_autograd().apply(logits, actions, legal, temperature, desc)
+  return _log_prob_forward(torch, desc, legal, logits, actions, temperature)[:2]
 
 
 def log_prob_backward(logits, actions, entropy, stats, grad_log_prob=None, grad_entropy=None, legal=None, temperature=1.0):
   """The gradient with respect to `logits` of `log_prob()`'s two results, from theirs (float32 [n], None: zero) and from the
   `entropy` and `stats` it returned.  Records nothing for autograd and waits for nothing: it may be captured."""
   torch = dev.require_torch('log_prob_backward()')
-  d, legal = _rows(logits, legal)
-  actions, temperature = _taken(actions, d.n, logits.device), _positive(temperature)
-  for t, shape, name in ((entropy, (d.n,), 'entropy'), (stats, (d.n, 2), 'stats')):
+  desc, legal, n, _, _ = _rows(torch, logits, legal)
+  actions, temperature = _taken(torch, actions, n, logits.device), _positive(temperature)
+  for t, shape, name in ((entropy, (n,), 'entropy'), (stats, (n, 2), 'stats')):
     if t.dtype != torch.float32 or tuple(t.shape) != shape or t.device != logits.device or not t.is_contiguous():
       raise ValueError('{} must be what log_prob(..., return_stats=True) returned'.format(name))
-  return _log_prob_backward(d, legal, logits, actions, temperature, entropy, stats, grad_log_prob, grad_entropy)
+  return _log_prob_backward(torch, desc, legal, logits, actions, temperature, entropy, stats, grad_log_prob, grad_entropy)

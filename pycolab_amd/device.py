@@ -99,6 +99,8 @@ def synchronize(device_id):
 
 
 # ---- the policy operators (rendering.project, actions.sample, actions.log_prob) work on PyTorch tensors ----------------
+# Their calls are small next to what they launch only if the way there is short: descriptions as packed bytes, the raw
+# stream, no context manager on the device that is current anyway.
 
 
 def require_torch(what):
@@ -108,17 +110,59 @@ def require_torch(what):
   return torch
 
 
+_kinds = None
+
+
 def policy_dtype(tensor, name):
   """The C ABI's number for a floating tensor's type."""
-  torch = torch_module()
-  kinds = {torch.float32: N.F32, torch.float16: N.F16, torch.bfloat16: N.BF16}
-  if tensor.dtype not in kinds:
+  global _kinds
+  if _kinds is None:
+    torch = torch_module()
+    _kinds = {torch.float32: N.F32, torch.float16: N.F16, torch.bfloat16: N.BF16}
+  kind = _kinds.get(tensor.dtype)
+  if kind is None:
     raise TypeError('{} must be float32, float16 or bfloat16, not {}'.format(name, tensor.dtype))
-  return kinds[tensor.dtype]
+  return kind
 
 
 def pointer(tensor):
   return None if tensor is None else tensor.data_ptr()
+
+
+def launch(device_id, function, *args):
+  """function(*args, stream) of the C ABI on `device_id`'s current stream."""
+  torch = torch_module()
+  if torch.cuda.current_device() != device_id:
+    with torch.cuda.device(device_id):
+      code = function(*args, torch.cuda.current_stream(device_id).cuda_stream)
+  else:
+    code = function(*args, _raw_stream(torch, device_id))
+  if code:
+    N.check(code)
+
+
+def _raw_stream(torch, device_id):
+  raw = getattr(torch._C, '_cuda_getCurrentRawStream', None)  # (the stream without the Python object around it)
+  return raw(device_id) if raw is not None else torch.cuda.current_stream(device_id).cuda_stream
+
+
+_sizes = {}
+
+
+def workspace(function, desc, device):
+  """(tensor or None, bytes): the workspace that `function` (pcx_..._size) asks for a description, for this call alone."""
+  key = (function, desc)
+  size = _sizes.get(key)
+  if size is None:
+    out = N.c_u64(0)
+    N.check(getattr(N.lib(), function)(desc, ctypes.byref(out)))
+    if len(_sizes) > 4096:
+      _sizes.clear()
+    size = _sizes[key] = int(out.value)
+  if not size:
+    return None, 0
+  torch = torch_module()
+  return torch.empty(size, dtype=torch.uint8, device=device), size
 
 
 def refuse_recording_in_capture(what, instead):
@@ -126,3 +170,9 @@ def refuse_recording_in_capture(what, instead):
   process: differentiable calls are refused under capture, the explicit pair of calls is what a graph holds."""
   if torch_module().cuda.is_current_stream_capturing():
     raise RuntimeError('{}() does not record gradients while a graph is captured: capture {} instead'.format(what, instead))
+
+
+def refuse_twice(what):
+  """Called in a backward pass: gradients are recorded there only when it is to be differentiated itself."""
+  if torch_module().is_grad_enabled():
+    raise RuntimeError('{}() cannot be differentiated twice'.format(what))

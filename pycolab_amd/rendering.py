@@ -686,6 +686,10 @@ class _Boards(object):
         self.offsets = [(1 + present.index(ord(c))) * view.pitch if ord(c) in present else -1 for c in layers]
 
 
+_NO_OFFSETS = bytes(8 * N.POST_MAX_DEPTH)
+_project_sizes = {}
+
+
 class _Projection(object):
   """The checked arguments of one projection: what the C ABI's description is made of."""
 
@@ -709,18 +713,16 @@ class _Projection(object):
     self.check_row(bias, 'bias', weight)
     if bias is not None and tuple(bias.shape) != (self.hidden,):
       raise ValueError('bias must be [{}], not {}'.format(self.hidden, list(bias.shape)))
-    self.torch_dtype = weight.dtype
-    d = self.desc = N.ProjectDesc()
-    d.cells, d.n_layers, d.hidden, d.dtype, d.activation = self.cells, depth, self.hidden, self.dtype, _ACTIVATIONS[activation]
-    for i, c in enumerate(layers):
-      d.chars[i] = ord(c)
+    self.torch_dtype, self.activation = weight.dtype, _ACTIVATIONS[activation]
+    chars = layers.encode('latin-1') if isinstance(layers, str) else bytes(ord(c) for c in layers)
+    self.tails = [N.PROJECT_TAIL.pack(self.cells, depth, self.hidden, self.dtype, self.activation, stacked, chars) for stacked in (0, 1)]
 
   def check_row(self, tensor, name, weight):
     if tensor is not None and (tensor.dtype != weight.dtype or tensor.device != weight.device):
       raise ValueError('{} must be {} on {}, like the weight'.format(name, weight.dtype, weight.device))
 
   def slope_dtype(self):
-    return self.torch_dtype if self.desc.activation == N.ACT_RELU else dev.torch_module().float32
+    return self.torch_dtype if self.activation == N.ACT_RELU else dev.torch_module().float32
 
   def check_rows(self, tensor, name, n, dtype=None):
     if tensor is None:
@@ -729,62 +731,66 @@ class _Projection(object):
       raise ValueError('{} must be {} [{}, {}] on {}'.format(name, dtype or self.torch_dtype, n, self.hidden, self.device))
 
   def at(self, boards):
-    """The description for these boards."""
+    """The description (the bytes of a pcx_project_desc) for these boards."""
     if boards.device_id != self.device.index:
       raise ValueError('the boards are on GPU {}, the weight is on GPU {}'.format(boards.device_id, self.device.index))
     if boards.rows * boards.cols != self.cells or (self.board and self.board != (boards.rows, boards.cols)):
       raise ValueError('the weight is for boards of {} cells, these are {} x {}'.format(
           '{} x {}'.format(*self.board) if self.board else self.cells, boards.rows, boards.cols))
-    d = self.desc
-    d.n, d.row_stride, d.stacked = boards.n, boards.row_stride, int(boards.offsets is not None)
-    if boards.offsets is not None:
-      for i, o in enumerate(boards.offsets):
-        d.layer_offset[i] = o
-    return d
+    if boards.offsets is None:
+      return N.PROJECT_HEAD.pack(boards.n, boards.row_stride) + _NO_OFFSETS + self.tails[0]
+    return (N.PROJECT_HEAD.pack(boards.n, boards.row_stride) +
+            N.PROJECT_OFFSETS.pack(*boards.offsets, *([0] * (N.POST_MAX_DEPTH - len(boards.offsets)))) + self.tails[1])
 
-  def sizes(self):
-    out = (N.c_u64(0), N.c_u64(0), N.c_u64(0))
-    N.check(N.lib().pcx_project_sizes(ctypes.byref(self.desc), *[ctypes.byref(x) for x in out]))
-    return [int(x.value) for x in out]
+  @staticmethod
+  def sizes(desc):
+    """Bytes of (the laid-out weight, the forward workspace, the backward workspace)."""
+    found = _project_sizes.get(desc)
+    if found is None:
+      out = (N.c_u64(0), N.c_u64(0), N.c_u64(0))
+      N.check(N.lib().pcx_project_sizes(desc, *[ctypes.byref(x) for x in out]))
+      if len(_project_sizes) > 4096:
+        _project_sizes.clear()
+      found = _project_sizes[desc] = tuple(int(x.value) for x in out)
+    return found
 
-  def pack(self, weight, packed=None):
+  def pack(self, desc, weight, packed=None):
     torch = dev.torch_module()
     if packed is None:
-      packed = torch.empty(self.sizes()[0], dtype=torch.uint8, device=self.device)
+      packed = torch.empty(self.sizes(desc)[0], dtype=torch.uint8, device=self.device)
     weight = weight.detach().contiguous()
-    N.check(N.lib().pcx_project_pack(ctypes.byref(self.desc), weight.data_ptr(), packed.data_ptr(), dev.current_stream(self.device.index)))
+    dev.launch(self.device.index, N.lib().pcx_project_pack, desc, weight.data_ptr(), packed.data_ptr())
     return packed
 
-  def forward(self, boards, packed, bias, residual, want_slope=False):
+  def forward(self, desc, boards, packed, bias, residual, want_slope=False):
     torch = dev.torch_module()
-    d = self.at(boards)
-    self.check_rows(residual, 'residual', boards.n)
+    if residual is not None:
+      self.check_rows(residual, 'residual', boards.n)
+      residual = residual.contiguous()
     out = torch.empty((boards.n, self.hidden), dtype=self.torch_dtype, device=self.device)
     slope = torch.empty(out.shape, dtype=self.slope_dtype(), device=self.device) if want_slope else None
-    scratch = self.sizes()[1]
-    ws = torch.empty(scratch, dtype=torch.uint8, device=self.device) if scratch else None
-    bias = None if bias is None else bias.detach().contiguous()
-    residual = None if residual is None else residual.detach().contiguous()
-    N.check(N.lib().pcx_project_forward(
-        ctypes.byref(d), boards.ptr, packed.data_ptr(), dev.pointer(bias), dev.pointer(residual), out.data_ptr(),
-        dev.pointer(slope), dev.pointer(ws), scratch, dev.current_stream(self.device.index)))
+    size = self.sizes(desc)[1]
+    scratch = torch.empty(size, dtype=torch.uint8, device=self.device) if size else None
+    if bias is not None:
+      bias = bias.contiguous()
+    dev.launch(self.device.index, N.lib().pcx_project_forward, desc, boards.ptr, packed.data_ptr(), dev.pointer(bias), dev.pointer(residual),
+               out.data_ptr(), dev.pointer(slope), dev.pointer(scratch), size)
     return out, slope
 
-  def backward(self, boards, grad, slope, want_weight, want_bias, weight_shape):
+  def backward(self, desc, boards, grad, slope, want_weight, want_bias, weight_shape):
     torch = dev.torch_module()
-    d = self.at(boards)
     self.check_rows(grad, 'grad', boards.n)
     self.check_rows(slope, 'slope', boards.n, self.slope_dtype())
     make = torch.zeros if boards.n == 0 else torch.empty
     dw = make(weight_shape, dtype=self.torch_dtype, device=self.device) if want_weight else None
     db = make((self.hidden,), dtype=self.torch_dtype, device=self.device) if want_bias else None
     if boards.n and (want_weight or want_bias):
-      scratch = self.sizes()[2]
-      ws = torch.empty(scratch, dtype=torch.uint8, device=self.device)
+      size = self.sizes(desc)[2]
+      scratch = torch.empty(size, dtype=torch.uint8, device=self.device)
       grad = grad.contiguous()
       slope = None if slope is None else slope.contiguous()
-      N.check(N.lib().pcx_project_backward(ctypes.byref(d), boards.ptr, grad.data_ptr(), dev.pointer(slope), dev.pointer(dw),
-                                           dev.pointer(db), ws.data_ptr(), scratch, dev.current_stream(self.device.index)))
+      dev.launch(self.device.index, N.lib().pcx_project_backward, desc, boards.ptr, grad.data_ptr(), dev.pointer(slope), dev.pointer(dw),
+                 dev.pointer(db), scratch.data_ptr(), size)
     return dw, db
 
 
@@ -821,10 +827,9 @@ class ObservationProjection(object):
     if torch.cuda.is_current_stream_capturing():
       raise RuntimeError('this ObservationProjection has not laid its weight out for stacked layers yet: call it once before '
                          'capturing a graph')
-    with torch.cuda.device(self._plan.device):
-      self._plan.desc.stacked = stacked
-      self._packs[stacked] = self._plan.pack(self._weight, self._packs.get(stacked))
-      torch.cuda.current_stream().synchronize()
+    desc = N.PROJECT_HEAD.pack(0, 0) + _NO_OFFSETS + self._plan.tails[stacked]  # (the layout depends on the weight alone)
+    self._packs[stacked] = self._plan.pack(desc, self._weight, self._packs.get(stacked))
+    torch.cuda.current_stream(self._plan.device).synchronize()
 
   def load(self, weight, bias=None):
     """New values for weight and bias (same shapes and types), in place: graphs that captured a call see them.  Waits for
@@ -845,13 +850,12 @@ class ObservationProjection(object):
     torch.cuda.synchronize(self._plan.device)
 
   def __call__(self, observation, residual=None):
-    torch = dev.torch_module()
     boards = _Boards(observation, self._layers)
+    desc = self._plan.at(boards)
     stacked = int(boards.offsets is not None)
     if stacked not in self._packs:
       self._lay_out(stacked)
-    with torch.cuda.device(self._plan.device):
-      out, _ = self._plan.forward(boards, self._packs[stacked], self._bias, residual)
+    out, _ = self._plan.forward(desc, boards, self._packs[stacked], self._bias, None if residual is None else residual.detach())
     return out[0] if boards.single else out
 
 
@@ -867,21 +871,20 @@ def _project_autograd():
     class ProjectBoards(torch.autograd.Function):
 
       @staticmethod
-      def forward(ctx, weight, bias, residual, plan, boards):
-        out, slope = plan.forward(boards, plan.pack(weight), bias, residual, want_slope=plan.desc.activation != N.ACT_NONE)
-        ctx.plan, ctx.boards, ctx.weight_shape = plan, boards, weight.shape
+      def forward(ctx, weight, bias, residual, plan, boards, desc):
+        out, slope = plan.forward(desc, boards, plan.pack(desc, weight), bias, residual, want_slope=plan.activation != N.ACT_NONE)
+        ctx.plan, ctx.boards, ctx.desc, ctx.weight_shape = plan, boards, desc, weight.shape
         # (the boards are an input like any other: a write to them before backward() is noticed where they are a tensor)
         ctx.save_for_backward(slope, boards.keep if isinstance(boards.keep, torch.Tensor) else None)
         return out
 
       @staticmethod
-      @torch.autograd.function.once_differentiable
       def backward(ctx, grad):
+        dev.refuse_twice('project')
         slope, _ = ctx.saved_tensors
         want = ctx.needs_input_grad
-        with torch.cuda.device(ctx.plan.device):
-          dw, db = ctx.plan.backward(ctx.boards, grad, slope, want[0], want[1], ctx.weight_shape)
-        return dw, db, grad if want[2] else None, None, None
+        dw, db = ctx.plan.backward(ctx.desc, ctx.boards, grad, slope, want[0], want[1], ctx.weight_shape)
+        return dw, db, grad if want[2] else None, None, None, None
 
     _project_function = ProjectBoards
   return _project_function
@@ -900,25 +903,23 @@ def project(boards, layers, weight, bias=None, activation=None, residual=None, r
   torch = dev.require_torch('project()')
   plan = _Projection(layers, weight, bias, activation)
   view = _Boards(boards, layers)
-  plan.at(view)
+  desc = plan.at(view)
   plan.check_rows(residual, 'residual', view.n)
-  with torch.cuda.device(plan.device):
-    if return_slope:
-      out, slope = plan.forward(view, plan.pack(weight), bias, residual, want_slope=activation is not None)
-      return (out[0] if view.single else out), slope
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (weight, bias, residual)):
-      dev.refuse_recording_in_capture('project', 'project(..., return_slope=True) and project_backward()')
-      out = _project_autograd().apply(weight, bias, residual, plan, view)
-    else:
-      out, _ = plan.forward(view, plan.pack(weight), bias, residual)
-  return out[0] if view.single else out
+  if not return_slope and torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (weight, bias, residual)):
+    dev.refuse_recording_in_capture('project', 'project(..., return_slope=True) and project_backward()')
+    out = _project_autograd().apply(weight, bias, residual, plan, view, desc)
+    return out[0] if view.single else out
+  bias, residual = (None if t is None else t.detach() for t in (bias, residual))
+  out, slope = plan.forward(desc, view, plan.pack(desc, weight), bias, residual, want_slope=return_slope and activation is not None)
+  out = out[0] if view.single else out
+  return (out, slope) if return_slope else out
 
 
 def project_backward(boards, layers, weight, grad, slope=None):
   """(grad_weight, grad_bias) of `project()` for the gradient `grad` [n, hidden] of its result; `slope` as it returned it.
   The residual's gradient is `grad`.  Records nothing for autograd and waits for nothing: it may be captured."""
-  torch = dev.require_torch('project_backward()')
+  dev.require_torch('project_backward()')
   # (which activation it was is in the slopes: relu's have the weight's type, the others' are float32)
   plan = _Projection(layers, weight, None, None if slope is None else 'relu' if slope.dtype == weight.dtype else 'silu')
-  with torch.cuda.device(plan.device):
-    return plan.backward(_Boards(boards, layers), grad.detach(), slope, True, True, weight.shape)
+  view = _Boards(boards, layers)
+  return plan.backward(plan.at(view), view, grad.detach(), slope, True, True, weight.shape)
