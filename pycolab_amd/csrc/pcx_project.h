@@ -75,6 +75,13 @@ __device__ __forceinline__ uint16_t part_of(float w, int p, int parts) {
   return (uint16_t)(u >> 16);
 }
 
+// The kernel's (one) argument where the runtime put it.  Its arrays are indexed there: indexed in the argument itself, the
+// compiler copies the whole structure into every lane's scratch memory.
+template <typename A>
+__device__ __forceinline__ const __attribute__((address_space(4))) A* argument() {
+  return (const __attribute__((address_space(4))) A*)__builtin_amdgcn_kernarg_segment_ptr();
+}
+
 // 16 bytes a lane straight from memory into LDS: lane i's land at lds + 16 i (lds: the same for the whole wave).
 __device__ __forceinline__ void copy_in(const uint8_t* from, uint8_t* lds) {
   __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)from, (__attribute__((address_space(3))) void*)lds, 16, 0, 0);

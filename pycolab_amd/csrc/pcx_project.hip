@@ -244,7 +244,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void pcx_project_forward_kernel(Fo
     if (tid < 256) lut[tid] = 0x44u;  // (0, 1), none
     __syncthreads();
     const int l = b * 16 + tid, p = l & 3, g = (l >> 2) & 3;
-    if (tid < 16 && l < s.layers) lut[s.chars[l]] = p < 3 ? (0x4000u >> g) | (uint32_t)((p | 12) * 0x11) : (0x40000000u >> g) | 0xCCu;
+    if (tid < 16 && l < s.layers) lut[argument<ForwardArgs>()->s.chars[l]] = p < 3 ? (0x4000u >> g) | (uint32_t)((p | 12) * 0x11) : (0x40000000u >> g) | 0xCCu;
   };
   // the run of (block, quad) units of this split
   const int units = blocks * s.quads;
@@ -316,7 +316,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void pcx_project_forward_kernel(Fo
 #pragma unroll
       for (int l = 0; l < 2; ++l) {
         const int layer = 2 * g + l;
-        const int64_t off = layer < s.layers ? s.layer_offset[layer] : -1;
+        const int64_t off = layer < s.layers ? argument<ForwardArgs>()->s.layer_offset[layer] : -1;
         on_next[l] = off >= 0 ? 0xFFFFFFFFu : 0u;
 #pragma unroll
         for (int m = 0; m < MT; ++m) nxt[m][l] = off >= 0 ? load16(row[m] + off, c) : u32x4{0, 0, 0, 0};
@@ -506,11 +506,15 @@ struct ForwardPlan { int mt, wm, wn, mblocks, nblocks, splits; uint64_t bytes; }
 ForwardPlan plan_forward(const Shape& s) {
   ForwardPlan p;
   // 4 x 2 tiles a wave make the most of a weight in LDS and of an expanded board.  Eight waves share a weight where the
-  // boards fill the chip with them (the weight then leaves L2 half as often); few boards take one tile a wave.
+  // boards fill the chip with them (the weight then leaves L2 half as often); where they do not fill it with four, a wave
+  // takes 2 x 2 tiles, and only then are the cells divided: joining costs 8 bytes a sum and part.
   p.mt = 4;
   p.wn = s.tiles >= 3 ? 2 : 1;
-  p.wm = p.wn == 2 && s.n * ((s.tiles + 3) / 4) >= 512 * 192 ? 4 : 4 / p.wn;
+  p.wm = 4 / p.wn;
+  const int64_t nblocks = (s.tiles + 2 * p.wn - 1) / (2 * p.wn);
   if (s.n <= 512) { p.mt = 1; p.wm = 1; p.wn = 4; }
+  else if (p.wn == 2 && s.n * nblocks >= 512 * 192) p.wm = 4;
+  else if ((s.n + 128 * p.wm - 1) / (128 * p.wm) * nblocks < SLOTS / 2) p.mt = 2;
   const int rows = p.wm * p.mt * 32, cols = (p.mt == 1 ? 1 : 2) * p.wn;
   p.mblocks = (int)((s.n + rows - 1) / rows);
   p.nblocks = (s.tiles + cols - 1) / cols;
@@ -537,8 +541,8 @@ template <int DT, int G>
 int forward_shape(const ForwardArgs& a, const ForwardPlan& p, unsigned grid, hipStream_t st) {
   if (p.mt == 1) return forward_go<DT, G, 1, 1, 1, 4>(a, grid, st);
   if (p.wm * p.wn == 8) return forward_go<DT, G, 4, 2, 4, 2>(a, grid, st);
-  if (p.wn == 2) return forward_go<DT, G, 4, 2, 2, 2>(a, grid, st);
-  return forward_go<DT, G, 4, 2, 4, 1>(a, grid, st);
+  if (p.wn == 2) return p.mt == 4 ? forward_go<DT, G, 4, 2, 2, 2>(a, grid, st) : forward_go<DT, G, 2, 2, 2, 2>(a, grid, st);
+  return p.mt == 4 ? forward_go<DT, G, 4, 2, 4, 1>(a, grid, st) : forward_go<DT, G, 2, 2, 4, 1>(a, grid, st);
 }
 template <int DT>
 int forward_type(const ForwardArgs& a, const ForwardPlan& p, unsigned grid, hipStream_t st) {

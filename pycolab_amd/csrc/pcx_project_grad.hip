@@ -136,7 +136,7 @@ __global__ __launch_bounds__(256, 2) void pcx_project_weight_grad(BackwardArgs a
   constexpr int MASKS = 32 * PITCH * 2;
   const Shape& s = a.s;
   extern __shared__ __align__(16) uint8_t lds[];
-  uint16_t* const lut = reinterpret_cast<uint16_t*>(lds + 2 * STAGE + 2 * MASKS);
+  uint16_t* const lut = reinterpret_cast<uint16_t*>(lds + 3 * STAGE + 2 * MASKS);
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = lane >> 5;
   const uint32_t tiles = (uint32_t)a.cell_blocks * a.layer_blocks * a.hblocks;
   // the tiles of one run of boards go to one XCD, whose L2 then serves dz and the boards once
@@ -150,12 +150,12 @@ __global__ __launch_bounds__(256, 2) void pcx_project_weight_grad(BackwardArgs a
   if constexpr (!STACKED) {
     lut[tid] = 0;
     __syncthreads();
-    if (tid < 8 && l0 + tid < s.layers) lut[s.chars[l0 + tid]] = (uint16_t)(128u << tid);
+    if (tid < 8 && l0 + tid < s.layers) lut[argument<BackwardArgs>()->s.chars[l0 + tid]] = (uint16_t)(128u << tid);
   }
   const int b0 = (int)((int64_t)a.blocks * split / a.splits), b1 = (int)((int64_t)a.blocks * (split + 1) / a.splits);
   const uint8_t* const src = a.frags + (int64_t)hb * NH * PARTS * 1024 + lane * 16;
   auto stage_in = [&](int b) {
-    uint8_t* const dst = lds + (b & 1) * STAGE;
+    uint8_t* const dst = lds + (b - b0) % 3 * STAGE;
 #pragma unroll
     for (int i = 0; i < NH * PARTS; ++i) {
       const int k = wave * NH * PARTS + i;  // (piece i of board step `wave`)
@@ -166,8 +166,8 @@ __global__ __launch_bounds__(256, 2) void pcx_project_weight_grad(BackwardArgs a
   const int pair = tid >> 3, cell = (tid & 7) * 4;
   const bool small = s.cells < QUAD;
   constexpr int PL = STACKED ? 8 : 1;
-  uint32_t raw[2][PL];
-  auto fetch = [&](int b) {
+  uint32_t raw[2][2][PL];  // [parity of the block]
+  auto fetch = [&](int b, uint32_t (&raw)[2][PL]) {
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
       const int64_t gr = (int64_t)b * BLK + pair * 2 + r;
@@ -175,15 +175,15 @@ __global__ __launch_bounds__(256, 2) void pcx_project_weight_grad(BackwardArgs a
 #pragma unroll
       for (int l = 0; l < PL; ++l) {
         raw[r][l] = 0;
-        const int64_t off = STACKED ? (l0 + l < s.layers ? s.layer_offset[l0 + l] : -1) : 0;
+        const int64_t off = STACKED ? (l0 + l < s.layers ? argument<BackwardArgs>()->s.layer_offset[l0 + l] : -1) : 0;
         if (off < 0) continue;
         if (small) raw[r][l] = edge_dword(at + off, cell, s.cells);
         else __builtin_memcpy(&raw[r][l], at + off + c0 + cell, 4);
       }
     }
   };
-  auto turn = [&](int b) {
-    uint8_t* const dst = lds + 2 * STAGE + (b & 1) * MASKS;
+  auto turn = [&](int b, const uint32_t (&raw)[2][PL]) {
+    uint8_t* const dst = lds + 3 * STAGE + (b & 1) * MASKS;
 #pragma unroll
     for (int c = 0; c < 4; ++c) {
       uint32_t m[2];
@@ -207,25 +207,32 @@ __global__ __launch_bounds__(256, 2) void pcx_project_weight_grad(BackwardArgs a
     for (int h = 0; h < NH; ++h)
 #pragma unroll
       for (int i = 0; i < 16; ++i) acc[l][h][i] = 0.0f;
+  // dz and the boards are two stages ahead: they come from beyond L2, which takes longer than a stage's 32 products a wave
+  // (one stage ahead: 94 us for 65,536 boards, two: 74).
   if (b0 < b1) {
-    fetch(b0);
+    fetch(b0, raw[0]);
     stage_in(b0);
+    if (b0 + 1 < b1) {
+      fetch(b0 + 1, raw[1]);
+      stage_in(b0 + 1);
+    }
   }
   __syncthreads();  // the table
-  if (b0 < b1) turn(b0);
+  if (b0 < b1) turn(b0, raw[0]);
   const bool work = l0 + wave * 2 < s.layers;
   const int shift = 7 - wave * 2;
-#pragma unroll 1
-  for (int b = b0; b < b1; ++b) {
-    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // (this wave's part of the turned boards is written)
-    stage_barrier();
-    if (b + 1 < b1) {
-      stage_in(b + 1);
-      fetch(b + 1);
+  auto block = [&](int b, uint32_t (&now)[2][PL], uint32_t (&next)[2][PL]) {
+    // this wave's part of the turned boards is written; block b's dz is here once no more than the NH * PARTS copies of
+    // block b + 1, the newest requests, are on their way
+    if (b + 1 < b1) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(NH * PARTS) : "memory");
+    else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    if (b + 2 < b1) {
+      fetch(b + 2, now);
+      stage_in(b + 2);
     }
     if (work) {
-      const uint8_t* const dz = lds + (b & 1) * STAGE + lane * 16;
-      const uint8_t* const masks = lds + 2 * STAGE + (b & 1) * MASKS + ((lane & 31) * PITCH + half * 8) * 2;
+      const uint8_t* const dz = lds + (b - b0) % 3 * STAGE + lane * 16;
+      const uint8_t* const masks = lds + 3 * STAGE + (b & 1) * MASKS + ((lane & 31) * PITCH + half * 8) * 2;
 #pragma unroll
       for (int kb = 0; kb < 4; ++kb) {
         const u32x4 m = *reinterpret_cast<const u32x4*>(masks + kb * 32);
@@ -245,7 +252,12 @@ __global__ __launch_bounds__(256, 2) void pcx_project_weight_grad(BackwardArgs a
           }
       }
     }
-    if (b + 1 < b1) turn(b + 1);
+    if (b + 1 < b1) turn(b + 1, next);
+  };
+#pragma unroll 1
+  for (int b = b0; b < b1; b += 2) {
+    block(b, raw[0], raw[1]);
+    if (b + 1 < b1) block(b + 1, raw[1], raw[0]);
   }
   const int c = c0 + (lane & 31);
   if (c < cb * QUAD || c >= s.cells) return;  // (the block before owns the cells this one shares with it)
@@ -328,7 +340,7 @@ BackwardPlan plan_backward(const Shape& s) {
 
 template <bool F16, int PARTS, bool STACKED, int NH>
 int grad_go(const BackwardArgs& a, unsigned grid, hipStream_t st) {
-  constexpr int LDS = 2 * 4 * NH * PARTS * 1024 + 2 * 32 * (BLK + 8) * 2 + 512;
+  constexpr int LDS = 3 * 4 * NH * PARTS * 1024 + 2 * 32 * (BLK + 8) * 2 + 512;
   auto* const kernel = &pcx_project_weight_grad<F16, PARTS, STACKED, NH>;
   if (LDS > 65536) PCX_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, LDS));
   hipLaunchKernelGGL(kernel, dim3(grid), dim3(256), LDS, st, a);
