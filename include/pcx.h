@@ -627,8 +627,8 @@ enum pcx_activation { PCX_ACT_NONE = 0, PCX_ACT_RELU = 1, PCX_ACT_SILU = 2, PCX_
  *   stacked == 0: `boards` holds uint8 characters [n][cells] (board b at b * row_stride): layer k of a cell is
  *     (character == chars[k]); the chars are distinct, characters that are none of them count nowhere;
  *   stacked != 0: `boards` holds uint8 layers (layer k of board b at b * row_stride + layer_offset[k], or nowhere, all
- *     zero, where the offset is negative), set where nonzero -- for observations whose layers overlap
- *     (occlusion_in_layers=False).
+ *     zero, where the offset is negative; less than 2 GB, and the board's first `cells` bytes are readable either way), set
+ *     where nonzero -- for observations whose layers overlap (occlusion_in_layers=False).
  * weight, bias, residual, out: `dtype` (PCX_F32, PCX_F16, PCX_BF16); weight [hidden][n_layers][cells], bias [hidden] or
  * NULL, residual and out [n][hidden], contiguous.  Sums are float32. */
 typedef struct pcx_project_desc {

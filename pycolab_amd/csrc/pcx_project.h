@@ -87,7 +87,9 @@ __device__ __forceinline__ void copy_in(const uint8_t* from, uint8_t* lds) {
   __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)from, (__attribute__((address_space(3))) void*)lds, 16, 0, 0);
 }
 // What copy_in() fetched has arrived, for every wave of the workgroup, and nobody reads the buffer of the stage before.
-__device__ __forceinline__ void stage_barrier() { asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory"); }
+// NEWER: how many requests at least were made after the copies that are waited for (requests complete in order).
+template <int NEWER>
+__device__ __forceinline__ void stage_barrier() { asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(NEWER) : "memory"); }
 
 // Bytes c .. c + 3 of a board of fewer than 32 cells; zeros past its end, which is never read.
 __device__ __forceinline__ uint32_t edge_dword(const uint8_t* row, int c, int cells) {

@@ -31,6 +31,9 @@ int make_shape(const pcx_project_desc* d, Shape* s, const char* who) {
     return set_error(PCX_E_INVALID, "%s: cells, layers or hidden units out of range", who);
   if (d->n < 0 || d->n > (int64_t)1 << 31) return set_error(PCX_E_INVALID, "%s: %lld boards", who, (long long)d->n);
   if (d->row_stride < 0) return set_error(PCX_E_INVALID, "%s: negative stride", who);
+  if (d->stacked)
+    for (int i = 0; i < d->n_layers; ++i)
+      if (d->layer_offset[i] >= (int64_t)1 << 31) return set_error(PCX_E_INVALID, "%s: a layer 2 GB or more from its board", who);
   if (!d->stacked)
     for (int i = 0; i < d->n_layers; ++i)
       for (int j = 0; j < i; ++j)
@@ -306,50 +309,60 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void pcx_project_forward_kernel(Fo
     }
     return v;
   };
+  // A stage's weights must have arrived, the boards' bytes requested after them need not: `loose` says that they were.
+  constexpr int LOADS = STACKED ? 2 * MT : MT;
+  bool loose = false;
+  auto arrive = [&]() {
+    if (loose) stage_barrier<LOADS>();
+    else stage_barrier<0>();
+    loose = false;
+  };
   int st = 0;
-  stage_in(0);
   if constexpr (STACKED) {
-    u32x4 cur[MT][2], nxt[MT][2];
-    uint32_t on[2], on_next[2] = {0, 0};  // 0 where the layer does not exist: its bytes are then another layer's
-    auto fetch = [&](int q, int g) {
-      const int c = quad_start(q, s.cells) + half * 16;
+    // The two layers of a (quad, group) unit, DEPTH - 1 units ahead: a unit is only 4 matrix steps, a trip to memory many.
+    constexpr int DEPTH = MT == 4 ? 2 : 4;
+    u32x4 ring[DEPTH][MT][2];
+    uint32_t on[DEPTH][2];  // 0 where the layer does not exist: its bytes are then the board's first
+    int fq = u0, fg = 0;
+    auto fetch = [&](u32x4 (&to)[MT][2], uint32_t (&keep)[2]) {
+      if (fq >= u1) return;
+      const int c = quad_start(fq, s.cells) + half * 16;
 #pragma unroll
       for (int l = 0; l < 2; ++l) {
-        const int layer = 2 * g + l;
+        const int layer = 2 * fg + l;
         const int64_t off = layer < s.layers ? argument<ForwardArgs>()->s.layer_offset[layer] : -1;
-        on_next[l] = off >= 0 ? 0xFFFFFFFFu : 0u;
+        keep[l] = off >= 0 ? 0xFFFFFFFFu : 0u;
 #pragma unroll
-        for (int m = 0; m < MT; ++m) nxt[m][l] = off >= 0 ? load16(row[m] + off, c) : u32x4{0, 0, 0, 0};
+        for (int m = 0; m < MT; ++m) to[m][l] = load16(row[m] + (off >= 0 ? off : 0), c);
       }
+      loose = !small;
+      if (++fg == s.groups) { fg = 0; ++fq; }
     };
 #pragma unroll
     for (int m = 0; m < MT; ++m) index[m] = 0x4444;
-    fetch(u0, 0);
-#pragma unroll 1
-    for (int q = u0; q < u1; ++q)
-#pragma unroll 1
-      for (int g = 0; g < s.groups; ++g) {
 #pragma unroll
-        for (int l = 0; l < 2; ++l) {
-          on[l] = on_next[l];
+    for (int k = 0; k < DEPTH - 1; ++k) fetch(ring[k], on[k]);
+    stage_in(0);
+    loose = false;
+    const int total = (u1 - u0) * s.groups;
+#pragma unroll 1
+    for (int i = 0; i < total; i += DEPTH)
 #pragma unroll
-          for (int m = 0; m < MT; ++m) cur[m][l] = nxt[m][l];
-        }
+      for (int k = 0; k < DEPTH; ++k) {
+        if (i + k >= total) break;
 #pragma unroll
         for (int part = 0; part < PARTS; ++part) {
-          stage_barrier();
+          arrive();
           if (st + 1 < stages) stage_in(st + 1);
-          if (part == 0) {
-            if (g + 1 < s.groups) fetch(q, g + 1);
-            else if (q + 1 < u1) fetch(q + 1, 0);
-          }
+          asm volatile("" ::: "memory");
+          if (part == 0) fetch(ring[(k + DEPTH - 1) % DEPTH], on[(k + DEPTH - 1) % DEPTH]);
           const uint8_t* const base = stage_base(st);
           read_right(base, 0);
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
 #pragma unroll
             for (int m = 0; m < MT; ++m) {
-              const uint32_t lo = set_bytes(cur[m][0][j]) & on[0], hi = set_bytes(cur[m][1][j]) & on[1];
+              const uint32_t lo = set_bytes(ring[k][m][0][j]) & on[k][0], hi = set_bytes(ring[k][m][1][j]) & on[k][1];
               left[m][0] = __builtin_amdgcn_perm(hi, lo, 0x040C000Cu);
               left[m][1] = __builtin_amdgcn_perm(hi, lo, 0x050C010Cu);
               left[m][2] = __builtin_amdgcn_perm(hi, lo, 0x060C020Cu);
@@ -366,8 +379,11 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void pcx_project_forward_kernel(Fo
       const int q = u < s.quads ? u : u - s.quads, c = quad_start(q, s.cells) + half * 16;
 #pragma unroll
       for (int m = 0; m < MT; ++m) nxt[m] = load16(row[m], c);
+      loose = !small;
     };
     fetch(u0);
+    stage_in(0);
+    loose = false;
     write_table(u0 < s.quads ? 0 : 1);
     __syncthreads();
 #pragma unroll 1
@@ -383,8 +399,9 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void pcx_project_forward_kernel(Fo
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         if (j % OCT == 0) {
-          stage_barrier();
+          arrive();
           if (st + 1 < stages) stage_in(st + 1);
+          asm volatile("" ::: "memory");
           if (j == 0 && u + 1 < u1) fetch(u + 1);
           read_right(stage_base(st), 0);
         }
@@ -398,7 +415,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void pcx_project_forward_kernel(Fo
 #pragma unroll
         for (int part = 0; part < PARTS; ++part) {
           if (part && part % PS == 0) {
-            stage_barrier();
+            arrive();
             if (st + 1 < stages) stage_in(st + 1);
             read_right(stage_base(st), 0);
           }

@@ -125,15 +125,19 @@ __device__ __forceinline__ f32x16 dense_step(u32x4 a, u32x4 b, f32x16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
 }
 
-// dw[h][l][c] over a run of boards: a workgroup owns NH tiles of hidden units x 32 cells x 8 layers (two layers a wave).
+// dw[h][l][c] over a run of boards: a workgroup owns NH tiles of hidden units x 32 cells x up to 2 LW layers (NH = 1: 4 LW).
 // The sum runs over boards, along which the features are not sparse: the dense instruction.  Its right operand is the
 // feature bit of 8 consecutive boards at one cell: the boards are turned round once per stage into LDS as a word of layer
-// bits per (cell, board), from which every layer's operand is one shift and one mask.
-template <bool F16, int PARTS, bool STACKED, int NH>
+// bits per (cell, board), from which every layer's operand is one shift and one mask.  A wave takes LW layers x half the
+// hidden units: one LDS read then serves LW operands, and every dz operand read LW products (with 2 layers x all units a
+// wave the LDS was the bound: 91 us for 65,536 boards x 256 units x 8 layers, 4 x half of them:
+// GRAD_US us).
+template <bool F16, int PARTS, bool STACKED, int NH, int LW>
 __global__ __launch_bounds__(256, 2) void pcx_project_weight_grad(BackwardArgs a) {
   constexpr int STAGE = 4 * NH * PARTS * 1024;
   constexpr int PITCH = BLK + 8;                // words per cell: 16-byte reads of one wave spread over the banks
   constexpr int MASKS = 32 * PITCH * 2;
+  constexpr int WH = NH == 1 ? 1 : 2, HW = NH / WH, WL = 4 / WH, LAYERS = WL * LW;  // waves along hidden units and layers
   const Shape& s = a.s;
   extern __shared__ __align__(16) uint8_t lds[];
   uint16_t* const lut = reinterpret_cast<uint16_t*>(lds + 3 * STAGE + 2 * MASKS);
@@ -146,11 +150,11 @@ __global__ __launch_bounds__(256, 2) void pcx_project_weight_grad(BackwardArgs a
   uint32_t t = id % tiles;
   const int hb = (int)(t % (uint32_t)a.hblocks); t /= (uint32_t)a.hblocks;
   const int lb = (int)(t % (uint32_t)a.layer_blocks), cb = (int)(t / (uint32_t)a.layer_blocks);
-  const int l0 = lb * 8, c0 = quad_start(cb, s.cells);
+  const int l0 = lb * LAYERS, c0 = quad_start(cb, s.cells);
   if constexpr (!STACKED) {
     lut[tid] = 0;
     __syncthreads();
-    if (tid < 8 && l0 + tid < s.layers) lut[argument<BackwardArgs>()->s.chars[l0 + tid]] = (uint16_t)(128u << tid);
+    if (tid < LAYERS && l0 + tid < s.layers) lut[argument<BackwardArgs>()->s.chars[l0 + tid]] = (uint16_t)(1u << (14 - tid));
   }
   const int b0 = (int)((int64_t)a.blocks * split / a.splits), b1 = (int)((int64_t)a.blocks * (split + 1) / a.splits);
   const uint8_t* const src = a.frags + (int64_t)hb * NH * PARTS * 1024 + lane * 16;
@@ -165,24 +169,28 @@ __global__ __launch_bounds__(256, 2) void pcx_project_weight_grad(BackwardArgs a
   // a thread turns two boards x four cells round
   const int pair = tid >> 3, cell = (tid & 7) * 4;
   const bool small = s.cells < QUAD;
-  constexpr int PL = STACKED ? 8 : 1;
-  uint32_t raw[2][2][PL];  // [parity of the block]
-  auto fetch = [&](int b, uint32_t (&raw)[2][PL]) {
+  constexpr int PL = STACKED ? LAYERS : 1;
+  int32_t offset[PL];  // STACKED: of this block's layers within a board, -1: nowhere (a board is less than 2 GB)
+#pragma unroll
+  for (int l = 0; l < PL; ++l) offset[l] = !STACKED ? 0 : l0 + l < s.layers ? (int32_t)argument<BackwardArgs>()->s.layer_offset[l0 + l] : -1;
+  auto fetch = [&](int b, uint32_t* raw) {  // [board of the pair][layer]
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
       const int64_t gr = (int64_t)b * BLK + pair * 2 + r;
       const uint8_t* const at = a.boards + (gr < s.n ? gr : s.n - 1) * s.row_stride;  // (boards past the end meet dz = 0)
 #pragma unroll
       for (int l = 0; l < PL; ++l) {
-        raw[r][l] = 0;
-        const int64_t off = STACKED ? (l0 + l < s.layers ? argument<BackwardArgs>()->s.layer_offset[l0 + l] : -1) : 0;
-        if (off < 0) continue;
-        if (small) raw[r][l] = edge_dword(at + off, cell, s.cells);
-        else __builtin_memcpy(&raw[r][l], at + off + c0 + cell, 4);
+        uint32_t v = 0;
+        if (small) {
+          if (offset[l] >= 0) v = edge_dword(at + offset[l], cell, s.cells);
+        } else {
+          __builtin_memcpy(&v, at + (offset[l] >= 0 ? offset[l] : 0) + c0 + cell, 4);
+        }
+        raw[r * PL + l] = v;
       }
     }
   };
-  auto turn = [&](int b, const uint32_t (&raw)[2][PL]) {
+  auto turn = [&](int b, const uint32_t* raw) {
     uint8_t* const dst = lds + 3 * STAGE + (b & 1) * MASKS;
 #pragma unroll
     for (int c = 0; c < 4; ++c) {
@@ -192,84 +200,90 @@ __global__ __launch_bounds__(256, 2) void pcx_project_weight_grad(BackwardArgs a
         if constexpr (STACKED) {
           m[r] = 0;
 #pragma unroll
-          for (int l = 0; l < 8; ++l) m[r] |= ((raw[r][l] >> (8 * c)) & 255u) ? 128u << l : 0u;
+          for (int l = 0; l < PL; ++l) m[r] |= offset[l] >= 0 && ((raw[r * PL + l] >> (8 * c)) & 255u) ? 1u << (14 - l) : 0u;
         } else {
-          m[r] = lut[(raw[r][0] >> (8 * c)) & 255u];
+          m[r] = lut[(raw[r] >> (8 * c)) & 255u];
         }
       }
       *reinterpret_cast<uint32_t*>(dst + ((cell + c) * PITCH + pair * 2) * 2) = m[0] | (m[1] << 16);
     }
   };
-  f32x16 acc[2][NH];
+  f32x16 acc[LW][HW];
 #pragma unroll
-  for (int l = 0; l < 2; ++l)
+  for (int l = 0; l < LW; ++l)
 #pragma unroll
-    for (int h = 0; h < NH; ++h)
+    for (int h = 0; h < HW; ++h)
 #pragma unroll
       for (int i = 0; i < 16; ++i) acc[l][h][i] = 0.0f;
-  // dz and the boards are two stages ahead: they come from beyond L2, which takes longer than a stage's 32 products a wave
-  // (one stage ahead: 94 us for 65,536 boards, two: 74).
+  const int wl = wave % WL, wh = wave / WL;
+  const bool work = l0 + wl * LW < s.layers;
+  auto multiply = [&](int b) {
+    const uint8_t* const dz = lds + (b - b0) % 3 * STAGE + lane * 16;
+    const uint8_t* const masks = lds + 3 * STAGE + (b & 1) * MASKS + ((lane & 31) * PITCH + half * 8) * 2;
+#pragma unroll
+    for (int kb = 0; kb < 4; ++kb) {
+      const u32x4 m = *reinterpret_cast<const u32x4*>(masks + kb * 32);
+      u32x4 right[LW];
+#pragma unroll
+      for (int l = 0; l < LW; ++l)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) right[l][e] = (m[e] << (wl * LW + l)) & 0x40004000u;
+#pragma unroll
+      for (int h = 0; h < HW; ++h)
+#pragma unroll
+        for (int p = 0; p < PARTS; ++p) {
+          const u32x4 left = *reinterpret_cast<const u32x4*>(dz + ((kb * NH + wh * HW + h) * PARTS + p) * 1024);
+#pragma unroll
+          for (int l = 0; l < LW; ++l) acc[l][h] = dense_step<F16>(left, right[l], acc[l][h]);
+        }
+    }
+  };
+  // dz is two stages ahead, the boards' bytes two: block b's dz is here once no more than the NH * PARTS copies of block
+  // b + 1, the newest requests, are on their way.
+  auto begin = [&](int b) {
+    if (b + 1 < b1) stage_barrier<NH * PARTS>();
+    else stage_barrier<0>();
+  };
+  uint32_t even[2 * PL], odd[2 * PL];
   if (b0 < b1) {
-    fetch(b0, raw[0]);
+    fetch(b0, even);
     stage_in(b0);
     if (b0 + 1 < b1) {
-      fetch(b0 + 1, raw[1]);
+      fetch(b0 + 1, odd);
       stage_in(b0 + 1);
     }
   }
   __syncthreads();  // the table
-  if (b0 < b1) turn(b0, raw[0]);
-  const bool work = l0 + wave * 2 < s.layers;
-  const int shift = 7 - wave * 2;
-  auto block = [&](int b, uint32_t (&now)[2][PL], uint32_t (&next)[2][PL]) {
-    // this wave's part of the turned boards is written; block b's dz is here once no more than the NH * PARTS copies of
-    // block b + 1, the newest requests, are on their way
-    if (b + 1 < b1) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(NH * PARTS) : "memory");
-    else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-    if (b + 2 < b1) {
-      fetch(b + 2, now);
-      stage_in(b + 2);
-    }
-    if (work) {
-      const uint8_t* const dz = lds + (b - b0) % 3 * STAGE + lane * 16;
-      const uint8_t* const masks = lds + 3 * STAGE + (b & 1) * MASKS + ((lane & 31) * PITCH + half * 8) * 2;
-#pragma unroll
-      for (int kb = 0; kb < 4; ++kb) {
-        const u32x4 m = *reinterpret_cast<const u32x4*>(masks + kb * 32);
-        u32x4 right[2];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          right[0][e] = (m[e] << shift) & 0x40004000u;
-          right[1][e] = (m[e] << (shift - 1)) & 0x40004000u;
-        }
-#pragma unroll
-        for (int h = 0; h < NH; ++h)
-#pragma unroll
-          for (int p = 0; p < PARTS; ++p) {
-            const u32x4 left = *reinterpret_cast<const u32x4*>(dz + ((kb * NH + h) * PARTS + p) * 1024);
-            acc[0][h] = dense_step<F16>(left, right[0], acc[0][h]);
-            acc[1][h] = dense_step<F16>(left, right[1], acc[1][h]);
-          }
-      }
-    }
-    if (b + 1 < b1) turn(b + 1, next);
-  };
+  if (b0 < b1) turn(b0, even);
 #pragma unroll 1
   for (int b = b0; b < b1; b += 2) {
-    block(b, raw[0], raw[1]);
-    if (b + 1 < b1) block(b + 1, raw[1], raw[0]);
+    begin(b);
+    if (b + 2 < b1) {
+      fetch(b + 2, even);
+      stage_in(b + 2);
+    }
+    if (work) multiply(b);
+    if (b + 1 >= b1) break;
+    turn(b + 1, odd);
+    begin(b + 1);
+    if (b + 3 < b1) {
+      fetch(b + 3, odd);
+      stage_in(b + 3);
+    }
+    if (work) multiply(b + 1);
+    if (b + 2 < b1) turn(b + 2, even);
   }
   const int c = c0 + (lane & 31);
   if (c < cb * QUAD || c >= s.cells) return;  // (the block before owns the cells this one shares with it)
 #pragma unroll
-  for (int l = 0; l < 2; ++l) {
-    const int layer = l0 + wave * 2 + l;
+  for (int l = 0; l < LW; ++l) {
+    const int layer = l0 + wl * LW + l;
     if (layer >= s.layers) continue;
 #pragma unroll
-    for (int h = 0; h < NH; ++h)
+    for (int h = 0; h < HW; ++h)
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
-        const int unit = (hb * NH + h) * 32 + 8 * (i >> 2) + 4 * half + (i & 3);
+        const int unit = (hb * NH + wh * HW + h) * 32 + 8 * (i >> 2) + 4 * half + (i & 3);
         if (unit < s.hidden) a.partial[(((int64_t)split * s.hidden + unit) * s.layers + layer) * s.cells + c] = SCALE<F16> * acc[l][h][i];
       }
   }
@@ -315,7 +329,7 @@ __global__ __launch_bounds__(256) void pcx_project_grad_join(BackwardArgs a, int
 
 // ---------------------------------------------------------------- plan
 
-struct BackwardPlan { int nh, htiles, hblocks, cell_blocks, layer_blocks, splits, bias_blocks, blocks, parts; uint64_t frag_bytes, bias_bytes, part_bytes; };
+struct BackwardPlan { int nh, lw, htiles, hblocks, cell_blocks, layer_blocks, splits, bias_blocks, blocks, parts; uint64_t frag_bytes, bias_bytes, part_bytes; };
 
 BackwardPlan plan_backward(const Shape& s) {
   BackwardPlan p;
@@ -324,7 +338,11 @@ BackwardPlan plan_backward(const Shape& s) {
   p.hblocks = (s.tiles + p.nh - 1) / p.nh;
   p.htiles = p.hblocks * p.nh;
   p.cell_blocks = s.quads;
-  p.layer_blocks = (s.layers + 7) / 8;
+  // Eight layers a workgroup, or four where that pads fewer (one tile of hidden units: always eight).
+  const int pad8 = (s.layers + 7) / 8 * 8, pad4 = (s.layers + 3) / 4 * 4;
+  p.lw = pad4 < pad8 || p.nh == 1 ? 2 : 4;
+  const int per = (p.nh == 1 ? 4 : 2) * p.lw;
+  p.layer_blocks = (s.layers + per - 1) / per;
   p.blocks = (int)((s.n + BLK - 1) / BLK);
   const int64_t tiles = (int64_t)p.hblocks * p.cell_blocks * p.layer_blocks;
   int64_t splits = SLOTS / tiles;
@@ -338,19 +356,19 @@ BackwardPlan plan_backward(const Shape& s) {
   return p;
 }
 
-template <bool F16, int PARTS, bool STACKED, int NH>
+template <bool F16, int PARTS, bool STACKED, int NH, int LW>
 int grad_go(const BackwardArgs& a, unsigned grid, hipStream_t st) {
   constexpr int LDS = 3 * 4 * NH * PARTS * 1024 + 2 * 32 * (BLK + 8) * 2 + 512;
-  auto* const kernel = &pcx_project_weight_grad<F16, PARTS, STACKED, NH>;
+  auto* const kernel = &pcx_project_weight_grad<F16, PARTS, STACKED, NH, LW>;
   if (LDS > 65536) PCX_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, LDS));
   hipLaunchKernelGGL(kernel, dim3(grid), dim3(256), LDS, st, a);
   return 0;
 }
 template <bool F16, int PARTS, bool STACKED>
 int grad_shape(const BackwardArgs& a, const BackwardPlan& p, unsigned grid, hipStream_t st) {
-  if (p.nh == 4) return grad_go<F16, PARTS, STACKED, 4>(a, grid, st);
-  if (p.nh == 2) return grad_go<F16, PARTS, STACKED, 2>(a, grid, st);
-  return grad_go<F16, PARTS, STACKED, 1>(a, grid, st);
+  if (p.nh == 1) return grad_go<F16, PARTS, STACKED, 1, 2>(a, grid, st);
+  if (p.nh == 2) return p.lw == 4 ? grad_go<F16, PARTS, STACKED, 2, 4>(a, grid, st) : grad_go<F16, PARTS, STACKED, 2, 2>(a, grid, st);
+  return p.lw == 4 ? grad_go<F16, PARTS, STACKED, 4, 4>(a, grid, st) : grad_go<F16, PARTS, STACKED, 4, 2>(a, grid, st);
 }
 template <int DT, int PARTS>
 int backward_parts(BackwardArgs& a, const BackwardPlan& p, hipStream_t st) {
