@@ -82,6 +82,14 @@ __device__ __forceinline__ const __attribute__((address_space(4))) A* argument()
   return (const __attribute__((address_space(4))) A*)__builtin_amdgcn_kernarg_segment_ptr();
 }
 
+template <bool F16>
+__device__ __forceinline__ f32x16 dense_step(u32x4 a, u32x4 b, f32x16 c) {
+  if constexpr (F16)
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+
 // 16 bytes a lane straight from memory into LDS: lane i's land at lds + 16 i (lds: the same for the whole wave).
 __device__ __forceinline__ void copy_in(const uint8_t* from, uint8_t* lds) {
   __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)from, (__attribute__((address_space(3))) void*)lds, 16, 0, 0);

@@ -8,8 +8,8 @@
 //   dz = dy act'(z),   dw[h][l][c] = sum_b dz[b][h] x[b][l][c],   dbias[h] = sum_b dz[b][h].
 // A cell shows one character, so of the four features (four layers of one cell) at most one is set: the left operand is
 // 2:4 sparse along the summed axis by construction, and v_smfmac_f32_32x32x32 multiplies it at 3,750 TFLOP/s where the
-// dense v_mfma_f32_32x32x16 gives 2,270 (both measured here, register operands only).  Overlapping layers use the same
-// instruction with two layers to a group of four (the other two weights are zero): the dense rate, one kernel.
+// dense v_mfma_f32_32x32x16 gives 2,270 (both measured here, register operands only).  Overlapping layers take the dense one,
+// 8 cells x 2 layers at a time.
 // A set feature is the number 2 -- the bit pattern 0x4000 in bfloat16 AND in float16 -- so that expanding a feature pair
 // is one shift and one mask; the other operand is halved instead (float16, whose small numbers have no bit to spare and
 // whose sums cannot leave float32's range: the sum is), which is exact down to the last subnormal bit.  float32 weights
@@ -61,7 +61,8 @@ using pcx::set_error;
 
 namespace {
 
-constexpr int FRAG = 2048;       // bytes of one right operand: 32 features x 32 hidden units x 2
+// bytes of one right operand: 32 features x 32 hidden units x 2, of stacked layers 16 x 32 x 2
+__host__ __device__ constexpr int frag_bytes(bool stacked) { return stacked ? 1024 : 2048; }
 
 // What a sum of the matrix unit is multiplied by: a feature is 2, and all weights but float16 ones are laid out halved.
 template <int DT> constexpr float SCALE = DT == PCX_F16 ? 0.5f : 1.0f;
@@ -91,8 +92,9 @@ __device__ __forceinline__ void activate(float z, float* y, float* slope) {
 // element e standing for cell start + 16 (e / 8) + 4 j + 2 hb + (e % 8) / 4 of the quad and position e % 4 of the group
 // (the lane layout of the instruction, measured: the sparse side's half A covers features 16 A .. 16 A + 15, the dense
 // side's element e feature 16 (e / 8) + 8 hb + e % 8).  The 16 bytes of elements 0..7 and of 8..15 of a lane are 1 KB apart,
-// so that a wave's LDS reads are contiguous.  A workgroup turns one quad of one group and tile round through LDS, so that
-// the weight is read in runs of 32 cells (a direct gather took 52 us for 5.6 million float32 weights; this one 20).
+// so that a wave's LDS reads are contiguous.  The dense instruction of stacked layers sums 16 features: element e of a
+// lane's 8 stands for cell start + 16 hb + 4 j + e / 2 and layer e % 2 of the group.  A workgroup turns one quad of one group and tile round through LDS, so that
+// the weight is read in runs of 32 cells (a direct gather took 52 us for 5.6 million float32 weights; this one 23).
 template <int DT>
 __global__ __launch_bounds__(256) void pcx_project_layout(Shape s, const typename Num<DT>::T* __restrict__ w, u32x4* __restrict__ packed) {
   __shared__ float in[32][4][33];
@@ -107,21 +109,22 @@ __global__ __launch_bounds__(256) void pcx_project_layout(Shape s, const typenam
   }
   __syncthreads();
   const int per = s.stacked || s.groups < 4 ? s.groups : 4;  // groups per block
-  for (int i = threadIdx.x; i < 4 * s.parts * 128; i += 256) {
-    const int lane = i & 63, e8 = (i >> 6) & 1, j = (i >> 7) & 3, part = i >> 9, hb = lane >> 5;
+  const int e8s = s.stacked ? 0 : 1;  // (the runs of 8 elements a lane has: 1 << e8s)
+  for (int i = threadIdx.x; i < (4 * s.parts * 64) << e8s; i += 256) {
+    const int lane = i & 63, e8 = (i >> 6) & e8s, j = (i >> (6 + e8s)) & 3, part = i >> (8 + e8s), hb = lane >> 5;
     u32x4 out = {0, 0, 0, 0};
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      const float v = in[lane & 31][e & 3][e8 * 16 + j * 4 + hb * 2 + (e >> 2)];
+      const float v = s.stacked ? in[lane & 31][e & 1][hb * 16 + j * 4 + (e >> 1)] : in[lane & 31][e & 3][e8 * 16 + j * 4 + hb * 2 + (e >> 2)];
       uint32_t bits;
       if constexpr (DT == PCX_F16) bits = __builtin_bit_cast(uint16_t, (_Float16)v);
       else bits = part_of(0.5f * v, part, s.parts);
       out[e >> 1] |= bits << (16 * (e & 1));
     }
     int64_t step;
-    if (s.stacked) step = (((int64_t)q * s.groups + g) * s.parts + part) * 4 + j;
+    if (s.stacked) step = (((int64_t)g * s.quads + q) * s.parts + part) * 4 + j;
     else step = ((((int64_t)(g / per) * s.quads + q) * 4 + j) * s.parts + part) * per + g % per;
-    packed[(step * s.tiles + tile) * 128 + e8 * 64 + lane] = out;
+    packed[((step * s.tiles + tile) << (6 + e8s)) + e8 * 64 + lane] = out;
   }
 }
 
@@ -143,6 +146,9 @@ struct ForwardArgs {
 // How many octets of a quad a stage holds: as many as leave two workgroups of four waves a CU, or one of eight.
 constexpr int octets_per_stage(int parts, int groups, int waves) {
   return parts > 1 ? 1 : groups == 1 ? 4 : groups == 2 ? (waves == 8 ? 4 : 2) : groups == 4 && waves == 8 ? 2 : 1;
+}
+constexpr int steps_per_stage(int parts, int groups, int waves) {
+  return groups == 0 ? (parts > 1 ? 4 : 8) : octets_per_stage(parts, groups, waves) * (parts == 3 && groups == 1 ? 3 : 1) * groups;
 }
 // bit 6 of every byte that is not zero
 __device__ __forceinline__ uint32_t set_bytes(uint32_t b) {
@@ -224,7 +230,8 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void pcx_project_forward_kernel(Fo
   constexpr int WAVES = WM * WN;
   constexpr int OCT = STACKED ? 4 : octets_per_stage(PARTS, G, WAVES);                     // octets per stage
   constexpr int PS = !STACKED && PARTS == 3 && G == 1 ? 3 : 1;                             // parts per stage
-  constexpr int STEPS = STACKED ? 4 : OCT * PS * G;                                        // matrix steps per stage
+  constexpr int STEPS = steps_per_stage(PARTS, G, WAVES);                                  // matrix steps per stage
+  constexpr int FRAG = frag_bytes(STACKED), PF = FRAG / 1024;
   constexpr int STAGE = STEPS * FR * FRAG;
   constexpr int PIECES = STAGE / 1024;        // 1 KB copies per stage
   constexpr int MROWS = WM * MT * 32;
@@ -238,7 +245,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void pcx_project_forward_kernel(Fo
   const int nb = (int)(id % (uint32_t)a.nblocks);
   const uint32_t rest = id / (uint32_t)a.nblocks;
   const int split = (int)(rest % (uint32_t)a.splits), mb = (int)(rest / (uint32_t)a.splits);
-  const int blocks = STACKED ? 1 : (s.groups + 3) / 4;
+  const int blocks = STACKED ? s.groups : (s.groups + 3) / 4;
   // A block's table by character: bits 0..3 and again 4..7 the positions of the two slots of a group -- they ascend: (p, 3)
   // with the feature in the low slot for p < 3, (0, 3) with it in the high one for 3 -- and bit 14 - g (30 - g) a feature of
   // group g in its low (high) slot.  (Two words a character save 6 of 21 instructions a cell quad and lose 6 % to the
@@ -249,10 +256,10 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void pcx_project_forward_kernel(Fo
     const int l = b * 16 + tid, p = l & 3, g = (l >> 2) & 3;
     if (tid < 16 && l < s.layers) lut[argument<ForwardArgs>()->s.chars[l]] = p < 3 ? (0x4000u >> g) | (uint32_t)((p | 12) * 0x11) : (0x40000000u >> g) | 0xCCu;
   };
-  // the run of (block, quad) units of this split
+  // the run of (block, quad) units of this split (STACKED: a block is a group)
   const int units = blocks * s.quads;
   const int u0 = (int)((int64_t)units * split / a.splits), u1 = (int)((int64_t)units * (split + 1) / a.splits);
-  const int per_unit = 4 * PARTS * (STACKED ? s.groups : G), stages = (u1 - u0) * per_unit / STEPS;
+  const int per_unit = 4 * PARTS * (STACKED ? 1 : G), stages = ((u1 - u0) * per_unit + STEPS - 1) / STEPS;
   const int tile0 = nb * FR, live = s.tiles - tile0 < FR ? s.tiles - tile0 : FR;
   const uint8_t* const src = a.packed + ((int64_t)u0 * per_unit * s.tiles + tile0) * FRAG + lane * 16;
   const int wm = wave / WN, wn = wave % WN, half = lane >> 5;
@@ -267,8 +274,8 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void pcx_project_forward_kernel(Fo
     uint8_t* const dst = lds + (st & 1) * STAGE;
 #pragma unroll
     for (int i = 0; i < (PIECES + WAVES - 1) / WAVES; ++i) {
-      const int k = wave + WAVES * i, step = k / (2 * FR), off = k % (2 * FR);  // 2 FR pieces of 1 KB to a step
-      if (k < PIECES && off < 2 * live) copy_in(src + ((int64_t)(st * STEPS + step) * s.tiles) * FRAG + off * 1024, dst + k * 1024);
+      const int k = wave + WAVES * i, step = k / (PF * FR), off = k % (PF * FR);  // PF FR pieces of 1 KB to a step
+      if (k < PIECES && off < PF * live) copy_in(src + ((int64_t)(st * STEPS + step) * s.tiles) * FRAG + off * 1024, dst + k * 1024);
     }
   };
   f32x16 acc[MT][NT];
@@ -282,19 +289,26 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void pcx_project_forward_kernel(Fo
   int index[MT];
   // One matrix step: step k of the stage at `base`.  The right operands are read one ahead, the first of a stage in
   // front of it.
-  u32x8 ahead;
+  typename std::conditional<STACKED, u32x4, u32x8>::type ahead;
   auto read_right = [&](const uint8_t* base, int i) {
     const uint8_t* const at = base + ((i / NT) * FR + i % NT) * FRAG;
-    const u32x4 b0 = *reinterpret_cast<const u32x4*>(at), b1 = *reinterpret_cast<const u32x4*>(at + 1024);
-    ahead = u32x8{b0[0], b0[1], b0[2], b0[3], b1[0], b1[1], b1[2], b1[3]};
+    const u32x4 b0 = *reinterpret_cast<const u32x4*>(at);
+    if constexpr (STACKED) {
+      ahead = b0;
+    } else {
+      const u32x4 b1 = *reinterpret_cast<const u32x4*>(at + 1024);
+      ahead = u32x8{b0[0], b0[1], b0[2], b0[3], b1[0], b1[1], b1[2], b1[3]};
+    }
   };
   auto multiply = [&](const uint8_t* base, int k) {
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
-      const u32x8 right = ahead;
+      const auto right = ahead;
       if (k * NT + t + 1 < STEPS * NT) read_right(base, k * NT + t + 1);
 #pragma unroll
-      for (int m = 0; m < MT; ++m) acc[m][t] = sparse_step<DT == PCX_F16>(left[m], right, acc[m][t], index[m]);
+      for (int m = 0; m < MT; ++m)
+        if constexpr (STACKED) acc[m][t] = dense_step<DT == PCX_F16>(left[m], right, acc[m][t]);
+        else acc[m][t] = sparse_step<DT == PCX_F16>(left[m], right, acc[m][t], index[m]);
     }
   };
   auto stage_base = [&](int st) { return lds + (st & 1) * STAGE + wn * NT * FRAG + lane * 16; };
@@ -310,7 +324,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void pcx_project_forward_kernel(Fo
     return v;
   };
   // A stage's weights must have arrived, the boards' bytes requested after them need not: `loose` says that they were.
-  constexpr int LOADS = STACKED ? 2 * MT : MT;
+  constexpr int LOADS = STACKED ? 4 * MT : MT;
   bool loose = false;
   auto arrive = [&]() {
     if (loose) stage_barrier<LOADS>();
@@ -319,13 +333,32 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void pcx_project_forward_kernel(Fo
   };
   int st = 0;
   if constexpr (STACKED) {
-    // The two layers of a (quad, group) unit, DEPTH - 1 units ahead: a unit is only 4 matrix steps, a trip to memory many.
-    constexpr int DEPTH = MT == 4 ? 2 : 4;
-    u32x4 ring[DEPTH][MT][2];
+    // The two layers of a (group, quad) unit, DEPTH - 1 units ahead: a unit is only 4 matrix steps, a trip to memory many.
+    // All quads of two layers follow each other, so that a board's bytes are read in the order in which they lie.
+    constexpr int DEPTH = 4;
+    // Layers lie at any byte: a lane reads the five aligned words around its 16 bytes (an aligned word never leaves the page
+    // of the byte that is wanted) and shifts them when they are used; loads at odd bytes took 42 us where these take 38.
+    struct Bytes { u32x4 v; uint32_t more, by; };
+    auto load_bytes = [&](const uint8_t* at, int c) {
+      Bytes x;
+      if (small) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x.v[i] = edge_dword(at, c + 4 * i, s.cells);
+        x.more = x.by = 0;
+      } else {
+        at += c;
+        x.by = (uint32_t)reinterpret_cast<uintptr_t>(at) & 3u;
+        const uint32_t* const words = reinterpret_cast<const uint32_t*>(at - x.by);
+        __builtin_memcpy(&x.v, words, 16);
+        x.more = words[x.by ? 4 : 3];
+      }
+      return x;
+    };
+    Bytes ring[DEPTH][MT][2];
     uint32_t on[DEPTH][2];  // 0 where the layer does not exist: its bytes are then the board's first
-    int fq = u0, fg = 0;
-    auto fetch = [&](u32x4 (&to)[MT][2], uint32_t (&keep)[2]) {
-      if (fq >= u1) return;
+    int fq = u0 % s.quads, fg = u0 / s.quads, fetched = u0;
+    auto fetch = [&](Bytes (&to)[MT][2], uint32_t (&keep)[2]) {
+      const bool last = ++fetched >= u1;  // (then the last unit again: the same number of requests for every one)
       const int c = quad_start(fq, s.cells) + half * 16;
 #pragma unroll
       for (int l = 0; l < 2; ++l) {
@@ -333,18 +366,16 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void pcx_project_forward_kernel(Fo
         const int64_t off = layer < s.layers ? argument<ForwardArgs>()->s.layer_offset[layer] : -1;
         keep[l] = off >= 0 ? 0xFFFFFFFFu : 0u;
 #pragma unroll
-        for (int m = 0; m < MT; ++m) to[m][l] = load16(row[m] + (off >= 0 ? off : 0), c);
+        for (int m = 0; m < MT; ++m) to[m][l] = load_bytes(row[m] + (off >= 0 ? off : 0), c);
       }
-      loose = !small;
-      if (++fg == s.groups) { fg = 0; ++fq; }
+      if (!last && ++fq == s.quads) { fq = 0; ++fg; }
     };
-#pragma unroll
-    for (int m = 0; m < MT; ++m) index[m] = 0x4444;
 #pragma unroll
     for (int k = 0; k < DEPTH - 1; ++k) fetch(ring[k], on[k]);
     stage_in(0);
-    loose = false;
-    const int total = (u1 - u0) * s.groups;
+    stage_barrier<0>();
+    const uint8_t* base = nullptr;
+    const int total = u1 - u0;
 #pragma unroll 1
     for (int i = 0; i < total; i += DEPTH)
 #pragma unroll
@@ -352,25 +383,36 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void pcx_project_forward_kernel(Fo
         if (i + k >= total) break;
 #pragma unroll
         for (int part = 0; part < PARTS; ++part) {
-          arrive();
-          if (st + 1 < stages) stage_in(st + 1);
-          asm volatile("" ::: "memory");
+          constexpr int PER = STEPS / 4;  // (PARTS = 1: units per stage)
+          if (PARTS > 1 || k % PER == 0) {
+            // a stage's weights must be here, the boards' bytes asked for behind it may be on their way
+            if (small || (PARTS > 1 && part != 1)) stage_barrier<0>();
+            else stage_barrier<PER * LOADS>();
+            if (st + 1 < stages) stage_in(st + 1);
+            asm volatile("" ::: "memory");
+            base = stage_base(st);
+            ++st;
+          }
           if (part == 0) fetch(ring[(k + DEPTH - 1) % DEPTH], on[(k + DEPTH - 1) % DEPTH]);
-          const uint8_t* const base = stage_base(st);
-          read_right(base, 0);
+          if (PARTS > 1 || k % PER == 0) read_right(base, 0);
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
 #pragma unroll
             for (int m = 0; m < MT; ++m) {
-              const uint32_t lo = set_bytes(ring[k][m][0][j]) & on[k][0], hi = set_bytes(ring[k][m][1][j]) & on[k][1];
+              uint32_t b[2];
+#pragma unroll
+              for (int l = 0; l < 2; ++l) {
+                const Bytes& x = ring[k][m][l];
+                b[l] = set_bytes(__builtin_amdgcn_alignbyte(j < 3 ? x.v[j < 3 ? j + 1 : 3] : x.more, x.v[j], x.by)) & on[k][l];
+              }
+              const uint32_t lo = b[0], hi = b[1];
               left[m][0] = __builtin_amdgcn_perm(hi, lo, 0x040C000Cu);
               left[m][1] = __builtin_amdgcn_perm(hi, lo, 0x050C010Cu);
               left[m][2] = __builtin_amdgcn_perm(hi, lo, 0x060C020Cu);
               left[m][3] = __builtin_amdgcn_perm(hi, lo, 0x070C030Cu);
             }
-            multiply(base, j);
+            multiply(base, PARTS > 1 ? j : k % (STEPS / 4) * 4 + j);
           }
-          ++st;
         }
       }
   } else {
@@ -435,7 +477,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void pcx_project_forward_kernel(Fo
   }
   // Out through LDS, 32 boards at a time and each wave by itself: a lane then has four neighbouring hidden units of one
   // board, and a wave writes whole rows of its tile.  The residual's rows are on their way one tile ahead and wait in LDS
-  // too (loaded where they are used, every row cost its own trip to memory: 583 us against 340 for 262,144 boards).
+  // too (loaded where they are used, every row cost its own trip to memory: 583 us against 315 for 262,144 boards of 300 cells x 8 layers).
   typedef typename Num<DT>::T T;
   constexpr int PITCH = NT * 32 + 4, LANES = NT * 8, ROUNDS = 32 * LANES / 64;  // lanes per row, rows per lane
   __syncthreads();
@@ -518,7 +560,7 @@ __global__ __launch_bounds__(256) void pcx_project_join(ForwardArgs a) {
 
 // ---------------------------------------------------------------- plan
 
-struct ForwardPlan { int mt, wm, wn, mblocks, nblocks, splits; uint64_t bytes; };
+struct ForwardPlan { int mt, nt, wm, wn, mblocks, nblocks, splits; uint64_t bytes; };
 
 ForwardPlan plan_forward(const Shape& s) {
   ForwardPlan p;
@@ -526,18 +568,24 @@ ForwardPlan plan_forward(const Shape& s) {
   // boards fill the chip with them (the weight then leaves L2 half as often); where they do not fill it with four, a wave
   // takes 2 x 2 tiles, and only then are the cells divided: joining costs 8 bytes a sum and part.
   p.mt = 4;
+  p.nt = 2;
   p.wn = s.tiles >= 3 ? 2 : 1;
   p.wm = 4 / p.wn;
   const int64_t nblocks = (s.tiles + 2 * p.wn - 1) / (2 * p.wn);
-  if (s.n <= 512) { p.mt = 1; p.wm = 1; p.wn = 4; }
+  // Stacked layers wait for the boards' bytes more than for the matrix units: small tiles of sums leave room for twice the
+  // waves (32,768 boards, 11 layers of 110 cells, 128 units: 2 x 2 tiles and four waves 47 us, 1 x 2 45, with eight 42).
+  if (s.stacked) { p.mt = 1; p.wm = 4; }
+  else if (s.n <= 512) { p.mt = p.nt = p.wm = 1; p.wn = 4; }
   else if (p.wn == 2 && s.n * nblocks >= 512 * 192) p.wm = 4;
   else if ((s.n + 128 * p.wm - 1) / (128 * p.wm) * nblocks < SLOTS / 2) p.mt = 2;
-  const int rows = p.wm * p.mt * 32, cols = (p.mt == 1 ? 1 : 2) * p.wn;
+  const int rows = p.wm * p.mt * 32, cols = p.nt * p.wn;
   p.mblocks = (int)((s.n + rows - 1) / rows);
   p.nblocks = (s.tiles + cols - 1) / cols;
   const int64_t groups = (int64_t)p.mblocks * p.nblocks;
-  int64_t splits = groups >= SLOTS / 2 || p.wm * p.wn == 8 ? 1 : SLOTS / groups;
-  if (splits > s.quads) splits = s.quads;
+  const int64_t slots = p.wm * p.wn == 8 ? SLOTS / 2 : SLOTS;
+  int64_t splits = groups >= slots / 2 || (p.wm * p.wn == 8 && !s.stacked) ? 1 : slots / groups;
+  const int64_t units = (int64_t)s.quads * (s.stacked ? s.groups : 1);
+  if (splits > units) splits = units;
   p.splits = (int)splits;
   p.bytes = splits > 1 ? (uint64_t)splits * s.n * s.hidden * 4 : 0;
   return p;
@@ -546,8 +594,8 @@ ForwardPlan plan_forward(const Shape& s) {
 template <int DT, int G, int MT, int NT, int WM, int WN>
 int forward_go(const ForwardArgs& a, unsigned grid, hipStream_t st) {
   constexpr int PARTS = DT == PCX_F32 ? 3 : 1, WAVES = WM * WN;
-  constexpr int STEPS = G == 0 ? 4 : octets_per_stage(PARTS, G, WAVES) * (PARTS == 3 && G == 1 ? 3 : 1) * G;
-  constexpr int ROWS_OUT = WAVES * 32 * (NT * 32 + 4) * 4 + WAVES * 32 * NT * 32 * (DT == PCX_F32 ? 4 : 2), STAGES = 2 * STEPS * NT * WN * FRAG;
+  constexpr int STEPS = steps_per_stage(PARTS, G, WAVES);
+  constexpr int ROWS_OUT = WAVES * 32 * (NT * 32 + 4) * 4 + WAVES * 32 * NT * 32 * (DT == PCX_F32 ? 4 : 2), STAGES = 2 * STEPS * NT * WN * frag_bytes(G == 0);
   constexpr int LDS = ROWS_OUT > STAGES ? ROWS_OUT : STAGES;
   auto* const kernel = &pcx_project_forward_kernel<DT, G, MT, NT, WM, WN>;
   if (LDS + 1024 > 65536) PCX_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, LDS));
@@ -564,7 +612,7 @@ int forward_shape(const ForwardArgs& a, const ForwardPlan& p, unsigned grid, hip
 template <int DT>
 int forward_type(const ForwardArgs& a, const ForwardPlan& p, unsigned grid, hipStream_t st) {
   int rc;
-  if (a.s.stacked) rc = forward_shape<DT, 0>(a, p, grid, st);
+  if (a.s.stacked) rc = p.wn == 2 ? forward_go<DT, 0, 1, 2, 4, 2>(a, grid, st) : forward_go<DT, 0, 1, 2, 4, 1>(a, grid, st);
   else if (a.s.groups == 1) rc = forward_shape<DT, 1>(a, p, grid, st);
   else if (a.s.groups == 2) rc = forward_shape<DT, 2>(a, p, grid, st);
   else if (a.s.groups == 3) rc = forward_shape<DT, 3>(a, p, grid, st);
@@ -584,7 +632,7 @@ extern "C" {
 int pcx_project_sizes(const pcx_project_desc* d, uint64_t* packed_bytes, uint64_t* forward_bytes, uint64_t* backward_bytes) {
   Shape s;
   if (int rc = make_shape(d, &s, "pcx_project_sizes")) return rc;
-  if (packed_bytes) *packed_bytes = (uint64_t)s.quads * 4 * s.groups * s.parts * s.tiles * FRAG;
+  if (packed_bytes) *packed_bytes = ((uint64_t)s.quads * s.groups + s.stacked) * 4 * s.parts * s.tiles * frag_bytes(s.stacked);
   if (forward_bytes) *forward_bytes = s.n ? plan_forward(s).bytes : 0;
   if (backward_bytes) *backward_bytes = s.n ? pcx::project::backward_bytes(s) : 0;
   return 0;

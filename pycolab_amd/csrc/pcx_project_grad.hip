@@ -117,21 +117,14 @@ __global__ __launch_bounds__(256) void pcx_project_turn(BackwardArgs a) {
   if (tid < 64 && h0 + tid < s.hidden) a.bias_part[(int64_t)blockIdx.x * s.hidden + h0 + tid] = (sums[0][tid] + sums[1][tid]) + (sums[2][tid] + sums[3][tid]);
 }
 
-template <bool F16>
-__device__ __forceinline__ f32x16 dense_step(u32x4 a, u32x4 b, f32x16 c) {
-  if constexpr (F16)
-    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
-  else
-    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
-}
-
 // dw[h][l][c] over a run of boards: a workgroup owns NH tiles of hidden units x 32 cells x up to 2 LW layers (NH = 1: 4 LW).
 // The sum runs over boards, along which the features are not sparse: the dense instruction.  Its right operand is the
 // feature bit of 8 consecutive boards at one cell: the boards are turned round once per stage into LDS as a word of layer
 // bits per (cell, board), from which every layer's operand is one shift and one mask.  A wave takes LW layers x half the
-// hidden units: one LDS read then serves LW operands, and every dz operand read LW products (with 2 layers x all units a
-// wave the LDS was the bound: 91 us for 65,536 boards x 256 units x 8 layers, 4 x half of them:
-// GRAD_US us).
+// hidden units (2,048 boards of 4,005 cells in float32: 106 us; 2 layers x all units 117).  65,536 boards of 300 cells x 8
+// layers x 256 units take 89 us.  The instructions alone take 47 of them (1.8 PFLOP/s): the masks' way through the LDS
+// after each barrier adds 11, dz's copies and the boards' turning, which the other workgroup's products hide in part, 26,
+// and the partial sums, as many as all registers of the card hold, 8.
 template <bool F16, int PARTS, bool STACKED, int NH, int LW>
 __global__ __launch_bounds__(256, 2) void pcx_project_weight_grad(BackwardArgs a) {
   constexpr int STAGE = 4 * NH * PARTS * 1024;
@@ -163,7 +156,7 @@ __global__ __launch_bounds__(256, 2) void pcx_project_weight_grad(BackwardArgs a
 #pragma unroll
     for (int i = 0; i < NH * PARTS; ++i) {
       const int k = wave * NH * PARTS + i;  // (piece i of board step `wave`)
-      copy_in(src + ((((int64_t)b * 4 + wave) * a.htiles) * PARTS + i) * 1024, dst + k * 1024);
+      copy_in(src + ((((int64_t)(b < b1 ? b : b1 - 1) * 4 + wave) * a.htiles) * PARTS + i) * 1024, dst + k * 1024);
     }
   };
   // a thread turns two boards x four cells round
@@ -190,23 +183,20 @@ __global__ __launch_bounds__(256, 2) void pcx_project_weight_grad(BackwardArgs a
       }
     }
   };
-  auto turn = [&](int b, const uint32_t* raw) {
+  auto turn = [&](int b, const uint32_t* raw, int c) {  // (of the thread's four cells the one numbered c)
     uint8_t* const dst = lds + 3 * STAGE + (b & 1) * MASKS;
+    uint32_t m[2];
 #pragma unroll
-    for (int c = 0; c < 4; ++c) {
-      uint32_t m[2];
+    for (int r = 0; r < 2; ++r) {
+      if constexpr (STACKED) {
+        m[r] = 0;
 #pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        if constexpr (STACKED) {
-          m[r] = 0;
-#pragma unroll
-          for (int l = 0; l < PL; ++l) m[r] |= offset[l] >= 0 && ((raw[r * PL + l] >> (8 * c)) & 255u) ? 1u << (14 - l) : 0u;
-        } else {
-          m[r] = lut[(raw[r] >> (8 * c)) & 255u];
-        }
+        for (int l = 0; l < PL; ++l) m[r] |= offset[l] >= 0 && ((raw[r * PL + l] >> (8 * c)) & 255u) ? 1u << (14 - l) : 0u;
+      } else {
+        m[r] = lut[(raw[r] >> (8 * c)) & 255u];
       }
-      *reinterpret_cast<uint32_t*>(dst + ((cell + c) * PITCH + pair * 2) * 2) = m[0] | (m[1] << 16);
     }
+    *reinterpret_cast<uint32_t*>(dst + ((cell + c) * PITCH + pair * 2) * 2) = m[0] | (m[1] << 16);
   };
   f32x16 acc[LW][HW];
 #pragma unroll
@@ -216,10 +206,17 @@ __global__ __launch_bounds__(256, 2) void pcx_project_weight_grad(BackwardArgs a
 #pragma unroll
       for (int i = 0; i < 16; ++i) acc[l][h][i] = 0.0f;
   const int wl = wave % WL, wh = wave / WL;
-  const bool work = l0 + wl * LW < s.layers;
-  auto multiply = [&](int b) {
+  // One block of boards: the block after the next is asked for, the next one's boards are turned round, this one's products
+  // are formed.  Blocks past the run's end are its last block again: they land in stages that nobody reads.
+  auto step = [&](int b, const uint32_t* next, uint32_t* later) {
+    stage_barrier<NH * PARTS>();  // (block b's dz is here; block b + 1's copies, the newest requests, may be on their way)
+    fetch(b + 2, later);
+    stage_in(b + 2);
     const uint8_t* const dz = lds + (b - b0) % 3 * STAGE + lane * 16;
     const uint8_t* const masks = lds + 3 * STAGE + (b & 1) * MASKS + ((lane & 31) * PITCH + half * 8) * 2;
+#pragma unroll
+    for (int c = 0; c < 4; ++c) turn(b + 1, next, c);
+    __builtin_amdgcn_s_setprio(1);  // (a wave that multiplies goes before the other workgroup's that turn: 94 -> 89 us)
 #pragma unroll
     for (int kb = 0; kb < 4; ++kb) {
       const u32x4 m = *reinterpret_cast<const u32x4*>(masks + kb * 32);
@@ -237,41 +234,24 @@ __global__ __launch_bounds__(256, 2) void pcx_project_weight_grad(BackwardArgs a
           for (int l = 0; l < LW; ++l) acc[l][h] = dense_step<F16>(left, right[l], acc[l][h]);
         }
     }
-  };
-  // dz is two stages ahead, the boards' bytes two: block b's dz is here once no more than the NH * PARTS copies of block
-  // b + 1, the newest requests, are on their way.
-  auto begin = [&](int b) {
-    if (b + 1 < b1) stage_barrier<NH * PARTS>();
-    else stage_barrier<0>();
+    __builtin_amdgcn_s_setprio(0);
   };
   uint32_t even[2 * PL], odd[2 * PL];
   if (b0 < b1) {
     fetch(b0, even);
     stage_in(b0);
-    if (b0 + 1 < b1) {
-      fetch(b0 + 1, odd);
-      stage_in(b0 + 1);
-    }
-  }
-  __syncthreads();  // the table
-  if (b0 < b1) turn(b0, even);
+    fetch(b0 + 1, odd);
+    stage_in(b0 + 1);
+    __syncthreads();  // the table
+#pragma unroll
+    for (int c = 0; c < 4; ++c) turn(b0, even, c);
 #pragma unroll 1
-  for (int b = b0; b < b1; b += 2) {
-    begin(b);
-    if (b + 2 < b1) {
-      fetch(b + 2, even);
-      stage_in(b + 2);
+    for (int b = b0; b < b1; b += 2) {
+      step(b, odd, even);
+      if (b + 1 >= b1) break;
+      step(b + 1, even, odd);
     }
-    if (work) multiply(b);
-    if (b + 1 >= b1) break;
-    turn(b + 1, odd);
-    begin(b + 1);
-    if (b + 3 < b1) {
-      fetch(b + 3, odd);
-      stage_in(b + 3);
-    }
-    if (work) multiply(b + 1);
-    if (b + 2 < b1) turn(b + 2, even);
+    stage_barrier<0>();  // (no copy may land after the workgroup's end)
   }
   const int c = c0 + (lane & 31);
   if (c < cb * QUAD || c >= s.cells) return;  // (the block before owns the cells this one shares with it)
