@@ -567,6 +567,11 @@ ForwardPlan plan_forward(const Shape& s) {
   // 4 x 2 tiles a wave make the most of a weight in LDS and of an expanded board.  Eight waves share a weight where the
   // boards fill the chip with them (the weight then leaves L2 half as often); where they do not fill it with four, a wave
   // takes 2 x 2 tiles, and only then are the cells divided: joining costs 8 bytes a sum and part.
+  // But every 128 boards fetch the weight anew, from beyond an XCD's 4 MB of L2 if it is large: from some 400 MB of that on
+  // (boards times the weight's bytes) eight waves of 512 boards stay, with the cells divided more often.  Float32 weights of
+  // 4,005 cells, 7 layers and 200 units: 2,048 boards 80 -> 69 us, 16,384 boards 749 -> 334; bfloat16 ones of 480 cells, 14
+  // layers and 512 units: 8,192 boards 70 -> 63, 4,096 boards 40 where eight waves take 51.
+  const int64_t packed = (int64_t)s.quads * 4 * s.groups * s.parts * s.tiles * frag_bytes(s.stacked);
   p.mt = 4;
   p.nt = 2;
   p.wn = s.tiles >= 3 ? 2 : 1;
@@ -576,14 +581,14 @@ ForwardPlan plan_forward(const Shape& s) {
   // waves (32,768 boards, 11 layers of 110 cells, 128 units: 2 x 2 tiles and four waves 47 us, 1 x 2 45, with eight 42).
   if (s.stacked) { p.mt = 1; p.wm = 4; }
   else if (s.n <= 512) { p.mt = p.nt = p.wm = 1; p.wn = 4; }
-  else if (p.wn == 2 && s.n * nblocks >= 512 * 192) p.wm = 4;
+  else if (p.wn == 2 && (s.n * nblocks >= 512 * 192 || s.n * packed >= (int64_t)50 << 30)) p.wm = 4;
   else if ((s.n + 128 * p.wm - 1) / (128 * p.wm) * nblocks < SLOTS / 2) p.mt = 2;
   const int rows = p.wm * p.mt * 32, cols = p.nt * p.wn;
   p.mblocks = (int)((s.n + rows - 1) / rows);
   p.nblocks = (s.tiles + cols - 1) / cols;
   const int64_t groups = (int64_t)p.mblocks * p.nblocks;
   const int64_t slots = p.wm * p.wn == 8 ? SLOTS / 2 : SLOTS;
-  int64_t splits = groups >= slots / 2 || (p.wm * p.wn == 8 && !s.stacked) ? 1 : slots / groups;
+  int64_t splits = groups > slots / 2 ? 1 : slots / groups;
   const int64_t units = (int64_t)s.quads * (s.stacked ? s.groups : 1);
   if (splits > units) splits = units;
   p.splits = (int)splits;
