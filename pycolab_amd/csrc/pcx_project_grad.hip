@@ -121,19 +121,27 @@ __global__ __launch_bounds__(256) void pcx_project_turn(BackwardArgs a) {
 // The sum runs over boards, along which the features are not sparse: the dense instruction.  Its right operand is the
 // feature bit of 8 consecutive boards at one cell: the boards are turned round once per stage into LDS as a word of layer
 // bits per (cell, board), from which every layer's operand is one shift and one mask.  A wave takes LW layers x half the
-// hidden units (2,048 boards of 4,005 cells in float32: 106 us; 2 layers x all units 117).  65,536 boards of 300 cells x 8
+// hidden units (2 layers x all units: float32 gradients of 2,048 boards of 4,005 cells 10 us slower).  65,536 boards of 300 cells x 8
 // layers x 256 units take 89 us.  The instructions alone take 47 of them (1.8 PFLOP/s): the masks' way through the LDS
 // after each barrier adds 11, dz's copies and the boards' turning, which the other workgroup's products hide in part, 26,
 // and the partial sums, as many as all registers of the card hold, 8.
+// Blocks of dz in LDS, one in use: three where that leaves room for two workgroups a CU, else two (dz in two or three parts;
+// one workgroup with three instead: 2,048 boards of 4,005 cells, float32 gradients 130 us against 105, 65,536 of 300 with
+// gelu and bfloat16 ones 216 against 166, the turning and joining included).
+template <int PARTS, int NH>
+struct Stage {
+  static constexpr int BYTES = 4 * NH * PARTS * 1024, MASKS = 32 * (BLK + 8) * 2, RING = 3 * BYTES + 2 * MASKS + 512 <= 80 * 1024 ? 3 : 2;
+  static constexpr int LDS = RING * BYTES + 2 * MASKS + 512;
+};
 template <bool F16, int PARTS, bool STACKED, int NH, int LW>
 __global__ __launch_bounds__(256, 2) void pcx_project_weight_grad(BackwardArgs a) {
-  constexpr int STAGE = 4 * NH * PARTS * 1024;
+  constexpr int STAGE = Stage<PARTS, NH>::BYTES, RING = Stage<PARTS, NH>::RING;
   constexpr int PITCH = BLK + 8;                // words per cell: 16-byte reads of one wave spread over the banks
-  constexpr int MASKS = 32 * PITCH * 2;
+  constexpr int MASKS = Stage<PARTS, NH>::MASKS;
   constexpr int WH = NH == 1 ? 1 : 2, HW = NH / WH, WL = 4 / WH, LAYERS = WL * LW;  // waves along hidden units and layers
   const Shape& s = a.s;
   extern __shared__ __align__(16) uint8_t lds[];
-  uint16_t* const lut = reinterpret_cast<uint16_t*>(lds + 3 * STAGE + 2 * MASKS);
+  uint16_t* const lut = reinterpret_cast<uint16_t*>(lds + RING * STAGE + 2 * MASKS);
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = lane >> 5;
   const uint32_t tiles = (uint32_t)a.cell_blocks * a.layer_blocks * a.hblocks;
   // the tiles of one run of boards go to one XCD, whose L2 then serves dz and the boards once
@@ -152,7 +160,7 @@ __global__ __launch_bounds__(256, 2) void pcx_project_weight_grad(BackwardArgs a
   const int b0 = (int)((int64_t)a.blocks * split / a.splits), b1 = (int)((int64_t)a.blocks * (split + 1) / a.splits);
   const uint8_t* const src = a.frags + (int64_t)hb * NH * PARTS * 1024 + lane * 16;
   auto stage_in = [&](int b) {
-    uint8_t* const dst = lds + (b - b0) % 3 * STAGE;
+    uint8_t* const dst = lds + (b - b0) % RING * STAGE;
 #pragma unroll
     for (int i = 0; i < NH * PARTS; ++i) {
       const int k = wave * NH * PARTS + i;  // (piece i of board step `wave`)
@@ -184,7 +192,7 @@ __global__ __launch_bounds__(256, 2) void pcx_project_weight_grad(BackwardArgs a
     }
   };
   auto turn = [&](int b, const uint32_t* raw, int c) {  // (of the thread's four cells the one numbered c)
-    uint8_t* const dst = lds + 3 * STAGE + (b & 1) * MASKS;
+    uint8_t* const dst = lds + RING * STAGE + (b & 1) * MASKS;
     uint32_t m[2];
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
@@ -209,11 +217,20 @@ __global__ __launch_bounds__(256, 2) void pcx_project_weight_grad(BackwardArgs a
   // One block of boards: the block after the next is asked for, the next one's boards are turned round, this one's products
   // are formed.  Blocks past the run's end are its last block again: they land in stages that nobody reads.
   auto step = [&](int b, const uint32_t* next, uint32_t* later) {
-    stage_barrier<NH * PARTS>();  // (block b's dz is here; block b + 1's copies, the newest requests, may be on their way)
-    fetch(b + 2, later);
-    stage_in(b + 2);
-    const uint8_t* const dz = lds + (b - b0) % 3 * STAGE + lane * 16;
-    const uint8_t* const masks = lds + 3 * STAGE + (b & 1) * MASKS + ((lane & 31) * PITCH + half * 8) * 2;
+    // block b's dz and block b + 1's boards must be here; what was asked for since then may be on its way
+    if constexpr (RING == 3) {
+      stage_barrier<NH * PARTS>();
+      fetch(b + 2, later);
+      stage_in(b + 2);
+    } else {
+      if (small) stage_barrier<0>();
+      else stage_barrier<2 * PL>();
+      stage_in(b + 1);
+      asm volatile("" ::: "memory");
+      fetch(b + 2, later);
+    }
+    const uint8_t* const dz = lds + (b - b0) % RING * STAGE + lane * 16;
+    const uint8_t* const masks = lds + RING * STAGE + (b & 1) * MASKS + ((lane & 31) * PITCH + half * 8) * 2;
 #pragma unroll
     for (int c = 0; c < 4; ++c) turn(b + 1, next, c);
     __builtin_amdgcn_s_setprio(1);  // (a wave that multiplies goes before the other workgroup's that turn: 94 -> 89 us)
@@ -240,8 +257,8 @@ __global__ __launch_bounds__(256, 2) void pcx_project_weight_grad(BackwardArgs a
   if (b0 < b1) {
     fetch(b0, even);
     stage_in(b0);
-    fetch(b0 + 1, odd);
-    stage_in(b0 + 1);
+    if constexpr (RING == 3) fetch(b0 + 1, odd), stage_in(b0 + 1);
+    else fetch(b0 + 1, odd);
     __syncthreads();  // the table
 #pragma unroll
     for (int c = 0; c < 4; ++c) turn(b0, even, c);
@@ -264,7 +281,13 @@ __global__ __launch_bounds__(256, 2) void pcx_project_weight_grad(BackwardArgs a
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
         const int unit = (hb * NH + wh * HW + h) * 32 + 8 * (i >> 2) + 4 * half + (i & 3);
-        if (unit < s.hidden) a.partial[(((int64_t)split * s.hidden + unit) * s.layers + layer) * s.cells + c] = SCALE<F16> * acc[l][h][i];
+        if (unit >= s.hidden) continue;
+        const int64_t at = ((int64_t)unit * s.layers + layer) * s.cells + c;
+        const float v = SCALE<F16> * acc[l][h][i];
+        if (a.splits > 1) a.partial[(int64_t)split * s.hidden * s.layers * s.cells + at] = v;
+        else if (s.dtype == PCX_F32) reinterpret_cast<float*>(a.grad_weight)[at] = v;  // (whole: nothing to join)
+        else if (s.dtype == PCX_F16) reinterpret_cast<_Float16*>(a.grad_weight)[at] = Num<PCX_F16>::put(v);
+        else reinterpret_cast<__bf16*>(a.grad_weight)[at] = Num<PCX_BF16>::put(v);
       }
   }
 }
@@ -314,7 +337,7 @@ struct BackwardPlan { int nh, lw, htiles, hblocks, cell_blocks, layer_blocks, sp
 BackwardPlan plan_backward(const Shape& s) {
   BackwardPlan p;
   p.parts = dz_parts(s);
-  p.nh = s.tiles >= 3 ? 4 : s.tiles;
+  p.nh = p.parts == 3 ? (s.tiles >= 2 ? 2 : 1) : s.tiles >= 3 ? 4 : s.tiles;  // (dz in three parts: two workgroups' LDS)
   p.hblocks = (s.tiles + p.nh - 1) / p.nh;
   p.htiles = p.hblocks * p.nh;
   p.cell_blocks = s.quads;
@@ -332,13 +355,13 @@ BackwardPlan plan_backward(const Shape& s) {
   p.bias_blocks = p.blocks < 512 ? p.blocks : 512;
   p.frag_bytes = (uint64_t)p.blocks * 4 * p.htiles * p.parts * 1024;
   p.bias_bytes = ((uint64_t)p.bias_blocks * s.hidden * 4 + 255) & ~255ull;
-  p.part_bytes = (uint64_t)p.splits * s.hidden * s.layers * s.cells * 4;
+  p.part_bytes = p.splits > 1 ? (uint64_t)p.splits * s.hidden * s.layers * s.cells * 4 : 0;
   return p;
 }
 
 template <bool F16, int PARTS, bool STACKED, int NH, int LW>
 int grad_go(const BackwardArgs& a, unsigned grid, hipStream_t st) {
-  constexpr int LDS = 3 * 4 * NH * PARTS * 1024 + 2 * 32 * (BLK + 8) * 2 + 512;
+  constexpr int LDS = Stage<PARTS, NH>::LDS;
   auto* const kernel = &pcx_project_weight_grad<F16, PARTS, STACKED, NH, LW>;
   if (LDS > 65536) PCX_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, LDS));
   hipLaunchKernelGGL(kernel, dim3(grid), dim3(256), LDS, st, a);
@@ -348,7 +371,8 @@ template <bool F16, int PARTS, bool STACKED>
 int grad_shape(const BackwardArgs& a, const BackwardPlan& p, unsigned grid, hipStream_t st) {
   if (p.nh == 1) return grad_go<F16, PARTS, STACKED, 1, 2>(a, grid, st);
   if (p.nh == 2) return p.lw == 4 ? grad_go<F16, PARTS, STACKED, 2, 4>(a, grid, st) : grad_go<F16, PARTS, STACKED, 2, 2>(a, grid, st);
-  return p.lw == 4 ? grad_go<F16, PARTS, STACKED, 4, 4>(a, grid, st) : grad_go<F16, PARTS, STACKED, 4, 2>(a, grid, st);
+  if constexpr (PARTS == 3) return set_error(PCX_E_INVALID, "pcx_project_backward: no such tile");
+  else return p.lw == 4 ? grad_go<F16, PARTS, STACKED, 4, 4>(a, grid, st) : grad_go<F16, PARTS, STACKED, 4, 2>(a, grid, st);
 }
 template <int DT, int PARTS>
 int backward_parts(BackwardArgs& a, const BackwardPlan& p, hipStream_t st) {
@@ -361,10 +385,11 @@ int backward_parts(BackwardArgs& a, const BackwardPlan& p, hipStream_t st) {
     const unsigned grid = (unsigned)a.chunk * 8u;
     if (int rc = a.s.stacked ? grad_shape<F16, PARTS, true>(a, p, grid, st) : grad_shape<F16, PARTS, false>(a, p, grid, st)) return rc;
     const int64_t wgs = ((int64_t)a.s.hidden * a.s.layers * a.s.cells + 1023) / 1024;
-    weight_blocks = (int)(wgs < 4096 ? wgs : 4096);
+    if (a.splits > 1) weight_blocks = (int)(wgs < 4096 ? wgs : 4096);
   }
   const int bias_blocks = a.grad_bias ? (a.s.hidden + 15) / 16 : 0;
-  hipLaunchKernelGGL((pcx_project_grad_join<DT>), dim3((unsigned)(weight_blocks + bias_blocks)), dim3(256), 0, st, a, weight_blocks);
+  if (weight_blocks + bias_blocks)
+    hipLaunchKernelGGL((pcx_project_grad_join<DT>), dim3((unsigned)(weight_blocks + bias_blocks)), dim3(256), 0, st, a, weight_blocks);
   return 0;
 }
 template <int DT>
