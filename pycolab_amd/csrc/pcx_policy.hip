@@ -108,8 +108,8 @@ __device__ __forceinline__ void load_keys(const Rows& rows, int64_t row, int j, 
 // exp(d) for d <= 0 in 64 bits, to about a unit in the last place: d = n ln 2 + r with ln 2 in two parts, the upper one short
 // enough that n times it is exact (the reduction of Cody and Waite), the Taylor series
 // of exp(r), |r| <= ln(2) / 2, to r^13 / 13! (the next term is 4e-18), and n in the exponent.
-// Four at a time: a chain of twenty dependent instructions leaves the unit idle, four side by side do not (33 million
-// logits: 20 -> 11 us); and the coefficients are held in scalar registers, which the four share -- left to itself the
+// Four at a time: a chain of twenty dependent instructions leaves the unit idle, four side by side do not (8 x 2^20
+// logits without rules: 41 -> 36 us, all launches included); and the coefficients are held in scalar registers, which the four share -- left to itself the
 // compiler copies each into vector registers for every element.
 __device__ __forceinline__ double scalar(double c) { asm("" : "+s"(c)); return c; }
 template <int N>
@@ -400,10 +400,9 @@ __device__ __forceinline__ int draw_action(Group<THREADS>& g, const double* w, d
   return (int)g.max(last) - 1;  // (u is one or more, or no number: the last one kept)
 }
 
-// The largest key t with at least k keys >= t; more than k keys are not 0.
+// The largest key t in [lo, hi] with at least k keys >= t; k keys or more are >= lo.
 template <int THREADS, int EP>
-__device__ __forceinline__ uint32_t find_rank(Group<THREADS>& g, const uint32_t* key, uint32_t k, uint32_t hi) {
-  uint32_t lo = 1;
+__device__ __forceinline__ uint32_t find_rank(Group<THREADS>& g, const uint32_t* key, uint32_t k, uint32_t lo, uint32_t hi) {
   while (lo < hi) {
     const uint32_t mid = hi - (hi - lo) / 2;
     uint32_t c = 0;
@@ -431,15 +430,16 @@ __device__ __forceinline__ uint32_t find_mass(Group<THREADS>& g, const uint32_t*
 }
 
 // The rules on a group's elements, EP neighbouring ones a thread in index order, of which best_key is the largest key (not
-// 0); `of` says how many actions the row has.  Which element is drawn.
+// 0) and `low` no more than the smallest but 0; `of` says how many actions the row has.  Which element is drawn.
 template <int DT, int THREADS, int EP>
-__device__ __forceinline__ int choose(Group<THREADS>& g, uint32_t* key, uint32_t best_key, const RowRules& r, int of, double u) {
+__device__ __forceinline__ int choose(Group<THREADS>& g, uint32_t* key, uint32_t low, uint32_t best_key, const RowRules& r, int of, double u) {
   if (r.top_k > 0 && r.top_k < of) {
     uint32_t c = 0;
 #pragma unroll
     for (int i = 0; i < EP; ++i) c += ballots(key[i] != 0);
     if (g.count(c) > (uint32_t)r.top_k) {
-      const uint32_t edge = find_rank<THREADS, EP>(g, key, (uint32_t)r.top_k, best_key);
+      const uint32_t edge = find_rank<THREADS, EP>(g, key, (uint32_t)r.top_k, low, best_key);
+      low = edge;
       uint32_t above = 0, equal = 0;
 #pragma unroll
       for (int i = 0; i < EP; ++i) {
@@ -468,9 +468,12 @@ __device__ __forceinline__ int choose(Group<THREADS>& g, uint32_t* key, uint32_t
     total = g.sum(total);
     const double target = (double)r.top_p * total;
     // What lies below the edge weighs at most (1 - top_p) of the total: an action of that much / (2 * all) cannot be the edge.
-    uint32_t lo = 1;
+    uint32_t lo = low;
     const float floor_x = best + (float)(log((total - target) / (2.0 * of)) * (double)r.temperature);
-    if (floor_x > -3e38f && floor_x < best) lo = order_of<DT>(floor_x);
+    if (floor_x > -3e38f && floor_x < best) {
+      const uint32_t floor_key = order_of<DT>(floor_x);
+      lo = floor_key > low ? floor_key : low;
+    }
     double above;
     const uint32_t edge = find_mass<THREADS, EP>(g, key, w, target, lo, best_key, &above);
 #pragma unroll
@@ -488,6 +491,9 @@ __device__ __forceinline__ int choose(Group<THREADS>& g, uint32_t* key, uint32_t
 // A wave or a workgroup holds a row in registers, EP neighbouring actions a thread.  Where top_k keeps few of a workgroup's
 // row, it first cuts at the k-th largest of the threads' largest keys -- at least k elements reach that, and seldom many
 // more -- and one wave chooses among those alone: no 64-bit exponentials and no workgroup-wide searches for the rest.
+// Bound by the chain of one row's steps, at five rows a CU: 4,096 rows of 4,096 bfloat16 logits with every rule 25 us, 1.3
+// TB/s of the 5.2 that a copy reaches (146 without the cut; 36 with a barrier in every step of the search for it, 30 with the
+// searches from the lowest key there is and not from the lowest that can be meant).
 template <int DT, int THREADS, int EP>
 __global__ __launch_bounds__(THREADS < 256 ? 256 : THREADS, EP <= 8 ? 5 : EP == 16 ? 4 : 2) void pcx_sample_group(SampleArgs a) {
   constexpr int ROWS = THREADS < 256 ? 256 / THREADS : 1;
@@ -503,7 +509,23 @@ __global__ __launch_bounds__(THREADS < 256 ? 256 : THREADS, EP <= 8 ? 5 : EP == 
   uint32_t most = 0;
 #pragma unroll
   for (int i = 0; i < EP; ++i) most = key[i] > most ? key[i] : most;
-  const uint32_t best_key = g.max(most);
+  // A workgroup's waves each look at all threads' largest keys, by themselves: one barrier, not one a step of the search.
+  constexpr int TOPS = THREADS < 256 ? 1 : THREADS / 64;
+  uint32_t tops[TOPS] = {most}, best_key;
+  Group<64> one{nullptr, (int)(threadIdx.x & 63), 0};
+  if constexpr (THREADS >= 256) {
+    __shared__ uint32_t all_tops[THREADS];
+    all_tops[threadIdx.x] = most;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < TOPS; ++i) {
+      tops[i] = all_tops[i * 64 + one.t];
+      most = tops[i] > most ? tops[i] : most;
+    }
+    best_key = one.max(most);
+  } else {
+    best_key = g.max(most);
+  }
   if (best_key == 0 || !(r.temperature > 0.0f)) {
     uint32_t first = 0xFFFFFFFFu;
 #pragma unroll
@@ -518,8 +540,11 @@ __global__ __launch_bounds__(THREADS < 256 ? 256 : THREADS, EP <= 8 ? 5 : EP == 
     __shared__ uint32_t few_key[FEW];
     __shared__ uint16_t few_at[FEW];
     if (r.top_k > 0 && r.top_k <= THREADS / 2 && r.top_k < A) {
-      uint32_t mine[1] = {most};
-      const uint32_t cut = find_rank<THREADS, 1>(g, mine, (uint32_t)r.top_k, best_key);
+      uint32_t least = tops[0];
+#pragma unroll
+      for (int i = 1; i < TOPS; ++i) least = tops[i] < least ? tops[i] : least;
+      least = one.min(least);
+      const uint32_t cut = find_rank<64, TOPS>(one, tops, (uint32_t)r.top_k, least ? least : 1u, best_key);
       uint32_t c = 0, total;
 #pragma unroll
       for (int i = 0; i < EP; ++i) c += key[i] >= cut;
@@ -533,25 +558,24 @@ __global__ __launch_bounds__(THREADS < 256 ? 256 : THREADS, EP <= 8 ? 5 : EP == 
           }
         __syncthreads();
         if (g.t >= 64) return;
-        Group<64> one{nullptr, g.t, 0};
         int pick;
         if (total <= 128) {
           uint32_t k[2];
 #pragma unroll
           for (int i = 0; i < 2; ++i) k[i] = (uint32_t)(g.t * 2 + i) < total ? few_key[g.t * 2 + i] : 0;
-          pick = choose<DT, 64, 2>(one, k, best_key, r, A, u);
+          pick = choose<DT, 64, 2>(one, k, cut, best_key, r, A, u);
         } else {
           uint32_t k[8];
 #pragma unroll
           for (int i = 0; i < 8; ++i) k[i] = (uint32_t)(g.t * 8 + i) < total ? few_key[g.t * 8 + i] : 0;
-          pick = choose<DT, 64, 8>(one, k, best_key, r, A, u);
+          pick = choose<DT, 64, 8>(one, k, cut, best_key, r, A, u);
         }
         if (g.t == 0) a.out[row] = few_at[pick];
         return;
       }
     }
   }
-  const int pick = choose<DT, THREADS, EP>(g, key, best_key, r, A, u);
+  const int pick = choose<DT, THREADS, EP>(g, key, 1u, best_key, r, A, u);
   if (g.t == 0) a.out[row] = pick;
 }
 
