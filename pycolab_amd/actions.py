@@ -127,13 +127,12 @@ def _taken(torch, actions, n, device):
 
 def _log_prob_forward(torch, desc, legal, logits, actions, temperature):
   n, device = logits.shape[0], logits.device
-  both = torch.empty((2, n), dtype=torch.float32, device=device)
-  log_prob, entropy = both.unbind(0)
+  log_prob = torch.empty((n,), dtype=torch.float32, device=device)
+  entropy = torch.empty((n,), dtype=torch.float32, device=device)
   stats = torch.empty((n, 2), dtype=torch.float32, device=device)
   scratch, size = dev.workspace('pcx_log_prob_size', desc, device)
-  start = both.data_ptr()
-  dev.launch(device.index, N.lib().pcx_log_prob, desc, temperature, logits.data_ptr(), dev.pointer(legal), actions.data_ptr(), start,
-             start + 4 * n, stats.data_ptr(), dev.pointer(scratch), size)
+  dev.launch(device.index, N.lib().pcx_log_prob, desc, temperature, logits.data_ptr(), dev.pointer(legal), actions.data_ptr(),
+             log_prob.data_ptr(), entropy.data_ptr(), stats.data_ptr(), dev.pointer(scratch), size)
   return log_prob, entropy, stats
 
 

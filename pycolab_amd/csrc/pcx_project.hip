@@ -70,7 +70,7 @@ template <int DT> constexpr float SCALE = DT == PCX_F16 ? 0.5f : 1.0f;
 template <int ACT>
 __device__ __forceinline__ void activate(float z, float* y, float* slope) {
   if constexpr (ACT == PCX_ACT_RELU) {
-    *y = z < 0.0f ? 0.0f : z; *slope = z > 0.0f ? 1.0f : 0.0f;  // (a NaN stays one)
+    *y = z < 0.0f ? 0.0f : z; *slope = z <= 0.0f ? 0.0f : 1.0f;  // (a NaN stays one)
   } else if constexpr (ACT == PCX_ACT_SILU) {
     const float s = 1.0f / (1.0f + expf(-z));
     *y = z * s; *slope = s * (1.0f + z * (1.0f - s));

@@ -46,6 +46,8 @@ __global__ __launch_bounds__(256) void pcx_project_turn(BackwardArgs a) {
   const T* const sl = reinterpret_cast<const T*>(a.slope);
   const float* const sl32 = reinterpret_cast<const float*>(a.slope);
   const bool relu = s.activation == PCX_ACT_RELU;
+  // (relu lets a gradient through or not: an infinite one that it stops is no NaN)
+  auto passes = [](T g, T k) { return Num<DT>::get(k) != 0.0f ? Num<DT>::get(g) : 0.0f; };
   const int r = tid >> 2, c0 = (tid & 3) * 16;  // a thread reads 16 neighbouring hidden units of one board
   float total = 0.0f;
   for (int b = blockIdx.x; b < a.blocks; b += gridDim.x) {
@@ -63,7 +65,7 @@ __global__ __launch_bounds__(256) void pcx_project_turn(BackwardArgs a) {
         } else if (relu) {
           const Sixteen k = *reinterpret_cast<const Sixteen*>(sl + at);
 #pragma unroll
-          for (int i = 0; i < 16; ++i) v[i] = Num<DT>::get(q.v[i]) * Num<DT>::get(k.v[i]);
+          for (int i = 0; i < 16; ++i) v[i] = passes(q.v[i], k.v[i]);
         } else {
           struct __align__(16) Floats { float v[16]; } k = *reinterpret_cast<const Floats*>(sl32 + at);
 #pragma unroll
@@ -74,7 +76,8 @@ __global__ __launch_bounds__(256) void pcx_project_turn(BackwardArgs a) {
         for (int i = 0; i < 16; ++i)
           if (h0 + c0 + i < s.hidden) {
             v[i] = Num<DT>::get(dy[at + i]);
-            if (sl) v[i] *= relu ? Num<DT>::get(sl[at + i]) : sl32[at + i];
+            if (sl && relu) v[i] = passes(dy[at + i], sl[at + i]);
+            else if (sl) v[i] *= sl32[at + i];
           }
       }
     }

@@ -583,7 +583,7 @@ class ObservationCharacterRepainter(object):
         d.chars[i] = ord(ch)
       pitch = (view.rows * view.cols + 3) & ~3
       self._post = _Post(source, d, np.uint8, (int(view.batch), 1 + len(self._out_chars), pitch))
-      self._repainted = _RepaintedPlanes(self._post, self._out_chars, view.rows, view.cols, pitch, device_id)
+      self._repainted = _RepaintedPlanes(self._post, self._out_chars, view.rows, view.cols, pitch, device_id, _engine_of(source))
     B = self._post.out_shape[0]
     planes, bad = self._post.run(host=B == 1)
     if bad and self._post.errors().any():
@@ -611,8 +611,8 @@ class ObservationCharacterRepainter(object):
 class _RepaintedPlanes(object):
   """The planes a repainter wrote, as a source for further post-processors."""
 
-  def __init__(self, post, out_chars, rows, cols, pitch, device_id):
-    self._post, self._out_chars = post, out_chars
+  def __init__(self, post, out_chars, rows, cols, pitch, device_id, origin):
+    self._post, self._out_chars, self._origin = post, out_chars, origin
     self.rows, self.cols, self.pitch, self._device_id = rows, cols, pitch, device_id
 
   def _planes_view(self):
@@ -637,6 +637,11 @@ class _RepaintedPlanes(object):
 _ACTIVATIONS = {None: N.ACT_NONE, 'relu': N.ACT_RELU, 'silu': N.ACT_SILU, 'tanh': N.ACT_TANH, 'gelu': N.ACT_GELU}
 
 
+def _engine_of(source):
+  """The engine whose steps change what a source of planes (itself, a cropper, repainted planes) holds."""
+  return getattr(source, '_engine', None) or getattr(source, '_origin', None) or source
+
+
 def _occluded(source):
   """Are this source's layers exactly `board == character`?"""
   engine = getattr(source, '_engine', None) or source
@@ -651,6 +656,7 @@ class _Boards(object):
     torch = dev.require_torch('a projection of observations')
     self.single = False
     self.offsets = None  # stacked layers: byte offsets within a board
+    self.written = None  # an Observation's engine and how many steps it had launched
     if isinstance(boards, torch.Tensor):
       self.keep, shape = boards, boards.shape
       if not boards.is_cuda:
@@ -679,11 +685,21 @@ class _Boards(object):
         raise RuntimeError('The layers {} have no entry that refers to an actual feature in the input observation, whose '
                            'features are {}.'.format(repr(layers), repr(present.decode('latin-1'))))
       self.keep = boards
+      engine = _engine_of(source)
+      self.written = engine, engine._steps_launched
       self.n, self.rows, self.cols = int(view.batch), view.rows, view.cols
       self.ptr, self.row_stride = view.planes, (1 + view.n_chars) * view.pitch
       self.single = self.n == 1
       if not _occluded(source):
         self.offsets = [(1 + present.index(ord(c))) * view.pitch if ord(c) in present else -1 for c in layers]
+
+  def check_unchanged(self, what):
+    """In a backward pass: does an Observation still hold what the forward pass read?  (Of a tensor, autograd knows.)"""
+    if self.written is not None:
+      engine, steps = self.written
+      if engine._native is None or engine._steps_launched != steps:
+        raise RuntimeError('{}(): the Observation was overwritten by a later step, or its engine closed, before the backward '
+                           'pass: pass a copy of its board, a tensor'.format(what))
 
 
 _NO_OFFSETS = bytes(8 * N.POST_MAX_DEPTH)
@@ -883,6 +899,8 @@ def _project_autograd():
         dev.refuse_twice('project')
         slope, _ = ctx.saved_tensors
         want = ctx.needs_input_grad
+        if want[0]:
+          ctx.boards.check_unchanged('project')
         dw, db = ctx.plan.backward(ctx.desc, ctx.boards, grad, slope, want[0], want[1], ctx.weight_shape)
         return dw, db, grad if want[2] else None, None, None, None
 
@@ -895,8 +913,9 @@ def project(boards, layers, weight, bias=None, activation=None, residual=None, r
   first layer.  Arguments, shapes and types as for `ObservationProjection`, which is the form for weights that stay; this
   one lays the weight out in every call.
 
-  An Observation is a view of the engine's planes, which the next step overwrites: for a backward pass after that, pass a
-  copy of the board (`observation.board.clone()`), a tensor.
+  An Observation is a view of the engine's planes, which the next step overwrites: a backward pass after that is refused;
+  pass a copy of the board (`observation.board.clone()`), a tensor.  A weight that is no finite number makes the results of
+  the boards that use it no finite numbers, and of others some.
 
   `return_slope=True`: no autograd; returns (out, slope) with slope = act'(...) (None without an activation), what
   `project_backward` takes -- the pair to capture into a graph."""

@@ -558,3 +558,20 @@ def test_a_rollout_and_a_gradient_step():
     engines[0].step_sampled(logits[:5], numbers[0][:5])
   for e in engines:
     e.close()
+
+
+@pytest.mark.gpu
+def test_results_changed_in_place():
+  x = torch.randn(6, 5, device='cuda', requires_grad=True)
+  taken = torch.tensor([0, 1, 2, 3, 4, -1], dtype=torch.int32, device='cuda')
+  lp, h = policy.log_prob(x, taken)
+  lp.mul_(2.0)
+  (lp.sum() + h.sum()).backward()
+  y = x.detach().clone().requires_grad_()
+  lp, h = policy.log_prob(y, taken)
+  (2.0 * lp.sum() + h.sum()).backward()
+  assert torch.equal(x.grad, y.grad)
+  lp, h = policy.log_prob(y, taken)
+  h.add_(1.0)  # (the gradient needs it as it was)
+  with pytest.raises(RuntimeError, match='inplace'):
+    h.sum().backward()

@@ -511,3 +511,55 @@ def test_other_streams_and_graphs():
       rendering.project(b, chars, leaf, c)
   torch.cuda.synchronize()
   assert torch.equal(rendering.project_backward(boards.cuda(), chars, w, grad, slope)[0], dw) and db.shape == (96,)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('dtype', DTYPES)
+def test_relu_stops_infinite_gradients(dtype):
+  """Where relu is shut nothing comes through, whatever the gradient is; a sum that is no number is not shut."""
+  for n, hidden in ((65, 16), (64, 13)):
+    chars, boards, weight, bias, _ = make(n, 3, 5, 7, hidden, dtype, 21)
+    bias[0], bias[1] = -1e4, float('nan')
+    w, c = weight.cuda().requires_grad_(), bias.cuda().requires_grad_()
+    out = rendering.project(boards.cuda(), chars, w, c, activation='relu')
+    grad = torch.ones(n, hidden, dtype=w.dtype, device='cuda')
+    grad[:, 0] = float('inf')
+    out.backward(grad)
+    assert not out[:, 0].any() and out[:, 1].isnan().all()
+    assert not c.grad[0].any() and not w.grad[0].any()
+    assert float(c.grad[1]) == n  # (whole numbers: exact)
+
+
+@pytest.mark.gpu
+def test_backward_after_the_observation_is_gone_is_refused():
+  import os
+  from pycolab_amd import cropping
+  from pycolab_amd.compiler import GameTemplate
+  from pycolab_amd.engine import Engine
+  path = os.path.join(os.path.dirname(__file__), 'golden', 'templates', 'better_scrolly_maze_L0.npz')
+  eng = Engine.from_template(GameTemplate.load(path), batch=9, auto_reset=True)
+  obs, _, _ = eng.its_showtime()
+  cropper = cropping.ScrollingCropper(rows=10, cols=30, to_track=['P'], scroll_margins=(2, 3))
+  cropper.set_engine(eng)
+  repainter = rendering.ObservationCharacterRepainter({'a': '@', 'b': '@', 'c': '@'})
+  sources = lambda obs: (obs, cropper.crop(obs), repainter(obs), repainter(cropper.crop(obs)))
+  shapes = ((45, 89), (10, 30), (45, 89), (10, 30))
+  weights = [torch.randn(8, 2, r, c, device='cuda').requires_grad_() for r, c in shapes]
+  for w, s in zip(weights, sources(obs)):  # in time
+    rendering.project(s, 'P@', w).sum().backward()
+    assert w.grad.abs().sum() > 0
+  late = [rendering.project(s, 'P@', w) for w, s in zip(weights, sources(obs))]
+  kept = rendering.project(obs.board.clone(), 'P@', weights[0])
+  residual = torch.zeros(9, 8, device='cuda', requires_grad=True)
+  only_residual = rendering.project(obs, 'P@', weights[0].detach(), residual=residual)
+  eng.play(torch.zeros(9, dtype=torch.int32).cuda())
+  for out in late:
+    with pytest.raises(RuntimeError, match='overwritten by a later step'):
+      out.sum().backward()
+  kept.sum().backward()
+  only_residual.sum().backward()
+  assert (residual.grad == 1).all()
+  out = rendering.project(eng.play(torch.zeros(9, dtype=torch.int32).cuda())[0], 'P@', weights[0])
+  eng.close()
+  with pytest.raises(RuntimeError, match='engine closed'):
+    out.sum().backward()
