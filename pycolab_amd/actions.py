@@ -127,9 +127,8 @@ def _taken(torch, actions, n, device):
 
 def _log_prob_forward(torch, desc, legal, logits, actions, temperature):
   n, device = logits.shape[0], logits.device
-  log_prob = torch.empty((n,), dtype=torch.float32, device=device)
-  entropy = torch.empty((n,), dtype=torch.float32, device=device)
   stats = torch.empty((n, 2), dtype=torch.float32, device=device)
+  log_prob, entropy = stats.new_empty(n), stats.new_empty(n)
   scratch, size = dev.workspace('pcx_log_prob_size', desc, device)
   dev.launch(device.index, N.lib().pcx_log_prob, desc, temperature, logits.data_ptr(), dev.pointer(legal), actions.data_ptr(),
              log_prob.data_ptr(), entropy.data_ptr(), stats.data_ptr(), dev.pointer(scratch), size)
@@ -137,13 +136,13 @@ def _log_prob_forward(torch, desc, legal, logits, actions, temperature):
 
 
 def _log_prob_backward(torch, desc, legal, logits, actions, temperature, entropy, stats, grad_log_prob, grad_entropy):
-  n, device = logits.shape[0], logits.device
-  grad = torch.empty(logits.shape, dtype=logits.dtype, device=device)
-  for g, name in ((grad_log_prob, 'grad_log_prob'), (grad_entropy, 'grad_entropy')):
-    if g is not None and (g.dtype != torch.float32 or g.dim() != 1 or g.shape[0] != n or g.device != device):
-      raise ValueError('{} must be float32 [{}] on {}'.format(name, n, device))
-  grad_log_prob, grad_entropy = (None if g is None else g.contiguous() for g in (grad_log_prob, grad_entropy))
-  dev.launch(device.index, N.lib().pcx_log_prob_backward, desc, temperature, logits.data_ptr(), dev.pointer(legal), actions.data_ptr(),
+  # (autograd calls this on a thread of its own, where every line costs several times what it does elsewhere)
+  grad = torch.empty_like(logits) if logits.is_contiguous() else logits.new_empty(logits.shape)
+  if grad_log_prob is not None and not grad_log_prob.is_contiguous():
+    grad_log_prob = grad_log_prob.contiguous()
+  if grad_entropy is not None and not grad_entropy.is_contiguous():
+    grad_entropy = grad_entropy.contiguous()
+  dev.launch(logits.get_device(), N.lib().pcx_log_prob_backward, desc, temperature, logits.data_ptr(), dev.pointer(legal), actions.data_ptr(),
              entropy.data_ptr(), stats.data_ptr(), dev.pointer(grad_log_prob), dev.pointer(grad_entropy), grad.data_ptr())
   return grad
 
@@ -156,6 +155,7 @@ def _log_prob_autograd():
   global _log_prob_function
   if _log_prob_function is None:
     torch = dev.torch_module()
+    grad_enabled = torch.is_grad_enabled
 
     class LogProb(torch.autograd.Function):
 
@@ -169,7 +169,8 @@ def _log_prob_autograd():
 
       @staticmethod
       def backward(ctx, grad_log_prob, grad_entropy):
-        dev.refuse_twice('log_prob')
+        if grad_enabled():
+          dev.refuse_twice('log_prob')
         logits, actions, legal, entropy, stats = ctx.saved_tensors
         if grad_log_prob is None and grad_entropy is None:
           return None, None, None, None, None
@@ -218,4 +219,7 @@ def log_prob_backward(logits, actions, entropy, stats, grad_log_prob=None, grad_
   for t, shape, name in ((entropy, (n,), 'entropy'), (stats, (n, 2), 'stats')):
     if t.dtype != torch.float32 or tuple(t.shape) != shape or t.device != logits.device or not t.is_contiguous():
       raise ValueError('{} must be what log_prob(..., return_stats=True) returned'.format(name))
-  return _log_prob_backward(torch, desc, legal, logits, actions, temperature, entropy, stats, grad_log_prob, grad_entropy)
+  for g, name in ((grad_log_prob, 'grad_log_prob'), (grad_entropy, 'grad_entropy')):
+    if g is not None and (g.dtype != torch.float32 or tuple(g.shape) != (n,) or g.device != logits.device):
+      raise ValueError('{} must be float32 [{}] on {}'.format(name, n, logits.device))
+  return _log_prob_backward(torch, desc, legal, logits.detach(), actions, temperature, entropy, stats, grad_log_prob, grad_entropy)

@@ -131,19 +131,27 @@ def pointer(tensor):
 
 def launch(device_id, function, *args):
   """function(*args, stream) of the C ABI on `device_id`'s current stream."""
-  torch = torch_module()
-  if torch.cuda.current_device() != device_id:
+  if _raw_stream is None:
+    _find_stream()
+  if _one_gpu or _current_device() == device_id:
+    code = function(*args, _raw_stream(device_id))
+  else:
+    torch = torch_module()
     with torch.cuda.device(device_id):
       code = function(*args, torch.cuda.current_stream(device_id).cuda_stream)
-  else:
-    code = function(*args, _raw_stream(torch, device_id))
   if code:
     N.check(code)
 
 
-def _raw_stream(torch, device_id):
-  raw = getattr(torch._C, '_cuda_getCurrentRawStream', None)  # (the stream without the Python object around it)
-  return raw(device_id) if raw is not None else torch.cuda.current_stream(device_id).cuda_stream
+_raw_stream = _one_gpu = _current_device = None
+
+
+def _find_stream():
+  global _raw_stream, _one_gpu, _current_device
+  torch = torch_module()
+  _one_gpu, _current_device = torch.cuda.device_count() == 1, torch.cuda.current_device
+  # (the stream without the Python object around it)
+  _raw_stream = getattr(torch._C, '_cuda_getCurrentRawStream', None) or (lambda i: torch.cuda.current_stream(i).cuda_stream)
 
 
 _sizes = {}

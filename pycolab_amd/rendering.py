@@ -794,15 +794,13 @@ class _Projection(object):
     return out, slope
 
   def backward(self, desc, boards, grad, slope, want_weight, want_bias, weight_shape):
-    torch = dev.torch_module()
-    self.check_rows(grad, 'grad', boards.n)
-    self.check_rows(slope, 'slope', boards.n, self.slope_dtype())
-    make = torch.zeros if boards.n == 0 else torch.empty
-    dw = make(weight_shape, dtype=self.torch_dtype, device=self.device) if want_weight else None
-    db = make((self.hidden,), dtype=self.torch_dtype, device=self.device) if want_bias else None
+    # (autograd calls this on a thread of its own, where every line costs several times what it does elsewhere)
+    make = grad.new_zeros if boards.n == 0 else grad.new_empty
+    dw = make(weight_shape) if want_weight else None
+    db = make(self.hidden) if want_bias else None
     if boards.n and (want_weight or want_bias):
       size = self.sizes(desc)[2]
-      scratch = torch.empty(size, dtype=torch.uint8, device=self.device)
+      scratch = grad.new_empty(size, dtype=dev.torch_module().uint8)
       grad = grad.contiguous()
       slope = None if slope is None else slope.contiguous()
       dev.launch(self.device.index, N.lib().pcx_project_backward, desc, boards.ptr, grad.data_ptr(), dev.pointer(slope), dev.pointer(dw),
@@ -883,6 +881,7 @@ def _project_autograd():
   global _project_function
   if _project_function is None:
     torch = dev.torch_module()
+    grad_enabled = torch.is_grad_enabled
 
     class ProjectBoards(torch.autograd.Function):
 
@@ -896,7 +895,8 @@ def _project_autograd():
 
       @staticmethod
       def backward(ctx, grad):
-        dev.refuse_twice('project')
+        if grad_enabled():
+          dev.refuse_twice('project')
         slope, _ = ctx.saved_tensors
         want = ctx.needs_input_grad
         if want[0]:
@@ -941,4 +941,7 @@ def project_backward(boards, layers, weight, grad, slope=None):
   # (which activation it was is in the slopes: relu's have the weight's type, the others' are float32)
   plan = _Projection(layers, weight, None, None if slope is None else 'relu' if slope.dtype == weight.dtype else 'silu')
   view = _Boards(boards, layers)
-  return plan.backward(plan.at(view), view, grad.detach(), slope, True, True, weight.shape)
+  desc = plan.at(view)
+  plan.check_rows(grad, 'grad', view.n)
+  plan.check_rows(slope, 'slope', view.n, plan.slope_dtype())
+  return plan.backward(desc, view, grad.detach(), slope, True, True, weight.shape)
