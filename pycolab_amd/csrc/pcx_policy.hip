@@ -109,8 +109,8 @@ __device__ __forceinline__ void load_keys(const Rows& rows, int64_t row, int j, 
 // enough that n times it is exact (the reduction of Cody and Waite), the Taylor series
 // of exp(r), |r| <= ln(2) / 2, to r^13 / 13! (the next term is 4e-18), and n in the exponent.
 // Four at a time: a chain of twenty dependent instructions leaves the unit idle, four side by side do not (8 x 2^20
-// logits without rules: 41 -> 36 us, all launches included); and the coefficients are held in scalar registers, which the four share -- left to itself the
-// compiler copies each into vector registers for every element.
+// logits without rules: 41 -> 36 us, all launches included); and the coefficients are held in scalar registers, which the
+// four share -- left to itself the compiler copies each into vector registers for every element.
 __device__ __forceinline__ double scalar(double c) { asm("" : "+s"(c)); return c; }
 template <int N>
 __device__ __forceinline__ void exp64(double* d) {
@@ -295,7 +295,7 @@ __device__ __forceinline__ void key_weights(const uint32_t* key, float best, dou
   weights<N>(x, best, rate, w);
 }
 
-// A thread holds a whole row: few actions, many rows.
+// A thread holds a whole row: few actions, many rows (2^20 rows of 5 float32 logits and legal flags: 16 us, 2.1 TB/s).
 template <int DT, int CAP>
 __global__ __launch_bounds__(256) void pcx_sample_rows(SampleArgs a) {
   typedef typename Logit<DT>::T T;
@@ -580,6 +580,11 @@ __global__ __launch_bounds__(THREADS < 256 ? 256 : THREADS, EP <= 8 ? 5 : EP == 
 }
 
 // ---- rows that no workgroup holds: divided among workgroups, one launch per question ------------------------------------
+//
+// The best logit; the edges of top_k and of top_p, a digit of the order key at a time; what each slice keeps; the slice and
+// the action that the number falls to.  8 x 2^20 float32 logits with top_p take 101 us in ten launches, of which one pass
+// over them, the floor, is 6.5: four more passes read them again (from the 256 MB cache: 7 us each if that were all), and the
+// chain of launches alone is 70 us, the time of a single row.
 
 constexpr int SLICE = 8192;    // actions per workgroup
 constexpr int WEP = 32;        // ... per thread of 256, all of them in flight before the first is looked at
@@ -659,11 +664,13 @@ __global__ __launch_bounds__(256) void pcx_sample_best(WideArgs w) {
   at = g.min(at);
   if (threadIdx.x == 0 && top) atomicMax(reinterpret_cast<unsigned long long*>(&w.state[row].best), (unsigned long long)top << 32 | (uint32_t)~at);
 }
-// Counts and weights per value of one digit, of the keys that agree with the digits found so far.
+// Weights (and counts, where top_k asks for them) per value of one digit, of the keys that agree with the digits found so
+// far: one pass over the logits, bound by the first digit's exponentials and LDS atomics (8 x 2^20 float32: 22 us; the second
+// digit 14, the third 10).  A slice a workgroup: with half the workgroups, two slices each, 4 us more.
 template <int DT>
-__global__ __launch_bounds__(256) void pcx_sample_digit(WideArgs w, int level, uint32_t needs) {
+__global__ __launch_bounds__(256) void pcx_sample_digit(WideArgs w, int level, uint32_t needs, int counts) {
   __shared__ unsigned long long mass[BINS];
-  __shared__ uint32_t count[BINS];
+  __shared__ uint32_t count[BINS], piles[4][768];
   const int row = blockIdx.y, lo = blockIdx.x * SLICE;
   const RowState st = w.state[row];
   if (level > 0 && !(st.active & needs)) return;
@@ -676,30 +683,58 @@ __global__ __launch_bounds__(256) void pcx_sample_digit(WideArgs w, int level, u
   const double rate = 1.0 / (double)r.temperature;
   for (int i = threadIdx.x; i < BINS; i += 256) { mass[i] = 0; count[i] = 0; }
   __syncthreads();
+  auto add = [&](const uint32_t* four) {
+    double v[4];
+    key_weights<DT, 4>(four, best, rate, v);
+#pragma unroll
+    for (int c = 0; c < 4; ++c)
+      if (four[c]) {
+        const uint32_t d = digit_of<DT>(four[c], level);
+        if (counts) atomicAdd(&count[d], 1u);
+        atomicAdd(&mass[d], (unsigned long long)(ldexp(v[c], w.scale) + 0.5));
+      }
+  };
+  if (level == 0) {
 #pragma unroll 1
-  for (int i = 0; i < WEP; i += 4) {
-    bool mine[4];
+    for (int i = 0; i < WEP; i += 4) {
+      add(key);
 #pragma unroll
-    for (int c = 0; c < 4; ++c) mine[c] = key[c] && same_prefix<DT>(key[c], st.prefix, level);
-    if (__ballot(mine[0] || mine[1] || mine[2] || mine[3])) {  // (later digits concern few)
-      double v[4];
-      key_weights<DT, 4>(key, best, rate, v);
-#pragma unroll
-      for (int c = 0; c < 4; ++c)
-        if (mine[c]) {
-          const uint32_t d = digit_of<DT>(key[c], level);
-          atomicAdd(&count[d], 1u);
-          atomicAdd(&mass[d], (unsigned long long)(ldexp(v[c], w.scale) + 0.5));
-        }
+      for (int c = 0; c < WEP - 4; ++c) key[c] = key[c + 4];
     }
+  } else {
+    // Later digits concern some of the keys: a wave piles those up and weighs them four a lane (weighed where they lie, with
+    // most lanes idle, the second digit of 8 x 2^20 float32 logits took 20 us, this way 14).
+    uint32_t* const pile = piles[threadIdx.x >> 6];
+    const uint32_t lane = threadIdx.x & 63;
+    uint32_t high = 0, four[4];
+#pragma unroll 1
+    for (int i = 0; i < WEP; i += 8) {
 #pragma unroll
-    for (int c = 0; c < WEP - 4; ++c) key[c] = key[c + 4];
+      for (int c = 0; c < 8; ++c) {
+        const bool mine = key[c] && same_prefix<DT>(key[c], st.prefix, level);
+        const uint64_t who = __ballot(mine);
+        if (mine) pile[high + __popcll(who & ((1ull << lane) - 1))] = key[c];
+        high += (uint32_t)__popcll(who);
+      }
+#pragma unroll
+      for (int c = 0; c < WEP - 8; ++c) key[c] = key[c + 8];
+      const bool end = i + 8 == WEP;
+      while (high >= 256 || (end && high)) {
+        const uint32_t from = high >= 256 ? high - 256 : 0;
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll
+        for (int c = 0; c < 4; ++c) four[c] = from + c * 64 + lane < high ? pile[from + c * 64 + lane] : 0u;
+        __builtin_amdgcn_wave_barrier();
+        high = from;
+        add(four);
+      }
+    }
   }
   __syncthreads();
   const int64_t at = ((int64_t)(level != 0) * w.batch + row) * BINS;
   for (int i = threadIdx.x; i < BINS; i += 256)
-    if (count[i]) {
-      atomicAdd(&w.count[at + i], count[i]);
+    if (count[i] || mass[i]) {
+      if (counts) atomicAdd(&w.count[at + i], count[i]);
       if (mass[i]) atomicAdd(reinterpret_cast<unsigned long long*>(&w.mass[at + i]), mass[i]);
     }
 }
@@ -749,7 +784,7 @@ __global__ __launch_bounds__(256) void pcx_sample_edge(WideArgs w, int level, in
     int bin_at = -1;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      if (!counts[i] || found != 0xFFFFFFFFu) continue;
+      if (!(by_mass ? masses[i] : counts[i]) || found != 0xFFFFFFFFu) continue;
       c_at = c_run;
       m_at = m_run;
       bin_at = BINS - 1 - ((int)threadIdx.x * 8 + i);
@@ -1160,10 +1195,10 @@ int sample_wide(const SampleArgs& a, void* workspace, hipStream_t st) {
     const bool k = a.rules.top_k_row || (a.rules.top_k > 0 && a.rules.top_k < a.rows.actions);
     const bool p_ = a.rules.top_p_row || a.rules.top_p < 1.0f;
     if (k || p_) {
-      hipLaunchKernelGGL((pcx_sample_digit<DT>), grid, block, 0, st, w, 0, 0u);
+      hipLaunchKernelGGL((pcx_sample_digit<DT>), grid, block, 0, st, w, 0, 0u, k);
       for (int by_mass = k ? 0 : 1; by_mass <= (p_ ? 1 : 0); ++by_mass)
         for (int level = 0; level < LEVELS<DT>; ++level) {
-          if (level) hipLaunchKernelGGL((pcx_sample_digit<DT>), grid, block, 0, st, w, level, by_mass ? 4u : 2u);
+          if (level) hipLaunchKernelGGL((pcx_sample_digit<DT>), grid, block, 0, st, w, level, by_mass ? 4u : 2u, !by_mass);
           hipLaunchKernelGGL((pcx_sample_edge<DT>), rows, block, 0, st, w, level, by_mass);
         }
     }
