@@ -1001,8 +1001,9 @@ template <int DT, int THREADS>
 __global__ __launch_bounds__(256) void pcx_log_prob_forward(LogProbArgs a) {
   typedef typename Logit<DT>::T T;
   constexpr int ROWS = 256 / THREADS, EP = THREADS == 64 ? 8 : 16;
-  __shared__ float shared[4][3];
+  __shared__ typename Group<THREADS>::Scratch scratch[ROWS];
   const int t = threadIdx.x % THREADS;
+  Group<THREADS> g{&scratch[threadIdx.x / THREADS], t, 0};
   const int64_t unit = (int64_t)blockIdx.x * ROWS + threadIdx.x / THREADS;
   if (unit >= a.rows.n * a.slices) return;
   const int64_t row = unit / a.slices;
@@ -1023,16 +1024,13 @@ __global__ __launch_bounds__(256) void pcx_log_prob_forward(LogProbArgs a) {
     soft_sums<EP>(x, big, a.rate, &s, &tt);
     v.join(big, s, tt, a.rate);
   }
-#pragma unroll
-  for (int k = 32; k >= 1; k >>= 1) {
-    const float m2 = __shfl_xor(v.m, k), s2 = __shfl_xor(v.s, k), t2 = __shfl_xor(v.t, k);
-    v.join(m2, s2, t2, a.rate);
-  }
-  if constexpr (THREADS > 64) {
-    if ((t & 63) == 0) { shared[t >> 6][0] = v.m; shared[t >> 6][1] = v.s; shared[t >> 6][2] = v.t; }
-    __syncthreads();
-    v = Soft{shared[0][0], shared[0][1], shared[0][2]};
-    for (int i = 1; i < THREADS / 64; ++i) v.join(shared[i][0], shared[i][1], shared[i][2], a.rate);
+  // the threads' parts relative to the row's largest logit, then plain sums
+  const uint32_t top = g.max(v.m > -INFINITY ? order_of<PCX_F32>(v.m) : 0u);
+  if (top) {
+    const float big = value_of<PCX_F32>(top), d = v.m == big ? 0.0f : (v.m - big) * a.rate, e = v.m > -INFINITY ? exp_of(d) : 0.0f;
+    v.t = g.sum(e > 0.0f ? e * fmaf(d, v.s, v.t) : 0.0f);
+    v.s = g.sum(e > 0.0f ? e * v.s : 0.0f);
+    v.m = big;
   }
   if (t != 0) return;
   if (a.slices > 1) a.partial[unit] = make_float4(v.m, v.s, v.t, 0.0f);
