@@ -99,12 +99,13 @@ __device__ __forceinline__ void copy_in(const uint8_t* from, uint8_t* lds) {
 template <int NEWER>
 __device__ __forceinline__ void stage_barrier() { asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(NEWER) : "memory"); }
 
-// Bytes c .. c + 3 of a board of fewer than 32 cells; zeros past its end, which is never read.
+// Bytes c .. c + 3 of a board of fewer than 32 cells; zeros past its end, which is never read (the last byte is, again: four
+// loads without branches, none of which waits for another).
 __device__ __forceinline__ uint32_t edge_dword(const uint8_t* row, int c, int cells) {
   uint32_t v = 0;
   for (int i = 0; i < 4; ++i)
-    if (c + i < cells) v |= (uint32_t)row[c + i] << (8 * i);
-  return v;
+    v |= (uint32_t)row[c + i < cells ? c + i : cells - 1] << (8 * i);
+  return c + 4 <= cells ? v : c < cells ? v & ((1u << (8 * (cells - c))) - 1u) : 0u;
 }
 
 }  // namespace project

@@ -538,23 +538,38 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void pcx_project_forward_kernel(Fo
 template <int DT>
 __global__ __launch_bounds__(256) void pcx_project_join(ForwardArgs a) {
   typedef typename Num<DT>::T T;
-  const int quads = (a.s.hidden + 3) / 4;
-  const int64_t total = a.s.n * quads, plane = a.s.n * a.s.hidden;
+  const int64_t plane = a.s.n * a.s.hidden;
+  if (!a.wide) {  // rows that do not keep four sums aligned: one a lane (four guarded ones: 31 us for 101 boards x
+                  // 19 units, this way 4)
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < plane; i += (int64_t)gridDim.x * 256) {
+      Four<T> bias = {}, res = {};
+      if (a.bias) bias.v[0] = reinterpret_cast<const T*>(a.bias)[i % a.s.hidden];
+      if (a.residual) res.v[0] = reinterpret_cast<const T*>(a.residual)[i];
+      float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+      const float* from = a.partial + i;
+#pragma unroll 8
+      for (int k = 0; k < a.splits; ++k, from += plane) sum[0] += *from;
+      by_activation(a.s.activation, [&](auto act) { finish<DT, decltype(act)::value>(a, i, sum, bias, res, 1); });
+    }
+    return;
+  }
+  const int quads = a.s.hidden / 4;
+  const int64_t total = a.s.n * quads;
   for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
     const int64_t row = i / quads;
-    const int col = (int)(i - row * quads) * 4, count = a.s.hidden - col < 4 ? a.s.hidden - col : 4;
+    const int col = (int)(i - row * quads) * 4;
     const float* from = a.partial + row * a.s.hidden + col;
     Four<T> bias = {}, res = {};
-    if (a.bias) bias = load_four(reinterpret_cast<const T*>(a.bias) + col, count, false);
-    if (a.residual) res = load_four(reinterpret_cast<const T*>(a.residual) + row * a.s.hidden + col, count, a.wide);
+    if (a.bias) bias = load_four(reinterpret_cast<const T*>(a.bias) + col, 4, false);
+    if (a.residual) res = load_four(reinterpret_cast<const T*>(a.residual) + row * a.s.hidden + col, 4, true);
     float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll 8
     for (int k = 0; k < a.splits; ++k, from += plane) {
-      const Four<float> v = load_four(from, count, a.wide);
+      const Four<float> v = load_four(from, 4, true);
 #pragma unroll
       for (int c = 0; c < 4; ++c) sum[c] += v.v[c];
     }
-    by_activation(a.s.activation, [&](auto act) { finish<DT, decltype(act)::value>(a, row * a.s.hidden + col, sum, bias, res, count); });
+    by_activation(a.s.activation, [&](auto act) { finish<DT, decltype(act)::value>(a, row * a.s.hidden + col, sum, bias, res, 4); });
   }
 }
 
@@ -624,7 +639,7 @@ int forward_type(const ForwardArgs& a, const ForwardPlan& p, unsigned grid, hipS
   else rc = forward_shape<DT, 4>(a, p, grid, st);
   if (rc) return rc;
   if (p.splits > 1) {
-    const int64_t wgs = (a.s.n * ((a.s.hidden + 3) / 4) + 255) / 256;
+    const int64_t wgs = (a.s.n * (a.wide ? a.s.hidden / 4 : a.s.hidden) + 255) / 256;
     hipLaunchKernelGGL((pcx_project_join<DT>), dim3((unsigned)(wgs < 2048 ? wgs : 2048)), dim3(256), 0, st, a);
   }
   return 0;

@@ -288,8 +288,8 @@ __global__ __launch_bounds__(256, 2) void pcx_project_weight_grad(BackwardArgs a
         const int64_t at = ((int64_t)unit * s.layers + layer) * s.cells + c;
         const float v = SCALE<F16> * acc[l][h][i];
         if (a.splits > 1) a.partial[(int64_t)split * s.hidden * s.layers * s.cells + at] = v;
-        else if (s.dtype == PCX_F32) reinterpret_cast<float*>(a.grad_weight)[at] = v;  // (whole: nothing to join)
-        else if (s.dtype == PCX_F16) reinterpret_cast<_Float16*>(a.grad_weight)[at] = Num<PCX_F16>::put(v);
+        else if (PARTS == 3) reinterpret_cast<float*>(a.grad_weight)[at] = v;  // (whole: nothing to join)
+        else if (F16 || (PARTS == 2 && s.dtype == PCX_F16)) reinterpret_cast<_Float16*>(a.grad_weight)[at] = Num<PCX_F16>::put(v);
         else reinterpret_cast<__bf16*>(a.grad_weight)[at] = Num<PCX_BF16>::put(v);
       }
   }
