@@ -579,6 +579,129 @@ __global__ __launch_bounds__(THREADS < 256 ? 256 : THREADS, EP <= 8 ? 5 : EP == 
   if (g.t == 0) a.out[row] = pick;
 }
 
+// ---- rows that no workgroup holds, of which top_k keeps few (or the temperature only the best) --------------------------
+//
+// A workgroup reads its row twice: once for every thread's largest key, whose k-th largest is the cut, once for the elements
+// that reach it, which go to one wave as in pcx_sample_group.  Where more than FEW do -- many equal logits -- the k-th largest
+// key of the row is searched for with a pass a step, and exactly the k elements that the rule keeps are taken.
+// Bound by the passes' loads, 16 neighbouring logits a thread in flight (32: 26 -> 30 us): 269 rows of 33,380 float16 logits with
+// top_k 40 and top_p take 26 us where the divided rows' launches below take 136, one row of 131,072 float32 ones 44 (62), of
+// 262,144 82 (63), 64 rows of those 95 (149).
+constexpr int TOP_THREADS = 512, TOP_EP = 16;
+template <int DT>
+__global__ __launch_bounds__(TOP_THREADS, 4) void pcx_sample_top(SampleArgs a) {
+  constexpr int FEW = 512, WAVES = TOP_THREADS / 64, TURN = TOP_THREADS * TOP_EP;
+  __shared__ Group<TOP_THREADS>::Scratch scratch;
+  __shared__ uint32_t all_tops[TOP_THREADS], few_key[FEW], few_at[FEW], sorted_key[FEW], sorted_at[FEW], found;
+  Group<TOP_THREADS> g{&scratch, (int)threadIdx.x, 0};
+  Group<64> one{nullptr, (int)(threadIdx.x & 63), 0};
+  const int64_t row = blockIdx.x;
+  const RowRules r = rules_of(a.rules, row);
+  const int A = a.rows.actions;
+  uint32_t key[TOP_EP];
+  // key[] of every turn of neighbouring elements, in index order
+  auto each = [&](auto f) {
+#pragma unroll 1
+    for (int64_t lo = 0; lo < A; lo += TURN) {
+      const int j = (int)lo + g.t * TOP_EP;  // (A is at most 2^24)
+      load_keys<DT, TOP_EP>(a.rows, row, j, A, key);
+      f(j);
+    }
+  };
+  uint32_t most = 0, first = 0;
+  each([&](int j) {
+#pragma unroll
+    for (int i = 0; i < TOP_EP; ++i)
+      if (key[i] > most) { most = key[i]; first = (uint32_t)(j + i); }
+  });
+  all_tops[g.t] = most;
+  if (g.t == 0) found = 0;
+  __syncthreads();
+  uint32_t tops[WAVES], best_key = 0, least = 0xFFFFFFFFu;
+#pragma unroll
+  for (int i = 0; i < WAVES; ++i) {
+    tops[i] = all_tops[i * 64 + one.t];
+    best_key = tops[i] > best_key ? tops[i] : best_key;
+    least = tops[i] < least ? tops[i] : least;
+  }
+  best_key = one.max(best_key);
+  if (best_key == 0 || !(r.temperature > 0.0f)) {
+    first = g.min(most == best_key ? first : 0xFFFFFFFFu);
+    if (g.t == 0) a.out[row] = best_key ? (int)first : NONE;
+    return;
+  }
+  least = one.min(least);
+  const uint32_t k = (uint32_t)r.top_k;
+  uint32_t cut = find_rank<64, WAVES>(one, tops, k, least ? least : 1u, best_key);
+  auto take = [&](bool yes, uint32_t what, uint32_t where) {
+    if (!yes) return;
+    const uint32_t at = atomicAdd(&found, 1u);
+    if (at < FEW) { few_key[at] = what; few_at[at] = where; }
+  };
+  each([&](int j) {
+#pragma unroll
+    for (int i = 0; i < TOP_EP; ++i) take(key[i] >= cut, key[i], (uint32_t)(j + i));
+  });
+  __syncthreads();
+  uint32_t total = found;
+  if (total > FEW) {
+    uint32_t lo = cut, hi = best_key;
+    while (lo < hi) {
+      const uint32_t mid = hi - (hi - lo) / 2;
+      uint32_t c = 0;
+      each([&](int) {
+#pragma unroll
+        for (int i = 0; i < TOP_EP; ++i) c += ballots(key[i] >= mid);
+      });
+      if (g.count(c) >= k) lo = mid; else hi = mid - 1;
+    }
+    uint32_t above = 0;
+    each([&](int) {
+#pragma unroll
+      for (int i = 0; i < TOP_EP; ++i) above += ballots(key[i] > lo);
+    });
+    uint32_t ties = k - g.count(above);  // how many of the row's elements with that very key are still kept, the first ones
+    if (g.t == 0) found = 0;
+    __syncthreads();
+    each([&](int j) {
+      uint32_t equal = 0, all;
+#pragma unroll
+      for (int i = 0; i < TOP_EP; ++i) equal += key[i] == lo;
+      uint32_t before = g.scan(equal, &all);
+#pragma unroll
+      for (int i = 0; i < TOP_EP; ++i) take(key[i] > lo || (key[i] == lo && before++ < ties), key[i], (uint32_t)(j + i));
+      ties = all < ties ? ties - all : 0u;
+    });
+    cut = lo;
+    __syncthreads();
+    total = found;
+  }
+  // in index order: an element's place is how many have a lower index
+  if ((uint32_t)g.t < total) {
+    const uint32_t at = few_at[g.t];
+    uint32_t place = 0;
+    for (uint32_t i = 0; i < total; ++i) place += few_at[i] < at;
+    sorted_key[place] = few_key[g.t];
+    sorted_at[place] = at;
+  }
+  __syncthreads();
+  if (g.t >= 64) return;
+  const double u = (double)a.uniforms[row];
+  int pick;
+  if (total <= 128) {
+    uint32_t some[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) some[i] = (uint32_t)(g.t * 2 + i) < total ? sorted_key[g.t * 2 + i] : 0;
+    pick = choose<DT, 64, 2>(one, some, cut, best_key, r, A, u);
+  } else {
+    uint32_t some[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) some[i] = (uint32_t)(g.t * 8 + i) < total ? sorted_key[g.t * 8 + i] : 0;
+    pick = choose<DT, 64, 8>(one, some, cut, best_key, r, A, u);
+  }
+  if (g.t == 0) a.out[row] = (int)sorted_at[pick];
+}
+
 // ---- rows that no workgroup holds: divided among workgroups, one launch per question ------------------------------------
 //
 // The best logit; the edges of top_k and of top_p, a digit of the order key at a time; what each slice keeps; the slice and
@@ -1142,6 +1265,7 @@ __global__ __launch_bounds__(256) void pcx_log_prob_rows_backward(LogProbArgs a)
 // ---------------------------------------------------------------- plans and entry points
 
 constexpr int ROW_IN_GROUP = 16384;  // actions a workgroup holds in registers
+constexpr int TOP_ALONE = 1 << 17, TOP_ROWS = 64;  // pcx_sample_top takes so many actions in any number of rows, or so many rows of any
 constexpr int WIDE_BATCH = 1024;     // rows per batch of launches beyond that
 constexpr int64_t CHUNK = 1 << 22;   // rows per launch otherwise (a grid has fewer than 2^32 threads)
 
@@ -1213,7 +1337,10 @@ int sample_wide(const SampleArgs& a, void* workspace, hipStream_t st) {
 template <int DT>
 int sample_type(const SampleArgs& all, void* workspace, hipStream_t st) {
   const int A = all.rows.actions;
-  if (A > ROW_IN_GROUP) return sample_wide<DT>(all, workspace, st);
+  // Few rows of very many actions are divided among workgroups even where one could choose by itself (pcx_sample_top's figures).
+  const bool few = (!all.rules.top_k_row && all.rules.top_k > 0 && all.rules.top_k <= TOP_THREADS / 2) || (!all.rules.temperature_row && all.rules.temperature == 0.0f);
+  const bool top = A > ROW_IN_GROUP && few && (A <= TOP_ALONE || all.rows.n >= TOP_ROWS);
+  if (A > ROW_IN_GROUP && !top) return sample_wide<DT>(all, workspace, st);
   for (int64_t row0 = 0; row0 < all.rows.n; row0 += CHUNK) {
     SampleArgs a = all;
     a.rows = rows_from(all.rows, row0, elem_size(DT));
@@ -1224,7 +1351,8 @@ int sample_type(const SampleArgs& all, void* workspace, hipStream_t st) {
     if (a.rules.top_p_row) a.rules.top_p_row += row0;
     if (a.rules.min_p_row) a.rules.min_p_row += row0;
     const dim3 block(256), per_thread((unsigned)((a.rows.n + 255) / 256)), per_wave((unsigned)((a.rows.n + 3) / 4)), per_group((unsigned)a.rows.n);
-    if (A <= 8) hipLaunchKernelGGL((pcx_sample_rows<DT, 8>), per_thread, block, 0, st, a);
+    if (top) hipLaunchKernelGGL((pcx_sample_top<DT>), per_group, dim3(TOP_THREADS), 0, st, a);
+    else if (A <= 8) hipLaunchKernelGGL((pcx_sample_rows<DT, 8>), per_thread, block, 0, st, a);
     else if (A <= 16) hipLaunchKernelGGL((pcx_sample_rows<DT, 16>), per_thread, block, 0, st, a);
     else if (A <= 128) hipLaunchKernelGGL((pcx_sample_group<DT, 64, 2>), per_wave, block, 0, st, a);
     else if (A <= 256) hipLaunchKernelGGL((pcx_sample_group<DT, 64, 4>), per_wave, block, 0, st, a);

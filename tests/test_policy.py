@@ -575,3 +575,32 @@ def test_results_changed_in_place():
   h.add_(1.0)  # (the gradient needs it as it was)
   with pytest.raises(RuntimeError, match='inplace'):
     h.sum().backward()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('dtype', DTYPES)
+@pytest.mark.parametrize('n,a', [(9, 16385), (5, 40001), (3, 262144), (2, 262145), (130, 270000)])
+def test_sample_few_of_very_many(n, a, dtype):
+  """Rows that no workgroup holds with a small top_k, or the best alone: random ones, ones of few values, ones of one value,
+  masked ones, best ones at either end."""
+  x, u = logits_of(n, a, dtype, a)
+  g = torch.Generator().manual_seed(a)
+  x[0] = torch.randint(-2, 3, (a,), generator=g).to(x.dtype)
+  x[1] = 0.25
+  legal = torch.ones(n, a, dtype=torch.bool)
+  if n > 2:
+    legal[2] = False
+    legal[2, a - 1] = True
+  if n > 4:
+    x[3] = -math.inf
+    x[3, a - 3:] = 1.0
+    x[4, a - 1] = math.inf
+    legal[4, :a // 2] = torch.rand(a // 2, generator=g) < 0.001
+  rows = slice(0, min(n, 12))  # (the plain form sorts)
+  for kw in (dict(top_k=1), dict(top_k=40, top_p=0.9), dict(top_k=256, temperature=0.7, min_p=0.01), dict(temperature=0.0), dict(top_k=257), dict(temperature=0.0, top_k=3)):
+    got = policy.sample(x.cuda(), u.cuda(), legal=legal.cuda(), **kw).cpu()
+    want = policy.sample(x[rows].cuda(), u[rows].cuda(), legal=legal[rows].cuda(), **kw).cpu()
+    assert torch.equal(got[rows], want)  # (130 rows or 12 of them: another way there)
+    check_sample(x[rows], u[rows], legal=legal[rows], **kw)
+  per_row = torch.tensor([0.0, 0.5, 1.0, 2.0])[torch.arange(n) % 4]
+  check_sample(x[rows], u[rows], legal=legal[rows], top_k=50, top_p=0.8, temperature=per_row[rows])
