@@ -97,15 +97,22 @@ __device__ __forceinline__ void activate(float z, float* y, float* slope) {
 // the weight is read in runs of 32 cells (a direct gather took 52 us for 5.6 million float32 weights; this one 23).
 template <int DT>
 __global__ __launch_bounds__(256) void pcx_project_layout(Shape s, const typename Num<DT>::T* __restrict__ w, u32x4* __restrict__ packed) {
-  __shared__ float in[32][4][33];
+  __shared__ float in[32][4 * 33 + 1];  // (an odd pitch: 32 hidden units in 32 banks)
   const int q = blockIdx.x, g = blockIdx.y, tile = blockIdx.z;
   const int start = quad_start(q, s.cells), mine = q * QUAD - start;  // (cells before `mine` belong to the quad before)
-  for (int i = threadIdx.x; i < 32 * 4 * 32; i += 256) {
-    const int c = i & 31, pos = (i >> 5) & 3, h = tile * 32 + (i >> 7), cell = start + c;
+  {  // (what does not exist is read as its neighbour and dropped: 16 loads in flight, not one after the other)
+    const int c = threadIdx.x & 31, pos = (threadIdx.x >> 5) & 3, cell = start + c;
     const int layer = s.stacked ? (pos < 2 ? g * 2 + pos : s.layers) : g * 4 + pos;
-    float v = 0.0f;
-    if (c >= mine && cell < s.cells && layer < s.layers && h < s.hidden) v = Num<DT>::get(w[((int64_t)h * s.layers + layer) * s.cells + cell]);
-    in[i >> 7][pos][c] = v;
+    const bool real = c >= mine && cell < s.cells && layer < s.layers;
+    const typename Num<DT>::T* const from = w + (layer < s.layers ? layer : 0) * (int64_t)s.cells + (cell < s.cells ? cell : 0);
+    float v[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const int h = tile * 32 + i * 2 + (threadIdx.x >> 7);
+      v[i] = Num<DT>::get(from[(int64_t)(h < s.hidden ? h : s.hidden - 1) * s.layers * s.cells]);
+    }
+#pragma unroll
+    for (int i = 0; i < 16; ++i) in[i * 2 + (threadIdx.x >> 7)][pos * 33 + c] = real && tile * 32 + i * 2 + (int)(threadIdx.x >> 7) < s.hidden ? v[i] : 0.0f;
   }
   __syncthreads();
   const int per = s.stacked || s.groups < 4 ? s.groups : 4;  // groups per block
@@ -115,7 +122,7 @@ __global__ __launch_bounds__(256) void pcx_project_layout(Shape s, const typenam
     u32x4 out = {0, 0, 0, 0};
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      const float v = s.stacked ? in[lane & 31][e & 1][hb * 16 + j * 4 + (e >> 1)] : in[lane & 31][e & 3][e8 * 16 + j * 4 + hb * 2 + (e >> 2)];
+      const float v = s.stacked ? in[lane & 31][(e & 1) * 33 + hb * 16 + j * 4 + (e >> 1)] : in[lane & 31][(e & 3) * 33 + e8 * 16 + j * 4 + hb * 2 + (e >> 2)];
       uint32_t bits;
       if constexpr (DT == PCX_F16) bits = __builtin_bit_cast(uint16_t, (_Float16)v);
       else bits = part_of(0.5f * v, part, s.parts);
