@@ -69,7 +69,7 @@ __device__ __forceinline__ bool allowed(float x, bool legal) { return legal && x
 template <int DT, int N>
 __device__ __forceinline__ void load_logits(const typename Logit<DT>::T* x_row, const uint8_t* l_row, int j, int end, float* x) {
   typedef typename Logit<DT>::T T;
-  constexpr int W = N % (16 / (int)sizeof(T)) == 0 ? 16 / (int)sizeof(T) : N % 4 == 0 ? 4 : 1;  // elements per load
+  constexpr int W = N % (16 / (int)sizeof(T)) == 0 ? 16 / (int)sizeof(T) : N % 4 == 0 ? 4 : 2 - N % 2;  // elements per load
 #pragma unroll
   for (int i = 0; i < N; i += W) {
     Pack<T, W> q = {};
@@ -139,7 +139,7 @@ __device__ __forceinline__ void exp64(double* d) {
 // exp((x - best) * rate); 0 for -infinity, 1 where x is the best, infinite or not.
 template <int N>
 __device__ __forceinline__ void weights(const float* x, float best, double rate, double* w) {
-  constexpr int AT_ONCE = N % 4 == 0 ? 4 : N % 2 == 0 ? 2 : 1;
+  constexpr int AT_ONCE = N % 4 == 0 ? 4 : N % 3 == 0 ? 3 : N % 2 == 0 ? 2 : 1;
 #pragma unroll
   for (int i = 0; i < N; i += AT_ONCE) {
     double d[AT_ONCE];
@@ -295,7 +295,8 @@ __device__ __forceinline__ void key_weights(const uint32_t* key, float best, dou
   weights<N>(x, best, rate, w);
 }
 
-// A thread holds a whole row: few actions, many rows (2^20 rows of 5 float32 logits and legal flags: 16 us, 2.1 TB/s).
+// A thread holds a whole row: few actions, many rows.  Bound by the 64-bit exponentials of CAP actions, those that do not exist
+// too: 2^20 rows of 5 float32 logits and legal flags 13.5 us with CAP = 6, 2.5 TB/s, 15.4 with 8.
 template <int DT, int CAP>
 __global__ __launch_bounds__(256) void pcx_sample_rows(SampleArgs a) {
   typedef typename Logit<DT>::T T;
@@ -1352,6 +1353,7 @@ int sample_type(const SampleArgs& all, void* workspace, hipStream_t st) {
     if (a.rules.min_p_row) a.rules.min_p_row += row0;
     const dim3 block(256), per_thread((unsigned)((a.rows.n + 255) / 256)), per_wave((unsigned)((a.rows.n + 3) / 4)), per_group((unsigned)a.rows.n);
     if (top) hipLaunchKernelGGL((pcx_sample_top<DT>), per_group, dim3(TOP_THREADS), 0, st, a);
+    else if (A <= 6) hipLaunchKernelGGL((pcx_sample_rows<DT, 6>), per_thread, block, 0, st, a);
     else if (A <= 8) hipLaunchKernelGGL((pcx_sample_rows<DT, 8>), per_thread, block, 0, st, a);
     else if (A <= 16) hipLaunchKernelGGL((pcx_sample_rows<DT, 16>), per_thread, block, 0, st, a);
     else if (A <= 128) hipLaunchKernelGGL((pcx_sample_group<DT, 64, 2>), per_wave, block, 0, st, a);
