@@ -117,7 +117,10 @@ __global__ __launch_bounds__(256) void pcx_project_turn(BackwardArgs a) {
   if (!a.grad_bias) return;
   sums[tid >> 6][tid & 63] = total;
   __syncthreads();
-  if (tid < 64 && h0 + tid < s.hidden) a.bias_part[(int64_t)blockIdx.x * s.hidden + h0 + tid] = (sums[0][tid] + sums[1][tid]) + (sums[2][tid] + sums[3][tid]);
+  if (tid >= 64 || h0 + tid >= s.hidden) return;
+  const float sum = (sums[0][tid] + sums[1][tid]) + (sums[2][tid] + sums[3][tid]);
+  if (a.bias_blocks > 1) a.bias_part[(int64_t)blockIdx.x * s.hidden + h0 + tid] = sum;
+  else reinterpret_cast<T*>(a.grad_bias)[h0 + tid] = Num<DT>::put(sum);  // (whole: nothing to join)
 }
 
 // dw[h][l][c] over a run of boards: a workgroup owns NH tiles of hidden units x 32 cells x up to 2 LW layers (NH = 1: 4 LW).
@@ -390,7 +393,7 @@ int backward_parts(BackwardArgs& a, const BackwardPlan& p, hipStream_t st) {
     const int64_t wgs = ((int64_t)a.s.hidden * a.s.layers * a.s.cells + 1023) / 1024;
     if (a.splits > 1) weight_blocks = (int)(wgs < 4096 ? wgs : 4096);
   }
-  const int bias_blocks = a.grad_bias ? (a.s.hidden + 15) / 16 : 0;
+  const int bias_blocks = a.grad_bias && a.bias_blocks > 1 ? (a.s.hidden + 15) / 16 : 0;
   if (weight_blocks + bias_blocks)
     hipLaunchKernelGGL((pcx_project_grad_join<DT>), dim3((unsigned)(weight_blocks + bias_blocks)), dim3(256), 0, st, a, weight_blocks);
   return 0;

@@ -774,7 +774,8 @@ class _Projection(object):
     torch = dev.torch_module()
     if packed is None:
       packed = torch.empty(self.sizes(desc)[0], dtype=torch.uint8, device=self.device)
-    weight = weight.detach().contiguous()
+    if not weight.is_contiguous():
+      weight = weight.detach().contiguous()
     dev.launch(self.device.index, N.lib().pcx_project_pack, desc, weight.data_ptr(), packed.data_ptr())
     return packed
 
@@ -784,10 +785,10 @@ class _Projection(object):
       self.check_rows(residual, 'residual', boards.n)
       residual = residual.contiguous()
     out = torch.empty((boards.n, self.hidden), dtype=self.torch_dtype, device=self.device)
-    slope = torch.empty(out.shape, dtype=self.slope_dtype(), device=self.device) if want_slope else None
+    slope = torch.empty_like(out, dtype=self.slope_dtype()) if want_slope else None
     size = self.sizes(desc)[1]
-    scratch = torch.empty(size, dtype=torch.uint8, device=self.device) if size else None
-    if bias is not None:
+    scratch = packed.new_empty(size) if size else None
+    if bias is not None and not bias.is_contiguous():
       bias = bias.contiguous()
     dev.launch(self.device.index, N.lib().pcx_project_forward, desc, boards.ptr, packed.data_ptr(), dev.pointer(bias), dev.pointer(residual),
                out.data_ptr(), dev.pointer(slope), dev.pointer(scratch), size)
