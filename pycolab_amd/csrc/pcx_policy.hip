@@ -1266,7 +1266,7 @@ __global__ __launch_bounds__(256) void pcx_log_prob_rows_backward(LogProbArgs a)
 // ---------------------------------------------------------------- plans and entry points
 
 constexpr int ROW_IN_GROUP = 16384;  // actions a workgroup holds in registers
-constexpr int TOP_ALONE = 1 << 17, TOP_ROWS = 64;  // pcx_sample_top takes so many actions in any number of rows, or so many rows of any
+constexpr int ROW_ALONE = 1 << 18;   // ... one goes through alone where top_k keeps few (pcx_sample_top has both sides' times)
 constexpr int WIDE_BATCH = 1024;     // rows per batch of launches beyond that
 constexpr int64_t CHUNK = 1 << 22;   // rows per launch otherwise (a grid has fewer than 2^32 threads)
 
@@ -1338,9 +1338,9 @@ int sample_wide(const SampleArgs& a, void* workspace, hipStream_t st) {
 template <int DT>
 int sample_type(const SampleArgs& all, void* workspace, hipStream_t st) {
   const int A = all.rows.actions;
-  // Few rows of very many actions are divided among workgroups even where one could choose by itself (pcx_sample_top's figures).
+  // (By the actions alone, not by how many rows there are: a row's answer must not depend on its batch.)
   const bool few = (!all.rules.top_k_row && all.rules.top_k > 0 && all.rules.top_k <= TOP_THREADS / 2) || (!all.rules.temperature_row && all.rules.temperature == 0.0f);
-  const bool top = A > ROW_IN_GROUP && few && (A <= TOP_ALONE || all.rows.n >= TOP_ROWS);
+  const bool top = A > ROW_IN_GROUP && few && A <= ROW_ALONE;
   if (A > ROW_IN_GROUP && !top) return sample_wide<DT>(all, workspace, st);
   for (int64_t row0 = 0; row0 < all.rows.n; row0 += CHUNK) {
     SampleArgs a = all;
