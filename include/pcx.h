@@ -652,7 +652,8 @@ int pcx_project_pack(const pcx_project_desc* d, const void* weight, void* packed
 int pcx_project_forward(const pcx_project_desc* d, const uint8_t* boards, const void* packed, const void* bias,
                         const void* residual, void* out, void* slope, void* workspace, uint64_t workspace_bytes, void* stream);
 /* Gradients from grad_out [n][hidden]: grad_weight [hidden][n_layers][cells] and grad_bias [hidden] (either may be
- * NULL); the residual's gradient is grad_out itself.  slope may be NULL for PCX_ACT_NONE. */
+ * NULL); the residual's gradient is grad_out itself.  slope may be NULL for PCX_ACT_NONE; grad_out is multiplied by it, and with
+ * PCX_ACT_RELU nothing comes through where it is 0, not even an infinity. */
 int pcx_project_backward(const pcx_project_desc* d, const uint8_t* boards, const void* grad_out, const void* slope,
                          void* grad_weight, void* grad_bias, void* workspace, uint64_t workspace_bytes, void* stream);
 

@@ -46,8 +46,9 @@ __global__ __launch_bounds__(256) void pcx_project_turn(BackwardArgs a) {
   const T* const sl = reinterpret_cast<const T*>(a.slope);
   const float* const sl32 = reinterpret_cast<const float*>(a.slope);
   const bool relu = s.activation == PCX_ACT_RELU;
-  // (relu lets a gradient through or not: an infinite one that it stops is no NaN)
-  auto passes = [](T g, T k) { return Num<DT>::get(k) != 0.0f ? Num<DT>::get(g) : 0.0f; };
+  // (relu lets a gradient through or not: an infinite one that it stops is no NaN.  Its slopes are 0 and 1; any others, of a
+  // caller who does not say which activation it was, multiply.)
+  auto passes = [](T g, T k) { return Num<DT>::get(k) != 0.0f ? Num<DT>::get(g) * Num<DT>::get(k) : 0.0f; };
   const int r = tid >> 2, c0 = (tid & 3) * 16;  // a thread reads 16 neighbouring hidden units of one board
   float total = 0.0f;
   for (int b = blockIdx.x; b < a.blocks; b += gridDim.x) {

@@ -935,12 +935,21 @@ def project(boards, layers, weight, bias=None, activation=None, residual=None, r
   return (out, slope) if return_slope else out
 
 
-def project_backward(boards, layers, weight, grad, slope=None):
-  """(grad_weight, grad_bias) of `project()` for the gradient `grad` [n, hidden] of its result; `slope` as it returned it.
-  The residual's gradient is `grad`.  Records nothing for autograd and waits for nothing: it may be captured."""
+def project_backward(boards, layers, weight, grad, slope=None, activation=None):
+  """(grad_weight, grad_bias) of `project()` for the gradient `grad` [n, hidden] of its result; `slope` as it
+  returned it, `activation` as it was given.  The residual's gradient is `grad`.  Records nothing for autograd and waits for
+  nothing: it may be captured.
+
+  Without `activation`, the gradient is multiplied by the slopes, and where a slope is 0 nothing comes through; named, a
+  smooth activation's slope of 0 makes an infinite gradient a NaN, as its formula does."""
   dev.require_torch('project_backward()')
-  # (which activation it was is in the slopes: relu's have the weight's type, the others' are float32)
-  plan = _Projection(layers, weight, None, None if slope is None else 'relu' if slope.dtype == weight.dtype else 'silu')
+  if activation is None and slope is not None:
+    # (16-bit weights: relu's slopes have their type, the others' are float32.  float32 weights: relu's rule multiplies by
+    # any slope and lets nothing through at 0.)
+    activation = 'relu' if slope.dtype == weight.dtype else 'silu'
+  elif activation is not None and slope is None:
+    raise ValueError('project_backward() needs the slopes of {}'.format(activation))
+  plan = _Projection(layers, weight, None, activation)
   view = _Boards(boards, layers)
   desc = plan.at(view)
   plan.check_rows(grad, 'grad', view.n)

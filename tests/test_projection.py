@@ -563,3 +563,25 @@ def test_backward_after_the_observation_is_gone_is_refused():
   eng.close()
   with pytest.raises(RuntimeError, match='engine closed'):
     out.sum().backward()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('dtype', DTYPES)
+@pytest.mark.parametrize('act', ACTS)
+def test_the_explicit_pair(act, dtype):
+  """project(return_slope=True) and project_backward(): the formula's gradients and autograd's own, whether or not the
+  activation is named again."""
+  for stacked in (False, True):
+    chars, boards, weight, bias, residual = make(130, 5, 5, 7, 40, dtype, 30, stacked, grid=act == 'relu')
+    y, tol, slope64, slope_tol = reference(chars, boards, weight, bias, act, residual)
+    b, w, c, r = (t.cuda() for t in (boards, weight, bias, residual))
+    grad = torch.randn(130, 40, generator=torch.Generator().manual_seed(31)).to(weight.dtype)
+    out, slope = rendering.project(b, chars, w, c, activation=act, residual=r, return_slope=True)
+    near(out, y, tol, 'forward')
+    assert (slope is None) == (act is None)
+    leaves = [w.clone().requires_grad_(), c.clone().requires_grad_()]
+    auto = torch.autograd.grad(rendering.project(b, chars, *leaves, activation=act, residual=r), leaves, grad.cuda())
+    for named in (dict(), dict(activation=act)):
+      dw, db = rendering.project_backward(b, chars, w, grad.cuda(), slope, **named)
+      check_grads(chars, boards, weight, grad, slope64, slope_tol, dw, db)
+      assert torch.equal(dw, auto[0]) and torch.equal(db, auto[1])
