@@ -936,9 +936,9 @@ def project(boards, layers, weight, bias=None, activation=None, residual=None, r
 
 
 def project_backward(boards, layers, weight, grad, slope=None, activation=None):
-  """(grad_weight, grad_bias) of `project()` for the gradient `grad` [n, hidden] of its result; `slope` as it
-  returned it, `activation` as it was given.  The residual's gradient is `grad`.  Records nothing for autograd and waits for
-  nothing: it may be captured.
+  """(grad_weight, grad_bias) of `project()` for the gradient `grad` of its result ([n, hidden]; of a batch-1 Observation
+  [hidden] too); `slope` as it returned it, `activation` as it was given.  The residual's gradient is `grad`.  Records
+  nothing for autograd and waits for nothing: it may be captured.
 
   Without `activation`, the gradient is multiplied by the slopes, and where a slope is 0 nothing comes through; named, a
   smooth activation's slope of 0 makes an infinite gradient a NaN, as its formula does."""
@@ -952,6 +952,8 @@ def project_backward(boards, layers, weight, grad, slope=None, activation=None):
   plan = _Projection(layers, weight, None, activation)
   view = _Boards(boards, layers)
   desc = plan.at(view)
+  if view.single and grad.dim() == 1:
+    grad = grad[None]
   plan.check_rows(grad, 'grad', view.n)
   plan.check_rows(slope, 'slope', view.n, plan.slope_dtype())
   return plan.backward(desc, view, grad.detach(), slope, True, True, weight.shape)

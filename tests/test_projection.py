@@ -585,3 +585,30 @@ def test_the_explicit_pair(act, dtype):
       dw, db = rendering.project_backward(b, chars, w, grad.cuda(), slope, **named)
       check_grads(chars, boards, weight, grad, slope64, slope_tol, dw, db)
       assert torch.equal(dw, auto[0]) and torch.equal(db, auto[1])
+
+
+def small_engine(batch, name='better_scrolly_maze_L0'):
+  import os
+  from pycolab_amd.compiler import GameTemplate
+  from pycolab_amd.engine import Engine
+  return Engine.from_template(GameTemplate.load(os.path.join(os.path.dirname(__file__), 'golden', 'templates', name + '.npz')), batch=batch, auto_reset=True)
+
+
+@pytest.mark.gpu
+def test_the_explicit_pair_of_one_observation():
+  """A batch-1 Observation: the result is [hidden], and so may its gradient be."""
+  eng = small_engine(1, 'scrolly_maze_L0')
+  obs, _, _ = eng.its_showtime()
+  w = torch.randn(24, 2, 10, 30, generator=torch.Generator().manual_seed(32)).cuda()
+  out, slope = rendering.project(obs, 'P#', w, activation='tanh', return_slope=True)
+  grad = torch.randn(24, generator=torch.Generator().manual_seed(33)).cuda()
+  assert out.shape == grad.shape
+  leaf = w.clone().requires_grad_()
+  want, = torch.autograd.grad(rendering.project(obs, 'P#', leaf, activation='tanh'), leaf, grad)
+  for g in (grad, grad[None]):
+    assert torch.equal(rendering.project_backward(obs, 'P#', w, g, slope, activation='tanh')[0], want)
+  with pytest.raises(ValueError):
+    rendering.project_backward(obs, 'P#', w, grad[:23], slope)
+  with pytest.raises(ValueError, match='slopes'):
+    rendering.project_backward(obs, 'P#', w, grad, activation='tanh')
+  eng.close()
