@@ -30,6 +30,7 @@ class ObservationCropper(object):
     self._out = None        # output planes [B, 1 + n_chars, pitch] (a device tensor with PyTorch)
     self._pitch = 0
     self._generation = 0    # bumped whenever the native cropper (and its buffers) is rebuilt
+    self._written = dev.Written()  # the output planes, by crop() or by the engine's step
     self._fused = False     # the engine's step kernel moves the window and writes the planes (fuse_croppers)
     self._feat_skip_since = 0
     self._feat_skip = 0     # ... and which of the window's own uint8 planes the kernel then no longer writes (1 layers, 2 board too)
@@ -61,6 +62,7 @@ class ObservationCropper(object):
     other._feat_skip = 0
     other._feat_skip_since = 0
     other._generation = 0
+    other._written = dev.Written()
     return other
 
   @property
@@ -105,6 +107,8 @@ class ObservationCropper(object):
       self._create_native()
     lib = N.lib()
     N.check(lib.pcx_cropper_crop(self._native, dev.current_stream(eng._device_id)))
+    if not self._fused:
+      self._written.count += 1
     chars = eng.template.chars
     B, P, r, c = eng.batch, 1 + len(chars), self._rows, self._cols
     if B == 1 or self._out is None or self._out.tensor is None:
@@ -324,6 +328,7 @@ def fuse_croppers(engine, croppers, only_crops=False):
     cr._fused = False
   for cr in croppers:
     cr._fused = True
+    cr._written.count += 1
   engine._only_crops = bool(only_crops) and bool(croppers)
   return True
 

@@ -83,6 +83,16 @@ class DeviceBuffer(object):
       pass
 
 
+class Written(object):
+  """How often kernels have written a device array that a caller may still be looking at (autograd's own counters do not see
+  them)."""
+
+  __slots__ = ('count',)
+
+  def __init__(self):
+    self.count = 0
+
+
 def current_stream(device_id):
   torch = torch_module()
   if torch is None:

@@ -84,6 +84,7 @@ class Engine(object):
     self._packed = None
     self._actions = None
     self._steps_launched = 0  # reset / step launches so far (fused epilogues know when they are fresh)
+    self._written = dev.Written()  # ... and what else has written the observation planes
     self._croppers = []
     self._fuse_request = None  # cropping.fuse_croppers() before its_showtime(): (croppers, only_crops)
     self._only_crops = False   # fused croppers only: the full-board planes are not written
@@ -294,8 +295,15 @@ class Engine(object):
     if template.n_plot_words and self._batch == 1:
       self._plot_to_device()  # what a Story copied into this game's Plot (storytelling.py:449-450) is what its programs start from
     N.check(lib.pcx_engine_reset(self._native, None, dev.current_stream(self._device_id)))
-    self._steps_launched += 1
+    self._launched(1)
     return self._result()
+
+  def _launched(self, steps):
+    self._steps_launched += steps
+    self._written.count += 1
+    for cropper in self._croppers:
+      if cropper._fused:  # (the same launch wrote its window)
+        cropper._written.count += 1
 
   # ---- plot words: the Plot entries device programs use (include/pcx.h PCX_PLOT_WORDS; examples/ordeal.py) ----------
   def plot_words(self):
@@ -376,7 +384,7 @@ class Engine(object):
         keep.upload(np.asarray(env_mask, np.uint8))
         ptr = keep.ptr
     N.check(N.lib().pcx_engine_reset(self._native, ptr, dev.current_stream(self._device_id)))
-    self._steps_launched += 1
+    self._launched(1)
     dev.synchronize(self._device_id)
     return self._result()
 
@@ -386,7 +394,7 @@ class Engine(object):
     ptr = self._stage_actions(actions)
     N.check(N.lib().pcx_engine_step(self._native, ptr, int(self._auto_reset),
                                     dev.current_stream(self._device_id)))
-    self._steps_launched += 1
+    self._launched(1)
 
   def step_n(self, action_tape):
     """`len(action_tape)` consecutive steps from a device int32 tensor (or host
@@ -407,7 +415,7 @@ class Engine(object):
       raise ValueError('action tape must have shape [T, batch]')
     N.check(N.lib().pcx_engine_step_n(self._native, ptr, int(steps), int(self._auto_reset),
                                       dev.current_stream(self._device_id)))
-    self._steps_launched += int(steps)
+    self._launched(int(steps))
     dev.synchronize(self._device_id)  # the staging buffer may be freed after this call
 
   def step_hashed(self, seed, t0, steps, env_offset=None):
@@ -419,7 +427,7 @@ class Engine(object):
     N.check(N.lib().pcx_engine_step_hashed(
         self._native, seed, env_offset, t0, steps, int(self._auto_reset),
         dev.current_stream(self._device_id)))
-    self._steps_launched += int(steps)
+    self._launched(int(steps))
 
   def step_sampled(self, logits, uniforms, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, legal=None):
     """One step with the actions `actions.sample()` draws from a policy's logits [batch, n_actions] and one number per
@@ -530,6 +538,11 @@ class Engine(object):
       raise ValueError('the checkpoint holds the state of {} cropper(s), this engine has {} attached: attach the same '
                        'croppers, in the same order, before import_state()'.format(len(parts), len(croppers)))
     blob = np.ascontiguousarray(blob)
+    with_observation = bool(blob[48:52].view(np.int32)[0]) if blob.size >= 64 else False  # StateHeader.with_observation
+    if with_observation:
+      self._written.count += 1
+    for cropper in croppers:  # (their windows are restored, or cut anew)
+      cropper._written.count += 1
     N.check(N.lib().pcx_engine_import_state(self._native, blob.ctypes.data, blob.nbytes))
     for cropper, part in zip(croppers, parts):
       if getattr(cropper, '_native', None) is None:
@@ -544,7 +557,6 @@ class Engine(object):
     # a feature stack fused into a cropper's window (ObservationToFeatureArray.fuse_into(engine, source=cropper)) was
     # written by the exporting engine's step kernel: recompute it from the window as restored (or recut), so that the
     # converter does not hand out the pre-import tensor as this step's
-    with_observation = bool(blob[48:52].view(np.int32)[0]) if blob.size >= 64 else False  # StateHeader.with_observation
     for cropper in croppers:
       feats = getattr(cropper, '_features', None)
       if feats is not None:

@@ -52,6 +52,7 @@ class _Post(object):
     lib = N.lib()
     N.check(lib.pcx_post_create(ctypes.byref(self.view), ctypes.byref(desc), self.device_id, ctypes.byref(handle)))
     self.handle = handle
+    self.written = dev.Written()
     self.out = None
     if dev.torch_module() is not None:
       self.out = dev.DeviceBuffer(self.out_shape, self.out_dtype, self.device_id)
@@ -60,6 +61,7 @@ class _Post(object):
   def run(self, host):
     lib = N.lib()
     N.check(lib.pcx_post_run(self.handle, dev.current_stream(self.device_id)))
+    self.written.count += 1
     if self.out is not None and self.out.tensor is not None and not host:
       seen = N.c_i32(0)
       N.check(lib.pcx_post_error_poll(self.handle, dev.current_stream(self.device_id), ctypes.byref(seen)))
@@ -642,6 +644,10 @@ def _engine_of(source):
   return getattr(source, '_engine', None) or getattr(source, '_origin', None) or source
 
 
+def _written_of(source):
+  return source._post.written if isinstance(source, _RepaintedPlanes) else source._written
+
+
 def _occluded(source):
   """Are this source's layers exactly `board == character`?"""
   engine = getattr(source, '_engine', None) or source
@@ -656,7 +662,7 @@ class _Boards(object):
     torch = dev.require_torch('a projection of observations')
     self.single = False
     self.offsets = None  # stacked layers: byte offsets within a board
-    self.written = None  # an Observation's engine and how many steps it had launched
+    self.written = None  # an Observation's engine, and [(what has been written, how often)]
     if isinstance(boards, torch.Tensor):
       self.keep, shape = boards, boards.shape
       if not boards.is_cuda:
@@ -686,7 +692,7 @@ class _Boards(object):
                            'features are {}.'.format(repr(layers), repr(present.decode('latin-1'))))
       self.keep = boards
       engine = _engine_of(source)
-      self.written = engine, engine._steps_launched
+      self.written = engine, [(w, w.count) for w in (engine._written, _written_of(source))]
       self.n, self.rows, self.cols = int(view.batch), view.rows, view.cols
       self.ptr, self.row_stride = view.planes, (1 + view.n_chars) * view.pitch
       self.single = self.n == 1
@@ -696,8 +702,8 @@ class _Boards(object):
   def check_unchanged(self, what):
     """In a backward pass: does an Observation still hold what the forward pass read?  (Of a tensor, autograd knows.)"""
     if self.written is not None:
-      engine, steps = self.written
-      if engine._native is None or engine._steps_launched != steps:
+      engine, counts = self.written
+      if engine._native is None or any(w.count != count for w, count in counts):
         raise RuntimeError('{}(): the Observation was overwritten by a later step, or its engine closed, before the backward '
                            'pass: pass a copy of its board, a tensor'.format(what))
 

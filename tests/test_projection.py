@@ -612,3 +612,26 @@ def test_the_explicit_pair_of_one_observation():
   with pytest.raises(ValueError, match='slopes'):
     rendering.project_backward(obs, 'P#', w, grad, activation='tanh')
   eng.close()
+
+
+@pytest.mark.gpu
+def test_backward_after_import_state():
+  """A checkpoint with its observation rewrites the planes, one without leaves them."""
+  from pycolab_amd import cropping
+  eng = small_engine(9)
+  obs, _, _ = eng.its_showtime()
+  cropper = cropping.ScrollingCropper(rows=10, cols=30, to_track=['P'], scroll_margins=(2, 3))
+  cropper.set_engine(eng)
+  cropper.crop(obs)
+  with_planes, without = eng.export_state(with_observation=True), eng.export_state()
+  obs = eng.play(torch.zeros(9, dtype=torch.int32).cuda())[0]
+  big, small = (torch.randn(8, 2, r, c, device='cuda').requires_grad_() for r, c in ((45, 89), (10, 30)))
+  out = rendering.project(obs, 'P@', big).sum()
+  eng.import_state(without)
+  torch.autograd.grad(out, big, retain_graph=True)
+  window = rendering.project(cropper.crop(obs), 'P@', small).sum()
+  eng.import_state(with_planes)
+  for late, weight in ((out, big), (window, small)):
+    with pytest.raises(RuntimeError, match='overwritten'):
+      torch.autograd.grad(late, weight)
+  eng.close()
