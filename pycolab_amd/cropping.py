@@ -80,6 +80,7 @@ class ObservationCropper(object):
   def _release(self):
     if self._native is not None:
       N.lib().pcx_cropper_destroy(self._native)  # (a fused cropper leaves its engine's step kernel first)
+      self._written.count += 1  # (the planes go; whoever still means to read them is told)
       self._native = None
       self._out = None
       self._fused = False

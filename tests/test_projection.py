@@ -635,3 +635,20 @@ def test_backward_after_import_state():
     with pytest.raises(RuntimeError, match='overwritten'):
       torch.autograd.grad(late, weight)
   eng.close()
+
+
+@pytest.mark.gpu
+def test_backward_after_a_cropper_let_go_of_its_window_is_refused():
+  from pycolab_amd import cropping
+  eng, other = small_engine(1), small_engine(1)
+  small = torch.randn(8, 2, 10, 30, device='cuda').requires_grad_()
+  obs, _, _ = eng.its_showtime()
+  other.its_showtime()
+  cropper = cropping.ScrollingCropper(rows=10, cols=30, to_track=['P'], scroll_margins=(2, 3))
+  cropper.set_engine(eng)
+  out = rendering.project(cropper.crop(obs), 'P@', small).sum()
+  cropper.set_engine(other)
+  with pytest.raises(RuntimeError, match='overwritten'):
+    torch.autograd.grad(out, small)
+  eng.close()
+  other.close()
