@@ -81,6 +81,7 @@ class ObservationCropper(object):
     if self._native is not None:
       N.lib().pcx_cropper_destroy(self._native)  # (a fused cropper leaves its engine's step kernel first)
       self._written.count += 1  # (the planes go; whoever still means to read them is told)
+      self._written = dev.Written()
       self._native = None
       self._out = None
       self._fused = False
@@ -179,6 +180,7 @@ class ObservationCropper(object):
       if dev.torch_module() is not None:  # the output planes are a tensor of ours: crop() hands out views of it
         self._out = dev.DeviceBuffer((eng.batch, 1 + len(eng.template.chars), self._pitch), np.uint8, eng._device_id)
         N.check(lib.pcx_cropper_bind_output(handle, self._out.ptr))
+      self._written = dev.Written(None if self._out is None else self._out.tensor)
 
   def _planes_view(self):
     view = N.PlanesView()

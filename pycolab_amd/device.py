@@ -8,6 +8,7 @@ in csrc/ -- nothing here computes.
 """
 
 import ctypes
+import weakref
 
 import numpy as np
 
@@ -85,12 +86,22 @@ class DeviceBuffer(object):
 
 class Written(object):
   """How often kernels have written a device array that a caller may still be looking at (autograd's own counters do not see
-  them)."""
+  them).  Whoever launches the writes holds it, and it holds the array, if there is a tensor of it: while it lives, the
+  tensor's storage can be found by its address and is no one else's."""
 
-  __slots__ = ('count',)
+  __slots__ = ('count', 'tensor', '__weakref__')
+  _by_storage = weakref.WeakValueDictionary()
 
-  def __init__(self):
+  def __init__(self, tensor=None):
     self.count = 0
+    self.tensor = tensor
+    if tensor is not None and tensor.numel():
+      Written._by_storage[tensor.untyped_storage().data_ptr()] = self
+
+  @classmethod
+  def of(cls, tensor):
+    """The one of the array that `tensor` is a view of, or None."""
+    return cls._by_storage.get(tensor.untyped_storage().data_ptr()) if tensor.numel() else None
 
 
 def current_stream(device_id):

@@ -84,7 +84,8 @@ class Engine(object):
     self._packed = None
     self._actions = None
     self._steps_launched = 0  # reset / step launches so far (fused epilogues know when they are fresh)
-    self._written = dev.Written()  # ... and what else has written the observation planes
+    self._written = dev.Written()  # what has written the observation planes: launches, import_state()
+    self._epilogue_written = None  # ... and the fused post-processor's array
     self._croppers = []
     self._fuse_request = None  # cropping.fuse_croppers() before its_showtime(): (croppers, only_crops)
     self._only_crops = False   # fused croppers only: the full-board planes are not written
@@ -98,6 +99,8 @@ class Engine(object):
     if self._epilogue is not None and self._epilogue[0] is not converter:
       self._epilogue[0]._epilogue_gone()  # the kernel feeds one array: the earlier converter is on its own again
     self._epilogue = (converter, out)
+    tensor = getattr(out, 'tensor', out)  # (a repainter's planes are a DeviceBuffer)
+    self._epilogue_written = dev.Written.of(tensor) or dev.Written(tensor)
     self._epilogue_only = bool(only)
 
   def _clear_epilogue(self, converter=None):
@@ -106,7 +109,7 @@ class Engine(object):
     if self._native is not None:
       N.check(N.lib().pcx_engine_set_epilogue(self._native, None))
     self._epilogue[0]._epilogue_gone()
-    self._epilogue = None
+    self._epilogue = self._epilogue_written = None
     self._epilogue_only = False
 
   def _register_cropper(self, cropper):
@@ -265,6 +268,7 @@ class Engine(object):
     mk = lambda shape, dt: dev.DeviceBuffer(shape, dt, self._device_id)
     self._bufs = dict(planes=mk((B, 1 + L, self._pitch), np.uint8), frame=mk((B,), np.int32),
                       error=mk((B,), np.uint8))
+    self._written = dev.Written(self._bufs['planes'].tensor)
     # what play() returns besides the observation, 10 bytes per environment, in
     # ONE allocation [reward i32 B | discount f32 B | reward_set u8 B | done u8 B]:
     # a multi-GPU consumer gathers it with a single collective and no packing
@@ -301,8 +305,10 @@ class Engine(object):
   def _launched(self, steps):
     self._steps_launched += steps
     self._written.count += 1
+    if self._epilogue_written is not None:  # (the same launch wrote it)
+      self._epilogue_written.count += 1
     for cropper in self._croppers:
-      if cropper._fused:  # (the same launch wrote its window)
+      if cropper._fused:  # (and its window)
         cropper._written.count += 1
 
   # ---- plot words: the Plot entries device programs use (include/pcx.h PCX_PLOT_WORDS; examples/ordeal.py) ----------
@@ -746,6 +752,7 @@ class Engine(object):
       # engine <-> cropper references form a cycle: without this the buffers would wait for the garbage collector
       self._croppers = []
       self._bufs, self._packed, self._actions, self._keepalive = {}, None, None, None
+      self._written = dev.Written()
 
   def __del__(self):
     try:

@@ -52,11 +52,11 @@ class _Post(object):
     lib = N.lib()
     N.check(lib.pcx_post_create(ctypes.byref(self.view), ctypes.byref(desc), self.device_id, ctypes.byref(handle)))
     self.handle = handle
-    self.written = dev.Written()
     self.out = None
     if dev.torch_module() is not None:
       self.out = dev.DeviceBuffer(self.out_shape, self.out_dtype, self.device_id)
       N.check(lib.pcx_post_bind_output(handle, self.out.ptr, self.out.nbytes))
+    self.written = dev.Written(None if self.out is None else self.out.tensor)
 
   def run(self, host):
     lib = N.lib()
@@ -662,7 +662,8 @@ class _Boards(object):
     torch = dev.require_torch('a projection of observations')
     self.single = False
     self.offsets = None  # stacked layers: byte offsets within a board
-    self.written = None  # an Observation's engine, and [(what has been written, how often)]
+    self.written = []  # of an Observation, or after watch(): [(what has been written, how often)]
+    self.engine = None
     if isinstance(boards, torch.Tensor):
       self.keep, shape = boards, boards.shape
       if not boards.is_cuda:
@@ -692,20 +693,25 @@ class _Boards(object):
                            'features are {}.'.format(repr(layers), repr(present.decode('latin-1'))))
       self.keep = boards
       engine = _engine_of(source)
-      self.written = engine, [(w, w.count) for w in (engine._written, _written_of(source))]
+      self.engine, self.written = engine, [(w, w.count) for w in (engine._written, _written_of(source))]
       self.n, self.rows, self.cols = int(view.batch), view.rows, view.cols
       self.ptr, self.row_stride = view.planes, (1 + view.n_chars) * view.pitch
       self.single = self.n == 1
       if not _occluded(source):
         self.offsets = [(1 + present.index(ord(c))) * view.pitch if ord(c) in present else -1 for c in layers]
 
+  def watch(self):
+    """A backward pass is to come.  (Of a tensor's writes autograd knows, but for what this package's kernels write to it.)"""
+    if isinstance(self.keep, dev.torch_module().Tensor):
+      written = dev.Written.of(self.keep)
+      self.written = [] if written is None else [(written, written.count)]
+    return self
+
   def check_unchanged(self, what):
-    """In a backward pass: does an Observation still hold what the forward pass read?  (Of a tensor, autograd knows.)"""
-    if self.written is not None:
-      engine, counts = self.written
-      if engine._native is None or any(w.count != count for w, count in counts):
-        raise RuntimeError('{}(): the Observation was overwritten by a later step, or its engine closed, before the backward '
-                           'pass: pass a copy of its board, a tensor'.format(what))
+    """In a backward pass: do the boards still show what the forward pass read?"""
+    if (self.engine is not None and self.engine._native is None) or any(w.count != count for w, count in self.written):
+      raise RuntimeError('{}(): the boards were overwritten by a later step (or crop, or conversion), or their engine closed, '
+                         'before the backward pass: pass a copy of the board, a tensor of its own'.format(what))
 
 
 _NO_OFFSETS = bytes(8 * N.POST_MAX_DEPTH)
@@ -920,8 +926,8 @@ def project(boards, layers, weight, bias=None, activation=None, residual=None, r
   first layer.  Arguments, shapes and types as for `ObservationProjection`, which is the form for weights that stay; this
   one lays the weight out in every call.
 
-  An Observation is a view of the engine's planes, which the next step overwrites: a backward pass after that is refused;
-  pass a copy of the board (`observation.board.clone()`), a tensor.  A weight that is no finite number makes the results of
+  An Observation, its board and what a converter returned are views of arrays that the next step, crop or conversion
+  overwrites: a backward pass after that is refused; pass a copy of the board (`observation.board.clone()`).  A weight that is no finite number makes the results of
   the boards that use it no finite numbers, and of others some.
 
   `return_slope=True`: no autograd; returns (out, slope) with slope = act'(...) (None without an activation), what
@@ -933,7 +939,7 @@ def project(boards, layers, weight, bias=None, activation=None, residual=None, r
   plan.check_rows(residual, 'residual', view.n)
   if not return_slope and torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (weight, bias, residual)):
     dev.refuse_recording_in_capture('project', 'project(..., return_slope=True) and project_backward()')
-    out = _project_autograd().apply(weight, bias, residual, plan, view, desc)
+    out = _project_autograd().apply(weight, bias, residual, plan, view.watch(), desc)
     return out[0] if view.single else out
   bias, residual = (None if t is None else t.detach() for t in (bias, residual))
   out, slope = plan.forward(desc, view, plan.pack(desc, weight), bias, residual, want_slope=return_slope and activation is not None)

@@ -652,3 +652,89 @@ def test_backward_after_a_cropper_let_go_of_its_window_is_refused():
     torch.autograd.grad(out, small)
   eng.close()
   other.close()
+
+
+@pytest.mark.gpu
+def test_backward_after_a_view_of_the_planes_was_overwritten_is_refused():
+  """The kernels write an engine's, a cropper's, a repainter's and a converter's arrays where autograd does not see it: a
+  backward pass over a tensor that lies in one of them is refused once it was written again."""
+  from pycolab_amd import cropping
+  eng = small_engine(9)
+  obs, _, _ = eng.its_showtime()
+  cropper = cropping.ScrollingCropper(rows=10, cols=30, to_track=['P'], scroll_margins=(2, 3))
+  cropper.set_engine(eng)
+  repainter = rendering.ObservationCharacterRepainter({'a': '@', 'b': '@', 'c': '@'})
+  converter = rendering.ObservationToArray({c: ord(c) for c in obs.layers}, dtype=np.uint8)
+  still = torch.zeros(9, dtype=torch.int32).cuda()
+  big, small = (torch.randn(8, 2, r, c, device='cuda').requires_grad_() for r, c in ((45, 89), (10, 30)))
+  run = lambda t, w: rendering.project(t, 'P@', w).sum()
+
+  def written(make_tensor, weight, again):
+    """make_tensor() -> a view; again() -> writes what it shows."""
+    out = run(make_tensor(), weight)
+    grad, = torch.autograd.grad(out, weight)  # in time
+    assert grad.abs().sum() > 0
+    out, copy = run(make_tensor(), weight), run(make_tensor().clone(), weight)
+    again()
+    torch.autograd.grad(copy, weight)
+    with pytest.raises(RuntimeError, match='overwritten'):
+      torch.autograd.grad(out, weight)
+
+  for view in (lambda: obs.board, lambda: obs.board[2:7], lambda: eng.planes_view()[:, 0], lambda: eng.planes_view()[:, 1:3]):
+    for again in (lambda: eng.step(still), lambda: eng.step_n(still[None]), lambda: eng.step_hashed(1, 0, 2), lambda: eng.reset()):
+      written(view, big, again)
+  written(lambda: cropper.crop(obs).board, small, lambda: cropper.crop(obs))
+  window = cropper.crop(obs).board
+  out = run(window, small)
+  eng.step(still)  # (the window is written by crop() alone)
+  torch.autograd.grad(out, small)
+  written(lambda: repainter(obs).board, big, lambda: repainter(obs))
+  written(lambda: converter(obs), big, lambda: converter(obs))
+  out = run(obs.board, big)
+  eng.close()  # (nobody writes the tensor any more)
+  torch.autograd.grad(out, big)
+
+
+@pytest.mark.gpu
+def test_backward_after_what_a_step_writes_besides_its_planes_is_refused():
+  """Fused croppers' windows and a fused converter's array are written by the step itself."""
+  from pycolab_amd import cropping
+  still = torch.zeros(9, dtype=torch.int32).cuda()
+  small = torch.randn(8, 2, 10, 30, device='cuda').requires_grad_()
+  eng = small_engine(9)
+  obs, _, _ = eng.its_showtime()
+  cropper = cropping.ScrollingCropper(rows=10, cols=30, to_track=['P'], scroll_margins=(2, 3))
+  assert cropping.fuse_croppers(eng, [cropper])
+  obs = eng.play(still)[0]
+  out = rendering.project(cropper.crop(obs).board, 'P@', small).sum()
+  eng.step(still)
+  with pytest.raises(RuntimeError, match='overwritten'):
+    torch.autograd.grad(out, small)
+  eng.close()
+  eng = small_engine(9, 'scrolly_maze_L0')
+  obs, _, _ = eng.its_showtime()
+  converter = rendering.ObservationToArray({c: ord(c) for c in obs.layers}, dtype=np.uint8)
+  assert converter.fuse_into(eng, force=True)
+  obs = eng.play(still)[0]
+  out = rendering.project(converter(obs), 'P@', small).sum()
+  eng.step(still)
+  with pytest.raises(RuntimeError, match='overwritten'):
+    torch.autograd.grad(out, small)
+  converter.unfuse()
+  eng.close()
+
+
+@pytest.mark.gpu
+def test_backward_over_a_view_after_import_state():
+  eng = small_engine(9)
+  obs, _, _ = eng.its_showtime()
+  with_planes, without = eng.export_state(with_observation=True), eng.export_state()
+  obs = eng.play(torch.zeros(9, dtype=torch.int32).cuda())[0]
+  big = torch.randn(8, 2, 45, 89, device='cuda').requires_grad_()
+  out = rendering.project(obs.board, 'P@', big).sum()
+  eng.import_state(without)
+  torch.autograd.grad(out, big, retain_graph=True)
+  eng.import_state(with_planes)
+  with pytest.raises(RuntimeError, match='overwritten'):
+    torch.autograd.grad(out, big)
+  eng.close()
