@@ -190,7 +190,7 @@ def _positive(temperature):
 
 def log_prob(logits, actions, legal=None, temperature=1.0, return_stats=False):
   """(log-probability of `actions`, entropy) of every row's policy softmax(logits / temperature) over the allowed actions:
-  two float32 tensors [n], differentiable in `logits` (float32, float16 or bfloat16 [n, actions]).
+  two float32 tensors [n], differentiable in `logits` (float32, float16 or bfloat16 [n, actions]) once, in reverse mode.
 
   `actions`: int32 [n], as `sample()` returned them.  -1 (`_native.ACTION_NONE`: nothing was allowed) has log-probability 0
   and adds nothing to the gradient; so does a row that allows nothing, whose entropy is 0 too.  An action that is not
@@ -204,6 +204,7 @@ def log_prob(logits, actions, legal=None, temperature=1.0, return_stats=False):
   actions, temperature = _taken(torch, actions, n, logits.device), _positive(temperature)
   if return_stats:
     return _log_prob_forward(torch, desc, legal, logits.detach(), actions, temperature)
+  dev.refuse_tangents('log_prob', logits)
   if logits.requires_grad and torch.is_grad_enabled():
     dev.refuse_recording_in_capture('log_prob', 'log_prob(..., return_stats=True) and log_prob_backward()')
     return _log_prob_autograd().apply(logits, actions, legal, temperature, desc)

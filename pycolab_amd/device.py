@@ -201,6 +201,17 @@ def refuse_recording_in_capture(what, instead):
     raise RuntimeError('{}() does not record gradients while a graph is captured: capture {} instead'.format(what, instead))
 
 
+def refuse_tangents(what, *tensors):
+  """Forward mode is not recorded: a tensor with a tangent looks like any other (it does not ask for gradients), and its
+  tangent would be dropped."""
+  forward = torch_module().autograd.forward_ad
+  if getattr(forward, '_current_level', 0) < 0:  # (nobody differentiates forward; without that number, ask each tensor)
+    return
+  for tensor in tensors:
+    if tensor is not None and forward.unpack_dual(tensor).tangent is not None:
+      raise RuntimeError('{}() has no forward-mode derivative'.format(what))
+
+
 def refuse_twice(what):
   """Called in a backward pass: gradients are recorded there only when it is to be differentiated itself."""
   if torch_module().is_grad_enabled():

@@ -922,8 +922,8 @@ def _project_autograd():
 
 
 def project(boards, layers, weight, bias=None, activation=None, residual=None, return_slope=False):
-  """`act(features @ weight.T + bias) + residual`, differentiable in `weight`, `bias` and `residual`: one training step's
-  first layer.  Arguments, shapes and types as for `ObservationProjection`, which is the form for weights that stay; this
+  """`act(features @ weight.T + bias) + residual`, differentiable in `weight`, `bias` and `residual` (once, in reverse
+  mode): one training step's first layer.  Arguments, shapes and types as for `ObservationProjection`, which is the form for weights that stay; this
   one lays the weight out in every call.
 
   An Observation, its board and what a converter returned are views of arrays that the next step, crop or conversion
@@ -937,6 +937,8 @@ def project(boards, layers, weight, bias=None, activation=None, residual=None, r
   view = _Boards(boards, layers)
   desc = plan.at(view)
   plan.check_rows(residual, 'residual', view.n)
+  if not return_slope:
+    dev.refuse_tangents('project', weight, bias, residual)
   if not return_slope and torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (weight, bias, residual)):
     dev.refuse_recording_in_capture('project', 'project(..., return_slope=True) and project_backward()')
     out = _project_autograd().apply(weight, bias, residual, plan, view.watch(), desc)

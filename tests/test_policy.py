@@ -604,3 +604,31 @@ def test_sample_few_of_very_many(n, a, dtype):
     check_sample(x[rows], u[rows], legal=legal[rows], **kw)
   per_row = torch.tensor([0.0, 0.5, 1.0, 2.0])[torch.arange(n) % 4]
   check_sample(x[rows], u[rows], legal=legal[rows], top_k=50, top_p=0.8, temperature=per_row[rows])
+
+
+@pytest.mark.gpu
+def test_tensors_with_a_tangent_are_told_apart():
+  from pycolab_amd import device as dev
+  plain = torch.ones(3)
+  dev.refuse_tangents('f', plain, None)
+  with torch.autograd.forward_ad.dual_level():
+    dual = torch.autograd.forward_ad.make_dual(torch.ones(3), torch.ones(3))
+    dev.refuse_tangents('f', plain, None)
+    with pytest.raises(RuntimeError, match='forward'):
+      dev.refuse_tangents('f', plain, dual)
+  assert not dual.requires_grad  # (which is why nothing else notices)
+
+
+@pytest.mark.gpu
+def test_log_prob_refuses_forward_mode_and_function_transforms():
+  x, taken = torch.randn(4, 5).cuda(), torch.zeros(4, dtype=torch.int32).cuda()
+  with torch.autograd.forward_ad.dual_level():
+    dual = torch.autograd.forward_ad.make_dual(x, torch.ones_like(x))
+    with pytest.raises(RuntimeError, match='forward'):
+      policy.log_prob(dual, taken)
+    policy.log_prob(x, taken)  # (no tangent)
+  f = lambda x: policy.log_prob(x, taken)[0]
+  for transform in (lambda: torch.func.jvp(f, (x,), (x,)), lambda: torch.func.grad(lambda x: f(x).sum())(x),
+                    lambda: torch.func.vmap(f)(torch.stack([x] * 2)), lambda: torch.func.vjp(f, x)):
+    with pytest.raises(RuntimeError):
+      transform()

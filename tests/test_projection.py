@@ -738,3 +738,21 @@ def test_backward_over_a_view_after_import_state():
   with pytest.raises(RuntimeError, match='overwritten'):
     torch.autograd.grad(out, big)
   eng.close()
+
+
+@pytest.mark.gpu
+def test_forward_mode_and_function_transforms_are_refused():
+  chars, boards, weight, bias, residual = make(6, 3, 4, 5, 16, 'float32', 50)
+  b, given = boards.cuda(), [t.cuda() for t in (weight, bias, residual)]
+  for i in range(3):
+    with torch.autograd.forward_ad.dual_level():
+      args = list(given)
+      args[i] = torch.autograd.forward_ad.make_dual(args[i], torch.ones_like(args[i]))
+      with pytest.raises(RuntimeError, match='forward'):
+        rendering.project(b, chars, args[0], args[1], residual=args[2])
+      rendering.project(b, chars, given[0], given[1], residual=given[2])  # (no tangent)
+  f = lambda w: rendering.project(b, chars, w, given[1])
+  for transform in (lambda: torch.func.jvp(f, (given[0],), (given[0],)), lambda: torch.func.grad(lambda w: f(w).sum())(given[0]),
+                    lambda: torch.func.vmap(f)(torch.stack([given[0]] * 2)), lambda: torch.func.vjp(f, given[0])):
+    with pytest.raises(RuntimeError):
+      transform()
