@@ -683,8 +683,9 @@ typedef struct pcx_sampling {
 } pcx_sampling;
 
 /* actions_out[row] = the first action, by index, at which the running sum of the kept actions' weights exceeds
- * uniforms[row] (in [0, 1)) of their total; PCX_ACTION_NONE where no action is allowed.  64-bit weights; the result
- * depends on the row alone.  The workspace (pcx_sample_size: 0 up to 16,384 actions) serves one call at a time. */
+ * uniforms[row] (in [0, 1)) of their total; PCX_ACTION_NONE where no action is allowed.  Weights and sums are 64-bit
+ * floats (over 16,384 actions, the sums that decide top_k's total and top_p's cut are of whole numbers, off by 2^-38 + actions
+ * 2^-55 of the total at most); the result depends on the row alone.  The workspace (pcx_sample_size: 0 up to 16,384 actions) serves one call at a time. */
 int pcx_sample_size(const pcx_logits_desc* d, uint64_t* bytes);
 int pcx_sample_actions(const pcx_logits_desc* d, const pcx_sampling* rules, const void* logits, const uint8_t* legal,
                        const float* uniforms, int32_t* actions_out, void* workspace, uint64_t workspace_bytes, void* stream);

@@ -13,7 +13,7 @@
 //
 // Sampling decides by where one number falls between two sums, so its weights and sums are 64-bit: a float32 sum would
 // pick another action once in some million rows.  MI355X multiplies and adds 64-bit floats at the rate of 32-bit ones,
-// which puts exp at about 25 instructions.  Sums that atomics build are 64-bit fixed point: their order does not matter.
+// which puts exp at about 25 instructions.  Sums that atomics build are whole numbers: their order does not matter.
 #include "pcx_internal.h"
 
 #include <cmath>
@@ -706,7 +706,7 @@ __global__ __launch_bounds__(TOP_THREADS, 4) void pcx_sample_top(SampleArgs a) {
 // ---- rows that no workgroup holds: divided among workgroups, one launch per question ------------------------------------
 //
 // The best logit; the edges of top_k and of top_p, a digit of the order key at a time; what each slice keeps; the slice and
-// the action that the number falls to.  8 x 2^20 float32 logits with top_p take 101 us in ten launches, of which one pass
+// the action that the number falls to.  8 x 2^20 float32 logits with top_p take 102 us in ten launches, of which one pass
 // over them, the floor, is 6.5: four more passes read them again (from the 256 MB cache: 7 us each if that were all), and the
 // chain of launches alone is 70 us, the time of a single row.
 
@@ -722,12 +722,28 @@ struct RowState {
   uint32_t active;             // bit 0: the row samples; 1: top_k cuts; 2: top_p cuts
 };
 struct Slot { double weight; uint64_t ties; };
+
+// Sums that atomics build are sums of whole numbers, so that their order does not matter; a word has 64 bits, and a tail of
+// many small weights must not vanish beside a large one.  So there are two words a bin: in LDS, of a slice's 2^13 weights, those
+// from 2^-12 of the best one's on in units of 2^-50, the smaller ones of 2^-62 (off by 2^-39 of themselves, and by 2^-39 of the
+// total, which is at least 1, if they are 2^24); in memory, a slice's bin below 2^-9 in units of 2^-62, exactly, and one from
+// there on in units of 2^-(63 - log2 A), off by A 2^-55 of itself.  A 64-bit float's sum of A numbers is known to A 2^-53.
+constexpr double SMALL = 1.0 / 4096.0;
+constexpr uint64_t LOW = 1ull << 53;  // (2^11 slices of less)
+// large 2^12 + small, in units of 2^-62: a word for memory, and which
+__device__ __forceinline__ uint64_t slice_sum(uint64_t large, uint64_t small, int scale, bool* is_low) {
+  *is_low = large < (LOW >> 12) && (large << 12) + small < LOW;  // (small is at most 2^63)
+  if (*is_low) return (large << 12) + small;
+  return (uint64_t)(ldexp((double)large, scale - 50) + ldexp((double)small, scale - 62) + 0.5);
+}
+__device__ __forceinline__ double weight_of(uint64_t high, uint64_t low, int scale) { return ldexp((double)high, -scale) + ldexp((double)low, -62); }
 struct WideArgs {
   SampleArgs a;
   int64_t row0;                // first row of this batch of launches
-  int32_t slices, scale;       // fixed-point weights: w * 2^scale
+  int32_t slices, scale;       // high words' unit: 2^-scale
   RowState* state;             // [rows]
-  uint64_t* mass;              // [2][rows][BINS]: the first digit's, the later digits'
+  uint64_t* high;              // [2][rows][BINS]: the first digit's, the later digits'
+  uint64_t* low;
   uint32_t* count;
   Slot* slots;                 // [rows][slices]
   int32_t batch;
@@ -753,7 +769,7 @@ __global__ __launch_bounds__(256) void pcx_sample_clear(WideArgs w) {
   const int row = blockIdx.x;
   for (int i = threadIdx.x; i < 2 * BINS; i += 256) {
     const int64_t at = ((int64_t)(i / BINS) * w.batch + row) * BINS + i % BINS;
-    w.mass[at] = 0;
+    w.high[at] = w.low[at] = 0;
     w.count[at] = 0;
   }
   if (threadIdx.x == 0) w.state[row] = RowState{};
@@ -789,15 +805,18 @@ __global__ __launch_bounds__(256) void pcx_sample_best(WideArgs w) {
   if (threadIdx.x == 0 && top) atomicMax(reinterpret_cast<unsigned long long*>(&w.state[row].best), (unsigned long long)top << 32 | (uint32_t)~at);
 }
 // Weights (and counts, where top_k asks for them) per value of one digit, of the keys that agree with the digits found so
-// far: one pass over the logits, bound by the first digit's exponentials and LDS atomics (8 x 2^20 float32: 22 us; the second
-// digit 14, the third 10).  A slice a workgroup: with half the workgroups, two slices each, 4 us more.
-template <int DT>
-__global__ __launch_bounds__(256) void pcx_sample_digit(WideArgs w, int level, uint32_t needs, int counts) {
-  __shared__ unsigned long long mass[BINS];
-  __shared__ uint32_t count[BINS], piles[4][768];
+// far: one pass over the logits, bound by the first digit's exponentials and LDS atomics (8 x 2^20 float32: 23 us; the second
+// digit 15, the third 11; a bin's two words of every slice added to memory: 34 and 22).  A slice a workgroup: with half the workgroups, two slices each, 4 us more.
+enum { FIRST = 0, BY_COUNT = 2, BY_MASS = 4 };  // the first digit; a later one of top_k's edge, of top_p's (a row's active bit)
+template <int DT, int KIND>
+__global__ __launch_bounds__(256) void pcx_sample_digit(WideArgs w, int level, int counts) {
+  // (40 KB at most: four workgroups a CU; three, with counts of 32 bits, 115 us where this takes 101: top_k = 5,000 of 8 x 2^20)
+  constexpr int PILE = 256, FULL = PILE - 64;
+  __shared__ unsigned long long mass[2 * BINS];
+  __shared__ uint32_t count[KIND == BY_MASS ? 1 : BINS / 2], piles[KIND == FIRST ? 1 : 4][KIND == FIRST ? 1 : PILE];  // (two counts a word)
   const int row = blockIdx.y, lo = blockIdx.x * SLICE;
   const RowState st = w.state[row];
-  if (level > 0 && !(st.active & needs)) return;
+  if (KIND != FIRST && !(st.active & KIND)) return;
   const RowRules r = rules_of(w.a.rules, w.row0 + row);
   const uint32_t best_key = (uint32_t)(st.best >> 32);
   if (!best_key || !(r.temperature > 0.0f)) return;
@@ -805,7 +824,11 @@ __global__ __launch_bounds__(256) void pcx_sample_digit(WideArgs w, int level, u
   load_slice<DT>(w, row, lo, key);
   const float best = value_of<DT>(best_key);
   const double rate = 1.0 / (double)r.temperature;
-  for (int i = threadIdx.x; i < BINS; i += 256) { mass[i] = 0; count[i] = 0; }
+  for (int i = threadIdx.x; i < BINS; i += 256) {
+    mass[i] = 0;
+    mass[BINS + i] = 0;
+    if constexpr (KIND != BY_MASS) count[i / 2] = 0;
+  }
   __syncthreads();
   auto add = [&](const uint32_t* four) {
     double v[4];
@@ -814,11 +837,13 @@ __global__ __launch_bounds__(256) void pcx_sample_digit(WideArgs w, int level, u
     for (int c = 0; c < 4; ++c)
       if (four[c]) {
         const uint32_t d = digit_of<DT>(four[c], level);
-        if (counts) atomicAdd(&count[d], 1u);
-        atomicAdd(&mass[d], (unsigned long long)(ldexp(v[c], w.scale) + 0.5));
+        if constexpr (KIND != BY_MASS)
+          if (counts) atomicAdd(&count[d / 2], d & 1 ? 65536u : 1u);
+        const bool small = v[c] < SMALL;
+        atomicAdd(&mass[small ? BINS + d : d], (unsigned long long)(ldexp(v[c], small ? 62 : 50) + 0.5));
       }
   };
-  if (level == 0) {
+  if constexpr (KIND == FIRST) {
 #pragma unroll 1
     for (int i = 0; i < WEP; i += 4) {
       add(key);
@@ -827,40 +852,45 @@ __global__ __launch_bounds__(256) void pcx_sample_digit(WideArgs w, int level, u
     }
   } else {
     // Later digits concern some of the keys: a wave piles those up and weighs them four a lane (weighed where they lie, with
-    // most lanes idle, the second digit of 8 x 2^20 float32 logits took 20 us, this way 14).
+    // most lanes idle, the second digit of 8 x 2^20 float32 logits took 20 us, this way 15).
     uint32_t* const pile = piles[threadIdx.x >> 6];
     const uint32_t lane = threadIdx.x & 63;
-    uint32_t high = 0, four[4];
-#pragma unroll 1
-    for (int i = 0; i < WEP; i += 8) {
+    uint32_t high = 0;
+    auto weigh = [&]() {
+      uint32_t four[4];
+      __builtin_amdgcn_wave_barrier();
 #pragma unroll
-      for (int c = 0; c < 8; ++c) {
+      for (int c = 0; c < 4; ++c) four[c] = c * 64 + lane < high ? pile[c * 64 + lane] : 0u;
+      __builtin_amdgcn_wave_barrier();
+      high = 0;
+      add(four);
+    };
+#pragma unroll 1
+    for (int i = 0; i < WEP; i += 4) {
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
         const bool mine = key[c] && same_prefix<DT>(key[c], st.prefix, level);
         const uint64_t who = __ballot(mine);
         if (mine) pile[high + __popcll(who & ((1ull << lane) - 1))] = key[c];
         high += (uint32_t)__popcll(who);
+        if (high > FULL) weigh();
       }
 #pragma unroll
-      for (int c = 0; c < WEP - 8; ++c) key[c] = key[c + 8];
-      const bool end = i + 8 == WEP;
-      while (high >= 256 || (end && high)) {
-        const uint32_t from = high >= 256 ? high - 256 : 0;
-        __builtin_amdgcn_wave_barrier();
-#pragma unroll
-        for (int c = 0; c < 4; ++c) four[c] = from + c * 64 + lane < high ? pile[from + c * 64 + lane] : 0u;
-        __builtin_amdgcn_wave_barrier();
-        high = from;
-        add(four);
-      }
+      for (int c = 0; c < WEP - 4; ++c) key[c] = key[c + 4];
     }
+    if (high) weigh();
   }
   __syncthreads();
-  const int64_t at = ((int64_t)(level != 0) * w.batch + row) * BINS;
-  for (int i = threadIdx.x; i < BINS; i += 256)
-    if (count[i] || mass[i]) {
-      if (counts) atomicAdd(&w.count[at + i], count[i]);
-      if (mass[i]) atomicAdd(reinterpret_cast<unsigned long long*>(&w.mass[at + i]), mass[i]);
+  const int64_t at = ((int64_t)(KIND != FIRST) * w.batch + row) * BINS;
+  for (int i = threadIdx.x; i < BINS; i += 256) {
+    if constexpr (KIND != BY_MASS)
+      if (const uint32_t n = (count[i / 2] >> (16 * (i & 1))) & 0xFFFFu) atomicAdd(&w.count[at + i], n);
+    if (mass[i] | mass[BINS + i]) {
+      bool is_low;
+      const uint64_t sum = slice_sum(mass[i], mass[BINS + i], w.scale, &is_low);
+      atomicAdd(reinterpret_cast<unsigned long long*>((is_low ? w.low : w.high) + at + i), (unsigned long long)sum);
     }
+  }
 }
 // Which bin of the digit the edge lies in.  by_mass: top_p's edge, else top_k's.
 template <int DT>
@@ -876,22 +906,30 @@ __global__ __launch_bounds__(256) void pcx_sample_edge(WideArgs w, int level, in
   if (level > 0 && !(st.active & (by_mass ? 4u : 2u))) return;
   const int64_t at = ((int64_t)(level != 0) * w.batch + row) * BINS;
   // thread 0 has the highest bins: eight a thread
-  uint64_t counts[8], masses[8], c_mine = 0, m_mine = 0, c_all, m_all;
+  uint64_t counts[8], c_mine = 0, c_all;
+  double masses[8], m_mine = 0.0, m_all;
+  const int64_t mine_at = at + BINS - 8 * ((int)threadIdx.x + 1);
+  const Pack<uint64_t, 8> high = *reinterpret_cast<const Pack<uint64_t, 8>*>(w.high + mine_at), low = *reinterpret_cast<const Pack<uint64_t, 8>*>(w.low + mine_at);
+  const Pack<uint32_t, 8> n = *reinterpret_cast<const Pack<uint32_t, 8>*>(w.count + mine_at);
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    const int bin = BINS - 1 - ((int)threadIdx.x * 8 + i);
-    counts[i] = w.count[at + bin];
-    masses[i] = w.mass[at + bin];
+    counts[i] = n.v[7 - i];
+    masses[i] = weight_of(high.v[7 - i], low.v[7 - i], w.scale);
     c_mine += counts[i];
     m_mine += masses[i];
-    if (level != 0) { w.count[at + bin] = 0; w.mass[at + bin] = 0; }  // for the next digit
   }
-  uint64_t c = g.scan(c_mine, &c_all), m = g.scan(m_mine, &m_all);
+  if (level != 0) {  // for the next digit
+    *reinterpret_cast<Pack<uint64_t, 8>*>(w.high + mine_at) = Pack<uint64_t, 8>{};
+    *reinterpret_cast<Pack<uint64_t, 8>*>(w.low + mine_at) = Pack<uint64_t, 8>{};
+    *reinterpret_cast<Pack<uint32_t, 8>*>(w.count + mine_at) = Pack<uint32_t, 8>{};
+  }
+  const uint64_t c = g.scan(c_mine, &c_all);
+  const double m = g.scan(m_mine, &m_all);
   if (level == 0) {
     st.above = 0.0;
     st.count_above = 0;
     if (by_mass) {
-      if (!(st.active & 2u)) st.total = ldexp((double)m_all, -w.scale);
+      if (!(st.active & 2u)) st.total = m_all;
       st.target = (double)r.top_p * st.total;
       if (r.top_p < 1.0f) st.active |= 4u;
     } else if (r.top_k > 0 && c_all > (uint64_t)r.top_k) {
@@ -904,27 +942,28 @@ __global__ __launch_bounds__(256) void pcx_sample_edge(WideArgs w, int level, in
   if (cuts) {
     // the first bin, from the top, at which the edge is reached
     uint32_t found = 0xFFFFFFFFu;
-    uint64_t c_run = c, m_run = m, c_at = 0, m_at = 0;  // ahead of the bin taken
+    uint64_t c_run = c, c_at = 0;
+    double m_run = m, m_at = 0.0;  // ahead of the bin taken
     int bin_at = -1;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      if (!(by_mass ? masses[i] : counts[i]) || found != 0xFFFFFFFFu) continue;
+      if (!(by_mass ? masses[i] > 0.0 : counts[i] > 0) || found != 0xFFFFFFFFu) continue;
       c_at = c_run;
       m_at = m_run;
       bin_at = BINS - 1 - ((int)threadIdx.x * 8 + i);
       c_run += counts[i];
       m_run += masses[i];
-      const bool reached = by_mass ? st.above + ldexp((double)m_run, -w.scale) >= st.target : st.count_above + c_run >= (uint64_t)r.top_k;
+      const bool reached = by_mass ? st.above + m_run >= st.target : st.count_above + c_run >= (uint64_t)r.top_k;
       if (reached) found = threadIdx.x;
     }
     uint32_t who = g.min(found);
-    // (sums of fixed-point weights can miss the target by their rounding: then the lowest bin that holds anything)
+    // (sums over parts can miss the target by their rounding: then the lowest bin that holds anything)
     const uint32_t lowest = g.max(bin_at >= 0 ? threadIdx.x : 0u);
     if (who == 0xFFFFFFFFu) who = lowest;
     const bool mine = who == threadIdx.x && bin_at >= 0;
     if (mine) {
       next.count_above = st.count_above + c_at;
-      next.above = st.above + ldexp((double)m_at, -w.scale);
+      next.above = st.above + m_at;
       next.prefix = (level == 0 ? 0u : st.prefix) | ((uint32_t)bin_at << digit_shift<DT>(level));
       if (level == LEVELS<DT> - 1) {
         const double tie = weight_of(value_of<DT>(next.prefix), value_of<DT>(best_key), 1.0 / (double)r.temperature);
@@ -1296,7 +1335,7 @@ int wide_slices(int actions) { return (actions + SLICE - 1) / SLICE; }
 uint64_t wide_bytes(int64_t n, int actions) {
   if (actions <= ROW_IN_GROUP) return 0;
   const uint64_t rows = (uint64_t)(n < WIDE_BATCH ? n : WIDE_BATCH);
-  return rows * (sizeof(RowState) + 2ull * BINS * 12 + (uint64_t)wide_slices(actions) * sizeof(Slot)) + 1024;
+  return rows * (sizeof(RowState) + 2ull * BINS * 20 + (uint64_t)wide_slices(actions) * sizeof(Slot)) + 1024;
 }
 // A row of logits is divided among workgroups where there are too few rows to fill the chip.
 int log_prob_slices(int64_t n, int actions) { return actions > 2 * SLICE && n < 2048 ? wide_slices(actions) : 1; }
@@ -1311,9 +1350,10 @@ int sample_wide(const SampleArgs& a, void* workspace, hipStream_t st) {
     w.row0 = row0;
     w.batch = (int32_t)(a.rows.n - row0 < WIDE_BATCH ? a.rows.n - row0 : WIDE_BATCH);
     w.slices = slices;
-    w.scale = 62 - log2a;
+    w.scale = 63 - log2a;
     uint8_t* p = reinterpret_cast<uint8_t*>(workspace);
-    w.mass = reinterpret_cast<uint64_t*>(p); p += (size_t)w.batch * 2 * BINS * 8;
+    w.high = reinterpret_cast<uint64_t*>(p); p += (size_t)w.batch * 2 * BINS * 8;
+    w.low = reinterpret_cast<uint64_t*>(p); p += (size_t)w.batch * 2 * BINS * 8;
     w.state = reinterpret_cast<RowState*>(p); p += (size_t)w.batch * sizeof(RowState);
     w.slots = reinterpret_cast<Slot*>(p); p += (size_t)w.batch * slices * sizeof(Slot);
     w.count = reinterpret_cast<uint32_t*>(p);
@@ -1323,10 +1363,11 @@ int sample_wide(const SampleArgs& a, void* workspace, hipStream_t st) {
     const bool k = a.rules.top_k_row || (a.rules.top_k > 0 && a.rules.top_k < a.rows.actions);
     const bool p_ = a.rules.top_p_row || a.rules.top_p < 1.0f;
     if (k || p_) {
-      hipLaunchKernelGGL((pcx_sample_digit<DT>), grid, block, 0, st, w, 0, 0u, k);
+      hipLaunchKernelGGL((pcx_sample_digit<DT, FIRST>), grid, block, 0, st, w, 0, k);
       for (int by_mass = k ? 0 : 1; by_mass <= (p_ ? 1 : 0); ++by_mass)
         for (int level = 0; level < LEVELS<DT>; ++level) {
-          if (level) hipLaunchKernelGGL((pcx_sample_digit<DT>), grid, block, 0, st, w, level, by_mass ? 4u : 2u, !by_mass);
+          if (level && by_mass) hipLaunchKernelGGL((pcx_sample_digit<DT, BY_MASS>), grid, block, 0, st, w, level, 0);
+          else if (level) hipLaunchKernelGGL((pcx_sample_digit<DT, BY_COUNT>), grid, block, 0, st, w, level, 1);
           hipLaunchKernelGGL((pcx_sample_edge<DT>), rows, block, 0, st, w, level, by_mass);
         }
     }

@@ -632,3 +632,35 @@ def test_log_prob_refuses_forward_mode_and_function_transforms():
                     lambda: torch.func.vmap(f)(torch.stack([x] * 2)), lambda: torch.func.vjp(f, x)):
     with pytest.raises(RuntimeError):
       transform()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('dtype', DTYPES)
+@pytest.mark.parametrize('log2a,bits', [(20, 43.5), (20, 46.0), (22, 41.5), (24, 39.25), (24, 50.0)])
+def test_sample_long_tails(log2a, bits, dtype):
+  """One action and 2^log2a - 1 equal ones of about 2^-bits of its weight each, itself the last one: what of the tail top_p
+  keeps, counted in 64 bits.  u = 0 then takes the first action if any of the tail is kept, a number halfway through the
+  kept tail's part of the total the action there."""
+  a = 1 << log2a
+  best = torch.tensor(0.0)
+  low = float(torch.tensor(-bits * math.log(2.0)).to(getattr(torch, dtype)))
+  w = math.exp(low)
+  tail = (a - 1) * w
+  total = 1.0 + tail
+  x = torch.full((1, a), low).to(getattr(torch, dtype))
+  x[0, a - 1] = best
+  x = x.cuda()
+  for k in range(1, 6):
+    p = 1.0 - k * 2.0 ** -24  # (exact in float32)
+    need = (p * total - 1.0) / w  # how many of the tail it takes
+    if abs(need) < 64 or abs(need - (a - 1)) < 64:
+      continue  # (on the border: the sums of the 64-bit formula are not that good)
+    kept = 0 if need < 0 else min(a - 1, math.ceil(need))
+    got = int(policy.sample(x, torch.zeros(1).cuda(), top_p=p).cpu())
+    assert got == (0 if kept else a - 1), (k, kept, got)
+    if not kept:
+      continue
+    u = float(np.float32(0.5 * kept * w / (1.0 + kept * w)))
+    at = u * (1.0 + kept * w) / w
+    got = int(policy.sample(x, torch.tensor([u]).cuda(), top_p=p).cpu())
+    assert abs(got - at) <= 1.0 + at * 2.0 ** -30, (k, kept, got, at)
