@@ -589,6 +589,10 @@ __global__ __launch_bounds__(THREADS < 256 ? 256 : THREADS, EP <= 8 ? 5 : EP == 
 // top_k 40 and top_p take 26 us where the divided rows' launches below take 136, one row of 131,072 float32 ones 44 (62), of
 // 262,144 82 (63), 64 rows of those 95 (149).
 constexpr int TOP_THREADS = 512, TOP_EP = 16;
+// Is this such a row?  By the row's own rules, however they were given, so that a row's answer does not depend on the others.
+__host__ __device__ __forceinline__ bool keeps_few(float temperature, int32_t top_k) {
+  return !(temperature > 0.0f) || (top_k > 0 && top_k <= TOP_THREADS / 2);
+}
 template <int DT>
 __global__ __launch_bounds__(TOP_THREADS, 4) void pcx_sample_top(SampleArgs a) {
   constexpr int FEW = 512, WAVES = TOP_THREADS / 64, TURN = TOP_THREADS * TOP_EP;
@@ -598,6 +602,7 @@ __global__ __launch_bounds__(TOP_THREADS, 4) void pcx_sample_top(SampleArgs a) {
   Group<64> one{nullptr, (int)(threadIdx.x & 63), 0};
   const int64_t row = blockIdx.x;
   const RowRules r = rules_of(a.rules, row);
+  if (!keeps_few(r.temperature, r.top_k)) return;
   const int A = a.rows.actions;
   uint32_t key[TOP_EP];
   // key[] of every turn of neighbouring elements, in index order
@@ -747,6 +752,7 @@ struct WideArgs {
   uint32_t* count;
   Slot* slots;                 // [rows][slices]
   int32_t batch;
+  int32_t others;              // rows that keep few are pcx_sample_top's
 };
 // The digits of a key, from the top: 11, 11 and 10 bits of 32; 11 and 5 of bfloat16's 16, 11 and 8 of float16's 19.
 template <int DT> constexpr int LEVELS = DT == PCX_F32 ? 3 : 2;
@@ -792,6 +798,10 @@ __global__ __launch_bounds__(256) void pcx_sample_best(WideArgs w) {
   __shared__ Group<256>::Scratch scratch;
   Group<256> g{&scratch, (int)threadIdx.x, 0};
   const int row = blockIdx.y, lo = blockIdx.x * SLICE;
+  if (w.others) {
+    const RowRules r = rules_of(w.a.rules, w.row0 + row);
+    if (keeps_few(r.temperature, r.top_k)) return;  // (no best: the next launches pass the row over)
+  }
   uint32_t key[WEP];
   load_slice<DT>(w, row, lo, key);
   uint32_t top = 0, at = 0xFFFFFFFFu;
@@ -1027,6 +1037,7 @@ __global__ __launch_bounds__(256) void pcx_sample_pick(WideArgs w) {
   const RowState st = w.state[row];
   const RowRules r = rules_of(w.a.rules, at);
   const uint32_t best_key = (uint32_t)(st.best >> 32);
+  if (w.others && keeps_few(r.temperature, r.top_k)) return;
   if (!best_key || !(r.temperature > 0.0f)) {
     if (threadIdx.x == 0) w.a.out[at] = best_key ? (int)~(uint32_t)st.best : NONE;
     return;
@@ -1341,7 +1352,7 @@ uint64_t wide_bytes(int64_t n, int actions) {
 int log_prob_slices(int64_t n, int actions) { return actions > 2 * SLICE && n < 2048 ? wide_slices(actions) : 1; }
 
 template <int DT>
-int sample_wide(const SampleArgs& a, void* workspace, hipStream_t st) {
+int sample_wide(const SampleArgs& a, bool others, void* workspace, hipStream_t st) {
   const int slices = wide_slices(a.rows.actions);
   int log2a = 0;
   while ((1 << log2a) < a.rows.actions) ++log2a;
@@ -1351,6 +1362,7 @@ int sample_wide(const SampleArgs& a, void* workspace, hipStream_t st) {
     w.batch = (int32_t)(a.rows.n - row0 < WIDE_BATCH ? a.rows.n - row0 : WIDE_BATCH);
     w.slices = slices;
     w.scale = 63 - log2a;
+    w.others = others;
     uint8_t* p = reinterpret_cast<uint8_t*>(workspace);
     w.high = reinterpret_cast<uint64_t*>(p); p += (size_t)w.batch * 2 * BINS * 8;
     w.low = reinterpret_cast<uint64_t*>(p); p += (size_t)w.batch * 2 * BINS * 8;
@@ -1379,10 +1391,16 @@ int sample_wide(const SampleArgs& a, void* workspace, hipStream_t st) {
 template <int DT>
 int sample_type(const SampleArgs& all, void* workspace, hipStream_t st) {
   const int A = all.rows.actions;
-  // (By the actions alone, not by how many rows there are: a row's answer must not depend on its batch.)
-  const bool few = (!all.rules.top_k_row && all.rules.top_k > 0 && all.rules.top_k <= TOP_THREADS / 2) || (!all.rules.temperature_row && all.rules.temperature == 0.0f);
-  const bool top = A > ROW_IN_GROUP && few && A <= ROW_ALONE;
-  if (A > ROW_IN_GROUP && !top) return sample_wide<DT>(all, workspace, st);
+  // (Which way a row goes, its actions and its own rules say, not how many rows there are: its answer must not depend on them.)
+  bool top = false;
+  if (A > ROW_IN_GROUP) {
+    const Rules& r = all.rules;
+    const bool every = keeps_few(r.temperature_row ? 1.0f : r.temperature, r.top_k_row ? 0 : r.top_k);  // whatever the rows' own rules say
+    top = A <= ROW_ALONE && (every || r.temperature_row || r.top_k_row);
+    if (!top || !every)
+      if (int rc = sample_wide<DT>(all, top, workspace, st)) return rc;
+    if (!top) return 0;
+  }
   for (int64_t row0 = 0; row0 < all.rows.n; row0 += CHUNK) {
     SampleArgs a = all;
     a.rows = rows_from(all.rows, row0, elem_size(DT));

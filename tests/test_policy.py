@@ -664,3 +664,31 @@ def test_sample_long_tails(log2a, bits, dtype):
     at = u * (1.0 + kept * w) / w
     got = int(policy.sample(x, torch.tensor([u]).cuda(), top_p=p).cpu())
     assert abs(got - at) <= 1.0 + at * 2.0 ** -30, (k, kept, got, at)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('a', [16385, 33380, 131072, 262144, 300000])
+def test_sample_rules_as_numbers_and_as_rows_agree(a):
+  """The same rule as a number and as an array row by row: the same actions, whichever kernels they take."""
+  n = 8
+  for dtype in DTYPES:
+    x, u = logits_of(n, a, dtype, a)
+    x[1] = -40.0
+    x[1, a - 1] = 0.0  # a long tail
+    x[2] = 0.5
+    x, u = x.cuda(), u.cuda()
+    u[1] = 0.0
+    for rule in (dict(top_k=1), dict(top_k=40, top_p=0.9), dict(top_k=256, top_p=1 - 2.0 ** -24), dict(top_k=257, top_p=1 - 2.0 ** -24), dict(top_k=a // 2, top_p=0.95),
+                 dict(top_p=1 - 2.0 ** -23), dict(temperature=0.0), dict(temperature=0.7, top_k=40, min_p=0.01), dict(min_p=0.001)):
+      want = policy.sample(x, u, **rule)
+      rows = {k: torch.full((n,), v, dtype=torch.int32 if k == 'top_k' else torch.float32).cuda() for k, v in rule.items()}
+      assert torch.equal(policy.sample(x, u, **rows), want), rule
+      for k in rule:
+        assert torch.equal(policy.sample(x, u, **dict(rule, **{k: rows[k]})), want), (rule, k)
+      assert torch.equal(policy.sample(x[1:4], u[1:4], **rule), want[1:4])
+    # rules of both kinds in one batch
+    ks = torch.tensor([1, 40, 0, 256, 257, a, 3, 0], dtype=torch.int32).cuda()
+    ts = torch.tensor([1.0, 0.7, 1.0, 0.5, 1.0, 1.0, 0.0, 0.0]).cuda()
+    got = policy.sample(x, u, top_k=ks, temperature=ts, top_p=0.9)
+    for i in range(n):
+      assert got[i] == policy.sample(x[i:i + 1], u[i:i + 1], top_k=int(ks[i]), temperature=float(ts[i]), top_p=0.9)[0], i
