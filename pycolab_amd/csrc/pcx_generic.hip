@@ -82,8 +82,8 @@ static std::string spec_header(const Consts& k, const std::vector<uint32_t>& tab
 // table-driven build (same results, PCX_DEBUG & 16 prints why); pcx_engine_launch_shape tells which one runs (30 / 31).
 namespace rtc {
 
-static const char* const OPTIONS[] = {"--offload-arch=gfx950", "-O3", "-std=c++17", "-DPCX_GENERIC_SPEC=\"pcx_generic_spec.h\""};
-constexpr int N_OPTIONS = 4;
+static const char* const OPTIONS[] = {"--offload-arch=gfx950", "-O3", "-std=c++17", PCX_RTC_NO_PACKED_FP32, "-DPCX_GENERIC_SPEC=\"pcx_generic_spec.h\""};
+constexpr int N_OPTIONS = sizeof OPTIONS / sizeof OPTIONS[0];
 
 static const char* const TU = "#include \"pcx_generic_kernel.h\"\n";
 static const pcx::rtc::Program PROGRAM = {RTC_NAMES, RTC_SOURCES, RTC_COUNT, TU, "pcx_generic_spec.hip", OPTIONS, N_OPTIONS, "pcx_generic_spec.h", "pcx_generic", "pcx generic"};

@@ -18,6 +18,9 @@
 
 #include <hip/hip_runtime.h>
 
+// Among every program's options, as in the Makefile: no packed FP32 arithmetic (some of its forms are not reliable on this part).
+#define PCX_RTC_NO_PACKED_FP32 "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"
+
 namespace pcx {
 namespace rtc {
 

@@ -55,9 +55,9 @@ namespace sm {
 // persistent shape on a run-time build.
 namespace jit {
 
-static const char* const OPTIONS[] = {"--offload-arch=gfx950", "-O3", "-std=c++17", "-DPCX_SM_SPEC=\"pcx_sm_spec.h\""};
+static const char* const OPTIONS[] = {"--offload-arch=gfx950", "-O3", "-std=c++17", PCX_RTC_NO_PACKED_FP32, "-DPCX_SM_SPEC=\"pcx_sm_spec.h\""};
 static const char* const TU = "#include \"pcx_scrolly_maze_kernel.h\"\n";
-static const rtc::Program PROGRAM = {RTC_NAMES, RTC_SOURCES, RTC_COUNT, TU, "pcx_sm_spec.hip", OPTIONS, 4, "pcx_sm_spec.h", "pcx_scrolly_maze", "pcx scrolly_maze"};
+static const rtc::Program PROGRAM = {RTC_NAMES, RTC_SOURCES, RTC_COUNT, TU, "pcx_sm_spec.hip", OPTIONS, sizeof OPTIONS / sizeof OPTIONS[0], "pcx_sm_spec.h", "pcx_scrolly_maze", "pcx scrolly_maze"};
 
 // The header a run-time build includes: the Consts as the persistent shape launches them and as init() leaves them, as words
 // (tools/gen_sm_shipped.py writes pcx_sm_shipped.h the same way).  `persistent_ok`: the persistent shape can take this

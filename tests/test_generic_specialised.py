@@ -261,3 +261,29 @@ def test_a_damaged_cache_entry_is_recompiled(monkeypatch, tmp_path):
   hip.reset()
   assert shape_of(hip) == 31
   assert os.path.getsize(tmp_path / entry) == good
+
+
+def test_run_time_builds_have_no_packed_float32_arithmetic(tmp_path, monkeypatch):
+  """As the library's own build (csrc/Makefile): a kernel that the compiler would give v_pk_fma_f32, built along with
+  the specialised one, and the run-time instances themselves, have none."""
+  import subprocess
+  objdump = '/opt/rocm/llvm/bin/llvm-objdump'
+  if not os.path.exists(objdump):
+    pytest.skip('no disassembler')
+  probe = tmp_path / 'probe.h'
+  probe.write_text('extern "C" __global__ void packed_probe(float2* a, const float2* b) { float2 x = a[threadIdx.x], y = b[threadIdx.x]; '
+                   'x.x = x.x * y.x + 1.0f; x.y = x.y * y.y + 1.0f; a[threadIdx.x] = x; }\n')
+  cache = tmp_path / 'cache'
+  monkeypatch.setenv('PCX_JIT_CACHE', str(cache))
+  log, n = ctypes.create_string_buffer(8192), ctypes.c_int64(0)
+  for extra, name, what in (('-include ' + str(probe), 'warehouse_L0', N.lib().pcx_generic_specialise_check), ('', 'marauders', N.lib().pcx_generic_specialise_check),
+                            ('', 'scrolly_custom_H', N.lib().pcx_scrolly_maze_specialise_check)):
+    monkeypatch.setenv('PCX_GENERIC_SPEC_DEFS', extra)
+    ct, keep = helpers.load_template(name).to_ctypes()
+    assert what(ctypes.byref(ct), log, len(log), ctypes.byref(n)) == 0, log.value.decode()[:2000]
+  built = [f for f in os.listdir(cache) if f.endswith('.hsaco')]
+  assert len(built) == 3
+  texts = [subprocess.run([objdump, '-d', str(cache / f)], capture_output=True, text=True, check=True).stdout for f in built]
+  assert sum('packed_probe' in t for t in texts) == 1
+  for f, text in zip(built, texts):
+    assert 'v_pk_add_f32' not in text and 'v_pk_mul_f32' not in text and 'v_pk_fma_f32' not in text, f
