@@ -756,3 +756,71 @@ def test_forward_mode_and_function_transforms_are_refused():
                     lambda: torch.func.vmap(f)(torch.stack([given[0]] * 2)), lambda: torch.func.vjp(f, given[0])):
     with pytest.raises(RuntimeError):
       transform()
+
+
+# Boards and hidden units that reach every instance of the product's kernel (a wave's tiles of boards x hidden units, the
+# workgroup's waves along them, and whether the cells are divided: a plan without a workspace is undivided).  450 units are 15
+# tiles, 50 are two; 35 cells are two quads.
+TILES = [(300, 450, True),     # 1 x 1, one wave x four
+         (700, 450, True),     # 2 x 2, two waves x two
+         (700, 50, True),      # 2 x 2, four waves x one
+         (16300, 450, True),   # 4 x 2, two waves x two: 64 x 4 workgroups of 256 boards
+         (16500, 450, False),  # ... 65 x 4
+         (24700, 450, False),  # 4 x 2, four waves x two: 98,304 boards of four tiles each and more
+         (130600, 50, True),   # 4 x 2, four waves x one: 256 workgroups of 512 boards
+         (131200, 50, False)]  # ... 257
+STACKED_TILES = [(700, 450, True), (5000, 450, False), (700, 50, True), (33000, 50, False)]  # 1 x 2, four waves x two and x one
+
+
+def check_on_device(n, layers, rows, cols, hidden, dtype, act, seed, stacked=False, divided=None, train=True):
+  """As check(), with the formulas in 64 bits on the device."""
+  chars, boards, weight, bias, residual = make(n, layers, rows, cols, hidden, dtype, seed, stacked, grid=act == 'relu')
+  if divided is not None:
+    d = desc(n=n, row_stride=boards[0].numel(), cells=rows * cols, n_layers=layers, hidden=hidden, stacked=int(stacked),
+             dtype={'float32': N.F32, 'float16': N.F16, 'bfloat16': N.BF16}[dtype])
+    for i, c in enumerate(chars):
+      d.chars[i] = ord(c)
+    assert (sizes(d)[1][1] > 0) == divided
+  boards, weight, bias, residual = (t.cuda() for t in (boards, weight, bias, residual))
+  y, tol, slope64, slope_tol = reference(chars, boards, weight, bias, act, residual)
+  got = rendering.ObservationProjection(chars, weight, bias, activation=act)(boards, residual=residual)
+  near(got, y.cpu(), tol.cpu(), 'forward')
+  out, slope = rendering.project(boards, chars, weight, bias, activation=act, residual=residual, return_slope=True)
+  assert torch.equal(out, got)
+  if slope is not None:
+    # (besides: silu's 1 - s is off by some 2 * 2^-24, which |z|, here below 10, multiplies)
+    near(slope, slope64.cpu(), (slope_tol + 24 * 2.0 ** -24).expand_as(slope64).cpu(), 'slope')
+  if not train:
+    return
+  grad = torch.randn(n, hidden, generator=torch.Generator().manual_seed(seed + 1)).to(weight.dtype).cuda()
+  dw, db = rendering.project_backward(boards, chars, weight, grad, slope, activation=act)
+  x, eps, tiny = features(chars, boards), torch.finfo(weight.dtype).eps, torch.finfo(weight.dtype).tiny
+  dz = grad.double() * slope64
+  off = grad.double().abs() * slope_tol + eps * (dz.abs() + grad.double().abs() * slope_tol) + tiny * eps
+  for g, left, what in ((dw.flatten(1), x, 'grad weight'), (db[:, None], torch.ones(n, 1, dtype=torch.float64, device='cuda'), 'grad bias')):
+    want = dz.t() @ left
+    tol = off.t() @ left + (n + 2) * 2.0 ** -23 * (dz.abs().t() @ left)
+    near(g, want.cpu(), (tol + eps / 2 * (want.abs() + tol) + tiny * eps).cpu(), what)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('dtype', DTYPES)
+@pytest.mark.parametrize('layers,act', [(3, 'silu'), (8, 'relu'), (11, 'tanh'), (16, 'gelu'), (20, None)])
+@pytest.mark.parametrize('n,hidden,divided', TILES)
+def test_every_tile_shape(n, hidden, divided, layers, act, dtype):
+  check_on_device(n, layers, 5, 7, hidden, dtype, act, 40, divided=divided)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('dtype', DTYPES)
+@pytest.mark.parametrize('n,hidden,divided', STACKED_TILES)
+def test_every_tile_shape_of_stacked_layers(n, hidden, divided, dtype):
+  for layers, act in ((1, 'gelu'), (7, 'relu'), (8, 'tanh'), (11, None), (12, 'silu')):
+    check_on_device(n, layers, 5, 7, hidden, dtype, act, 41, stacked=True, divided=divided)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('dtype,n,layers,rows,cols,hidden', [('float32', 2048, 7, 45, 89, 200), ('bfloat16', 8192, 14, 16, 30, 512)])
+def test_weights_beyond_the_cache(dtype, n, layers, rows, cols, hidden):
+  """50 GB and more of boards times the weight's bytes: eight waves, the cells divided."""
+  check_on_device(n, layers, rows, cols, hidden, dtype, 'gelu', 42, divided=True)
