@@ -150,6 +150,13 @@ def pointer(tensor):
   return None if tensor is None else tensor.data_ptr()
 
 
+def raw_stream(device_id):
+  """`device_id`'s current stream, as the C ABI takes it."""
+  if _raw_stream is None:
+    _find_stream()
+  return _raw_stream(device_id)
+
+
 def launch(device_id, function, *args):
   """function(*args, stream) of the C ABI on `device_id`'s current stream."""
   if _raw_stream is None:

@@ -835,8 +835,8 @@ class ObservationProjection(object):
   [n, len(layers), rows, cols] of stacked layers, and returns [n, hidden] of the weight's type (a batch-1 Observation:
   [hidden]).  `residual`: [n, hidden] or None.  Boards whose layers are `board == character` (the default engine) are
   read as characters; with `occlusion_in_layers=False` the layer planes are read.  Characters of a board that are not
-  among `layers` count nowhere.  Sums are float32.  Nothing waits for the device, so a call can be captured into a graph;
-  gradients are `project()`'s business."""
+  among `layers` count nowhere.  Sums are float32.  Nothing waits for the device, so a call can be captured into a graph
+  (keep this object as long as the graph); gradients are `project()`'s business."""
 
   def __init__(self, layers, weight, bias=None, activation=None):
     self._activation = activation
@@ -845,6 +845,7 @@ class ObservationProjection(object):
     self._weight = weight.detach().clone()
     self._bias = None if bias is None else bias.detach().clone()
     self._packs = {}
+    self._streams = set()  # (stacked, stream) that a laid-out weight has been used on
     self._lay_out(0)
 
   def _lay_out(self, stacked):
@@ -882,6 +883,14 @@ class ObservationProjection(object):
     stacked = int(boards.offsets is not None)
     if stacked not in self._packs:
       self._lay_out(stacked)
+    used = stacked, dev.raw_stream(self._plan.device.index)
+    if used not in self._streams:
+      # (their memory is not given to others, when this object goes, before that stream has passed the calls made on it)
+      stream = dev.torch_module().cuda.current_stream(self._plan.device)
+      for kept in (self._packs[stacked], self._bias):
+        if kept is not None:
+          kept.record_stream(stream)
+      self._streams.add(used)
     out, _ = self._plan.forward(desc, boards, self._packs[stacked], self._bias, None if residual is None else residual.detach())
     return out[0] if boards.single else out
 

@@ -824,3 +824,29 @@ def test_every_tile_shape_of_stacked_layers(n, hidden, divided, dtype):
 def test_weights_beyond_the_cache(dtype, n, layers, rows, cols, hidden):
   """50 GB and more of boards times the weight's bytes: eight waves, the cells divided."""
   check_on_device(n, layers, rows, cols, hidden, dtype, 'gelu', 42, divided=True)
+
+
+@pytest.mark.gpu
+def test_a_projection_dropped_while_another_stream_uses_it():
+  """Its laid-out weight must not become another tensor's memory before that stream has read it."""
+  chars, boards, weight, bias, residual = make(700, 8, 10, 30, 96, 'bfloat16', 51)
+  b, r = boards.cuda(), residual.cuda()
+  for stacked in (False, True):
+    x = torch.stack([(b == ord(c)) for c in chars], 1) if stacked else b
+    want = rendering.project(x, chars, weight.cuda(), bias.cuda(), activation='tanh', residual=r)
+    proj = rendering.ObservationProjection(chars, weight.cuda(), bias.cuda(), activation='tanh')
+    proj(x)
+    side, busy = torch.cuda.Stream(), torch.cuda.Event()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+      torch.cuda._sleep(200_000_000)  # (some tens of milliseconds and more)
+      got = proj(x, residual=r)
+      busy.record()
+    held = [(t.data_ptr(), t.numel() * t.element_size()) for t in (proj._packs[int(stacked)], proj._bias)]  # (what that call reads)
+    del proj
+    taken = [torch.empty(size, dtype=torch.uint8, device='cuda').fill_(255) for _, size in held for _ in range(3)]
+    assert not busy.query(), 'the other stream was through too early to tell'
+    for ptr, size in held:
+      assert not any(t.data_ptr() < ptr + size and ptr < t.data_ptr() + t.numel() for t in taken)
+    torch.cuda.synchronize()
+    assert torch.equal(got, want)
