@@ -90,7 +90,8 @@ def sample(logits, uniforms, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, leg
   `temperature` 0 takes the best action.  Each of the four is a number or a device array [n] (float32; `top_k` int32), row by
   row.  A row that allows nothing gives `_native.ACTION_NONE` (-1), the engine's `None`.
 
-  `out`: an int32 tensor [n] to write into.  Nothing waits for the device; calls can be captured into a graph."""
+  `out`: an int32 tensor [n] to write into (autograd counts it as a change in place: a backward pass that needs its old values
+  is refused; of a replayed graph's writes it does not know).  Nothing waits for the device; calls can be captured into a graph."""
   torch = dev.require_torch('sample()')
   desc, legal, n, _, index = _rows(torch, logits, legal)
   device = logits.device
@@ -108,7 +109,8 @@ def sample(logits, uniforms, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, leg
   rules = N.SAMPLING.pack(0.0 if t_row is not None else float(temperature), 0.0 if p_row is not None else float(top_p),
                           0.0 if m_row is not None else float(min_p), 0 if k_row is not None else top_k,
                           dev.pointer(t_row) or 0, dev.pointer(k_row) or 0, dev.pointer(p_row) or 0, dev.pointer(m_row) or 0)
-  if out is None:
+  given = out is not None
+  if not given:
     out = torch.empty((n,), dtype=torch.int32, device=device)
   elif out.dtype != torch.int32 or out.device != device or tuple(out.shape) != (n,) or not out.is_contiguous():
     raise ValueError('out must be a contiguous int32 tensor [{}] on {}'.format(n, device))
@@ -116,6 +118,8 @@ def sample(logits, uniforms, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, leg
   scratch, size = dev.workspace('pcx_sample_size', desc, device)
   dev.launch(index, N.lib().pcx_sample_actions, desc, rules, logits.data_ptr(), dev.pointer(legal), uniforms.data_ptr(), out.data_ptr(),
              dev.pointer(scratch), size)
+  if given:  # (a log_prob() of the actions that lay there may still wait for its backward pass)
+    torch.autograd.graph.increment_version(out)
   return out
 
 

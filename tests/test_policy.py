@@ -692,3 +692,26 @@ def test_sample_rules_as_numbers_and_as_rows_agree(a):
     got = policy.sample(x, u, top_k=ks, temperature=ts, top_p=0.9)
     for i in range(n):
       assert got[i] == policy.sample(x[i:i + 1], u[i:i + 1], top_k=int(ks[i]), temperature=float(ts[i]), top_p=0.9)[0], i
+
+
+@pytest.mark.gpu
+def test_backward_after_the_actions_were_drawn_anew_is_refused():
+  """A buffer of actions that sample(out=...) writes again before the gradient of the old ones' log-probability."""
+  x, u = logits_of(40, 9, 'float32', 60)
+  leaf, u = x.cuda().requires_grad_(), u.cuda()
+  taken = torch.empty(40, dtype=torch.int32, device='cuda')
+  policy.sample(leaf, u, out=taken)
+  lp, _ = policy.log_prob(leaf, taken)
+  policy.sample(leaf, u.flip(0), out=taken)
+  with pytest.raises(RuntimeError, match='modified by an inplace operation'):
+    lp.sum().backward()
+  with pytest.raises(RuntimeError, match='modified by an inplace operation'):  # a part of it is it, too
+    both = policy.log_prob(leaf, taken)[0]
+    policy.sample(leaf[:3], u[:3], out=taken[:3])
+    both.sum().backward()
+  policy.log_prob(leaf, taken)[0].sum().backward()
+  want = policy.log_prob_backward(leaf, taken, *policy.log_prob(leaf, taken, return_stats=True)[1:], torch.ones(40, device='cuda'))
+  assert torch.equal(leaf.grad, want)
+  with torch.inference_mode():  # (a tensor of no version)
+    held = torch.empty(40, dtype=torch.int32, device='cuda')
+    assert torch.equal(policy.sample(x.cuda(), u, out=held), policy.sample(x.cuda(), u))
