@@ -151,6 +151,12 @@ def _log_prob_backward(torch, desc, legal, logits, actions, temperature, entropy
   return grad
 
 
+def _layout(logits, actions, legal, entropy, stats):
+  """Where and how the arrays of a backward pass lie: what the forward pass's description of them goes by."""
+  return (logits.data_ptr(), logits.dtype, logits.shape, logits.stride(), None if legal is None else (legal.data_ptr(), legal.stride()), actions.data_ptr(),
+          entropy.data_ptr(), stats.data_ptr())
+
+
 _log_prob_function = None
 
 
@@ -167,7 +173,7 @@ def _log_prob_autograd():
       def forward(ctx, logits, actions, legal, temperature, desc):
         ctx.set_materialize_grads(False)
         log_prob, entropy, stats = _log_prob_forward(torch, desc, legal, logits, actions, temperature)
-        ctx.desc, ctx.temperature = desc, temperature
+        ctx.desc, ctx.temperature, ctx.layout = desc, temperature, _layout(logits, actions, legal, entropy, stats)
         ctx.save_for_backward(logits, actions, legal, entropy, stats)
         return log_prob, entropy
 
@@ -178,6 +184,11 @@ def _log_prob_autograd():
         logits, actions, legal, entropy, stats = ctx.saved_tensors
         if grad_log_prob is None and grad_entropy is None:
           return None, None, None, None, None
+        if _layout(logits, actions, legal, entropy, stats) != ctx.layout:
+          # (what was saved went elsewhere meanwhile -- torch.autograd.graph.saved_tensors_hooks, checkpoint -- and what came
+          # back is laid out in its own way)
+          return (log_prob_backward(logits, actions, entropy, stats, grad_log_prob, grad_entropy, legal, ctx.temperature), None, None, None,
+                  None)
         return (_log_prob_backward(torch, ctx.desc, legal, logits, actions, ctx.temperature, entropy, stats, grad_log_prob, grad_entropy),
                 None, None, None, None)
 

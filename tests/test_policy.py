@@ -715,3 +715,38 @@ def test_backward_after_the_actions_were_drawn_anew_is_refused():
   with torch.inference_mode():  # (a tensor of no version)
     held = torch.empty(40, dtype=torch.int32, device='cuda')
     assert torch.equal(policy.sample(x.cuda(), u, out=held), policy.sample(x.cuda(), u))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('dtype', DTYPES)
+@pytest.mark.parametrize('a', [5, 200, 3000])
+def test_log_prob_whose_saved_tensors_went_elsewhere(a, dtype):
+  """What autograd saved comes back laid out in its own way: copies on the host, a forward pass made anew."""
+  from torch.utils.checkpoint import checkpoint
+  n = 30
+  base, u = logits_of(n, 2 * a + 7, dtype, a)
+  mask = torch.rand(n, 3 * a, generator=torch.Generator().manual_seed(a)) < 0.7
+  taken = (u * a).int().cuda()
+  g = torch.randn(2, n, generator=torch.Generator().manual_seed(1)).cuda()
+  wide, legal = base.cuda(), mask.cuda()
+  for allowed in (None, legal[:, a:2 * a], legal[0, :a]):
+    view = wide[:, 5:5 + a]
+    lp, h, stats = policy.log_prob(view, taken, legal=allowed, return_stats=True)
+    want = policy.log_prob_backward(view, taken, h, stats, g[0], g[1], legal=allowed)
+
+    def grads(run):
+      leaf = wide.clone().requires_grad_()
+      out = run(lambda x: policy.log_prob(x[:, 5:5 + a], taken, legal=allowed), leaf)
+      assert torch.equal(out[0], lp) and torch.equal(out[1], h)
+      torch.autograd.backward(out, [g[0], g[1]])
+      assert not leaf.grad[:, :5].any() and not leaf.grad[:, 5 + a:].any()
+      return leaf.grad[:, 5:5 + a]
+
+    def on_the_host(f, x):
+      with torch.autograd.graph.save_on_cpu():
+        return f(x)
+
+    assert torch.equal(grads(lambda f, x: f(x)), want)
+    assert torch.equal(grads(on_the_host), want)
+    for reentrant in (False, True):
+      assert torch.equal(grads(lambda f, x: checkpoint(f, x, use_reentrant=reentrant)), want)
