@@ -683,7 +683,8 @@ class _Boards(object):
       self.n, self.rows, self.cols = int(shape[0]), int(shape[-2]), int(shape[-1])
       if (self.cols > 1 and boards.stride(-1) != 1) or (self.rows > 1 and boards.stride(-2) != self.cols):
         raise ValueError('the cells of a board must lie one after the other (rows * cols contiguous bytes)')
-      self.device_id, self.ptr, self.row_stride = boards.device.index, boards.data_ptr(), int(boards.stride(0))
+      self.strides = boards.stride()
+      self.device_id, self.ptr, self.row_stride = boards.device.index, boards.data_ptr(), int(self.strides[0])
     else:
       source = _source_of(boards)
       view, self.device_id = source._planes_view()
@@ -911,19 +912,28 @@ def _project_autograd():
       def forward(ctx, weight, bias, residual, plan, boards, desc):
         out, slope = plan.forward(desc, boards, plan.pack(desc, weight), bias, residual, want_slope=plan.activation != N.ACT_NONE)
         ctx.plan, ctx.boards, ctx.desc, ctx.weight_shape = plan, boards, desc, weight.shape
-        # (the boards are an input like any other: a write to them before backward() is noticed where they are a tensor)
-        ctx.save_for_backward(slope, boards.keep if isinstance(boards.keep, torch.Tensor) else None)
+        # (the boards are an input like any other, where they are a tensor and the weight's gradient reads them: a write to
+        # them before backward() is noticed)
+        ctx.save_for_backward(slope, boards.keep if ctx.needs_input_grad[0] and isinstance(boards.keep, torch.Tensor) else None)
         return out
 
       @staticmethod
       def backward(ctx, grad):
         if grad_enabled():
           dev.refuse_twice('project')
-        slope, _ = ctx.saved_tensors
-        want = ctx.needs_input_grad
-        if want[0]:
-          ctx.boards.check_unchanged('project')
-        dw, db = ctx.plan.backward(ctx.desc, ctx.boards, grad, slope, want[0], want[1], ctx.weight_shape)
+        slope, saved = ctx.saved_tensors
+        plan, boards, desc, want = ctx.plan, ctx.boards, ctx.desc, ctx.needs_input_grad
+        if saved is not None and (saved.data_ptr() != boards.ptr or saved.stride() != boards.strides):
+          # (what was saved went elsewhere meanwhile -- torch.autograd.graph.saved_tensors_hooks, checkpoint -- and what came
+          # back, as it was then, is laid out in its own way)
+          boards = _Boards(saved, plan.layers)
+          desc = plan.at(boards)
+          if boards.n != ctx.boards.n:
+            raise ValueError('project(): {} boards came back of {} saved'.format(boards.n, ctx.boards.n))
+        elif want[0]:
+          boards.check_unchanged('project')
+        plan.check_rows(slope, 'slope', boards.n, plan.slope_dtype())
+        dw, db = plan.backward(desc, boards, grad, slope, want[0], want[1], ctx.weight_shape)
         return dw, db, grad if want[2] else None, None, None, None
 
     _project_function = ProjectBoards

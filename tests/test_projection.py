@@ -850,3 +850,49 @@ def test_a_projection_dropped_while_another_stream_uses_it():
       assert not any(t.data_ptr() < ptr + size and ptr < t.data_ptr() + t.numel() for t in taken)
     torch.cuda.synchronize()
     assert torch.equal(got, want)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('act', ACTS)
+@pytest.mark.parametrize('stacked', [False, True])
+@pytest.mark.parametrize('dtype', DTYPES)
+def test_gradients_whose_saved_tensors_went_elsewhere(dtype, stacked, act):
+  """What autograd saved comes back laid out in its own way: copies on the host, a forward pass made anew."""
+  from torch.utils.checkpoint import checkpoint
+  n = 70
+  chars, boards, weight, bias, residual = make(n, 6, 5, 9, 40, dtype, 61, stacked)
+  many = torch.zeros((n, 3) + tuple(boards.shape[1:]), dtype=torch.uint8)  # the boards lie apart
+  many[:, 1] = boards
+  many, given, grad = many.cuda(), [t.cuda() for t in (weight, bias, residual)], torch.randn(n, 40, generator=torch.Generator().manual_seed(2)).to(weight.dtype).cuda()
+  out, slope = rendering.project(boards.cuda(), chars, given[0], given[1], activation=act, residual=given[2], return_slope=True)
+  want = rendering.project_backward(boards.cuda(), chars, given[0], grad, slope, activation=act) + (grad,)
+
+  def on_the_host(f, *leaves):
+    with torch.autograd.graph.save_on_cpu():
+      return f(*leaves)
+
+  for run, later in ((lambda f, *leaves: f(*leaves), False), (on_the_host, False), (on_the_host, True),
+                     (lambda f, *leaves: checkpoint(f, *leaves, use_reentrant=False), False),
+                     (lambda f, *leaves: checkpoint(f, *leaves, use_reentrant=True), False)):
+    held = many.clone()
+    leaves = [t.clone().requires_grad_() for t in given]
+    y = run(lambda w, b, r: rendering.project(held[:, 1], chars, w, b, activation=act, residual=r), *leaves)
+    assert torch.equal(y, out)
+    if later:  # (the copy on the host is of the boards as they were)
+      held.zero_()
+    y.backward(grad)
+    assert all(torch.equal(leaf.grad, w) for leaf, w in zip(leaves, want))
+
+
+@pytest.mark.gpu
+def test_a_frozen_weight_leaves_the_boards_free():
+  """The gradients of bias and residual read no boards: those may be written again before."""
+  chars, boards, weight, bias, residual = make(40, 5, 4, 8, 24, 'float32', 62)
+  b, w, grad = boards.cuda(), weight.cuda(), torch.ones(40, 24).cuda()
+  _, slope = rendering.project(b, chars, w, bias.cuda(), activation='tanh', return_slope=True)
+  want = rendering.project_backward(b, chars, w, grad, slope, activation='tanh')[1]
+  leaves = [bias.cuda().requires_grad_(), residual.cuda().requires_grad_()]
+  y = rendering.project(b, chars, w, leaves[0], activation='tanh', residual=leaves[1])
+  b.zero_()
+  y.backward(grad)
+  assert torch.equal(leaves[0].grad, want) and torch.equal(leaves[1].grad, grad)
