@@ -871,9 +871,10 @@ class ObservationProjection(object):
                                                                        'no' if self._bias is None else 'a'))
     _Projection(self._layers, weight, bias, self._activation)  # (checks)
     torch.cuda.synchronize(self._plan.device)  # nobody reads the old values any more
-    self._weight.copy_(weight.detach())
-    if bias is not None:
-      self._bias.copy_(bias.detach())
+    with torch.inference_mode():  # (made in it, the copies can be written nowhere else)
+      self._weight.copy_(weight)
+      if bias is not None:
+        self._bias.copy_(bias)
     for stacked in list(self._packs):
       self._lay_out(stacked)
     torch.cuda.synchronize(self._plan.device)

@@ -896,3 +896,21 @@ def test_a_frozen_weight_leaves_the_boards_free():
   b.zero_()
   y.backward(grad)
   assert torch.equal(leaves[0].grad, want) and torch.equal(leaves[1].grad, grad)
+
+
+@pytest.mark.gpu
+def test_a_projection_made_in_inference_mode_takes_new_values():
+  chars, boards, weight, bias, _ = make(40, 5, 4, 8, 24, 'bfloat16', 63)
+  b, w, c = boards.cuda(), weight.cuda(), bias.cuda()
+  with torch.inference_mode():
+    proj = rendering.ObservationProjection(chars, -w, -c, activation='silu')
+    proj(b)
+  leaf = w.clone().requires_grad_()
+  proj.load(leaf, c)
+  want = rendering.project(b, chars, w, c, activation='silu')
+  assert torch.equal(proj(b), want)
+  other = rendering.ObservationProjection(chars, -w, -c, activation='silu')
+  with torch.inference_mode():
+    other.load(w, c)
+    assert torch.equal(other(b), want)
+  assert leaf._version == 0 and torch.equal(other(b), want)
