@@ -586,8 +586,11 @@ __global__ __launch_bounds__(THREADS < 256 ? 256 : THREADS, EP <= 8 ? 5 : EP == 
 // that reach it, which go to one wave as in pcx_sample_group.  Where more than FEW do -- many equal logits -- the k-th largest
 // key of the row is searched for with a pass a step, and exactly the k elements that the rule keeps are taken.
 // Bound by the passes' loads, 16 neighbouring logits a thread in flight (32: 26 -> 30 us): 269 rows of 33,380 float16 logits with
-// top_k 40 and top_p take 26 us where the divided rows' launches below take 136, one row of 131,072 float32 ones 44 (62), of
-// 262,144 82 (63), 64 rows of those 95 (149).
+// top_k 40 and top_p take 26 us where the divided rows' launches below take 136, one row of 131,072 float32 ones 44 (65), of
+// 262,144 82 (65), 64 rows of those 94 (156); with top_k 256 ten more; the best alone
+// of 262,144 36, where divided rows of 300,000 take 16.  So the limit weighs 20 us of a few long rows against 60 of
+// many: how many there are cannot decide, since the two ways round their sums in different places and a row's answer must
+// not depend on the others.
 constexpr int TOP_THREADS = 512, TOP_EP = 16;
 // Is this such a row?  By the row's own rules, however they were given, so that a row's answer does not depend on the others.
 __host__ __device__ __forceinline__ bool keeps_few(float temperature, int32_t top_k) {
@@ -711,9 +714,9 @@ __global__ __launch_bounds__(TOP_THREADS, 4) void pcx_sample_top(SampleArgs a) {
 // ---- rows that no workgroup holds: divided among workgroups, one launch per question ------------------------------------
 //
 // The best logit; the edges of top_k and of top_p, a digit of the order key at a time; what each slice keeps; the slice and
-// the action that the number falls to.  8 x 2^20 float32 logits with top_p take 102 us in ten launches, of which one pass
+// the action that the number falls to.  8 x 2^20 float32 logits with top_p take 101 us in ten launches, of which one pass
 // over them, the floor, is 6.5: four more passes read them again (from the 256 MB cache: 7 us each if that were all), and the
-// chain of launches alone is 70 us, the time of a single row.
+// chain of launches alone is 65 us, the time of a single row.
 
 constexpr int SLICE = 8192;    // actions per workgroup
 constexpr int WEP = 32;        // ... per thread of 256, all of them in flight before the first is looked at

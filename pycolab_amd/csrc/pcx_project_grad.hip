@@ -129,9 +129,10 @@ __global__ __launch_bounds__(256) void pcx_project_turn(BackwardArgs a) {
 // feature bit of 8 consecutive boards at one cell: the boards are turned round once per stage into LDS as a word of layer
 // bits per (cell, board), from which every layer's operand is one shift and one mask.  A wave takes LW layers x half the
 // hidden units (2 layers x all units: float32 gradients of 2,048 boards of 4,005 cells 10 us slower).  65,536 boards of 300 cells x 8
-// layers x 256 units take 89 us.  The instructions alone take 47 of them (1.8 PFLOP/s): the masks' way through the LDS
-// after each barrier adds 11, dz's copies and the boards' turning, which the other workgroup's products hide in part, 26,
-// and the partial sums, as many as all registers of the card hold, 8.
+// layers x 256 units take 77 us, and 89 for some 20 ms after the GPU was idle, until its clocks have settled.  Of those 89 the
+// instructions alone take 47 (1.8 PFLOP/s): the masks' way through the LDS after each barrier adds 11, dz's copies and the
+// boards' turning, which the other workgroup's products hide in part, 26, and the partial sums, as many as all registers of
+// the card hold, 8.
 // Blocks of dz in LDS, one in use: three where that leaves room for two workgroups a CU, else two (dz in two or three parts;
 // one workgroup with three instead: 2,048 boards of 4,005 cells, float32 gradients 130 us against 105, 65,536 of 300 with
 // gelu and bfloat16 ones 216 against 166, the turning and joining included).

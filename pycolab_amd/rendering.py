@@ -947,8 +947,9 @@ def project(boards, layers, weight, bias=None, activation=None, residual=None, r
   one lays the weight out in every call.
 
   An Observation, its board and what a converter returned are views of arrays that the next step, crop or conversion
-  overwrites: a backward pass after that is refused; pass a copy of the board (`observation.board.clone()`).  A weight that is no finite number makes the results of
-  the boards that use it no finite numbers, and of others some.
+  overwrites: a backward pass after that is refused (where a replayed graph wrote them, nobody knows: do not); pass a copy
+  of the board (`observation.board.clone()`).  A weight that is no finite number makes the results of the boards that use it
+  no finite numbers, and of others some.
 
   `return_slope=True`: no autograd; returns (out, slope) with slope = act'(...) (None without an activation), what
   `project_backward` takes -- the pair to capture into a graph."""
