@@ -750,3 +750,42 @@ def test_log_prob_whose_saved_tensors_went_elsewhere(a, dtype):
     assert torch.equal(grads(on_the_host), want)
     for reentrant in (False, True):
       assert torch.equal(grads(lambda f, x: checkpoint(f, x, use_reentrant=reentrant)), want)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('n,a', [((1 << 22) + 37, 3), ((1 << 22) + 37, 16), ((1 << 22) + 37, 20), (1024 + 37, 16500), (1024 + 37, 270000)])
+def test_more_rows_than_one_launch_takes(n, a):
+  """The rows behind the first 2^22 (1,024 of more than 16,384 actions) give what they give by themselves."""
+  dtype = torch.bfloat16 if a > 100 else torch.float32
+  g = torch.Generator(device='cuda').manual_seed(a)
+  x = torch.randn(n, a, generator=g, device='cuda', dtype=dtype).mul_(2)
+  u, legal = torch.rand(n, generator=g, device='cuda'), torch.rand(n, a, generator=g, device='cuda', dtype=dtype) < 0.8
+  legal[n - 3] = False
+  rules = dict(temperature=torch.rand(n, generator=g, device='cuda') + 0.5, top_k=torch.randint(0, 300, (n,), generator=g, device='cuda', dtype=torch.int32),
+               top_p=torch.rand(n, generator=g, device='cuda') * 0.3 + 0.75, min_p=torch.rand(n, generator=g, device='cuda') * 0.01)
+  rules['temperature'][1::5] = 0.0
+  g_lp, g_h = torch.randn(n, generator=g, device='cuda'), torch.randn(n, generator=g, device='cuda')
+  for kw in (dict(), dict(top_p=0.9), dict(top_k=40, temperature=0.7), rules):
+    got = policy.sample(x, u, legal=legal, **kw)
+    lp, h, stats = policy.log_prob(x, got, legal=legal, temperature=0.8, return_stats=True)
+    grad = policy.log_prob_backward(x, got, h, stats, g_lp, g_h, legal=legal, temperature=0.8)
+    for part in (slice(0, 9), slice(n - 47, n)):
+      some = {k: v[part] if isinstance(v, torch.Tensor) else v for k, v in kw.items()}
+      want = policy.sample(x[part], u[part], legal=legal[part], **some)
+      assert torch.equal(got[part], want)
+      # (log_prob may divide few long rows: other sums, so they are held against 64 bits)
+      exact, p, h64, _, ok = soft64(x[part].cpu(), legal[part].cpu(), 0.8)
+      at = want.cpu().long().clamp(min=0)[:, None]
+      there = want.cpu() >= 0
+      lp64 = torch.where(there, exact.gather(1, at)[:, 0], torch.zeros_like(h64))
+      off = (a / 64 + 24) * 2.0 ** -22 + 2.0 ** -21 * (lp64.abs() + math.log(a) + 1)
+      off_h = (a / 64 + 24) * 2.0 ** -22 * (h64 + 2 * (math.log(a) + 1)) + 2.0 ** -21 * (math.log(a) + 1)
+      assert ((lp[part].cpu().double() - lp64).abs() <= off).all() and ((h[part].cpu().double() - h64).abs() <= off_h).all()
+      one = torch.zeros_like(p).scatter_(1, at, 1.0) * there[:, None]
+      gl, gh = (g_lp[part].cpu().double() * there)[:, None], g_h[part].cpu().double()[:, None]
+      term = torch.where(p > 0, p * (exact + h64[:, None]), torch.zeros_like(p))
+      want64 = torch.where(ok, (gl * (one - p) - gh * term) / 0.8, torch.zeros_like(p))
+      # p is off by `off` of itself, log p and H by off + off_h
+      size = gl.abs() * (one + p) + gh.abs() * p * (torch.where(p > 0, exact.abs(), torch.zeros_like(p)) + h64[:, None] + 1)
+      tol = size * 4 * (off + off_h)[:, None] + torch.finfo(dtype).eps / 2 * want64.abs() + 2.0 ** -100
+      assert ((grad[part].cpu().double() - want64).abs() <= tol).all()

@@ -914,3 +914,28 @@ def test_a_projection_made_in_inference_mode_takes_new_values():
     other.load(w, c)
     assert torch.equal(other(b), want)
   assert leaf._version == 0 and torch.equal(other(b), want)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('dtype', DTYPES)
+@pytest.mark.parametrize('n,hidden', [(70, 64), (3000, 48), (70, 19)])
+def test_arrays_at_any_element(n, hidden, dtype):
+  """Bias, residual, gradient and slopes that begin in the middle of a word or of four elements: the same numbers."""
+  chars, boards, weight, bias, residual = make(n, 6, 7, 9, hidden, dtype, 64)
+  b, w = boards.cuda(), weight.cuda()
+
+  def moved(t, by):  # the same numbers `by` elements into an allocation
+    held = torch.empty(t.numel() + 8, dtype=t.dtype, device='cuda')[by:by + t.numel()].view(t.shape)
+    return held.copy_(t)
+
+  grad = torch.randn(n, hidden, generator=torch.Generator().manual_seed(3)).to(weight.dtype)
+  shifted = torch.empty(b.numel() + 8, dtype=torch.uint8, device='cuda')
+  for act in ('relu', 'gelu'):
+    want, slope = rendering.project(b, chars, w, bias.cuda(), activation=act, residual=residual.cuda(), return_slope=True)
+    grads = rendering.project_backward(b, chars, w, grad.cuda(), slope, activation=act)
+    for by in (1, 2, 3):
+      at = shifted[by:by + b.numel()].view(b.shape).copy_(b)
+      out, k = rendering.project(at, chars, moved(weight, by), moved(bias, by), activation=act, residual=moved(residual, by), return_slope=True)
+      assert torch.equal(out, want) and torch.equal(k, slope)
+      got = rendering.project_backward(at, chars, w, moved(grad, by), moved(slope, by), activation=act)
+      assert torch.equal(got[0], grads[0]) and torch.equal(got[1], grads[1])
