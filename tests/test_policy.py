@@ -789,3 +789,33 @@ def test_more_rows_than_one_launch_takes(n, a):
       size = gl.abs() * (one + p) + gh.abs() * p * (torch.where(p > 0, exact.abs(), torch.zeros_like(p)) + h64[:, None] + 1)
       tol = size * 4 * (off + off_h)[:, None] + torch.finfo(dtype).eps / 2 * want64.abs() + 2.0 ** -100
       assert ((grad[part].cpu().double() - want64).abs() <= tol).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('n,a,stride', [((1 << 20) + 3, 2100, 2100), (300, 20000, 1 << 23), (40, 1 << 20, (1 << 26) + 8)])
+def test_offsets_beyond_31_bits(n, a, stride):
+  """Logits of 2^31 elements and more: the last rows give what they give by themselves."""
+  g = torch.Generator(device='cuda').manual_seed(a)
+  held = torch.empty((n - 1) * stride + a, dtype=torch.bfloat16, device='cuda')
+  assert held.numel() > 1 << 31
+  x = held.as_strided((n, a), (stride, 1))
+  for lo in range(0, n, 1 << 16):
+    x[lo:lo + (1 << 16)].normal_(0, 2, generator=g)
+  u = torch.rand(n, generator=g, device='cuda')
+  g_lp, g_h = torch.randn(n, generator=g, device='cuda'), torch.randn(n, generator=g, device='cuda')
+  for kw in (dict(top_p=0.9), dict(top_k=40, temperature=0.7), dict(temperature=0.0)):
+    got = policy.sample(x, u, **kw)
+    lp, h, stats = policy.log_prob(x, got, return_stats=True)
+    for part in (slice(0, 5), slice(n // 2, n // 2 + 5), slice(n - 5, n)):
+      near = x[part].contiguous()
+      assert torch.equal(got[part], policy.sample(near, u[part], **kw))
+      exact, _, h64, _, _ = soft64(near.cpu(), None, 1.0)
+      lp64 = exact.gather(1, got[part].cpu().long()[:, None])[:, 0]
+      off = (a / 64 + 24) * 2.0 ** -22
+      assert ((lp[part].cpu().double() - lp64).abs() <= off + 2.0 ** -21 * (lp64.abs() + math.log(a) + 1)).all()
+      assert ((h[part].cpu().double() - h64).abs() <= off * (h64 + 2 * (math.log(a) + 1)) + 2.0 ** -21 * (math.log(a) + 1)).all()
+  if n * a < 1 << 31:
+    return
+  grad = policy.log_prob_backward(x, got, h, stats, g_lp, g_h)
+  for part in (slice(0, 5), slice(n // 2, n // 2 + 5), slice(n - 5, n)):
+    assert torch.equal(grad[part], policy.log_prob_backward(x[part], got[part], h[part], stats[part], g_lp[part], g_h[part]))

@@ -939,3 +939,39 @@ def test_arrays_at_any_element(n, hidden, dtype):
       assert torch.equal(out, want) and torch.equal(k, slope)
       got = rendering.project_backward(at, chars, w, moved(grad, by), moved(slope, by), activation=act)
       assert torch.equal(got[0], grads[0]) and torch.equal(got[1], grads[1])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('rows,cols,hidden,dtype,act,stacked', [(3, 4, 1056, 'bfloat16', 'relu', False), (3, 4, 1056, 'bfloat16', 'relu', True),
+                                                                (42, 50, 8, 'float16', None, False), (42, 17, 8, 'float16', None, True)])
+def test_offsets_beyond_31_bits(rows, cols, hidden, dtype, act, stacked):
+  """Results of 2^31 elements and more, boards of 2^32 bytes and more.  All numbers are small multiples of 1/16 and all sums
+  of them exact, so the last boards give what they give by themselves, and the gradients are whole numbers."""
+  n, layers = (1 << 21) + 5, 3
+  g = torch.Generator(device='cuda').manual_seed(rows)
+  chars, cells = ' !"', rows * cols
+  if stacked:
+    boards = torch.randint(0, 2, (n, layers, rows, cols), generator=g, device='cuda', dtype=torch.uint8)
+  else:
+    boards = torch.randint(32, 36, (n, rows, cols), generator=g, device='cuda', dtype=torch.uint8)
+  assert n * hidden >= 1 << 31 or boards.numel() >= 1 << 32
+  dt = getattr(torch, dtype)
+  weight = (torch.randint(-8, 9, (hidden, layers, rows, cols), generator=g, device='cuda').float() / 16).to(dt)
+  bias = (torch.randint(-8, 9, (hidden,), generator=g, device='cuda').float() / 16).to(dt)
+  out, slope = rendering.project(boards, chars, weight, bias, activation=act, return_slope=True)
+  for part in (slice(0, 40), slice(n // 2, n // 2 + 40), slice(n - 40, n)):
+    want, want_slope = rendering.project(boards[part], chars, weight, bias, activation=act, return_slope=True)
+    assert torch.equal(out[part], want)
+    assert slope is None or torch.equal(slope[part], want_slope)
+  grad = torch.randint(-1, 2, (n, hidden), generator=g, device='cuda', dtype=torch.int8).to(dt)
+  dw, db = rendering.project_backward(boards, chars, weight, grad, slope, activation=act)
+  want, want_b = torch.zeros(hidden, layers * cells, dtype=torch.float64, device='cuda'), torch.zeros(hidden, dtype=torch.float64, device='cuda')
+  for lo in range(0, n, 1 << 16):
+    part = boards[lo:lo + (1 << 16)]
+    x = part.flatten(1) if stacked else torch.stack([part == ord(c) for c in chars], 1).flatten(1)
+    dz = grad[lo:lo + (1 << 16)].double()
+    if slope is not None:
+      dz = dz * slope[lo:lo + (1 << 16)]
+    want += dz.t().contiguous() @ x.double()
+    want_b += dz.sum(0)
+  assert torch.equal(dw.flatten(1), want.to(dt)) and torch.equal(db, want_b.to(dt))
