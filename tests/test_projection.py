@@ -975,3 +975,21 @@ def test_offsets_beyond_31_bits(rows, cols, hidden, dtype, act, stacked):
     want += dz.t().contiguous() @ x.double()
     want_b += dz.sum(0)
   assert torch.equal(dw.flatten(1), want.to(dt)) and torch.equal(db, want_b.to(dt))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('stacked', [False, True])
+@pytest.mark.parametrize('n,layers,rows,cols,hidden,dtype', [(5, 2, 1024, 1024, 3, 'bfloat16'), (700, 1, 512, 1024, 2, 'float16'), (3, 32, 100, 101, 5, 'float32'),
+                                                             (70, 3, 2, 2, 1 << 16, 'float16'), (600, 2, 1, 1, 1 << 16, 'float32')])
+def test_the_largest_boards_and_layers(n, layers, rows, cols, hidden, dtype, stacked):
+  """A million cells a board, 65,536 units, 32 layers.  Small multiples of 1/16: all sums are exact."""
+  chars, boards, weight, bias, residual = make(n, layers, rows, cols, hidden, dtype, 65, stacked, grid=True)
+  b, w, c = boards.cuda(), weight.cuda(), bias.cuda()
+  grad = torch.randint(-1, 2, (n, hidden), generator=torch.Generator().manual_seed(4)).to(weight.dtype).cuda()
+  x = features(chars, b).float()  # (as are float32's products and sums of these numbers)
+  want = x @ w.flatten(1).float().t().contiguous() + c.float()
+  got = rendering.project(b, chars, w, c)
+  assert torch.equal(got, want.to(w.dtype))
+  dw, db = rendering.project_backward(b, chars, w, grad)
+  assert torch.equal(dw.flatten(1), (grad.float().t().contiguous() @ x).to(w.dtype))
+  assert torch.equal(db, grad.float().sum(0).to(w.dtype))
