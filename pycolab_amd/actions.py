@@ -215,6 +215,8 @@ def log_prob(logits, actions, legal=None, temperature=1.0, return_stats=False):
   `return_stats=True`: no autograd; returns (log_prob, entropy, stats), what `log_prob_backward` takes -- the pair to
   capture into a graph."""
   torch = dev.require_torch('log_prob()')
+  if not return_stats and torch.is_grad_enabled():
+    actions, legal = dev.saveable(torch, actions), dev.saveable(torch, legal)
   desc, legal, n, _, _ = _rows(torch, logits, legal)
   actions, temperature = _taken(torch, actions, n, logits.device), _positive(temperature)
   if return_stats:

@@ -208,6 +208,11 @@ def refuse_recording_in_capture(what, instead):
     raise RuntimeError('{}() does not record gradients while a graph is captured: capture {} instead'.format(what, instead))
 
 
+def saveable(torch, tensor):
+  """The tensor, or a copy where it was made in inference mode -- in a rollout, say: autograd saves no such tensor."""
+  return tensor.clone() if isinstance(tensor, torch.Tensor) and tensor.is_inference() else tensor
+
+
 def refuse_tangents(what, *tensors):
   """Forward mode is not recorded: a tensor with a tangent looks like any other (it does not ask for gradients), and its
   tangent would be dropped."""

@@ -955,6 +955,8 @@ def project(boards, layers, weight, bias=None, activation=None, residual=None, r
   `project_backward` takes -- the pair to capture into a graph."""
   torch = dev.require_torch('project()')
   plan = _Projection(layers, weight, bias, activation)
+  if not return_slope and weight.requires_grad and torch.is_grad_enabled():
+    boards = dev.saveable(torch, boards)
   view = _Boards(boards, layers)
   desc = plan.at(view)
   plan.check_rows(residual, 'residual', view.n)

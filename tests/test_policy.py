@@ -819,3 +819,22 @@ def test_offsets_beyond_31_bits(n, a, stride):
   grad = policy.log_prob_backward(x, got, h, stats, g_lp, g_h)
   for part in (slice(0, 5), slice(n // 2, n // 2 + 5), slice(n - 5, n)):
     assert torch.equal(grad[part], policy.log_prob_backward(x[part], got[part], h[part], stats[part], g_lp[part], g_h[part]))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('a', [5, 300, 20000])
+def test_what_a_rollout_in_inference_mode_left(a):
+  """Actions and masks made in inference mode serve a gradient afterwards."""
+  x, u = (t.cuda() for t in logits_of(40, a, 'float32', 66))
+  legal = torch.rand(40, a, generator=torch.Generator().manual_seed(5)).cuda() < 0.8
+  with torch.inference_mode():
+    mask, one = legal.clone(), legal[0].clone()
+    taken, free = policy.sample(x, u, legal=mask), policy.sample(x, u, legal=one)
+  for t, m, plain in ((taken, mask, legal), (free, one, legal[0])):
+    assert t.is_inference() and m.is_inference()
+    grads = []
+    for allowed, drawn in ((m, t), (plain, t.clone())):
+      leaf = x.clone().requires_grad_()
+      lp, h = policy.log_prob(leaf, drawn, legal=allowed)
+      grads += torch.autograd.grad(lp.sum() + 0.1 * h.sum(), leaf)
+    assert torch.equal(*grads)

@@ -993,3 +993,41 @@ def test_the_largest_boards_and_layers(n, layers, rows, cols, hidden, dtype, sta
   dw, db = rendering.project_backward(b, chars, w, grad)
   assert torch.equal(dw.flatten(1), (grad.float().t().contiguous() @ x).to(w.dtype))
   assert torch.equal(db, grad.float().sum(0).to(w.dtype))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('stacked', [False, True])
+def test_boards_that_a_rollout_in_inference_mode_left(stacked):
+  chars, boards, weight, bias, _ = make(50, 5, 6, 7, 40, 'float32', 67, stacked)
+  b, grad = boards.cuda(), torch.randn(50, 40, generator=torch.Generator().manual_seed(6)).cuda()
+  with torch.inference_mode():
+    kept = torch.stack([b, b], 1)[:, 1]
+  assert kept.is_inference() and not kept.is_contiguous()
+  grads = []
+  for given in (b, kept):
+    leaves = [weight.cuda().requires_grad_(), bias.cuda().requires_grad_()]
+    grads.append(torch.autograd.grad(rendering.project(given, chars, *leaves, activation='tanh'), leaves, grad))
+  assert all(torch.equal(p, q) for p, q in zip(*grads))
+  frozen = bias.cuda().requires_grad_()
+  only, = torch.autograd.grad(rendering.project(kept, chars, weight.cuda(), frozen, activation='tanh'), frozen, grad)
+  assert torch.equal(only, grads[0][1])
+
+
+@pytest.mark.gpu
+def test_an_engine_stepped_in_inference_mode():
+  eng = small_engine(9)
+  with torch.inference_mode():
+    obs, _, _ = eng.its_showtime()
+    board = obs.board
+  big = torch.randn(8, 2, 45, 89, generator=torch.Generator().manual_seed(7)).cuda().requires_grad_()
+  want, = torch.autograd.grad(rendering.project(obs.board.clone(), 'P@', big).sum(), big)
+  for boards in (board, obs):
+    out = rendering.project(boards, 'P@', big).sum()
+    got, = torch.autograd.grad(out, big)
+    assert torch.equal(got, want)
+  out, late = rendering.project(board, 'P@', big).sum(), rendering.project(obs, 'P@', big).sum()
+  eng.step(torch.zeros(9, dtype=torch.int32).cuda())
+  assert torch.equal(torch.autograd.grad(out, big)[0], want)  # (of a copy)
+  with pytest.raises(RuntimeError, match='overwritten'):
+    torch.autograd.grad(late, big)
+  eng.close()
